@@ -255,6 +255,123 @@ int s2s_profile_only(s2s_ctx *ctx, const char *kernel);
  * Reference: the stage loop of src/gpu.rs:481-529 / src/cpu.rs:1516-1581. */
 int s2s_rstb_device(s2s_ctx *ctx, int stage, int hp, int wp, const float *d_in, float *d_out);
 
+/* ---- transformer operators on device buffers ------------------------------- */
+/* Attention, rotary positions and the root-mean-square norm for tokens of any
+ * count and layout, where the forward above has window attention on 8x8
+ * windows, a 15x15 position-bias table and LayerNorm. No reference counterpart.
+ *
+ * They need no context. Every array is device memory of the stream's device
+ * (`stream` is a hipStream_t; NULL is the current device's default stream)
+ * unless it is called a host array; memory of another device and plain host
+ * memory are refused. A call checks its arguments, enqueues its kernels on
+ * `stream` and returns without waiting; it allocates nothing, keeps nothing of
+ * its arrays and can be captured into a graph. Any number of calls may run at
+ * once if none writes what another reads or writes, workspaces included. Sums,
+ * softmax statistics and norms are held in 32 bits; results are rounded once. */
+
+/* Element types. */
+enum s2s_dtype { S2S_F32 = 0, S2S_F16 = 1, S2S_BF16 = 2, S2S_E4M3 = 3 };
+
+/* An array [batch][tokens][heads][width]: channels are adjacent, the other
+ * strides are in elements. They may be any non-negative numbers (0 repeats an
+ * input over that dimension); a written array's elements may not overlap. */
+typedef struct s2s_tokens {
+    void *data;
+    int64_t batch, token, head;
+} s2s_tokens;
+
+/* softmax(bias + cap tanh(scale q k / cap)) v, for every query token i and query
+ * head h (which reads key head h / (q_heads / k_heads)):
+ *  - key j takes part if j < k_lens[b]; under `causal`, if also j <= P(i), the
+ *    query's place among the keys, P(i) = k_lens[b] - q_lens[b] + i, or
+ *    j < prefix[b]; with documents, if also q_docs[b][i] == k_docs[b][j] >= 0.
+ *    Whatever other keys' k and v hold (NaN and infinities too) has no effect.
+ *  - the score is scale q.k, capped if cap > 0; then - slopes[h] |d| and
+ *    + table[h][clamp(d + table_size / 2, 0, table_size - 1)] are added, d =
+ *    q_pos[b][i] - k_pos[b][j] or, without positions, P(i) - j. A bias of
+ *    minus infinity takes the key out.
+ *  - a query with no key gives zeros. Queries from q_lens[b] on are not
+ *    written. Lengths are taken as clamped to [0, tokens], prefix to k_lens.
+ * (dy, dx) biases of an image's tokens: positions y * S + x with S at least
+ * twice the width less one tell every (dy, dx) apart.
+ * Width up to 128. Scores and sums are f32 (f32 arrays: f32 products too); for
+ * f16 and bf16 the softmax's weights are rounded to that type before they
+ * multiply v. `out` may not overlap an input. */
+typedef struct s2s_attention_args {
+    int dtype; /* of q, k, v, out: S2S_F32, S2S_F16 or S2S_BF16 */
+    int batch, q_tokens, k_tokens, q_heads, k_heads, width;
+    int causal;
+    float scale;
+    float cap; /* 0: none */
+    s2s_tokens q, k, v, out;
+    const int32_t *q_lens, *k_lens; /* [batch], or NULL: all tokens */
+    const int32_t *prefix;          /* [batch], or NULL; only with causal */
+    const int32_t *q_docs, *k_docs; /* [batch][tokens], both or neither */
+    int64_t q_docs_batch, k_docs_batch; /* their batch strides (0: shared) */
+    const int32_t *q_pos, *k_pos;       /* [batch][tokens], both or neither */
+    int64_t q_pos_batch, k_pos_batch;
+    const float *slopes; /* [q_heads], or NULL */
+    const float *table;  /* [q_heads][table_size], or NULL */
+    int table_size;      /* odd */
+} s2s_attention_args;
+
+/* The bytes of device memory (16-byte aligned) that `s2s_attention` needs for
+ * these sizes (0: none): it goes by dtype and the six sizes and reads nothing
+ * else of `args`. */
+int s2s_attention_workspace(const s2s_attention_args *args, uint64_t *bytes);
+
+/* One call of the attention. `workspace` belongs to the call until its work on
+ * `stream` is done: calls (and replays of captured ones) that may overlap on
+ * the device need one each, calls of one stream can share one. Its contents
+ * need no preparation and are left undefined. */
+int s2s_attention(const s2s_attention_args *args, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* Rotary positions with up to four axes: the pair p of every head of q (and k)
+ * is turned by the angle pos[b][token][pair_axis[p]] * inv_freq[p]. Pairs are
+ * channels (p, p + pairs), or (2p, 2p + 1) if `adjacent`; channels from 2 pairs
+ * on are copied. `inverse` turns the other way (the transpose: the gradient).
+ * Angles are reduced in 64-bit fixed point, so far positions lose nothing.
+ * Tokens from lens[b] on are not written. The outputs may be the inputs (with
+ * the same strides) and may not overlap them otherwise. */
+typedef struct s2s_rotary_args {
+    int dtype; /* S2S_F32, S2S_F16 or S2S_BF16 */
+    int batch, tokens, q_heads, k_heads /* 0: no k */, width;
+    int axes, pairs; /* axes 1 to 4; pairs 1 to 128, 2 * pairs <= width */
+    int adjacent, inverse;
+    s2s_tokens q, k, q_out, k_out;
+    const int32_t *pos; /* [batch][tokens][axes] */
+    int64_t pos_batch;  /* its batch stride (0: shared) */
+    const int32_t *lens; /* [batch], or NULL */
+    const double *inv_freq;   /* HOST [pairs]: radians per position, finite, |.| < 2^20 */
+    const uint8_t *pair_axis; /* HOST [pairs] */
+} s2s_rotary_args;
+
+int s2s_rotary(const s2s_rotary_args *args, void *stream);
+
+/* out = h / sqrt(mean(h^2) + eps) * (weight + weight_offset) for every row of
+ * h = x + res, the sum stored in `sum` too if that is not NULL. out_dtype is
+ * dtype, or S2S_E4M3: then every `group` columns (0: the row; else a multiple of
+ * 8) share a scale, scales[row][column / group] = max(largest |out| of them /
+ * 448, 2^-126), and the stored codes are out / scale to the nearest e4m3 (ties
+ * to even, OCP e4m3fn). `sum` and an `out` of dtype may be x or res (with the
+ * same stride) and may not overlap them otherwise. */
+typedef struct s2s_rms_norm_args {
+    int dtype, out_dtype;
+    int64_t rows;
+    int cols;
+    const void *x;
+    const void *res; /* or NULL: no addition */
+    void *sum;       /* or NULL */
+    void *out;
+    int64_t x_stride, res_stride, sum_stride, out_stride; /* of rows, in elements */
+    const float *weight; /* [cols] */
+    float weight_offset, eps;
+    float *scales; /* [rows][ceil(cols / group)], contiguous; S2S_E4M3 only */
+    int group;
+} s2s_rms_norm_args;
+
+int s2s_rms_norm(const s2s_rms_norm_args *args, void *stream);
+
 /* ---- self-test ------------------------------------------------------------ */
 
 /* `gpu::selftest(&Weights)` behind `--cuda-selftest` (reference

@@ -4,6 +4,8 @@ Layout of this package:
   csrc/            the HIP kernels and the C ABI (include/swin2sr_hip.h)
   Makefile         builds libswin2sr_hip.so with hipcc --offload-arch=gfx950
   abi.py           ctypes binding of the ABI and the `Backend` mirror (HipBackend)
+  ops.py           the transformer operators on device buffers: attention, rotary
+                   positions, root-mean-square norm
   model.py         architectures, synthetic checkpoints (crate tensor names) and inputs
   tiling.py        the crate's tile loop and memory policy over the Backend interface
   formats.py       the crate's on-disk formats: converted-checkpoint safetensors with the
@@ -16,4 +18,5 @@ from . import model  # noqa: F401
 from . import hip  # noqa: F401
 from . import tiling  # noqa: F401
 from . import formats  # noqa: F401
+from . import ops  # noqa: F401
 from .abi import HipBackend, S2SError, device_info, load_library  # noqa: F401

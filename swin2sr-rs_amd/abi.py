@@ -41,6 +41,40 @@ class Tensor_(C.Structure):
                 ("shape", C.c_int64 * 4)]
 
 
+class Tokens_(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("batch", C.c_int64), ("token", C.c_int64), ("head", C.c_int64)]
+
+
+class Attention_(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("batch", C.c_int), ("q_tokens", C.c_int), ("k_tokens", C.c_int),
+                ("q_heads", C.c_int), ("k_heads", C.c_int), ("width", C.c_int), ("causal", C.c_int),
+                ("scale", C.c_float), ("cap", C.c_float),
+                ("q", Tokens_), ("k", Tokens_), ("v", Tokens_), ("out", Tokens_),
+                ("q_lens", C.c_void_p), ("k_lens", C.c_void_p), ("prefix", C.c_void_p),
+                ("q_docs", C.c_void_p), ("k_docs", C.c_void_p),
+                ("q_docs_batch", C.c_int64), ("k_docs_batch", C.c_int64),
+                ("q_pos", C.c_void_p), ("k_pos", C.c_void_p),
+                ("q_pos_batch", C.c_int64), ("k_pos_batch", C.c_int64),
+                ("slopes", C.c_void_p), ("table", C.c_void_p), ("table_size", C.c_int)]
+
+
+class Rotary_(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("batch", C.c_int), ("tokens", C.c_int), ("q_heads", C.c_int),
+                ("k_heads", C.c_int), ("width", C.c_int), ("axes", C.c_int), ("pairs", C.c_int),
+                ("adjacent", C.c_int), ("inverse", C.c_int),
+                ("q", Tokens_), ("k", Tokens_), ("q_out", Tokens_), ("k_out", Tokens_),
+                ("pos", C.c_void_p), ("pos_batch", C.c_int64), ("lens", C.c_void_p),
+                ("inv_freq", C.POINTER(C.c_double)), ("pair_axis", C.POINTER(C.c_uint8))]
+
+
+class RmsNorm_(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("out_dtype", C.c_int), ("rows", C.c_int64), ("cols", C.c_int),
+                ("x", C.c_void_p), ("res", C.c_void_p), ("sum", C.c_void_p), ("out", C.c_void_p),
+                ("x_stride", C.c_int64), ("res_stride", C.c_int64), ("sum_stride", C.c_int64),
+                ("out_stride", C.c_int64), ("weight", C.c_void_p), ("weight_offset", C.c_float),
+                ("eps", C.c_float), ("scales", C.c_void_p), ("group", C.c_int)]
+
+
 _lib = None
 
 FP = C.POINTER(C.c_float)
@@ -75,6 +109,10 @@ EXPORTS = {
     "s2s_profile_query": (C.c_int, [C.c_void_p, C.c_char_p, C.POINTER(C.c_double), C.POINTER(C.c_int)]),
     "s2s_profile_only": (C.c_int, [C.c_void_p, C.c_char_p]),
     "s2s_rstb_device": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
+    "s2s_attention_workspace": (C.c_int, [C.POINTER(Attention_), C.POINTER(C.c_uint64)]),
+    "s2s_attention": (C.c_int, [C.POINTER(Attention_), C.c_void_p, C.c_uint64, C.c_void_p]),
+    "s2s_rotary": (C.c_int, [C.POINTER(Rotary_), C.c_void_p]),
+    "s2s_rms_norm": (C.c_int, [C.POINTER(RmsNorm_), C.c_void_p]),
     "s2s_test_window_map": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int32),
                                       C.POINTER(C.c_uint8)]),
     "s2s_test_qkv_windows": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, FP, FP, FP,
