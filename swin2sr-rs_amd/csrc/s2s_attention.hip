@@ -1,90 +1,111 @@
-// s2s_attention.hip - attention over token arrays of any layout: capped scores,
-// biases by distance, document, causal and prefix masks, grouped heads.
-#include <algorithm>
-#include <cmath>
-
-#include "s2s_device.h"
-#include "s2s_kernels.h"
-#include "s2s_ops.h"
+// s2s_attention.hip - the attention operator's launcher: how a call is cut over the
+// chip, its workspace, and the documents' tile summary.
+#include "s2s_attention.h"
 
 namespace {
 
-// One wave per query row: 64 keys at a time, a lane per key for the scores,
-// then a lane per channel for the products with v.
-template <typename T>
-__global__ __launch_bounds__(64) void k_attn_row(AttnOpArgs a) {
-    const int lane = threadIdx.x;
-    const long long id = blockIdx.x;
-    const int h = (int)(id % a.hq), i = (int)(id / a.hq % a.nq), b = (int)(id / a.hq / a.nq);
-    const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
-    const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.nk) : a.nk;
-    if (i >= ql) return;
-    const int at = kl - ql + i;
-    int lim = kl;
-    if (a.causal) lim = min(kl, max(at + 1, a.prefix ? a.prefix[b] : 0));
-    const T *q = (const T *)a.q + b * a.sq.b + i * a.sq.t + h * a.sq.h;
-    const T *k = (const T *)a.k + b * a.sk.b + (h / a.group) * a.sk.h;
-    const T *v = (const T *)a.v + b * a.sv.b + (h / a.group) * a.sv.h;
-    const int doc = a.q_docs ? a.q_docs[b * a.q_docs_b + i] : 0;
-    if (a.q_docs && doc < 0) lim = 0;
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int j0 = 0; j0 < lim; j0 += 64) {
-        const int j = j0 + lane;
-        bool ok = j < lim;
-        if (ok && a.q_docs) ok = a.k_docs[b * a.k_docs_b + j] == doc;
-        float s = -INFINITY;
-        if (ok) {
-            s = 0.f;
-            for (int d = 0; d < a.width; ++d) s = fmaf((float)q[d], (float)k[j * a.sk.t + d], s);
-            s *= a.scale;
-            if (a.cap > 0.f) s = a.cap * tanhf(s / a.cap);
-            const int dist = a.q_pos ? a.q_pos[b * a.q_pos_b + i] - a.k_pos[b * a.k_pos_b + j] : at - j;
-            if (a.slopes) s -= a.slopes[h] * fabsf((float)dist);
-            if (a.table) {
-                const int half = a.table_size / 2;
-                s += a.table[(long long)h * a.table_size + min(max(dist, -half), half) + half];
-            }
-        }
-        float top = s;
-        for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-        const float mn = fmaxf(m, top);
-        const float p = mn == -INFINITY ? 0.f : expf(s - mn), f = mn == -INFINITY ? 0.f : expf(m - mn);
-        m = mn;
-        l = l * f + p;
-        o0 *= f;
-        o1 *= f;
-        for (int x = 0; x < min(64, lim - j0); ++x) {
-            const float px = __shfl(p, x);
-            if (!__shfl((int)ok, x)) continue;
-            const T *vr = v + (j0 + x) * a.sv.t;
-            if (lane < a.width) o0 = fmaf(px, (float)vr[lane], o0);
-            if (lane + 64 < a.width) o1 = fmaf(px, (float)vr[lane + 64], o1);
-        }
-    }
-    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
-    const float r = l > 0.f || l != l ? 1.f / l : 0.f;
-    T *out = (T *)a.out + b * a.so.b + i * a.so.t + h * a.so.h;
-    if (lane < a.width) out[lane] = (T)(o0 * r);
-    if (lane + 64 < a.width) out[lane + 64] = (T)(o1 * r);
+int round_up(int v, int m) { return (v + m - 1) / m * m; }
+
+// Columns of at most 16 share one set of waves that split each key tile; more take
+// waves of 16 or 32 columns. Where that leaves CUs without work the keys are cut
+// into ranges whose sums a second kernel joins.
+attn::Cut cut_of(int dtype, const AttnOpArgs &a) {
+    attn::Cut c;
+    const long long cols = (long long)a.group * a.nq, pairs = (long long)a.batch * a.hk;
+    const int cus = cu_count();
+    c.dp = round_up(std::max(a.width, 1), 32);
+    c.wk = cols <= 16;
+    c.nb = c.wk || cols <= 64 || (cols + 127) / 128 * pairs < 2 * cus ? 1 : 2;
+    c.tk = dtype == 0 && !c.wk ? 32 : 64;
+    const int per = c.wk ? 16 : 64 * c.nb;
+    c.tiles = (int)((cols + per - 1) / per);
+    // ranges of 4 tiles at least, workgroups for two per CU at most
+    const long long blocks = std::max(1LL, pairs * c.tiles), want = 2LL * cus;
+    const long long nt = ((long long)a.nk + c.tk - 1) / c.tk;
+    c.splits = (int)std::max(1LL, std::min({want / blocks, nt / 4, 256LL}));
+    return c;
 }
 
-template <typename T>
-hipError_t attention_type(const AttnOpArgs &a, void *, hipStream_t st) {
-    const long long n = (long long)a.batch * a.hq * a.nq;
-    if (n > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_attn_row<T>), dim3((unsigned)n), dim3(64), 0, st, a);
-    return hipGetLastError();
+int meta_tiles(const attn::Cut &c, const AttnOpArgs &a) { return (a.nk + c.tk - 1) / c.tk; }
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+// {smallest id >= 0, largest, smallest of all} of a key tile's documents: a wave
+// per tile.
+__global__ __launch_bounds__(256) void k_doc_tiles(AttnOpArgs a, int tk, int tiles, int4 *meta) {
+    const int lane = threadIdx.x & 63;
+    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= (long long)a.batch * tiles) return;
+    const int b = (int)(id / tiles), t = (int)(id - (long long)b * tiles);
+    const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.nk) : a.nk;
+    const int j = t * tk + lane;
+    int lo = 0x7fffffff, hi = -1, all = 0x7fffffff;
+    if (lane < tk && j < kl) {
+        all = a.k_docs[b * a.k_docs_b + j];
+        if (all >= 0) lo = hi = all;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        lo = min(lo, __shfl_xor(lo, m));
+        hi = max(hi, __shfl_xor(hi, m));
+        all = min(all, __shfl_xor(all, m));
+    }
+    if (lane == 0) meta[id] = make_int4(lo, hi, all, 0);
+}
+
+// The largest power of two in bytes, up to 16, that an array's address, strides
+// and width are multiples of.
+int aligned_bytes(const void *p, const Strides &s, int width, int size) {
+    unsigned long long m = (unsigned long long)(uintptr_t)p | (unsigned long long)((s.b | s.t | s.h) * size) | 16;
+    m |= (unsigned long long)width * size;
+    return (int)(m & (~m + 1));
 }
 
 }  // namespace
 
-size_t attn_op_workspace(int, const AttnOpArgs &) { return 0; }
+size_t attn_op_workspace(int dtype, const AttnOpArgs &a) {
+    const attn::Cut c = cut_of(dtype, a);
+    size_t n = round16((size_t)a.batch * meta_tiles(c, a) * sizeof(int4));
+    if (c.splits > 1) {
+        const size_t rows = (size_t)a.batch * a.hk * c.splits * a.group * a.nq;
+        n += rows * c.dp * 4 + rows * 8;
+    }
+    return n;
+}
 
 hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStream_t st) {
+    const attn::Cut c = cut_of(dtype, a);
+    AttnLaunch L{};
+    L.cols = a.group * a.nq;
+    L.tiles = c.tiles;
+    L.splits = c.splits;
+    const int size = dtype == 0 ? 4 : 2;
+    char *w = (char *)ws;
+    const int mt = meta_tiles(c, a);
+    const size_t meta_bytes = round16((size_t)a.batch * mt * sizeof(int4));
+    if (c.splits > 1) {
+        const size_t rows = (size_t)a.batch * a.hk * c.splits * L.cols;
+        L.part_o = (float *)(w + meta_bytes);
+        L.part_ml = L.part_o + rows * c.dp;
+    }
+    // a summary of few tiles would skip nothing
+    if (a.k_docs && mt > 4) {
+        L.meta = (const int4 *)w;
+        L.meta_tiles = mt;
+        const long long n = (long long)a.batch * mt;
+        hipLaunchKernelGGL(k_doc_tiles, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, (int4 *)w);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    int al = aligned_bytes(a.q, a.sq, a.width, size);
+    if (a.nk > 0) al = std::min(al, std::min(aligned_bytes(a.k, a.sk, a.width, size), aligned_bytes(a.v, a.sv, a.width, size)));
+    L.vec = std::min(al, 8);
+    L.out_vec = aligned_bytes(a.out, a.so, a.width, size) >= 4 * size;
+    const bool aligned = al >= 16;
     switch (dtype) {
-        case 0: return attention_type<float>(a, ws, st);
-        case 1: return attention_type<half_t>(a, ws, st);
-        case 2: return attention_type<bfloat_t>(a, ws, st);
+        case 0: return launch_attention_f32(a, L, c, aligned, st);
+        case 1: return launch_attention_f16(a, L, c, aligned, st);
+        case 2: return launch_attention_bf16(a, L, c, aligned, st);
     }
     return hipErrorInvalidValue;
 }
