@@ -23,6 +23,41 @@
 #include "s2s_kernels.h"
 #include "s2s_ops.h"
 
+constexpr float kAttnLog2e = 1.4426950408889634f;
+
+// How a product q k becomes an exponent in powers of two.
+struct AttnScore {
+    float c1;    // without a cap: its factor; with one: 2 log2(e) / cap of scale q k
+    float capl;  // cap in powers of two
+    // cap tanh(z) for |z| <= 0.375 as x (p0 + p1 x^2 + p2 x^4 + p3 x^6) of the product x: tanh(z)
+    // / z to 7e-8 (least squares, weights iterated towards equal ripple), three
+    // fused operations where the exponential takes two transcendentals, and no
+    // cancellation near zero. poly_max: the |x| that it holds for.
+    float p0, p1, p2, p3, poly_max;
+    bool general;  // a bias other than slopes by token distance
+    void set(const AttnOpArgs &a) {
+        // a negative or zero scale would turn masked minus infinities round: scores in
+        // powers of two at once, with no slope
+        general = a.table || a.k_pos || (!(a.cap > 0.f) && !(a.scale > 1e-30f));
+        c1 = a.scale * kAttnLog2e;
+        capl = a.cap * kAttnLog2e;
+        p0 = p1 = p2 = p3 = 0.f;
+        poly_max = -1.f;
+        if (a.cap > 0.f) {
+            const float z = a.scale / a.cap, w = z * z;
+            c1 = z * (2.f * kAttnLog2e);
+            // the coefficients and powers of x in the normal range
+            if (std::fabs(z) > 1e-5f && std::fabs(z) < 1e5f && a.cap < 1e6f) {
+                p0 = capl * z;
+                p1 = p0 * w * -0.33332333f;
+                p2 = p0 * w * w * 0.13289726f;
+                p3 = p0 * w * w * w * -0.04848728f;
+                poly_max = 0.375f / std::fabs(z);
+            }
+        }
+    }
+};
+
 // What a launch adds to the call's arguments.
 struct AttnLaunch {
     int cols;       // group * nq
@@ -34,6 +69,7 @@ struct AttnLaunch {
     float *part_ml;  // [batch * hk][splits][cols][2]: reference and sum of the weights
     const int4 *meta;  // documents: [batch][key tiles] {smallest, largest id >= 0, smallest id, 0}
     int meta_tiles;
+    AttnScore score;
 };
 
 namespace attn {
@@ -42,7 +78,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = kAttnLog2e;
 
 template <typename T>
 struct Type;
@@ -98,6 +134,31 @@ __device__ __forceinline__ int v_slot(int r, int c) {
     }
 }
 
+// A resource of less than 2^31 bytes (64 rows of 2^22 elements are 2^30 at most).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void *p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, bytes, 0x00020000);
+}
+
+// LDS by byte address: a lane's address once per tile, what is constant in the
+// instruction's offset.
+typedef __attribute__((address_space(3))) char lds_t;
+template <typename V>
+__device__ __forceinline__ V lds_read(const lds_t *p, int off) {
+    return *(const __attribute__((address_space(3))) V *)(p + off);
+}
+__device__ __forceinline__ s4 lds_read_tr(const lds_t *p, int off) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(p + off));
+}
+// The address itself, kept from being split into a loop-invariant part per use.
+__device__ __forceinline__ const lds_t *opaque(const lds_t *p) {
+    unsigned x = (unsigned)(size_t)p;
+    asm volatile("" : "+v"(x));
+    return (const lds_t *)(size_t)x;
+}
+__device__ __forceinline__ const lds_t *lds_xor(const lds_t *p, unsigned m) {
+    return (const lds_t *)(size_t)((unsigned)(size_t)p ^ m);
+}
+
 // max and sum over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48)
 __device__ __forceinline__ void swap16(float &a, float &b) {
     asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
@@ -106,6 +167,31 @@ __device__ __forceinline__ float col_max(float x) {
     float y = x;
     swap16(x, y);
     return half_max(fmaxf(x, y));
+}
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+
+// The kernel's arguments, read again: what only the end of the kernel needs would
+// otherwise take scalar registers through the loop.
+struct AttnParams {
+    AttnOpArgs a;
+    AttnLaunch L;
+};
+__device__ __forceinline__ const __attribute__((address_space(4))) AttnParams *late_params() {
+    auto p = (const __attribute__((address_space(4))) AttnParams *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
+// max of three as one instruction (fmaxf quiets each operand first); a NaN is dropped
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
 }
 __device__ __forceinline__ float col_sum(float x) {
     float y = x;
@@ -177,10 +263,12 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 //  WK false: wave w has columns 16 NB w .. + 16 NB of the tile's 64 NB, all keys.
 //  WK true (at most 16 columns): every wave has all columns and a quarter of each
 //  key tile (one block of 16 keys of 64); the four sums meet in LDS at the end.
+//  GEN: with what AttnScore::general asks for. Apart, since the registers of those
+//  paths would be spilled around the others' loop.
 // K and V tiles of TK keys are copied straight into LDS, two buffers each, the
 // next tile in flight while one is computed. ALIGNED: rows of 16-byte multiples,
 // copied by the DMA; otherwise through registers in narrower accesses.
-template <typename T, int DP, int NB, bool WK, bool ALIGNED>
+template <typename T, int DP, int NB, bool WK, bool ALIGNED, bool GEN>
 struct Kernel {
     typedef Type<T> Ty;
     typedef typename Ty::V Vec;
@@ -198,8 +286,19 @@ struct Kernel {
     static constexpr size_t kJoin = WK ? (size_t)4 * 16 * (DP + 4) * 4 : 0;
     static constexpr size_t kLds = 4 * kTile > kJoin ? 4 * kTile : kJoin;
 
-    static __device__ void run(const AttnOpArgs &a, const AttnLaunch &L, char *lds) {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // What a tile needs that is the same for all of the workgroup.
+    struct Uniform {
+        const int *k_docs, *k_pos;  // of this batch entry, or null
+        const float *table;
+        int half;  // the table's middle
+        int kl;
+        bool capped, slopes, general;
+        AttnScore sc;
+    };
+
+    // (inlined into the kernel always: late_params has no meaning in a called function)
+    static __device__ __forceinline__ void run(const AttnOpArgs &a, const AttnLaunch &L, char *lds) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = wave_of();
         const int n16 = lane & 15, q = lane >> 4;
         // tile-major, so that with a multiple of 8 (batch, key head) pairs one XCD
         // keeps a pair's keys in its L2, and the tiles with the most keys (the last
@@ -217,15 +316,14 @@ struct Kernel {
 
         // the columns of this lane
         const int wc0 = WK ? c0 : c0 + wave * 16 * NB;
-        int tok[NB], lim[NB], doc[NB], at[NB];
-        const float *tab[NB];
+        int lim[NB], doc[NB], at[NB];
+        int tab[NB];  // the head's row of the table
         float slope[NB];
         Vec qf[NB][KS];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int c = wc0 + nb * 16 + n16, i = c / a.group, h = kvh * a.group + (c - i * a.group);
             const bool ok = i < ql;
-            tok[nb] = ok ? i : -1;
             lim[nb] = ok ? limit(i) : 0;
             doc[nb] = 0;
             if (a.q_docs && ok) {
@@ -234,7 +332,7 @@ struct Kernel {
             }
             at[nb] = a.q_pos && ok ? a.q_pos[b * a.q_pos_b + i] : kl - ql + i;
             slope[nb] = a.slopes && ok ? a.slopes[h] * kLog2e : 0.f;
-            tab[nb] = a.table ? a.table + (long long)(ok ? h : 0) * a.table_size : nullptr;
+            tab[nb] = ok ? h * a.table_size : 0;
             const T *row = (const T *)a.q + b * a.sq.b + (long long)(ok ? i : 0) * a.sq.t + h * a.sq.h;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -303,26 +401,39 @@ struct Kernel {
             return t_end;
         };
 
-        // copying a tile: this thread's chunks
-        const T *kbase = (const T *)a.k + b * a.sk.b + kvh * a.sk.h;
-        const T *vbase = (const T *)a.v + b * a.sv.b + kvh * a.sv.h;
-        const int kst = (int)a.sk.t, vst = (int)a.sv.t;  // below 2^22
+        // copying a tile: this thread's chunks. With the DMA a row past the keys lies
+        // past the resource, whose size is the rows that are left (token strides are
+        // no smaller than the width on this path), and reads as zeros, as does a
+        // chunk past the width
+        const T *kp = (const T *)a.k + b * a.sk.b + kvh * a.sk.h;
+        const T *vp = (const T *)a.v + b * a.sv.b + kvh * a.sv.h;
+        const int kst = (int)a.sk.t, vst = (int)a.sv.t, kstep = TK * kst, vstep = TK * vst;  // (strides up to 2^22)
+        // a wave's next chunks are STEP rows on; the permutations repeat every 16
+        constexpr int STEP = 256 / CH, PER = STEP < 16 ? 16 / STEP : 1;
+        int koff[PER], voff[PER];
+#pragma unroll
+        for (int p = 0; ALIGNED && p < PER; ++p) {
+            const int r = (wave * 64 + lane) / CH + p * STEP, sl = lane & (CH - 1);
+            const int kc = (k_slot<CH>(r, sl) & (CH - 1)) * E, vc = (v_slot<CH, F32>(r, sl) & (CH - 1)) * E;
+            koff[p] = kc < a.width ? (r * kst + kc) * (int)sizeof(T) : 0x60000000;
+            voff[p] = vc < a.width ? (r * vst + vc) * (int)sizeof(T) : 0x60000000;
+        }
         auto stage = [&](int t, int buf) {
             char *kd = lds + buf * 2 * kTile, *vd = kd + kTile;
-            const long long j0 = (long long)t * TK;
-            const T *kp = kbase + j0 * kst, *vp = vbase + j0 * vst;
-            const int left = kl - t * TK;
+            const int left = min(kl - t * TK, TK);
             if constexpr (ALIGNED) {
-                const __amdgpu_buffer_rsrc_t kr = buf_rsrc(kp, BUF_MAX_BYTES), vr = buf_rsrc(vp, BUF_MAX_BYTES);
+                const __amdgpu_buffer_rsrc_t kr = tile_rsrc(kp, left * kst * (int)sizeof(T)),
+                                             vr = tile_rsrc(vp, left * vst * (int)sizeof(T));
+                int ko[PER], vo[PER];
+#pragma unroll
+                for (int p = 0; p < PER; ++p) {
+                    ko[p] = koff[p], vo[p] = voff[p];
+                    asm volatile("" : "+v"(ko[p]), "+v"(vo[p]));  // (sums formed here, not kept)
+                }
 #pragma unroll
                 for (int n = 0; n < LOADS; ++n) {
-                    const int s = (n * 4 + wave) * 64 + lane, r = s / CH;
-                    const int kc = k_slot<CH>(r, s & (CH - 1)) & (CH - 1), vc = v_slot<CH, F32>(r, s & (CH - 1)) & (CH - 1);
-                    const bool ok = r < left;
-                    dma16(kr, (float *)(kd + (size_t)(n * 4 + wave) * 1024),
-                          ok && kc * E < a.width ? (r * kst + kc * E) * (int)sizeof(T) : BUF_OOB);
-                    dma16(vr, (float *)(vd + (size_t)(n * 4 + wave) * 1024),
-                          ok && vc * E < a.width ? (r * vst + vc * E) * (int)sizeof(T) : BUF_OOB);
+                    dma16(kr, (float *)(kd + (size_t)(n * 4 + wave) * 1024), ko[n % PER] + n / PER * (PER * STEP) * kst * (int)sizeof(T));
+                    dma16(vr, (float *)(vd + (size_t)(n * 4 + wave) * 1024), vo[n % PER] + n / PER * (PER * STEP) * vst * (int)sizeof(T));
                 }
             } else {
                 v4u x[2][LOADS];
@@ -353,23 +464,41 @@ struct Kernel {
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db][nb] = f4v{0.f, 0.f, 0.f, 0.f};
         }
-        const float c1 = a.cap > 0.f ? a.scale / a.cap * (2.f * kLog2e) : a.scale * kLog2e;
-        const float capl = a.cap * kLog2e;
-        const bool biased = a.slopes || a.table;
+
+        // this lane's first K and V addresses in a buffer: the others differ by a constant
+        // or by the bits that count chunks (steps of K, channel blocks of V)
+        const lds_t *base = (const lds_t *)lds;
+        const lds_t *kl0 = base + k_slot<CH>((WK ? 16 * wave : 0) + n16, q) * 16;
+        const int vr0 = (WK ? 16 * wave : 0) + 4 * q + (F32 ? 0 : n16 >> 2);
+        const lds_t *vl0 = base + kTile + v_slot<CH, F32>(vr0, F32 ? n16 >> 2 : (n16 >> 1) & 1) * 16 +
+                           (F32 ? (n16 & 3) * 4 : (n16 & 1) * 8);
+
+        Uniform u;
+        u.k_docs = a.k_docs ? a.k_docs + b * a.k_docs_b : nullptr;
+        u.k_pos = GEN && a.k_pos ? a.k_pos + b * a.k_pos_b : nullptr;
+        u.table = GEN ? a.table : nullptr;
+        u.half = a.table_size >> 1;
+        u.kl = kl;
+        u.capped = a.cap > 0.f;
+        u.slopes = a.slopes != nullptr;
+        u.general = GEN && L.score.general;
+        u.sc = L.score;
 
         int t = next(split * per), buf = 0;
+        kp += (long long)t * kstep, vp += (long long)t * vstep;
         if (t < t_end) stage(t, 0);
         while (t < t_end) {
             const bool one_doc = !a.q_docs || (L.meta && ((whole >> (t - live_at)) & 1));
             const int tn = next(t + 1);
             if constexpr (ALIGNED) WAIT_VMCNT(0);
             lds_sync();
+            kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
             if (tn < t_end) stage(tn, buf ^ 1);
             const int j0 = t * TK + (WK ? 16 * wave : 0);  // the wave's first key
             if (j0 < w_max) {
-                const char *kd = lds + buf * 2 * kTile, *vd = kd + kTile;
-                const bool full = j0 + 16 * KB <= w_min && one_doc && !a.table;
-                tile(a, L, kd, vd, j0, b, kl, full, biased, c1, capl, lim, doc, at, slope, tab, qf, o, m, l);
+                const int at_buf = buf * 2 * (int)kTile;
+                const bool full = j0 + 16 * KB <= w_min && one_doc && !(GEN && u.table);
+                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), base + at_buf + kTile, j0, full, lim, doc, at, slope, tab, qf, o, m, l);
             }
             t = tn;
             buf ^= 1;
@@ -414,28 +543,27 @@ struct Kernel {
             }
         }
         // out, or the sums of this key range
+        const auto *late = late_params();
+        const int group = late->a.group, splits = late->L.splits, width = late->a.width, vec = late->L.out_vec;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            if (tok[nb] < 0) continue;
-            const int c = wc0 + nb * 16 + n16;
-            if (L.splits > 1) {
-                const long long row = ((long long)bh * L.splits + split) * L.cols + c;
-                float *po = L.part_o + row * DP;
-                if (q == 0 && (!WK || wave == 0)) {
-                    L.part_ml[2 * row] = m[nb];
-                    L.part_ml[2 * row + 1] = l[nb];
-                }
+            const int c = wc0 + nb * 16 + n16, i = c / group;
+            if (i >= ql) continue;
+            if (splits > 1) {
+                const long long row = ((long long)bh * splits + split) * late->L.cols + c;
+                float *po = late->L.part_o + row * DP, *ml = late->L.part_ml + 2 * row;
+                if (q == 0 && (!WK || wave == 0)) ml[0] = m[nb], ml[1] = l[nb];
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
                     if (!WK || (db & 3) == wave) *(f4v *)(po + db * 16 + 4 * q) = o[db][nb];
             } else {
-                const int h = kvh * a.group + (c - tok[nb] * a.group);
-                T *row = (T *)a.out + b * a.so.b + (long long)tok[nb] * a.so.t + h * a.so.h;
+                const int h = kvh * group + (c - i * group);
+                T *row = (T *)late->a.out + b * late->a.so.b + (long long)i * late->a.so.t + h * late->a.so.h;
                 const float r = l[nb] == 0.f ? 0.f : 1.f / l[nb];
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
                     if (WK && (db & 3) != wave) continue;
-                    store(row, db * 16 + 4 * q, a.width, L.out_vec, o[db][nb] * r);
+                    store(row, db * 16 + 4 * q, width, vec, o[db][nb] * r);
                 }
             }
         }
@@ -454,118 +582,149 @@ struct Kernel {
         }
     }
 
-    // V^T's operand for channel block db: the keys of blocks 2 j and 2 j + 1 (f32: of
-    // block j, one key per lane group and register). With WK the wave's one block.
-    static __device__ __forceinline__ Vec v_operand(const char *vd, int j, int db, int lane) {
-        const int n16 = lane & 15, q = lane >> 4, wave = threadIdx.x >> 6;
+    // V^T's operand for channel block db (vl: the lane's address for it): the keys of
+    // blocks 2 j and 2 j + 1 (f32: of block j, one key per lane group and register). With
+    // WK the wave's one block.
+    static __device__ __forceinline__ Vec v_operand(const lds_t *vl, int j) {
         if constexpr (F32) {
-            f4v x;
-            const int r0 = 16 * (WK ? wave : j) + 4 * q, c = 16 * db + n16;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = *(const float *)(vd + v_slot<CH, F32>(r0 + i, c >> 2) * 16 + (c & 3) * 4);
-            return x;
+            const int r = j * 16 * CH * 16;
+            return f4v{lds_read<float>(vl, r), lds_read<float>(vl, r + CH * 16), lds_read<float>(vl, r + 2 * CH * 16),
+                       lds_read<float>(vl, r + 3 * CH * 16)};
         } else {
-            const int r = 16 * (WK ? wave : 2 * j) + 4 * q + (n16 >> 2), c = 16 * db + 4 * (n16 & 3);
             union {
                 s4 h[2];
                 Vec v;
             } u;
-            u.h[0] = read_tr(vd + v_slot<CH, F32>(r, c >> 3) * 16 + (c & 4) * 2);
+            u.h[0] = lds_read_tr(vl, j * 32 * CH * 16);
             if constexpr (WK) u.h[1] = s4{0, 0, 0, 0};
-            else u.h[1] = read_tr(vd + v_slot<CH, F32>(r + 16, c >> 3) * 16 + (c & 4) * 2);
+            else u.h[1] = lds_read_tr(vl, (j * 32 + 16) * CH * 16);
             return u.v;
         }
     }
-    static __device__ __forceinline__ s4 read_tr(const char *p) {
-        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)p);
-    }
+    static __device__ __forceinline__ const lds_t *v_block(const lds_t *vl, int db) { return lds_xor(vl, db << (F32 ? 6 : 5)); }
 
     // The wave's keys of one tile: scores, softmax step, products with V.
-    static __device__ __forceinline__ void tile(const AttnOpArgs &a, const AttnLaunch &L, const char *kd, const char *vd,
-                                                int j0, int b, int kl, bool full, bool biased, float c1, float capl,
-                                                const int *lim, const int *doc, const int *at, const float *slope,
-                                                const float *const *tab, const Vec (*qf)[KS], f4v (*o)[NB], float *m,
-                                                float *l) {
-        const int lane = threadIdx.x & 63, n16 = lane & 15, q = lane >> 4, wave = threadIdx.x >> 6;
+    static __device__ __forceinline__ void tile(const Uniform &u, const lds_t *kl0, const lds_t *vl0, const lds_t *vd,
+                                                int j0, bool full, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
+                                                const Vec (*qf)[KS], f4v (*o)[NB], float *m, float *l) {
+        const int lane = threadIdx.x & 63, q = lane >> 4;
         f4v s[KB][NB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) s[kb][nb] = f4v{0.f, 0.f, 0.f, 0.f};
+        const lds_t *kls[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kls[ks] = lds_xor(kl0, ks << 6);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const int r = 16 * (WK ? wave : kb) + n16;
-                const Vec x = *(const Vec *)(kd + k_slot<CH>(r, 4 * ks + q) * 16);
+                const Vec x = lds_read<Vec>(kls[ks], kb * 16 * CH * 16);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) s[kb][nb] = mma(x, qf[nb][ks], s[kb][nb]);
             }
-        // scores in powers of two
-        if (a.cap > 0.f) {
-            // cap tanh(z) = cap (1 - 2 / (e^2z + 1))
+        // what is left of a score is a factor to powers of two, except where a cap or a
+        // bias made it powers of two already
+        const AttnScore &sc = u.sc;
+        float unit = sc.c1;
+        if (u.capped) {
+            float big = 0.f;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
+                for (int nb = 0; nb < NB; ++nb) big = max3_abs(max3_abs(big, s[kb][nb][0], s[kb][nb][1]), s[kb][nb][2], s[kb][nb][3]);
+            if (__any(big > sc.poly_max)) {
+                // cap tanh(z) = cap (1 - 2 / (e^2z + 1))
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(s[kb][nb][i] * c1);
-                        s[kb][nb][i] = fmaf(-2.f * capl, __builtin_amdgcn_rcpf(e + 1.f), capl);
-                    }
-        } else {
+                for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+                    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) s[kb][nb] *= c1;
+                        for (int i = 0; i < 4; ++i) {
+                            const float e = __builtin_amdgcn_exp2f(s[kb][nb][i] * sc.c1);
+                            s[kb][nb][i] = fmaf(-2.f * sc.capl, __builtin_amdgcn_rcpf(e + 1.f), sc.capl);
+                        }
+            } else {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = s[kb][nb][i], w = x * x;
+                            s[kb][nb][i] = x * fmaf(w, fmaf(w, fmaf(w, sc.p3, sc.p2), sc.p1), sc.p0);
+                        }
+            }
+            unit = 1.f;
         }
-        int kpos = 0, kdoc = 0;
-        const int jl = j0 + min(lane, 16 * KB - 1);
-        if (biased && a.k_pos) kpos = a.k_pos[b * a.k_pos_b + min(jl, kl - 1)];
-        if (!full && a.k_docs) kdoc = a.k_docs[b * a.k_docs_b + min(jl, kl - 1)];
-        if (biased) {
+        // a lane per key for what is read per key
+        const int jl = min(j0 + min(lane, 16 * KB - 1), u.kl - 1);
+        if (GEN && u.general) {
+            const int kpos = u.k_pos ? u.k_pos[jl] : 0;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int jr = 16 * kb + 4 * q + i;
-                    const int kp = a.k_pos ? __shfl(kpos, jr) : j0 + jr;
+                    const int kp = u.k_pos ? __shfl(kpos, jr) : j0 + jr;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         const int dist = at[nb] - kp;
-                        float x = s[kb][nb][i];
-                        if (a.slopes) x = fmaf(-slope[nb], fabsf((float)dist), x);
-                        if (a.table) x = add_bias(x, entry(a, tab[nb], dist));
+                        float x = fmaf(-slope[nb], fabsf((float)dist), s[kb][nb][i] * unit);
+                        if (u.table) x = add_bias(x, entry(u, tab[nb], dist));
                         // lowest values stay numbers, so that a row of them is even
                         s[kb][nb][i] = x < -1e30f && x != -INFINITY ? -1e30f : x;
                     }
                 }
+            unit = 1.f;
+        } else if (u.slopes) {
+            // distances of neighbours differ by what the register says
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const float d0 = (float)(at[nb] - j0 - 4 * q);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        s[kb][nb][i] = fmaf(-slope[nb], fabsf(d0 - (float)(16 * kb + i)), s[kb][nb][i] * unit);
+            }
+            unit = 1.f;
         }
         if (!full) {
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+            for (int nb = 0; nb < NB; ++nb) {
+                const int n = lim[nb] - j0 - 4 * q;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int jr = 16 * kb + 4 * q + i;
-                    const int kdv = a.k_docs ? __shfl(kdoc, jr) : 0;
+                for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        const bool ok = j0 + jr < lim[nb] && (!a.k_docs || kdv == doc[nb]);
-                        if (!ok) s[kb][nb][i] = -INFINITY;
+                    for (int i = 0; i < 4; ++i)
+                        if (16 * kb + i >= n) s[kb][nb][i] = -INFINITY;
+            }
+            if (u.k_docs) {
+                const int kdoc = u.k_docs[jl];
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int d = __shfl(kdoc, 16 * kb + 4 * q + i);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                            if (d != doc[nb]) s[kb][nb][i] = -INFINITY;
                     }
-                }
+            }
         }
         // the running reference: rescaled only where a score passes it by 2^kLazy
         float top[NB];
         bool grow = false;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            float x = -INFINITY;
+            float x = s[0][nb][0];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x = fmaxf(x, s[kb][nb][i]);
-            top[nb] = col_max(x);
+                x = kb ? max3(max3(x, s[kb][nb][0], s[kb][nb][1]), s[kb][nb][2], s[kb][nb][3])
+                       : max3(max3(x, s[kb][nb][1], s[kb][nb][2]), s[kb][nb][3], s[kb][nb][3]);
+            top[nb] = col_max(x) * unit;
             grow |= top[nb] > m[nb] + Ty::kLazy;
         }
         if (__any(grow)) {
@@ -581,170 +740,205 @@ struct Kernel {
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const float ref = (m[nb] == -INFINITY ? 0.f : m[nb]) - Ty::kShift;
-            float sum = 0.f;
+            const float ref = Ty::kShift - (m[nb] == -INFINITY ? 0.f : m[nb]);
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(s[kb][nb][i] - ref);
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[kb][nb][i], unit, ref));
                     s[kb][nb][i] = p;
-                    sum += p;
+                    sum[i] += p;
                 }
-            l[nb] += sum;
+            l[nb] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         // a masked key's weight is zero, and zero times an infinity is none: with such
         // values among a masked tile's v they are added key by key
-        bool wildv = false;
         if (!full) {
+            bool w = false;
 #pragma unroll
-            for (int j = 0; j < (F32 || WK ? KB : KB / 2); ++j)
+            for (int db = 0; db < DB; ++db) {
 #pragma unroll
-                for (int db = 0; db < DB; ++db) wildv |= any_wild(v_operand(vd, j, db, lane));
-            wildv = __any(wildv);
+                for (int j = 0; j < (F32 || WK ? KB : KB / 2); ++j) w |= any_wild(v_operand(v_block(vl0, db), j));
+                __builtin_amdgcn_sched_barrier(0);  // (few operands at a time)
+            }
+            if (__any(w)) {
+                products<true>(vl0, s, o);
+                wild_products(u, vd, j0, lim, doc, at, tab, o);
+                return;
+            }
         }
-        products(vd, lane, s, o, wildv);
-        if (wildv) wild_products(a, vd, j0, b, kl, lim, doc, at, tab, o);
+        products<false>(vl0, s, o);
     }
 
-    static __device__ __forceinline__ float entry(const AttnOpArgs &a, const float *tab, int dist) {
-        const int half = a.table_size >> 1;
-        return tab[min(max(dist, -half), half) + half];
+    static __device__ __forceinline__ float entry(const Uniform &u, int tab, int dist) {
+        return u.table[tab + min(max(dist, -u.half), u.half) + u.half];
     }
     // bias in powers of two; minus infinity takes the key out whatever its score
     static __device__ __forceinline__ float add_bias(float x, float bias) {
         return bias == -INFINITY ? -INFINITY : fmaxf(bias, -2e38f) * kLog2e + x;
     }
 
-    static __device__ __forceinline__ void products(const char *vd, int lane, const f4v (*s)[NB], f4v (*o)[NB], bool clean) {
+    // O^T += V^T P^T; CLEAN: without V's infinities and NaN
+    template <bool CLEAN>
+    static __device__ __forceinline__ void products(const lds_t *vl0, const f4v (*s)[NB], f4v (*o)[NB]) {
         constexpr int J = F32 || WK ? KB : KB / 2;
+        Vec p[J][NB];
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            Vec p[NB];
+        for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                if constexpr (F32) p[nb] = s[j][nb];
+                if constexpr (F32) p[j][nb] = s[j][nb];
                 else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        p[nb][i] = (T)s[WK ? 0 : 2 * j][nb][i];
-                        p[nb][4 + i] = WK ? (T)0.f : (T)s[WK ? 0 : 2 * j + 1][nb][i];
+                        p[j][nb][i] = (T)s[WK ? 0 : 2 * j][nb][i];
+                        p[j][nb][4 + i] = WK ? (T)0.f : (T)s[WK ? 0 : 2 * j + 1][nb][i];
                     }
                 }
             }
 #pragma unroll
-            for (int db = 0; db < DB; ++db) {
-                Vec x = v_operand(vd, j, db, lane);
-                if (clean) {
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                Vec x = v_operand(v_block(vl0, db), j);
+                if constexpr (CLEAN) {
 #pragma unroll
                     for (int e = 0; e < E; ++e)
                         if (wild((float)x[e])) x[e] = (T)0.f;
                 }
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) o[db][nb] = mma(x, p[nb], o[db][nb]);
+                for (int nb = 0; nb < NB; ++nb) o[db][nb] = mma(x, p[j][nb], o[db][nb]);
             }
-        }
     }
 
     // The infinities and NaN of the tile's v, added to the columns that read their key.
-    static __device__ __forceinline__ void wild_products(const AttnOpArgs &a, const char *vd, int j0, int b, int kl,
-                                                      const int *lim, const int *doc, const int *at,
-                                                      const float *const *tab, f4v (*o)[NB]) {
-        const int lane = threadIdx.x & 63, q = lane >> 4, wave = threadIdx.x >> 6;
+    static __device__ __forceinline__ void wild_products(const Uniform &u, const lds_t *vd, int j0, const int *lim,
+                                                         const int *doc, const int *at, const int *tab, f4v (*o)[NB]) {
+        const int lane = threadIdx.x & 63, q = lane >> 4, wave = wave_of();
+#pragma unroll 1
         for (int jr = 0; jr < 16 * KB; ++jr) {
             const int j = j0 + jr;
-            if (j >= kl) break;
+            if (j >= u.kl) break;
             const int r = (WK ? 16 * wave : 0) + jr;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                bool ok = j < lim[nb] && (!a.k_docs || a.k_docs[b * a.k_docs_b + j] == doc[nb]);
-                if (ok && a.table)
-                    ok = entry(a, tab[nb], at[nb] - (a.k_pos ? a.k_pos[b * a.k_pos_b + j] : j)) != -INFINITY;
+                bool ok = j < lim[nb] && (!u.k_docs || u.k_docs[j] == doc[nb]);
+                if (GEN && ok && u.table) ok = entry(u, tab[nb], at[nb] - (u.k_pos ? u.k_pos[j] : j)) != -INFINITY;
                 if (!ok) continue;
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int c = 16 * db + 4 * q + i;
-                        const float v = (float)*(const T *)(vd + v_slot<CH, F32>(r, c / E) * 16 + (c % E) * sizeof(T));
+                        const float v = (float)lds_read<T>(vd, v_slot<CH, F32>(r, c / E) * 16 + (c % E) * (int)sizeof(T));
                         if (wild(v)) o[db][nb][i] += v;
+                        __builtin_amdgcn_sched_barrier(0);
                     }
             }
         }
     }
 };
 
-template <typename T, int DP, int NB, bool WK, bool ALIGNED>
+template <typename T, int DP, int NB, bool WK, bool ALIGNED, bool GEN>
 __global__ __launch_bounds__(256, 2) void k_attn(AttnOpArgs a, AttnLaunch L) {
+    static_assert(sizeof(AttnOpArgs) % 8 == 0 && alignof(AttnLaunch) == 8, "late_params reads the two as one struct");
     extern __shared__ __align__(16) char lds[];
-    Kernel<T, DP, NB, WK, ALIGNED>::run(a, L, lds);
+    Kernel<T, DP, NB, WK, ALIGNED, GEN>::run(a, L, lds);
 }
 
-// The key ranges' sums of one column: a wave per column, a lane per two channels.
+// The key ranges' sums of one column: a workgroup each, its threads over the ranges
+// for their weights and then over (channel, every 256 / DP-th range), so that the
+// reads of all ranges are in flight together.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void k_attn_join(AttnOpArgs a, AttnLaunch L) {
-    const int lane = threadIdx.x & 63;
-    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int c = (int)(id % L.cols);
-    const long long bh = id / L.cols;
-    const int b = (int)(bh / a.hk), kvh = (int)(bh - (long long)b * a.hk);
-    if (b >= a.batch) return;
+    constexpr int G = 256 / DP;
+    const int tid = threadIdx.x;
+    const int c = blockIdx.x % L.cols, bh = blockIdx.x / L.cols;
+    const int b = bh / a.hk, kvh = bh - b * a.hk;
     const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
     const int i = c / a.group;
     if (i >= ql) return;
-    const long long row0 = bh * L.splits * L.cols + c;
-    float top = -INFINITY;
-    for (int s = 0; s < L.splits; ++s) top = fmaxf(top, L.part_ml[2 * (row0 + (long long)s * L.cols)]);
-    if (top == -INFINITY) top = 0.f;
-    float ls = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int s = 0; s < L.splits; ++s) {
-        const long long row = row0 + (long long)s * L.cols;
-        const float ms = L.part_ml[2 * row], l = L.part_ml[2 * row + 1];
-        if (l == 0.f) continue;  // no key in this range
-        const float f = ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms - top);
-        ls = fmaf(f, l, ls);
-        const float *po = L.part_o + row * DP;
-        if (lane < DP) o0 = fmaf(f, po[lane], o0);
-        if (lane + 64 < DP) o1 = fmaf(f, po[lane + 64], o1);
+    const long long row0 = (long long)bh * L.splits * L.cols + c;
+    __shared__ float weight[256], part[256], stat[8];
+    float ms = -INFINITY, l = 0.f;
+    if (tid < L.splits) {
+        const long long row = row0 + (long long)tid * L.cols;
+        ms = L.part_ml[2 * row];
+        l = L.part_ml[2 * row + 1];
     }
-    const float r = ls == 0.f ? 0.f : 1.f / ls;
-    const int h = kvh * a.group + (c - i * a.group);
-    T *out = (T *)a.out + b * a.so.b + (long long)i * a.so.t + h * a.so.h;
-    if (lane < a.width) out[lane] = (T)(o0 * r);
-    if (lane + 64 < a.width) out[lane + 64] = (T)(o1 * r);
+    float top = half_max(ms);
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) top = fmaxf(top, __shfl_xor(top, m));
+    if ((tid & 63) == 0) stat[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
+    // a range without keys has weight zero; one whose sum is NaN passes it on
+    const float f = l == 0.f ? 0.f : (ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms - top));
+    weight[tid] = f;
+    float ls = l == 0.f ? 0.f : f * l;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) ls += __shfl_xor(ls, m);
+    if ((tid & 63) == 0) stat[4 + (tid >> 6)] = ls;
+    __syncthreads();
+    ls = (stat[4] + stat[5]) + (stat[6] + stat[7]);
+    const int d = tid % DP, g = tid / DP;
+    float o = 0.f;
+    if (g < G) {
+#pragma unroll 4
+        for (int s = g; s < L.splits; s += G) {
+            const float w = weight[s], x = L.part_o[(row0 + (long long)s * L.cols) * DP + d];
+            o += w == 0.f ? 0.f : w * x;
+        }
+        part[tid] = o;
+    }
+    __syncthreads();
+    if (tid < a.width) {
+        o = 0.f;
+#pragma unroll
+        for (int k = 0; k < G; ++k) o += part[k * DP + tid];
+        const int h = kvh * a.group + (c - i * a.group);
+        T *out = (T *)a.out + b * a.so.b + (long long)i * a.so.t + h * a.so.h;
+        out[tid] = (T)(ls == 0.f ? 0.f : o / ls);
+    }
 }
 
-// How a call is cut, from its type and sizes alone (the workspace goes by it).
+// How a call is cut.
 struct Cut {
     int dp, nb, tk;
     bool wk;
     int tiles, splits;
 };
 
-template <typename T, int DP, int NB, bool WK, bool ALIGNED>
+template <typename T, int DP, int NB, bool WK, bool ALIGNED, bool GEN>
 hipError_t launch(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
-    typedef Kernel<T, DP, NB, WK, ALIGNED> K;
+    typedef Kernel<T, DP, NB, WK, ALIGNED, GEN> K;
+    static_assert(K::kLds <= 163840, "LDS");
     const long long blocks = (long long)a.batch * a.hk * L.tiles * L.splits;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    if (K::kLds > 65536) {
-        static_assert(K::kLds <= 163840, "LDS");
-        const hipError_t e = hipFuncSetAttribute((const void *)k_attn<T, DP, NB, WK, ALIGNED>,
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)K::kLds);
-        if (e != hipSuccess) return e;
-    }
-    hipLaunchKernelGGL((k_attn<T, DP, NB, WK, ALIGNED>), dim3((unsigned)blocks), dim3(256), K::kLds, st, a, L);
+    hipLaunchKernelGGL((k_attn<T, DP, NB, WK, ALIGNED, GEN>), dim3((unsigned)blocks), dim3(256), K::kLds, st, a, L);
     return hipGetLastError();
 }
 
+// Unaligned arrays and general biases take the kernels of 16 columns a wave.
 template <typename T, int DP>
 hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, bool aligned, hipStream_t st) {
     hipError_t e;
-    if (c.wk) e = aligned ? launch<T, DP, 1, true, true>(a, L, st) : launch<T, DP, 1, true, false>(a, L, st);
-    else if (c.nb == 1) e = aligned ? launch<T, DP, 1, false, true>(a, L, st) : launch<T, DP, 1, false, false>(a, L, st);
-    else e = aligned ? launch<T, DP, 2, false, true>(a, L, st) : launch<T, DP, 2, false, false>(a, L, st);
+    const bool gen = L.score.general;
+    if (c.wk)
+        e = !aligned ? launch<T, DP, 1, true, false, true>(a, L, st)
+            : gen    ? launch<T, DP, 1, true, true, true>(a, L, st)
+                     : launch<T, DP, 1, true, true, false>(a, L, st);
+    else if (c.nb == 1)
+        e = !aligned ? launch<T, DP, 1, false, false, true>(a, L, st)
+            : gen    ? launch<T, DP, 1, false, true, true>(a, L, st)
+                     : launch<T, DP, 1, false, true, false>(a, L, st);
+    else
+        e = launch<T, DP, 2, false, true, false>(a, L, st);
     if (e != hipSuccess || L.splits == 1) return e;
     const long long rows = (long long)a.batch * a.hk * L.cols;
-    hipLaunchKernelGGL((k_attn_join<T, DP>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, L);
+    if (rows > 0x7fffffffLL) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_attn_join<T, DP>), dim3((unsigned)rows), dim3(256), 0, st, a, L);
     return hipGetLastError();
 }
 

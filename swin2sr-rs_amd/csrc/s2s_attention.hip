@@ -8,19 +8,19 @@ int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
 // Columns of at most 16 share one set of waves that split each key tile; more take
 // waves of 16 or 32 columns. Where that leaves CUs without work the keys are cut
-// into ranges whose sums a second kernel joins.
-attn::Cut cut_of(int dtype, const AttnOpArgs &a) {
+// into ranges whose sums a second kernel joins. `narrow`: waves of 16 only.
+attn::Cut cut_of(int dtype, const AttnOpArgs &a, bool narrow) {
     attn::Cut c;
     const long long cols = (long long)a.group * a.nq, pairs = (long long)a.batch * a.hk;
     const int cus = cu_count();
     c.dp = round_up(std::max(a.width, 1), 32);
     c.wk = cols <= 16;
-    c.nb = c.wk || cols <= 64 || (cols + 127) / 128 * pairs < 2 * cus ? 1 : 2;
+    c.nb = narrow || c.wk || cols <= 64 || (cols + 127) / 128 * pairs < 2 * cus ? 1 : 2;
     c.tk = dtype == 0 && !c.wk ? 32 : 64;
     const int per = c.wk ? 16 : 64 * c.nb;
     c.tiles = (int)((cols + per - 1) / per);
-    // ranges of 4 tiles at least, workgroups for two per CU at most
-    const long long blocks = std::max(1LL, pairs * c.tiles), want = 2LL * cus;
+    // ranges of 4 tiles at least, workgroups for two per CU (four of the narrow ones) at most
+    const long long blocks = std::max(1LL, pairs * c.tiles), want = (c.wk && c.dp <= 64 ? 4LL : 2LL) * cus;
     const long long nt = ((long long)a.nk + c.tk - 1) / c.tk;
     c.splits = (int)std::max(1LL, std::min({want / blocks, nt / 4, 256LL}));
     return c;
@@ -63,23 +63,35 @@ int aligned_bytes(const void *p, const Strides &s, int width, int size) {
 
 }  // namespace
 
+// The most that either cut of these sizes needs: which one runs goes by strides and
+// biases too.
 size_t attn_op_workspace(int dtype, const AttnOpArgs &a) {
-    const attn::Cut c = cut_of(dtype, a);
-    size_t n = round16((size_t)a.batch * meta_tiles(c, a) * sizeof(int4));
-    if (c.splits > 1) {
-        const size_t rows = (size_t)a.batch * a.hk * c.splits * a.group * a.nq;
-        n += rows * c.dp * 4 + rows * 8;
+    size_t most = 0;
+    for (const bool narrow : {false, true}) {
+        const attn::Cut c = cut_of(dtype, a, narrow);
+        size_t n = round16((size_t)a.batch * meta_tiles(c, a) * sizeof(int4));
+        if (c.splits > 1) {
+            const size_t rows = (size_t)a.batch * a.hk * c.splits * a.group * a.nq;
+            n += rows * c.dp * 4 + rows * 8;
+        }
+        most = std::max(most, n);
     }
-    return n;
+    return most;
 }
 
 hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStream_t st) {
-    const attn::Cut c = cut_of(dtype, a);
+    const int size = dtype == 0 ? 4 : 2;
     AttnLaunch L{};
+    L.score.set(a);
+    int al = aligned_bytes(a.q, a.sq, a.width, size);
+    if (a.nk > 0) al = std::min(al, std::min(aligned_bytes(a.k, a.sk, a.width, size), aligned_bytes(a.v, a.sv, a.width, size)));
+    L.vec = std::min(al, 8);
+    L.out_vec = aligned_bytes(a.out, a.so, a.width, size) >= 4 * size;
+    const bool aligned = al >= 16 && (a.nk <= 1 || (a.sk.t >= a.width && a.sv.t >= a.width));
+    const attn::Cut c = cut_of(dtype, a, !aligned || L.score.general);
     L.cols = a.group * a.nq;
     L.tiles = c.tiles;
     L.splits = c.splits;
-    const int size = dtype == 0 ? 4 : 2;
     char *w = (char *)ws;
     const int mt = meta_tiles(c, a);
     const size_t meta_bytes = round16((size_t)a.batch * mt * sizeof(int4));
@@ -97,11 +109,6 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    int al = aligned_bytes(a.q, a.sq, a.width, size);
-    if (a.nk > 0) al = std::min(al, std::min(aligned_bytes(a.k, a.sk, a.width, size), aligned_bytes(a.v, a.sv, a.width, size)));
-    L.vec = std::min(al, 8);
-    L.out_vec = aligned_bytes(a.out, a.so, a.width, size) >= 4 * size;
-    const bool aligned = al >= 16;
     switch (dtype) {
         case 0: return launch_attention_f32(a, L, c, aligned, st);
         case 1: return launch_attention_f16(a, L, c, aligned, st);

@@ -180,6 +180,7 @@ int s2s_attention(const s2s_attention_args *a, void *workspace, uint64_t workspa
     if (a->q_pos && !a->slopes && !a->table) return refuse("%s: positions without slopes or table", op);
     if (a->table && (a->table_size < 1 || a->table_size % 2 == 0 || a->table_size > (1 << 24)))
         return refuse("%s: a table of %d entries: an odd number up to 2^24 is wanted", op, a->table_size);
+    if (a->table && (long long)a->q_heads * a->table_size > (1 << 30)) return refuse("%s: a table over 2^30 entries", op);
     if (a->q_docs_batch < 0 || a->k_docs_batch < 0 || a->q_pos_batch < 0 || a->k_pos_batch < 0 ||
         a->q_docs_batch > kMaxStride || a->k_docs_batch > kMaxStride || a->q_pos_batch > kMaxStride ||
         a->k_pos_batch > kMaxStride)
