@@ -80,6 +80,8 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = kAttnLog2e;
 
+enum { CAP = 1, SLOPES = 2, ANY = 4, GENERAL = 8 };
+
 template <typename T>
 struct Type;
 // V: 16 bytes of elements. kShift: weights are 2^kShift times e^(s - max), so that f16's
@@ -135,9 +137,26 @@ __device__ __forceinline__ int v_slot(int r, int c) {
 }
 
 // A resource of less than 2^31 bytes (64 rows of 2^22 elements are 2^30 at most).
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void *p, int bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, bytes, 0x00020000);
+__device__ __forceinline__ v4u tile_rsrc(const void *p, int bytes) {
+    const unsigned long long x = (unsigned long long)p;
+    return v4u{(unsigned)x, (unsigned)(x >> 32) & 0xffffu, (unsigned)bytes, 0x00020000u};
 }
+// The direct copy of dma16 (16 bytes a lane to LDS address `to` + 16 * lane) as an
+// instruction the compiler does not see through: it takes the transposing LDS
+// read for a reader of whatever copy is in flight and waits for all of them in front
+// of it, which leaves no copy in flight during the products. The kernel waits by
+// itself, before the barrier that opens the tile. There is no result register; the
+// wait states are those of a resource in scalar registers that a VALU instruction
+// wrote.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is reserved, and named as what it changes)
+__device__ __forceinline__ void tile_dma(v4u rsrc, unsigned to, int off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(to), "v"(off), "s"(rsrc)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
 
 // LDS by byte address: a lane's address once per tile, what is constant in the
 // instruction's offset.
@@ -182,16 +201,10 @@ __device__ __forceinline__ const __attribute__((address_space(4))) AttnParams *l
     return p;
 }
 
-// max of three as one instruction (fmaxf quiets each operand first); a NaN is dropped
+// The IEEE 754-2019 maximum (v_maximum3_f32), which passes a NaN on; fmaxf would quiet
+// each operand first. A column with a NaN among its scores is NaN whatever its reference.
 __device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
-}
-__device__ __forceinline__ float max3_abs(float a, float b, float c) {
-    float d;
-    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 __device__ __forceinline__ float col_sum(float x) {
     float y = x;
@@ -263,13 +276,15 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 //  WK false: wave w has columns 16 NB w .. + 16 NB of the tile's 64 NB, all keys.
 //  WK true (at most 16 columns): every wave has all columns and a quarter of each
 //  key tile (one block of 16 keys of 64); the four sums meet in LDS at the end.
-//  GEN: with what AttnScore::general asks for. Apart, since the registers of those
-//  paths would be spilled around the others' loop.
+//  MODE: CAP and SLOPES are known (0 to 3), or asked for in every tile (ANY), or these and
+//  what AttnScore::general stands for (GENERAL). Paths that a kernel might take and
+//  does not cost it registers, spilled around its loop, and copies where they meet.
 // K and V tiles of TK keys are copied straight into LDS, two buffers each, the
 // next tile in flight while one is computed. ALIGNED: rows of 16-byte multiples,
 // copied by the DMA; otherwise through registers in narrower accesses.
-template <typename T, int DP, int NB, bool WK, bool ALIGNED, bool GEN>
+template <typename T, int DP, int NB, bool WK, bool ALIGNED, int MODE>
 struct Kernel {
+    static constexpr bool GEN = MODE == GENERAL;
     typedef Type<T> Ty;
     typedef typename Ty::V Vec;
     static constexpr bool F32 = sizeof(T) == 4;
@@ -284,7 +299,7 @@ struct Kernel {
     static constexpr int LOADS = TK * CH / 256;          // chunks per thread and tile
     static constexpr size_t kTile = (size_t)TK * CH * 16;
     static constexpr size_t kJoin = WK ? (size_t)4 * 16 * (DP + 4) * 4 : 0;
-    static constexpr size_t kLds = 4 * kTile > kJoin ? 4 * kTile : kJoin;
+    static constexpr size_t kLds = (4 * kTile > kJoin ? 4 * kTile : kJoin) + 16;  // (and four flags)
 
     // What a tile needs that is the same for all of the workgroup.
     struct Uniform {
@@ -347,7 +362,7 @@ struct Kernel {
         }
         // keys that any column of the workgroup (of the wave) may read, and that all may
         const int i_last = min(ql - 1, (c0 + COLS - 1) / a.group);
-        const int wg_max = limit(i_last);
+        const int wg_max = limit(i_last), wg_min = limit(c0 / a.group);
         const int w_first = min(ql - 1, wc0 / a.group), w_last = min(ql - 1, (wc0 + 16 * NB - 1) / a.group);
         const bool w_any = wc0 < ql * a.group;
         const int w_max = w_any ? limit(w_last) : 0, w_min = limit(w_first);
@@ -418,12 +433,12 @@ struct Kernel {
             koff[p] = kc < a.width ? (r * kst + kc) * (int)sizeof(T) : 0x60000000;
             voff[p] = vc < a.width ? (r * vst + vc) * (int)sizeof(T) : 0x60000000;
         }
+        const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(const lds_t *)lds);
         auto stage = [&](int t, int buf) {
-            char *kd = lds + buf * 2 * kTile, *vd = kd + kTile;
             const int left = min(kl - t * TK, TK);
             if constexpr (ALIGNED) {
-                const __amdgpu_buffer_rsrc_t kr = tile_rsrc(kp, left * kst * (int)sizeof(T)),
-                                             vr = tile_rsrc(vp, left * vst * (int)sizeof(T));
+                const v4u kr = tile_rsrc(kp, left * kst * (int)sizeof(T)), vr = tile_rsrc(vp, left * vst * (int)sizeof(T));
+                const unsigned to = lds0 + buf * 2 * (unsigned)kTile + wave * 1024;
                 int ko[PER], vo[PER];
 #pragma unroll
                 for (int p = 0; p < PER; ++p) {
@@ -432,8 +447,8 @@ struct Kernel {
                 }
 #pragma unroll
                 for (int n = 0; n < LOADS; ++n) {
-                    dma16(kr, (float *)(kd + (size_t)(n * 4 + wave) * 1024), ko[n % PER] + n / PER * (PER * STEP) * kst * (int)sizeof(T));
-                    dma16(vr, (float *)(vd + (size_t)(n * 4 + wave) * 1024), vo[n % PER] + n / PER * (PER * STEP) * vst * (int)sizeof(T));
+                    tile_dma(kr, to + n * 4096, ko[n % PER] + n / PER * (PER * STEP) * kst * (int)sizeof(T));
+                    tile_dma(vr, to + (unsigned)kTile + n * 4096, vo[n % PER] + n / PER * (PER * STEP) * vst * (int)sizeof(T));
                 }
             } else {
                 v4u x[2][LOADS];
@@ -446,6 +461,7 @@ struct Kernel {
                         x[1][n] = load_chunk<T>(vp + (long long)r * vst, c * E, a.width, L.vec);
                     }
                 }
+                char *kd = lds + buf * 2 * kTile, *vd = kd + kTile;
 #pragma unroll
                 for (int n = 0; n < LOADS; ++n) {
                     const int s = n * 256 + tid, r = s / CH, c = s & (CH - 1);
@@ -494,11 +510,27 @@ struct Kernel {
             lds_sync();
             kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
             if (tn < t_end) stage(tn, buf ^ 1);
+            const int at_buf = buf * 2 * (int)kTile;
+            if (!(t * TK + TK <= wg_min && one_doc) || (GEN && u.table)) {
+                // a masked key's weight is zero, and zero times an infinity is none: with
+                // such values in the V of a tile that not every column reads whole, they are
+                // added by themselves to the columns that do read them, and taken out
+                lds_t *vd = (lds_t *)lds + at_buf + kTile;
+                auto *flag = (__attribute__((address_space(3))) int *)((lds_t *)lds + 4 * kTile);
+                const bool w = __any(any_wild_chunk(vd));
+                if (lane == 0) flag[wave] = w;
+                lds_sync();
+                if (__builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3])) {
+                    wild_products(u, vd, t * TK + (WK ? 16 * wave : 0), lim, doc, at, tab, o);
+                    lds_sync();
+                    remove_wild(vd);
+                    lds_sync();
+                }
+            }
             const int j0 = t * TK + (WK ? 16 * wave : 0);  // the wave's first key
             if (j0 < w_max) {
-                const int at_buf = buf * 2 * (int)kTile;
                 const bool full = j0 + 16 * KB <= w_min && one_doc && !(GEN && u.table);
-                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), base + at_buf + kTile, j0, full, lim, doc, at, slope, tab, qf, o, m, l);
+                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, lim, doc, at, slope, tab, qf, o, m, l);
             }
             t = tn;
             buf ^= 1;
@@ -604,8 +636,8 @@ struct Kernel {
     static __device__ __forceinline__ const lds_t *v_block(const lds_t *vl, int db) { return lds_xor(vl, db << (F32 ? 6 : 5)); }
 
     // The wave's keys of one tile: scores, softmax step, products with V.
-    static __device__ __forceinline__ void tile(const Uniform &u, const lds_t *kl0, const lds_t *vl0, const lds_t *vd,
-                                                int j0, bool full, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
+    static __device__ __forceinline__ void tile(const Uniform &u, const lds_t *kl0, const lds_t *vl0, int j0,
+                                                bool full, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
                                                 const Vec (*qf)[KS], f4v (*o)[NB], float *m, float *l) {
         const int lane = threadIdx.x & 63, q = lane >> 4;
         f4v s[KB][NB];
@@ -628,13 +660,16 @@ struct Kernel {
         // bias made it powers of two already
         const AttnScore &sc = u.sc;
         float unit = sc.c1;
-        if (u.capped) {
+        if (MODE < ANY ? (MODE & CAP) != 0 : u.capped) {
             float big = 0.f;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) big = max3_abs(max3_abs(big, s[kb][nb][0], s[kb][nb][1]), s[kb][nb][2], s[kb][nb][3]);
-            if (__any(big > sc.poly_max)) {
+                for (int nb = 0; nb < NB; ++nb) {
+                    big = max3(big, fabsf(s[kb][nb][0]), fabsf(s[kb][nb][1]));
+                    big = max3(big, fabsf(s[kb][nb][2]), fabsf(s[kb][nb][3]));
+                }
+            if (__any(!(big <= sc.poly_max))) {
                 // cap tanh(z) = cap (1 - 2 / (e^2z + 1))
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
@@ -678,7 +713,7 @@ struct Kernel {
                     }
                 }
             unit = 1.f;
-        } else if (u.slopes) {
+        } else if (MODE < ANY ? (MODE & SLOPES) != 0 : u.slopes) {
             // distances of neighbours differ by what the register says
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -721,9 +756,7 @@ struct Kernel {
         for (int nb = 0; nb < NB; ++nb) {
             float x = s[0][nb][0];
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-                x = kb ? max3(max3(x, s[kb][nb][0], s[kb][nb][1]), s[kb][nb][2], s[kb][nb][3])
-                       : max3(max3(x, s[kb][nb][1], s[kb][nb][2]), s[kb][nb][3], s[kb][nb][3]);
+            for (int kb = 0; kb < KB; ++kb) x = max3(max3(x, s[kb][nb][0], s[kb][nb][1]), s[kb][nb][2], s[kb][nb][3]);
             top[nb] = col_max(x) * unit;
             grow |= top[nb] > m[nb] + Ty::kLazy;
         }
@@ -731,7 +764,8 @@ struct Kernel {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const float mn = fmaxf(m[nb], top[nb]);
-                const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nb] - mn);
+                // (no reference yet: sums of zero, or infinities of v that stay)
+                const float f = m[nb] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nb] - mn);
                 m[nb] = mn;
                 l[nb] *= f;
 #pragma unroll
@@ -752,23 +786,7 @@ struct Kernel {
                 }
             l[nb] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
-        // a masked key's weight is zero, and zero times an infinity is none: with such
-        // values among a masked tile's v they are added key by key
-        if (!full) {
-            bool w = false;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) {
-#pragma unroll
-                for (int j = 0; j < (F32 || WK ? KB : KB / 2); ++j) w |= any_wild(v_operand(v_block(vl0, db), j));
-                __builtin_amdgcn_sched_barrier(0);  // (few operands at a time)
-            }
-            if (__any(w)) {
-                products<true>(vl0, s, o);
-                wild_products(u, vd, j0, lim, doc, at, tab, o);
-                return;
-            }
-        }
-        products<false>(vl0, s, o);
+        products(vl0, s, o);
     }
 
     static __device__ __forceinline__ float entry(const Uniform &u, int tab, int dist) {
@@ -779,8 +797,7 @@ struct Kernel {
         return bias == -INFINITY ? -INFINITY : fmaxf(bias, -2e38f) * kLog2e + x;
     }
 
-    // O^T += V^T P^T; CLEAN: without V's infinities and NaN
-    template <bool CLEAN>
+    // O^T += V^T P^T
     static __device__ __forceinline__ void products(const lds_t *vl0, const f4v (*s)[NB], f4v (*o)[NB]) {
         constexpr int J = F32 || WK ? KB : KB / 2;
         Vec p[J][NB];
@@ -801,15 +818,25 @@ struct Kernel {
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                Vec x = v_operand(v_block(vl0, db), j);
-                if constexpr (CLEAN) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (wild((float)x[e])) x[e] = (T)0.f;
-                }
+                const Vec x = v_operand(v_block(vl0, db), j);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) o[db][nb] = mma(x, p[j][nb], o[db][nb]);
             }
+    }
+
+    // Whether this thread's share of the tile's V (as it lies in LDS) holds an infinity or
+    // NaN, and their removal.
+    static __device__ __forceinline__ bool any_wild_chunk(const lds_t *vd) {
+        bool w = false;
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) w |= any_wild(lds_read<Vec>(vd, (n * 256 + (int)threadIdx.x) * 16));
+        return w;
+    }
+    static __device__ __forceinline__ void remove_wild(lds_t *vd) {
+        for (int n = 0; n < LOADS * E; ++n) {
+            auto *p = (__attribute__((address_space(3))) T *)(vd + (n * 256 + (int)threadIdx.x) * (int)sizeof(T));
+            if (wild((float)*p)) *p = (T)0.f;
+        }
     }
 
     // The infinities and NaN of the tile's v, added to the columns that read their key.
@@ -840,11 +867,11 @@ struct Kernel {
     }
 };
 
-template <typename T, int DP, int NB, bool WK, bool ALIGNED, bool GEN>
+template <typename T, int DP, int NB, bool WK, bool ALIGNED, int MODE>
 __global__ __launch_bounds__(256, 2) void k_attn(AttnOpArgs a, AttnLaunch L) {
     static_assert(sizeof(AttnOpArgs) % 8 == 0 && alignof(AttnLaunch) == 8, "late_params reads the two as one struct");
     extern __shared__ __align__(16) char lds[];
-    Kernel<T, DP, NB, WK, ALIGNED, GEN>::run(a, L, lds);
+    Kernel<T, DP, NB, WK, ALIGNED, MODE>::run(a, L, lds);
 }
 
 // The key ranges' sums of one column: a workgroup each, its threads over the ranges
@@ -910,13 +937,13 @@ struct Cut {
     int tiles, splits;
 };
 
-template <typename T, int DP, int NB, bool WK, bool ALIGNED, bool GEN>
+template <typename T, int DP, int NB, bool WK, bool ALIGNED, int MODE>
 hipError_t launch(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
-    typedef Kernel<T, DP, NB, WK, ALIGNED, GEN> K;
+    typedef Kernel<T, DP, NB, WK, ALIGNED, MODE> K;
     static_assert(K::kLds <= 163840, "LDS");
     const long long blocks = (long long)a.batch * a.hk * L.tiles * L.splits;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_attn<T, DP, NB, WK, ALIGNED, GEN>), dim3((unsigned)blocks), dim3(256), K::kLds, st, a, L);
+    hipLaunchKernelGGL((k_attn<T, DP, NB, WK, ALIGNED, MODE>), dim3((unsigned)blocks), dim3(256), K::kLds, st, a, L);
     return hipGetLastError();
 }
 
@@ -926,15 +953,17 @@ hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, 
     hipError_t e;
     const bool gen = L.score.general;
     if (c.wk)
-        e = !aligned ? launch<T, DP, 1, true, false, true>(a, L, st)
-            : gen    ? launch<T, DP, 1, true, true, true>(a, L, st)
-                     : launch<T, DP, 1, true, true, false>(a, L, st);
+        e = !aligned ? launch<T, DP, 1, true, false, GENERAL>(a, L, st)
+            : gen    ? launch<T, DP, 1, true, true, GENERAL>(a, L, st)
+                     : launch<T, DP, 1, true, true, ANY>(a, L, st);
     else if (c.nb == 1)
-        e = !aligned ? launch<T, DP, 1, false, false, true>(a, L, st)
-            : gen    ? launch<T, DP, 1, false, true, true>(a, L, st)
-                     : launch<T, DP, 1, false, true, false>(a, L, st);
+        e = !aligned ? launch<T, DP, 1, false, false, GENERAL>(a, L, st)
+            : gen    ? launch<T, DP, 1, false, true, GENERAL>(a, L, st)
+                     : launch<T, DP, 1, false, true, ANY>(a, L, st);
+    else if (a.cap > 0.f)
+        e = a.slopes ? launch<T, DP, 2, false, true, CAP | SLOPES>(a, L, st) : launch<T, DP, 2, false, true, CAP>(a, L, st);
     else
-        e = launch<T, DP, 2, false, true, false>(a, L, st);
+        e = a.slopes ? launch<T, DP, 2, false, true, SLOPES>(a, L, st) : launch<T, DP, 2, false, true, 0>(a, L, st);
     if (e != hipSuccess || L.splits == 1) return e;
     const long long rows = (long long)a.batch * a.hk * L.cols;
     if (rows > 0x7fffffffLL) return hipErrorInvalidValue;

@@ -135,6 +135,7 @@ CASES = {
     "step": case("bf16", B=4, Lq=1, Lk=900, H=8, KV=2, D=128, order="cache", causal=True, cap=50.0, k_lens=[900, 1, 333, 0]),
     "step_f16_slopes": case("f16", B=1, Lq=1, Lk=5003, H=16, KV=2, order="cache", causal=True, slopes=True),
     "step_f32": case("f32", B=2, Lq=1, Lk=1500, H=4, KV=4, D=64, order="cache", causal=True, table=63),
+    "step_f32_128": case("f32", B=2, Lq=1, Lk=700, H=4, KV=2, D=128, order="cache", causal=True),
     "step_4": case("bf16", B=2, Lq=4, Lk=2100, H=8, KV=2, D=128, order="cache", causal=True, prefix=[0, 2099]),
     "step_documents": case("f16", B=2, Lq=2, Lk=1100, H=4, KV=2, D=96, order="cache", docs=scattered),
     "group_33": case("f16", B=1, Lq=2, Lk=700, H=33, KV=1, D=32),
