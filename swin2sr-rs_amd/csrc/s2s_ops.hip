@@ -39,69 +39,71 @@ __device__ __forceinline__ void sincos_turns(unsigned long long f, float &s, flo
     c = ((q + 1) & 2) ? -cc : cc;
 }
 
-// One thread: V pairs of one token (their angles once) in the heads h0, h0 + hs,
-// ... of q and of k, or V of the channels that are copied. Neighbouring threads
-// take neighbouring pairs of a token, then the next token, so that a wave reads
-// whole rows; heads are split over gridDim.y until the launch fills the chip.
+// A workgroup takes `tb` tokens of q and k. Their sines and cosines are made once, in
+// LDS; then the threads walk the tokens' heads in memory order, a unit of V pairs (or of
+// V channels that are copied) at a time, neighbours next to each other across heads, so
+// that a wave's accesses are whole runs whatever the width. (A thread that kept its
+// angles in registers and looped over heads touched a run per head: 45 us for 2 x
+// 23400 tokens of 6 + 6 f32 heads of 30, of which every run is 120 bytes.)
 template <typename T, bool ADJ, int V, bool ALIGNED = true>
-__global__ __launch_bounds__(256) void k_rotary(RotaryArgs a, int per_token) {
+__global__ __launch_bounds__(256) void k_rotary(RotaryArgs a, int tb, int per_head) {
     typedef VecOf<T, ADJ ? 2 * V : V, ALIGNED ? (ADJ ? 2 * V : V) : 1> Vec;
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long tok = id / per_token;
-    const int g = (int)(id - tok * per_token);
-    if (tok >= (long long)a.batch * a.tokens) return;
-    const int b = (int)(tok / a.tokens), t = (int)(tok - (long long)b * a.tokens);
-    if (a.lens && t >= a.lens[b]) return;
-    const T *q = (const T *)a.q + b * a.sq.b + t * a.sq.t;
-    T *qo = (T *)a.qo + b * a.sqo.b + t * a.sqo.t;
-    const T *k = (const T *)a.k + b * a.sk.b + t * a.sk.t;
-    T *ko = (T *)a.ko + b * a.sko.b + t * a.sko.t;
-    const int heads = a.hq + a.hk, rot = a.pairs / V;
-    if (g < rot) {
-        float sn[V], cs[V];
-        const int *pos = a.pos + b * a.pos_b + (long long)t * a.axes;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int p = g * V + i;
-            sincos_turns((unsigned long long)(long long)pos[a.axis[p]] * a.freq[p], sn[i], cs[i]);
-        }
-        const int c0 = ADJ ? g * 2 * V : g * V, c1 = ADJ ? c0 + 1 : c0 + a.pairs;
-#pragma unroll 4
-        for (int h = blockIdx.y; h < heads; h += gridDim.y) {
+    typedef VecOf<T, V, ALIGNED ? V : 1> Part;
+    extern __shared__ float2 turn[];  // [tb][pairs]
+    const int tid = threadIdx.x, heads = a.hq + a.hk, rot = a.pairs / V;
+    const long long tok0 = (long long)blockIdx.x * tb, all = (long long)a.batch * a.tokens;
+    const int n_tok = (int)min((long long)tb, all - tok0);
+    for (int i = tid; i < n_tok * a.pairs; i += 256) {
+        const int t = i / a.pairs, p = i - t * a.pairs;
+        const long long b = (tok0 + t) / a.tokens, at = (tok0 + t) - b * a.tokens;
+        const int pos = a.pos[b * a.pos_b + at * a.axes + a.axis[p]];
+        float2 x;
+        sincos_turns((unsigned long long)(long long)pos * a.freq[p], x.y, x.x);
+        turn[i] = x;
+    }
+    __syncthreads();
+    // unit (token t, head h, g) of this thread, and the step of 256 units
+    const int dg = 256 % per_head, dh = 256 / per_head;
+    int g = tid % per_head, h = tid / per_head, t = 0;
+    while (h >= heads) h -= heads, ++t;
+    while (t < n_tok) {
+        const int b = (int)((tok0 + t) / a.tokens), at = (int)((tok0 + t) - (long long)b * a.tokens);
+        if (!a.lens || at < a.lens[b]) {
             const bool isq = h < a.hq;
-            const T *src = isq ? q + h * a.sq.h : k + (h - a.hq) * a.sk.h;
-            T *dst = isq ? qo + h * a.sqo.h : ko + (h - a.hq) * a.sko.h;
-            Vec x = *(const Vec *)(src + c0);
-            if (ADJ) {
-                Vec o;
+            const T *src = isq ? (const T *)a.q + b * a.sq.b + at * a.sq.t + h * a.sq.h
+                               : (const T *)a.k + b * a.sk.b + at * a.sk.t + (h - a.hq) * a.sk.h;
+            T *dst = isq ? (T *)a.qo + b * a.sqo.b + at * a.sqo.t + h * a.sqo.h
+                         : (T *)a.ko + b * a.sko.b + at * a.sko.t + (h - a.hq) * a.sko.h;
+            if (g < rot) {
+                const float2 *cs = turn + t * a.pairs + g * V;
+                const int c0 = ADJ ? g * 2 * V : g * V, c1 = ADJ ? c0 : c0 + a.pairs;
+                Vec x = *(const Vec *)(src + c0), o;
+                if (ADJ) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float u = (float)x.e[2 * i], w = (float)x.e[2 * i + 1];
-                    o.e[2 * i] = (T)fmaf(u, cs[i], -w * sn[i]);
-                    o.e[2 * i + 1] = (T)fmaf(u, sn[i], w * cs[i]);
+                    for (int i = 0; i < V; ++i) {
+                        const float u = (float)x.e[2 * i], w = (float)x.e[2 * i + 1];
+                        o.e[2 * i] = (T)fmaf(u, cs[i].x, -w * cs[i].y);
+                        o.e[2 * i + 1] = (T)fmaf(u, cs[i].y, w * cs[i].x);
+                    }
+                } else {
+                    Vec y = *(const Vec *)(src + c1), r;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float u = (float)x.e[i], w = (float)y.e[i];
+                        o.e[i] = (T)fmaf(u, cs[i].x, -w * cs[i].y);
+                        r.e[i] = (T)fmaf(u, cs[i].y, w * cs[i].x);
+                    }
+                    *(Vec *)(dst + c1) = r;
                 }
                 *(Vec *)(dst + c0) = o;
             } else {
-                Vec y = *(const Vec *)(src + c1), o, r;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float u = (float)x.e[i], w = (float)y.e[i];
-                    o.e[i] = (T)fmaf(u, cs[i], -w * sn[i]);
-                    r.e[i] = (T)fmaf(u, sn[i], w * cs[i]);
-                }
-                *(Vec *)(dst + c0) = o;
-                *(Vec *)(dst + c1) = r;
+                const int c = 2 * a.pairs + (g - rot) * V;
+                *(Part *)(dst + c) = *(const Part *)(src + c);
             }
         }
-    } else {
-        typedef VecOf<T, V> Part;
-        const int c = 2 * a.pairs + (g - rot) * V;
-        for (int h = blockIdx.y; h < heads; h += gridDim.y) {
-            const bool isq = h < a.hq;
-            const T *src = isq ? q + h * a.sq.h : k + (h - a.hq) * a.sk.h;
-            T *dst = isq ? qo + h * a.sqo.h : ko + (h - a.hq) * a.sko.h;
-            *(Part *)(dst + c) = *(const Part *)(src + c);
-        }
+        g += dg, h += dh;
+        if (g >= per_head) g -= per_head, ++h;
+        while (h >= heads) h -= heads, ++t;
     }
 }
 
@@ -123,34 +125,36 @@ hipError_t rotary_of(const RotaryArgs &a, hipStream_t st) {
     int v = ADJ ? w / 2 : w;
     while (v > 1 && (a.pairs % v || (a.width - 2 * a.pairs) % v)) v /= 2;
     v = std::max(v, 1);
-    const int per_token = (a.pairs + a.width - 2 * a.pairs) / v;
-    const long long items = (long long)a.batch * a.tokens * per_token, blocks = (items + 255) / 256;
+    const int per_head = (a.pairs + a.width - 2 * a.pairs) / v;
+    // tokens per workgroup: 8 units a thread, fewer where that leaves CUs without work
+    const long long units = (long long)(a.hq + a.hk) * per_head, all = (long long)a.batch * a.tokens;
+    const long long fill = std::max(1LL, all / (4LL * cu_count()));
+    const int tb = (int)std::max(1LL, std::min({(2048 + units - 1) / units, fill, 16LL}));
+    const long long blocks = (all + tb - 1) / tb;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    // threads enough for 8 waves on every SIMD, before heads are looped over
-    const long long want = (long long)cu_count() * 2048;
-    const int hs = (int)std::max(1LL, std::min((long long)(a.hq + a.hk), want / std::max(1LL, blocks * 256)));
-    const dim3 grid((unsigned)blocks, (unsigned)hs);
+    const dim3 grid((unsigned)blocks);
+    const size_t lds = (size_t)tb * a.pairs * sizeof(float2);
     switch (v) {
         case 8:
             if constexpr (!ADJ && sizeof(T) == 2) {
-                hipLaunchKernelGGL((k_rotary<T, ADJ, 8>), grid, dim3(256), 0, st, a, per_token);
+                hipLaunchKernelGGL((k_rotary<T, ADJ, 8>), grid, dim3(256), lds, st, a, tb, per_head);
                 break;
             }
             return hipErrorInvalidValue;
         case 4:
             if constexpr (!(ADJ && sizeof(T) == 4)) {
-                hipLaunchKernelGGL((k_rotary<T, ADJ, 4>), grid, dim3(256), 0, st, a, per_token);
+                hipLaunchKernelGGL((k_rotary<T, ADJ, 4>), grid, dim3(256), lds, st, a, tb, per_head);
                 break;
             }
             return hipErrorInvalidValue;
         case 2:
-            hipLaunchKernelGGL((k_rotary<T, ADJ, 2>), grid, dim3(256), 0, st, a, per_token);
+            hipLaunchKernelGGL((k_rotary<T, ADJ, 2>), grid, dim3(256), lds, st, a, tb, per_head);
             break;
         default:
             if (ADJ && w < 2)
-                hipLaunchKernelGGL((k_rotary<T, ADJ, 1, false>), grid, dim3(256), 0, st, a, per_token);
+                hipLaunchKernelGGL((k_rotary<T, ADJ, 1, false>), grid, dim3(256), lds, st, a, tb, per_head);
             else
-                hipLaunchKernelGGL((k_rotary<T, ADJ, 1>), grid, dim3(256), 0, st, a, per_token);
+                hipLaunchKernelGGL((k_rotary<T, ADJ, 1>), grid, dim3(256), lds, st, a, tb, per_head);
     }
     return hipGetLastError();
 }
@@ -173,6 +177,14 @@ __device__ __forceinline__ float wave_sum(float v) {
 __device__ __forceinline__ unsigned char to_e4m3(float v) {
     v = v > 448.f ? 448.f : (v < -448.f ? -448.f : v);
     return (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xff);
+}
+
+// Four codes in a word.
+__device__ __forceinline__ unsigned to_e4m3x4(float a, float b, float c, float d) {
+    auto clip = [](float v) { return v > 448.f ? 448.f : (v < -448.f ? -448.f : v); };
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(clip(a), clip(b), 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(clip(c), clip(d), w, true);
+    return (unsigned)w;
 }
 
 // The largest magnitude of a row or group; NaN where one is among them (a
@@ -253,14 +265,172 @@ __global__ __launch_bounds__(256) void k_rms_norm_rows(RmsNormArgs a) {
     }
 }
 
-template <typename T>
-hipError_t rms_type(bool e4m3, const RmsNormArgs &a, hipStream_t st) {
-    const dim3 grid((unsigned)a.rows);
-    if (e4m3)
-        hipLaunchKernelGGL((k_rms_norm_rows<T, true>), grid, dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((k_rms_norm_rows<T, false>), grid, dim3(256), 0, st, a);
+// The rows of a workgroup in registers: TPR threads a row (256 / TPR rows at once), NC
+// chunks of V elements (16 bytes) a thread, so that x and the residual are read once and
+// nothing is read again; the weights stay in registers over the rows that the workgroup
+// walks. A group of the scales is a power of two of chunks, which neighbouring lanes hold.
+template <typename T, bool E4M3, int TPR, int NC>
+__global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
+    constexpr int V = 16 / sizeof(T);
+    typedef VecOf<T, V> Vec;
+    const int tid = threadIdx.x, lane = tid & 63, r0 = tid / TPR, tr = tid % TPR;
+    const int chunks = a.cols / V;
+    __shared__ float part[2][4];
+    float wt[NC][V];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        const int c = (n * TPR + tr) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) wt[n][e] = 0.f;
+        if (c < a.cols) {
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const float4 w = *(const float4 *)(a.weight + c + e);
+                wt[n][e] = w.x + a.offset, wt[n][e + 1] = w.y + a.offset;
+                wt[n][e + 2] = w.z + a.offset, wt[n][e + 3] = w.w + a.offset;
+            }
+        }
+    }
+    for (long long row = (long long)blockIdx.x * (256 / TPR) + r0;; row += (long long)gridDim.x * (256 / TPR)) {
+        // (uniform in a wave, and in the workgroup where rows share it)
+        if (row >= a.rows) break;
+        const T *x = (const T *)a.x + row * a.xs;
+        const T *res = a.res ? (const T *)a.res + row * a.rs : nullptr;
+        float h[NC][V];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const int i = n * TPR + tr;
+            Vec u{}, v{};
+            if (i < chunks) {
+                u = *(const Vec *)(x + i * V);
+                if (res) v = *(const Vec *)(res + i * V);
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) h[n][e] = (float)u.e[e] + (float)v.e[e];
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int e = 0; e < V; ++e) ss = fmaf(h[n][e], h[n][e], ss);
+        if (a.sum) {
+            T *sum = (T *)a.sum + row * a.ss;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                const int i = n * TPR + tr;
+                Vec u;
+#pragma unroll
+                for (int e = 0; e < V; ++e) u.e[e] = (T)h[n][e];
+                if (i < chunks) *(Vec *)(sum + i * V) = u;
+            }
+        }
+        ss = wave_sum(ss);
+        if constexpr (TPR == 256) {
+            // two sets of words in turn: a row's are read before the next but one writes them
+            if (lane == 0) part[0][tid >> 6] = ss;
+            __syncthreads();
+            ss = (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]);
+        }
+        const float inv = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int e = 0; e < V; ++e) h[n][e] = h[n][e] * inv * wt[n][e];
+        if constexpr (!E4M3) {
+            T *out = (T *)a.out + row * a.os;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                const int i = n * TPR + tr;
+                Vec u;
+#pragma unroll
+                for (int e = 0; e < V; ++e) u.e[e] = (T)h[n][e];
+                if (i < chunks) *(Vec *)(out + i * V) = u;
+            }
+            if constexpr (TPR == 256) __syncthreads();
+        } else {
+            unsigned char *out = (unsigned char *)a.out + row * a.os;
+            float *scales = a.scales + row * a.groups;
+            float top[NC];
+            const int gl = a.groups == 1 ? 64 : a.group / V;  // lanes of a group
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                top[n] = 0.f;
+#pragma unroll
+                for (int e = 0; e < V; ++e) top[n] = nan_max(top[n], fabsf(h[n][e]));
+            }
+            if (a.groups == 1) {
+#pragma unroll
+                for (int n = 1; n < NC; ++n) top[0] = nan_max(top[0], top[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                if (n && a.groups == 1) {
+                    top[n] = top[0];
+                    continue;
+                }
+#pragma unroll
+                for (int m = 1; m < 64; m *= 2)
+                    if (m < gl) top[n] = nan_max(top[n], __shfl_xor(top[n], m));
+                if (a.groups == 1) {
+                    if constexpr (TPR == 256) {
+                        if (lane == 0) part[1][tid >> 6] = top[0];
+                        __syncthreads();
+                        top[0] = nan_max(nan_max(part[1][0], part[1][1]), nan_max(part[1][2], part[1][3]));
+                    }
+                }
+            }
+            if constexpr (TPR == 256)
+                if (a.groups != 1) __syncthreads();
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                const int i = n * TPR + tr;
+                const float s = e4m3_scale(top[n]), r = 1.0f / s;
+                VecOf<unsigned, V / 4> code;
+#pragma unroll
+                for (int e = 0; e < V; e += 4) code.e[e / 4] = to_e4m3x4(h[n][e] * r, h[n][e + 1] * r, h[n][e + 2] * r, h[n][e + 3] * r);
+                if (i < chunks) {
+                    *(VecOf<unsigned, V / 4> *)(out + i * V) = code;
+                    if (a.groups == 1 ? i == 0 : (lane & (gl - 1)) == 0) scales[a.groups == 1 ? 0 : i / gl] = s;
+                }
+            }
+        }
+    }
+}
+
+template <typename T, bool E4M3, int TPR, int NC>
+hipError_t rms_launch(const RmsNormArgs &a, hipStream_t st) {
+    const long long blocks = (a.rows + 256 / TPR - 1) / (256 / TPR);
+    // at most 8 workgroups a CU, which then walk their rows with the weights at hand
+    const long long most = 8LL * cu_count();
+    hipLaunchKernelGGL((k_rms_norm<T, E4M3, TPR, NC>), dim3((unsigned)std::min(blocks, most)), dim3(256), 0, st, a);
     return hipGetLastError();
+}
+
+template <typename T, bool E4M3>
+hipError_t rms_type(const RmsNormArgs &a, hipStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    auto fits = [](const void *p, long long stride, int size, int bytes) {
+        return !p || ((uintptr_t)p % bytes == 0 && stride * size % bytes == 0);
+    };
+    const int gl = a.groups == 1 ? 1 : a.group / V;
+    const bool vec = a.cols % V == 0 && a.cols <= 8 * 256 * V && fits(a.x, a.xs, sizeof(T), 16) &&
+                     fits(a.res, a.rs, sizeof(T), 16) && fits(a.sum, a.ss, sizeof(T), 16) &&
+                     fits(a.out, a.os, E4M3 ? 1 : sizeof(T), E4M3 ? V : 16) && fits(a.weight, 0, 4, 16) &&
+                     (!E4M3 || a.groups == 1 || (a.group % V == 0 && (gl & (gl - 1)) == 0 && gl <= 64));
+    if (!vec) {
+        hipLaunchKernelGGL((k_rms_norm_rows<T, E4M3>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+        return hipGetLastError();
+    }
+    // a wave per row up to 2 chunks a lane, and up to 4 where there are rows for the chip
+    const int chunks = a.cols / V;
+    const bool many = a.rows >= 16LL * cu_count();
+    if (chunks <= 64) return rms_launch<T, E4M3, 64, 1>(a, st);
+    if (chunks <= 128) return rms_launch<T, E4M3, 64, 2>(a, st);
+    if (chunks <= 256) return many ? rms_launch<T, E4M3, 64, 4>(a, st) : rms_launch<T, E4M3, 256, 1>(a, st);
+    if (chunks <= 512) return rms_launch<T, E4M3, 256, 2>(a, st);
+    if (chunks <= 768) return rms_launch<T, E4M3, 256, 3>(a, st);
+    if (chunks <= 1024) return rms_launch<T, E4M3, 256, 4>(a, st);
+    return rms_launch<T, E4M3, 256, 8>(a, st);
 }
 
 }  // namespace
@@ -276,9 +446,9 @@ hipError_t launch_rotary_op(int dtype, const RotaryArgs &a, hipStream_t st) {
 
 hipError_t launch_rms_norm_op(int dtype, bool e4m3, const RmsNormArgs &a, hipStream_t st) {
     switch (dtype) {
-        case 0: return rms_type<float>(e4m3, a, st);
-        case 1: return rms_type<half_t>(e4m3, a, st);
-        case 2: return rms_type<bfloat_t>(e4m3, a, st);
+        case 0: return e4m3 ? rms_type<float, true>(a, st) : rms_type<float, false>(a, st);
+        case 1: return e4m3 ? rms_type<half_t, true>(a, st) : rms_type<half_t, false>(a, st);
+        case 2: return e4m3 ? rms_type<bfloat_t, true>(a, st) : rms_type<bfloat_t, false>(a, st);
     }
     return hipErrorInvalidValue;
 }
