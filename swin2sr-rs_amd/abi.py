@@ -110,9 +110,9 @@ EXPORTS = {
     "s2s_profile_only": (C.c_int, [C.c_void_p, C.c_char_p]),
     "s2s_rstb_device": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
     "s2s_attention_workspace": (C.c_int, [C.POINTER(Attention_), C.POINTER(C.c_uint64)]),
-    "s2s_attention": (C.c_int, [C.POINTER(Attention_), C.c_void_p, C.c_uint64, C.c_void_p]),
-    "s2s_rotary": (C.c_int, [C.POINTER(Rotary_), C.c_void_p]),
-    "s2s_rms_norm": (C.c_int, [C.POINTER(RmsNorm_), C.c_void_p]),
+    "s2s_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "s2s_rotary": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "s2s_rms_norm": (C.c_int, [C.c_void_p, C.c_void_p]),
     "s2s_test_window_map": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int32),
                                       C.POINTER(C.c_uint8)]),
     "s2s_test_qkv_windows": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, FP, FP, FP,

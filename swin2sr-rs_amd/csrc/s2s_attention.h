@@ -58,6 +58,23 @@ struct AttnScore {
     }
 };
 
+// n / d for 0 <= n < 2^31 by a multiplication: a division takes some twenty
+// instructions, and the small launches do little else.
+struct FastDiv {
+    unsigned m;
+    int s, d;
+    void set(int by) {
+        d = by;
+        for (s = 0; (1LL << s) < by;) ++s;
+        m = (unsigned)((((1ULL << s) - by) << 32) / by + 1);
+    }
+#ifdef __HIP_DEVICE_COMPILE__
+    __device__ int of(int n) const { return (int)((__umulhi((unsigned)n, m) + (unsigned)n) >> s); }
+#else
+    int of(int n) const { return n / d; }
+#endif
+};
+
 // What a launch adds to the call's arguments.
 struct AttnLaunch {
     int cols;       // group * nq
@@ -69,6 +86,9 @@ struct AttnLaunch {
     float *part_ml;  // [batch * hk][splits][cols][2]: reference and sum of the weights
     const int4 *meta;  // documents: [batch][key tiles] {smallest, largest id >= 0, smallest id, 0}
     int meta_tiles;
+    const int4 *col_docs;  // [batch][tiles] the same of a column tile's queries, and its key tiles
+    const int *order;      // [batch][tiles] column tiles with the most key tiles first, or null
+    FastDiv by_pairs, by_tiles, by_hk, by_group;
     AttnScore score;
 };
 
@@ -141,7 +161,7 @@ __device__ __forceinline__ v4u tile_rsrc(const void *p, int bytes) {
     const unsigned long long x = (unsigned long long)p;
     return v4u{(unsigned)x, (unsigned)(x >> 32) & 0xffffu, (unsigned)bytes, 0x00020000u};
 }
-// The direct copy of dma16 (16 bytes a lane to LDS address `to` + 16 * lane) as an
+// The direct copy of dma16 (16 or 4 bytes a lane to LDS address `to` + bytes * lane) as an
 // instruction the compiler does not see through: it takes the transposing LDS
 // read for a reader of whatever copy is in flight and waits for all of them in front
 // of it, which leaves no copy in flight during the products. The kernel waits by
@@ -150,11 +170,19 @@ __device__ __forceinline__ v4u tile_rsrc(const void *p, int bytes) {
 // wrote.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // (m0 is reserved, and named as what it changes)
+template <int BYTES>
 __device__ __forceinline__ void tile_dma(v4u rsrc, unsigned to, int off) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :
-                 : "s"(to), "v"(off), "s"(rsrc)
-                 : "memory", "m0");
+    static_assert(BYTES == 16 || BYTES == 4, "the copies' sizes");
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :
+                     : "s"(to), "v"(off), "s"(rsrc)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                     :
+                     : "s"(to), "v"(off), "s"(rsrc)
+                     : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
@@ -280,9 +308,9 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 //  what AttnScore::general stands for (GENERAL). Paths that a kernel might take and
 //  does not cost it registers, spilled around its loop, and copies where they meet.
 // K and V tiles of TK keys are copied straight into LDS, two buffers each, the
-// next tile in flight while one is computed. ALIGNED: rows of 16-byte multiples,
-// copied by the DMA; otherwise through registers in narrower accesses.
-template <typename T, int DP, int NB, bool WK, bool ALIGNED, int MODE>
+// next tile in flight while one is computed. ALIGN: bytes of one copy by the DMA
+// (16, or 4 for rows of 4-byte multiples), or 0: through registers, by elements.
+template <typename T, int DP, int NB, bool WK, int ALIGN, int MODE>
 struct Kernel {
     static constexpr bool GEN = MODE == GENERAL;
     typedef Type<T> Ty;
@@ -297,6 +325,7 @@ struct Kernel {
     static constexpr int CH = CHD <= 4 ? 4 : CHD <= 8 ? 8 : CHD <= 16 ? 16 : 32;
     static constexpr int COLS = WK ? 16 : 64 * NB;       // columns per workgroup
     static constexpr int LOADS = TK * CH / 256;          // chunks per thread and tile
+    static constexpr int UNIT = ALIGN ? ALIGN : 16, SUB = 16 / UNIT;  // the copies' units, per chunk
     static constexpr size_t kTile = (size_t)TK * CH * 16;
     static constexpr size_t kJoin = WK ? (size_t)4 * 16 * (DP + 4) * 4 : 0;
     static constexpr size_t kLds = (4 * kTile > kJoin ? 4 * kTile : kJoin) + 16;  // (and four flags)
@@ -318,10 +347,10 @@ struct Kernel {
         // tile-major, so that with a multiple of 8 (batch, key head) pairs one XCD
         // keeps a pair's keys in its L2, and the tiles with the most keys (the last
         // ones, under the causal mask) start first
-        const int nbh = a.batch * a.hk;
-        const int bh = blockIdx.x % nbh, rest = blockIdx.x / nbh;
-        const int ct = L.tiles - 1 - rest % L.tiles, split = rest / L.tiles;
-        const int b = bh / a.hk, kvh = bh - b * a.hk;
+        const int rest = L.by_pairs.of(blockIdx.x), bh = blockIdx.x - rest * (a.batch * a.hk);
+        const int split = L.by_tiles.of(rest), rank = rest - split * L.tiles;
+        const int b = L.by_hk.of(bh), kvh = bh - b * a.hk;
+        const int ct = L.order ? L.order[b * L.tiles + rank] : L.tiles - 1 - rank;
         const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
         const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.nk) : a.nk;
         const int c0 = ct * COLS;
@@ -337,7 +366,7 @@ struct Kernel {
         Vec qf[NB][KS];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const int c = wc0 + nb * 16 + n16, i = c / a.group, h = kvh * a.group + (c - i * a.group);
+            const int c = wc0 + nb * 16 + n16, i = L.by_group.of(c), h = kvh * a.group + (c - i * a.group);
             const bool ok = i < ql;
             lim[nb] = ok ? limit(i) : 0;
             doc[nb] = 0;
@@ -354,40 +383,26 @@ struct Kernel {
                 const int c = (4 * ks + q) * E;
                 v4u x = {0, 0, 0, 0};
                 if (ok && c < a.width) {
-                    if constexpr (ALIGNED) x = *(const v4u *)(row + c);
+                    if constexpr (ALIGN == 16) x = *(const v4u *)(row + c);
                     else x = load_chunk<T>(row, c, a.width, L.vec);
                 }
                 qf[nb][ks] = __builtin_bit_cast(Vec, x);
             }
         }
         // keys that any column of the workgroup (of the wave) may read, and that all may
-        const int i_last = min(ql - 1, (c0 + COLS - 1) / a.group);
-        const int wg_max = limit(i_last), wg_min = limit(c0 / a.group);
-        const int w_first = min(ql - 1, wc0 / a.group), w_last = min(ql - 1, (wc0 + 16 * NB - 1) / a.group);
+        const int i_last = min(ql - 1, L.by_group.of(c0 + COLS - 1));
+        const int wg_max = limit(i_last), wg_min = limit(L.by_group.of(c0));
+        const int w_first = min(ql - 1, L.by_group.of(wc0)), w_last = min(ql - 1, L.by_group.of(wc0 + 16 * NB - 1));
         const bool w_any = wc0 < ql * a.group;
         const int w_max = w_any ? limit(w_last) : 0, w_min = limit(w_first);
-        // documents of the workgroup's columns
+        // documents of the workgroup's columns, where key tiles can be passed over
         int q_lo = 0, q_hi = 0, q_min = 0;
-        if (a.q_docs) {
-            q_lo = 0x7fffffff, q_hi = -1, q_min = 0x7fffffff;
-            const int i_first = c0 / a.group;
-            for (int i = i_first + lane; i <= i_last; i += 64) {
-                const int d = a.q_docs[b * a.q_docs_b + i];
-                q_min = min(q_min, d);
-                if (d >= 0) q_lo = min(q_lo, d), q_hi = max(q_hi, d);
-            }
-#pragma unroll
-            for (int m = 1; m < 64; m *= 2) {
-                q_lo = min(q_lo, __shfl_xor(q_lo, m));
-                q_hi = max(q_hi, __shfl_xor(q_hi, m));
-                q_min = min(q_min, __shfl_xor(q_min, m));
-            }
-            q_lo = __builtin_amdgcn_readfirstlane(q_lo);
-            q_hi = __builtin_amdgcn_readfirstlane(q_hi);
-            q_min = __builtin_amdgcn_readfirstlane(q_min);
+        if (L.meta) {
+            const int4 x = L.col_docs[b * L.tiles + ct];
+            q_lo = x.x, q_hi = x.y, q_min = x.z;
         }
         const int nt = q_hi < 0 ? 0 : (wg_max + TK - 1) / TK;
-        const int per = (nt + L.splits - 1) / L.splits;
+        const int per = L.splits == 1 ? nt : (nt + L.splits - 1) / L.splits;
         const int t_end = min(nt, (split + 1) * per);
 
         // the next tile from t on that holds a key some column's document has, and
@@ -417,28 +432,29 @@ struct Kernel {
         };
 
         // copying a tile: this thread's chunks. With the DMA a row past the keys lies
-        // past the resource, whose size is the rows that are left (token strides are
+        // past the resource, which ends with the last row that is left (token strides are
         // no smaller than the width on this path), and reads as zeros, as does a
         // chunk past the width
         const T *kp = (const T *)a.k + b * a.sk.b + kvh * a.sk.h;
         const T *vp = (const T *)a.v + b * a.sv.b + kvh * a.sv.h;
         const int kst = (int)a.sk.t, vst = (int)a.sv.t, kstep = TK * kst, vstep = TK * vst;  // (strides up to 2^22)
-        // a wave's next chunks are STEP rows on; the permutations repeat every 16
-        constexpr int STEP = 256 / CH, PER = STEP < 16 ? 16 / STEP : 1;
+        // a wave's next units are STEP rows on; the permutations repeat every 16
+        constexpr int ROW = CH * SUB, STEP = 256 / ROW, PER = STEP < 16 ? 16 / STEP : 1;
         int koff[PER], voff[PER];
 #pragma unroll
-        for (int p = 0; ALIGNED && p < PER; ++p) {
-            const int r = (wave * 64 + lane) / CH + p * STEP, sl = lane & (CH - 1);
-            const int kc = (k_slot<CH>(r, sl) & (CH - 1)) * E, vc = (v_slot<CH, F32>(r, sl) & (CH - 1)) * E;
+        for (int p = 0; ALIGN && p < PER; ++p) {
+            const int i = wave * 64 + lane, r = i / ROW + p * STEP, sl = i % ROW / SUB, sub = i % SUB * (E / SUB);
+            const int kc = (k_slot<CH>(r, sl) & (CH - 1)) * E + sub, vc = (v_slot<CH, F32>(r, sl) & (CH - 1)) * E + sub;
             koff[p] = kc < a.width ? (r * kst + kc) * (int)sizeof(T) : 0x60000000;
             voff[p] = vc < a.width ? (r * vst + vc) * (int)sizeof(T) : 0x60000000;
         }
         const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(const lds_t *)lds);
         auto stage = [&](int t, int buf) {
             const int left = min(kl - t * TK, TK);
-            if constexpr (ALIGNED) {
-                const v4u kr = tile_rsrc(kp, left * kst * (int)sizeof(T)), vr = tile_rsrc(vp, left * vst * (int)sizeof(T));
-                const unsigned to = lds0 + buf * 2 * (unsigned)kTile + wave * 1024;
+            if constexpr (ALIGN > 0) {
+                const v4u kr = tile_rsrc(kp, ((left - 1) * kst + a.width) * (int)sizeof(T)),
+                          vr = tile_rsrc(vp, ((left - 1) * vst + a.width) * (int)sizeof(T));
+                const unsigned to = lds0 + buf * 2 * (unsigned)kTile + wave * 64 * UNIT;
                 int ko[PER], vo[PER];
 #pragma unroll
                 for (int p = 0; p < PER; ++p) {
@@ -446,9 +462,9 @@ struct Kernel {
                     asm volatile("" : "+v"(ko[p]), "+v"(vo[p]));  // (sums formed here, not kept)
                 }
 #pragma unroll
-                for (int n = 0; n < LOADS; ++n) {
-                    tile_dma(kr, to + n * 4096, ko[n % PER] + n / PER * (PER * STEP) * kst * (int)sizeof(T));
-                    tile_dma(vr, to + (unsigned)kTile + n * 4096, vo[n % PER] + n / PER * (PER * STEP) * vst * (int)sizeof(T));
+                for (int n = 0; n < LOADS * SUB; ++n) {
+                    tile_dma<UNIT>(kr, to + n * 256 * UNIT, ko[n % PER] + n / PER * (PER * STEP) * kst * (int)sizeof(T));
+                    tile_dma<UNIT>(vr, to + (unsigned)kTile + n * 256 * UNIT, vo[n % PER] + n / PER * (PER * STEP) * vst * (int)sizeof(T));
                 }
             } else {
                 v4u x[2][LOADS];
@@ -506,7 +522,7 @@ struct Kernel {
         while (t < t_end) {
             const bool one_doc = !a.q_docs || (L.meta && ((whole >> (t - live_at)) & 1));
             const int tn = next(t + 1);
-            if constexpr (ALIGNED) WAIT_VMCNT(0);
+            if constexpr (ALIGN > 0) WAIT_VMCNT(0);
             lds_sync();
             kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
             if (tn < t_end) stage(tn, buf ^ 1);
@@ -579,7 +595,7 @@ struct Kernel {
         const int group = late->a.group, splits = late->L.splits, width = late->a.width, vec = late->L.out_vec;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const int c = wc0 + nb * 16 + n16, i = c / group;
+            const int c = wc0 + nb * 16 + n16, i = (int)((__umulhi((unsigned)c, late->L.by_group.m) + (unsigned)c) >> late->L.by_group.s);
             if (i >= ql) continue;
             if (splits > 1) {
                 const long long row = ((long long)bh * splits + split) * late->L.cols + c;
@@ -640,6 +656,22 @@ struct Kernel {
                                                 bool full, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
                                                 const Vec (*qf)[KS], f4v (*o)[NB], float *m, float *l) {
         const int lane = threadIdx.x & 63, q = lane >> 4;
+        // a lane per key for what is read per key
+        const int jl = min(j0 + min(lane, 16 * KB - 1), u.kl - 1);
+        // the table's entries on their way while the scores are made
+        int kpos = 0;
+        float bias[GEN ? KB : 1][4][GEN ? NB : 1];
+        if (GEN && u.table) {
+            if (u.k_pos) kpos = u.k_pos[jl];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int jr = 16 * kb + 4 * q + i, kp = u.k_pos ? __shfl(kpos, jr) : j0 + jr;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) bias[GEN ? kb : 0][i][GEN ? nb : 0] = entry(u, tab[nb], at[nb] - kp);
+                }
+        }
         f4v s[KB][NB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -693,25 +725,31 @@ struct Kernel {
             }
             unit = 1.f;
         }
-        // a lane per key for what is read per key
-        const int jl = min(j0 + min(lane, 16 * KB - 1), u.kl - 1);
         if (GEN && u.general) {
-            const int kpos = u.k_pos ? u.k_pos[jl] : 0;
+            if (u.slopes) {
+                if (u.k_pos && !u.table) kpos = u.k_pos[jl];
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int jr = 16 * kb + 4 * q + i, kp = u.k_pos ? __shfl(kpos, jr) : j0 + jr;
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                            s[kb][nb][i] = fmaf(-slope[nb], fabsf((float)(at[nb] - kp)), s[kb][nb][i] * unit);
+                    }
+                unit = 1.f;
+            }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int jr = 16 * kb + 4 * q + i;
-                    const int kp = u.k_pos ? __shfl(kpos, jr) : j0 + jr;
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        const int dist = at[nb] - kp;
-                        float x = fmaf(-slope[nb], fabsf((float)dist), s[kb][nb][i] * unit);
-                        if (u.table) x = add_bias(x, entry(u, tab[nb], dist));
+                        float x = s[kb][nb][i] * unit;
+                        if (u.table) x = add_bias(x, bias[GEN ? kb : 0][i][GEN ? nb : 0]);
                         // lowest values stay numbers, so that a row of them is even
                         s[kb][nb][i] = x < -1e30f && x != -INFINITY ? -1e30f : x;
                     }
-                }
             unit = 1.f;
         } else if (MODE < ANY ? (MODE & SLOPES) != 0 : u.slopes) {
             // distances of neighbours differ by what the register says
@@ -867,11 +905,11 @@ struct Kernel {
     }
 };
 
-template <typename T, int DP, int NB, bool WK, bool ALIGNED, int MODE>
+template <typename T, int DP, int NB, bool WK, int ALIGN, int MODE>
 __global__ __launch_bounds__(256, 2) void k_attn(AttnOpArgs a, AttnLaunch L) {
     static_assert(sizeof(AttnOpArgs) % 8 == 0 && alignof(AttnLaunch) == 8, "late_params reads the two as one struct");
     extern __shared__ __align__(16) char lds[];
-    Kernel<T, DP, NB, WK, ALIGNED, MODE>::run(a, L, lds);
+    Kernel<T, DP, NB, WK, ALIGN, MODE>::run(a, L, lds);
 }
 
 // The key ranges' sums of one column: a workgroup each, its threads over the ranges
@@ -937,33 +975,36 @@ struct Cut {
     int tiles, splits;
 };
 
-template <typename T, int DP, int NB, bool WK, bool ALIGNED, int MODE>
+template <typename T, int DP, int NB, bool WK, int ALIGN, int MODE>
 hipError_t launch(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
-    typedef Kernel<T, DP, NB, WK, ALIGNED, MODE> K;
+    typedef Kernel<T, DP, NB, WK, ALIGN, MODE> K;
     static_assert(K::kLds <= 163840, "LDS");
     const long long blocks = (long long)a.batch * a.hk * L.tiles * L.splits;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_attn<T, DP, NB, WK, ALIGNED, MODE>), dim3((unsigned)blocks), dim3(256), K::kLds, st, a, L);
+    hipLaunchKernelGGL((k_attn<T, DP, NB, WK, ALIGN, MODE>), dim3((unsigned)blocks), dim3(256), K::kLds, st, a, L);
     return hipGetLastError();
 }
 
-// Unaligned arrays and general biases take the kernels of 16 columns a wave.
+// Arrays that are not of 16-byte multiples and general biases take the kernels of 16
+// columns a wave.
+template <typename T, int DP, bool WK>
+hipError_t launch_narrow(const AttnOpArgs &a, const AttnLaunch &L, int align, hipStream_t st) {
+    if (align == 0) return launch<T, DP, 1, WK, 0, GENERAL>(a, L, st);
+    if (align < 16) return launch<T, DP, 1, WK, 4, GENERAL>(a, L, st);
+    return L.score.general ? launch<T, DP, 1, WK, 16, GENERAL>(a, L, st) : launch<T, DP, 1, WK, 16, ANY>(a, L, st);
+}
+
 template <typename T, int DP>
-hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, bool aligned, hipStream_t st) {
+hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, int align, hipStream_t st) {
     hipError_t e;
-    const bool gen = L.score.general;
     if (c.wk)
-        e = !aligned ? launch<T, DP, 1, true, false, GENERAL>(a, L, st)
-            : gen    ? launch<T, DP, 1, true, true, GENERAL>(a, L, st)
-                     : launch<T, DP, 1, true, true, ANY>(a, L, st);
+        e = launch_narrow<T, DP, true>(a, L, align, st);
     else if (c.nb == 1)
-        e = !aligned ? launch<T, DP, 1, false, false, GENERAL>(a, L, st)
-            : gen    ? launch<T, DP, 1, false, true, GENERAL>(a, L, st)
-                     : launch<T, DP, 1, false, true, ANY>(a, L, st);
+        e = launch_narrow<T, DP, false>(a, L, align, st);
     else if (a.cap > 0.f)
-        e = a.slopes ? launch<T, DP, 2, false, true, CAP | SLOPES>(a, L, st) : launch<T, DP, 2, false, true, CAP>(a, L, st);
+        e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES>(a, L, st) : launch<T, DP, 2, false, 16, CAP>(a, L, st);
     else
-        e = a.slopes ? launch<T, DP, 2, false, true, SLOPES>(a, L, st) : launch<T, DP, 2, false, true, 0>(a, L, st);
+        e = a.slopes ? launch<T, DP, 2, false, 16, SLOPES>(a, L, st) : launch<T, DP, 2, false, 16, 0>(a, L, st);
     if (e != hipSuccess || L.splits == 1) return e;
     const long long rows = (long long)a.batch * a.hk * L.cols;
     if (rows > 0x7fffffffLL) return hipErrorInvalidValue;
@@ -972,17 +1013,17 @@ hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, 
 }
 
 template <typename T>
-hipError_t launch_type(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, bool aligned, hipStream_t st) {
+hipError_t launch_type(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, int align, hipStream_t st) {
     switch (c.dp) {
-        case 32: return launch_width<T, 32>(a, L, c, aligned, st);
-        case 64: return launch_width<T, 64>(a, L, c, aligned, st);
-        case 96: return launch_width<T, 96>(a, L, c, aligned, st);
-        default: return launch_width<T, 128>(a, L, c, aligned, st);
+        case 32: return launch_width<T, 32>(a, L, c, align, st);
+        case 64: return launch_width<T, 64>(a, L, c, align, st);
+        case 96: return launch_width<T, 96>(a, L, c, align, st);
+        default: return launch_width<T, 128>(a, L, c, align, st);
     }
 }
 
 }  // namespace attn
 
-hipError_t launch_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, bool aligned, hipStream_t st);
-hipError_t launch_attention_f16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, bool aligned, hipStream_t st);
-hipError_t launch_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, bool aligned, hipStream_t st);
+hipError_t launch_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_attention_f16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);

@@ -53,6 +53,68 @@ __global__ __launch_bounds__(256) void k_doc_tiles(AttnOpArgs a, int tk, int til
     if (lane == 0) meta[id] = make_int4(lo, hi, all, 0);
 }
 
+// The same of the queries of a column tile, and how many key tiles hold a document of
+// theirs: a wave per column tile.
+__global__ __launch_bounds__(256) void k_doc_columns(AttnOpArgs a, int tk, int key_tiles, int per, int tiles, const int4 *meta,
+                                                     int4 *col) {
+    const int lane = threadIdx.x & 63;
+    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= (long long)a.batch * tiles) return;
+    const int b = (int)(id / tiles), t = (int)(id - (long long)b * tiles);
+    const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
+    int lo = 0x7fffffff, hi = -1, all = 0x7fffffff;
+    const int first = t * per / a.group, last = min(ql - 1, (t * per + per - 1) / a.group);
+    for (int i = first + lane; i <= last; i += 64) {
+        const int d = a.q_docs[b * a.q_docs_b + i];
+        all = min(all, d);
+        if (d >= 0) lo = min(lo, d), hi = max(hi, d);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        lo = min(lo, __shfl_xor(lo, m));
+        hi = max(hi, __shfl_xor(hi, m));
+        all = min(all, __shfl_xor(all, m));
+    }
+    int live = 0;
+    for (int k = lane; k < key_tiles; k += 64) {
+        const int4 x = meta[(long long)b * key_tiles + k];
+        live += x.x <= hi && x.y >= lo;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) live += __shfl_xor(live, m);
+    if (lane == 0) col[id] = make_int4(lo, hi, all, live);
+}
+
+// Column tiles by falling number of key tiles, to 256 steps: a workgroup per batch
+// entry. (Tiles of one step come in any order; no result goes by it.)
+__global__ __launch_bounds__(256) void k_doc_order(int tiles, const int4 *col, int *order) {
+    __shared__ int bin[256], most;
+    const int tid = threadIdx.x;
+    col += (long long)blockIdx.x * tiles, order += (long long)blockIdx.x * tiles;
+    bin[tid] = 0;
+    if (tid == 0) most = 1;
+    __syncthreads();
+    for (int t = tid; t < tiles; t += 256) atomicMax(&most, col[t].w);
+    __syncthreads();
+    const float step = 255.f / (float)most;
+    auto of = [&](int t) { return 255 - min(255, (int)((float)col[t].w * step)); };
+    for (int t = tid; t < tiles; t += 256) atomicAdd(&bin[of(t)], 1);
+    __syncthreads();
+    int n = bin[tid];  // its sum over the steps before
+    for (int m = 1; m < 256; m *= 2) {
+        __syncthreads();
+        const int x = tid >= m ? bin[tid - m] : 0;
+        __syncthreads();
+        bin[tid] += x;
+    }
+    __syncthreads();
+    n = bin[tid] - n;
+    __syncthreads();
+    bin[tid] = n;
+    __syncthreads();
+    for (int t = tid; t < tiles; t += 256) order[atomicAdd(&bin[of(t)], 1)] = t;
+}
+
 // The largest power of two in bytes, up to 16, that an array's address, strides
 // and width are multiples of.
 int aligned_bytes(const void *p, const Strides &s, int width, int size) {
@@ -63,13 +125,18 @@ int aligned_bytes(const void *p, const Strides &s, int width, int size) {
 
 }  // namespace
 
+// The documents' summaries: of key tiles, of column tiles, the column tiles' order.
+size_t doc_bytes(const attn::Cut &c, const AttnOpArgs &a) {
+    return (size_t)a.batch * ((size_t)meta_tiles(c, a) + c.tiles) * sizeof(int4) + round16((size_t)a.batch * c.tiles * sizeof(int));
+}
+
 // The most that either cut of these sizes needs: which one runs goes by strides and
 // biases too.
 size_t attn_op_workspace(int dtype, const AttnOpArgs &a) {
     size_t most = 0;
     for (const bool narrow : {false, true}) {
         const attn::Cut c = cut_of(dtype, a, narrow);
-        size_t n = round16((size_t)a.batch * meta_tiles(c, a) * sizeof(int4));
+        size_t n = doc_bytes(c, a);
         if (c.splits > 1) {
             const size_t rows = (size_t)a.batch * a.hk * c.splits * a.group * a.nq;
             n += rows * c.dp * 4 + rows * 8;
@@ -87,32 +154,46 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
     if (a.nk > 0) al = std::min(al, std::min(aligned_bytes(a.k, a.sk, a.width, size), aligned_bytes(a.v, a.sv, a.width, size)));
     L.vec = std::min(al, 8);
     L.out_vec = aligned_bytes(a.out, a.so, a.width, size) >= 4 * size;
-    const bool aligned = al >= 16 && (a.nk <= 1 || (a.sk.t >= a.width && a.sv.t >= a.width));
-    const attn::Cut c = cut_of(dtype, a, !aligned || L.score.general);
+    // (rows that overlap have no end that the copies' resource could tell: by elements)
+    const int align = a.sk.t < a.width || a.sv.t < a.width ? 0 : al >= 16 ? 16 : al >= 4 ? 4 : 0;
+    const attn::Cut c = cut_of(dtype, a, align < 16 || L.score.general);
     L.cols = a.group * a.nq;
     L.tiles = c.tiles;
     L.splits = c.splits;
     char *w = (char *)ws;
     const int mt = meta_tiles(c, a);
-    const size_t meta_bytes = round16((size_t)a.batch * mt * sizeof(int4));
+    L.by_pairs.set(a.batch * a.hk);
+    L.by_tiles.set(c.tiles);
+    L.by_hk.set(a.hk);
+    L.by_group.set(a.group);
     if (c.splits > 1) {
         const size_t rows = (size_t)a.batch * a.hk * c.splits * L.cols;
-        L.part_o = (float *)(w + meta_bytes);
+        L.part_o = (float *)(w + doc_bytes(c, a));
         L.part_ml = L.part_o + rows * c.dp;
     }
     // a summary of few tiles would skip nothing
     if (a.k_docs && mt > 4) {
-        L.meta = (const int4 *)w;
+        int4 *meta = (int4 *)w, *col = meta + (size_t)a.batch * mt;
+        int *order = (int *)(col + (size_t)a.batch * c.tiles);
+        const int per = c.wk ? 16 : 64 * c.nb;
+        L.meta = meta;
         L.meta_tiles = mt;
-        const long long n = (long long)a.batch * mt;
-        hipLaunchKernelGGL(k_doc_tiles, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, (int4 *)w);
+        L.col_docs = col;
+        const long long nk = (long long)a.batch * mt, nc = (long long)a.batch * c.tiles;
+        hipLaunchKernelGGL(k_doc_tiles, dim3((unsigned)((nk + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, meta);
+        hipLaunchKernelGGL(k_doc_columns, dim3((unsigned)((nc + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, per, c.tiles, meta, col);
+        // documents of different sizes make column tiles of different work; the longest first
+        if (c.tiles >= 8) {
+            L.order = order;
+            hipLaunchKernelGGL(k_doc_order, dim3((unsigned)a.batch), dim3(256), 0, st, c.tiles, col, order);
+        }
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     switch (dtype) {
-        case 0: return launch_attention_f32(a, L, c, aligned, st);
-        case 1: return launch_attention_f16(a, L, c, aligned, st);
-        case 2: return launch_attention_bf16(a, L, c, aligned, st);
+        case 0: return launch_attention_f32(a, L, c, align, st);
+        case 1: return launch_attention_f16(a, L, c, align, st);
+        case 2: return launch_attention_bf16(a, L, c, align, st);
     }
     return hipErrorInvalidValue;
 }

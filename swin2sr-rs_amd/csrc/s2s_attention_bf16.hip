@@ -1,6 +1,6 @@
 // s2s_attention_bf16.hip - the attention kernels of s2s_attention.h for bf16 arrays.
 #include "s2s_attention.h"
 
-hipError_t launch_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, bool aligned, hipStream_t st) {
-    return attn::launch_type<bfloat_t>(a, L, c, aligned, st);
+hipError_t launch_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st) {
+    return attn::launch_type<bfloat_t>(a, L, c, align, st);
 }

@@ -14,9 +14,10 @@ library's message; shapes and types that do not fit raise it too.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Sequence
 
-from .abi import Attention_, RmsNorm_, Rotary_, S2SError, Tokens_, check, load_library
+from .abi import Attention_, S2SError, check, last_error, load_library
 
 F32, F16, BF16, E4M3 = 0, 1, 2, 3
 _NAMES = {"f32": F32, "float32": F32, "f16": F16, "float16": F16, "bf16": BF16, "bfloat16": BF16,
@@ -55,8 +56,15 @@ def _type(dtype) -> int:
         return code
 
 
+_int32 = {}
+
+
 def _is_int32(dtype) -> bool:
-    return str(dtype) in ("torch.int32", "int32", "i32")
+    try:
+        return _int32[dtype]
+    except KeyError:
+        _int32[dtype] = str(dtype) in ("torch.int32", "int32", "i32")
+        return _int32[dtype]
 
 
 def _is_f32(dtype) -> bool:
@@ -77,20 +85,27 @@ def _contiguous(a) -> bool:
     return True
 
 
-def _tokens(where: Tokens_, a, shape, dtype: int, op: str, name: str):
-    """An array [batch][tokens][heads][width] into its C struct."""
-    if tuple(a.shape) != shape or _type(a.dtype) != dtype:
+def _tokens(a, shape, dtype: int, op: str, name: str):
+    """An array [batch][tokens][heads][width] as its C struct's fields."""
+    if a.shape != shape or _type(a.dtype) != dtype:
         raise S2SError(f"{op}: {name} is {tuple(a.shape)} of {a.dtype}, wanted {shape} of the call's type")
-    s = a.stride()
-    if s[3] != 1 and shape[3] > 1:
+    b, t, h, d = a.stride()
+    if d != 1 and shape[3] > 1:
         raise S2SError(f"{op}: the channels of {name} are not adjacent")
-    where.data, where.batch, where.token, where.head = a.data_ptr(), s[0], s[1], s[2]
+    return a.data_ptr(), b, t, h
+
+
+# The argument structs as one pack each (a call's fields set one by one through
+# ctypes take as long as the call): the C structs' layout, null pointers as 0.
+_ATTENTION = struct.Struct("@8i2f 4q4q4q4q 3P 2P2q 2P2q 2Pi0q")
+_ROTARY = struct.Struct("@10i 4q4q4q4q Pq3P")
+_RMS = struct.Struct("@2iqi4P4qP2fPi0q")
 
 
 def _vector(a, n: int, op: str, name: str):
-    """A contiguous int32 vector of n."""
+    """A contiguous int32 vector of n: its address, 0 for none."""
     if a is None:
-        return None
+        return 0
     _need(tuple(a.shape) == (n,) and _is_int32(a.dtype) and _contiguous(a), f"{op}: {name} is no int32 vector of {n}")
     return a.data_ptr()
 
@@ -98,7 +113,7 @@ def _vector(a, n: int, op: str, name: str):
 def _per_token(a, batch: int, tokens: int, op: str, name: str):
     """int32 [batch][tokens], or [tokens] shared by the batch: address and batch stride."""
     if a is None:
-        return None, 0
+        return 0, 0
     shape, s = tuple(a.shape), tuple(a.stride())
     _need(_is_int32(a.dtype) and shape in ((tokens,), (batch, tokens)) and (s[-1] == 1 or tokens <= 1),
           f"{op}: {name} is not int32 [{batch}][{tokens}] or [{tokens}] with adjacent tokens")
@@ -124,13 +139,12 @@ class Attention:
         sizes = (batch, q_tokens, k_tokens, q_heads, k_heads, width)
         _need(all(-2 ** 31 <= n < 2 ** 31 for n in sizes), "attention: a size that is no 32-bit int")
         self.lib = load_library()
-        a = self.args = Attention_()
-        a.dtype = self.dtype = _type(dtype)
-        a.batch, a.q_tokens, a.k_tokens = batch, q_tokens, k_tokens
-        a.q_heads, a.k_heads, a.width = q_heads, k_heads, width
-        a.scale = float(scale) if scale is not None else max(width, 1) ** -0.5
-        a.cap, a.causal = float(cap), int(bool(causal))
+        self.dtype = _type(dtype)
+        self.head = (self.dtype, batch, q_tokens, k_tokens, q_heads, k_heads, width, int(bool(causal)),
+                     float(scale) if scale is not None else max(width, 1) ** -0.5, float(cap))
+        self.batch, self.q_tokens, self.k_tokens, self.q_heads = batch, q_tokens, k_tokens, q_heads
         self.q_shape, self.k_shape = (batch, q_tokens, q_heads, width), (batch, k_tokens, k_heads, width)
+        a = Attention_(*self.head)
         n = C.c_uint64()
         check(self.lib.s2s_attention_workspace(C.byref(a), C.byref(n)), "attention")
         self.workspace_bytes = n.value
@@ -141,44 +155,47 @@ class Attention:
         [batch][k_tokens][k_heads][width]; lengths and prefix int32 [batch];
         documents and positions int32 [batch][tokens] or [tokens]; slopes f32
         [q_heads]; table f32 [q_heads][odd]."""
-        a = Attention_.from_buffer_copy(self.args)
-        op = "attention"
-        _tokens(a.q, q, self.q_shape, self.dtype, op, "q")
-        _tokens(a.k, k, self.k_shape, self.dtype, op, "k")
-        _tokens(a.v, v, self.k_shape, self.dtype, op, "v")
-        _tokens(a.out, out, self.q_shape, self.dtype, op, "out")
-        if q_lens is not None:
-            a.q_lens = _vector(q_lens, a.batch, op, "q_lens")
-        if k_lens is not None:
-            a.k_lens = _vector(k_lens, a.batch, op, "k_lens")
-        if prefix is not None:
-            a.prefix = _vector(prefix, a.batch, op, "prefix")
+        op, dt, batch, nq, nk = "attention", self.dtype, self.batch, self.q_tokens, self.k_tokens
+        arrays = (*_tokens(q, self.q_shape, dt, op, "q"), *_tokens(k, self.k_shape, dt, op, "k"),
+                  *_tokens(v, self.k_shape, dt, op, "v"), *_tokens(out, self.q_shape, dt, op, "out"))
+        lens = (_vector(q_lens, batch, op, "q_lens"), _vector(k_lens, batch, op, "k_lens"), _vector(prefix, batch, op, "prefix"))
+        docs = pos = (0, 0, 0, 0)
         if q_docs is not None or k_docs is not None:
-            a.q_docs, a.q_docs_batch = _per_token(q_docs, a.batch, a.q_tokens, op, "q_docs")
-            a.k_docs, a.k_docs_batch = _per_token(k_docs, a.batch, a.k_tokens, op, "k_docs")
+            (a, sa), (b, sb) = _per_token(q_docs, batch, nq, op, "q_docs"), _per_token(k_docs, batch, nk, op, "k_docs")
+            docs = (a, b, sa, sb)
         if q_pos is not None or k_pos is not None:
-            a.q_pos, a.q_pos_batch = _per_token(q_pos, a.batch, a.q_tokens, op, "q_pos")
-            a.k_pos, a.k_pos_batch = _per_token(k_pos, a.batch, a.k_tokens, op, "k_pos")
+            (a, sa), (b, sb) = _per_token(q_pos, batch, nq, op, "q_pos"), _per_token(k_pos, batch, nk, op, "k_pos")
+            pos = (a, b, sa, sb)
+        slope_ptr = table_ptr = entries = 0
         if slopes is not None:
-            _need(tuple(slopes.shape) == (a.q_heads,) and _is_f32(slopes.dtype) and _contiguous(slopes),
-                  f"{op}: slopes is no f32 vector of {a.q_heads}")
-            a.slopes = slopes.data_ptr()
+            _need(slopes.shape == (self.q_heads,) and _is_f32(slopes.dtype) and _contiguous(slopes),
+                  f"{op}: slopes is no f32 vector of {self.q_heads}")
+            slope_ptr = slopes.data_ptr()
         if table is not None:
-            _need(len(table.shape) == 2 and table.shape[0] == a.q_heads and _is_f32(table.dtype) and _contiguous(table),
-                  f"{op}: table is no contiguous f32 [{a.q_heads}][entries]")
-            a.table, a.table_size = table.data_ptr(), table.shape[1]
+            _need(len(table.shape) == 2 and table.shape[0] == self.q_heads and _is_f32(table.dtype) and _contiguous(table),
+                  f"{op}: table is no contiguous f32 [{self.q_heads}][entries]")
+            table_ptr, entries = table.data_ptr(), table.shape[1]
+            _need(entries < 2 ** 31, f"{op}: a table of {entries} entries")
+        args = _ATTENTION.pack(*self.head, *arrays, *lens, *docs, *pos, slope_ptr, table_ptr, entries)
         ws, n = (None, 0) if workspace is None else (workspace.data_ptr(), _bytes(workspace))
-        check(self.lib.s2s_attention(C.byref(a), ws, n, stream), op)
+        if self.lib.s2s_attention(args, ws, n, stream):
+            raise S2SError(f"{op}: {last_error()}")
         return out
+
+
+_SIZES = {}
 
 
 def _bytes(a) -> int:
     n = 1
     for d in a.shape:
         n *= d
-    _need(_contiguous(a), "workspace: not contiguous")
-    size = {"u8": 1, "uint8": 1, "i32": 4, "int32": 4, "f32": 4, "float32": 4}.get(str(a.dtype).replace("torch.", ""))
-    _need(size is not None, f"workspace: of {a.dtype}, wanted u8, i32 or f32")
+    size = _SIZES.get(a.dtype)
+    if size is None:
+        size = {"u8": 1, "uint8": 1, "i32": 4, "int32": 4, "f32": 4, "float32": 4}.get(str(a.dtype).replace("torch.", ""))
+        _need(size is not None, f"workspace: of {a.dtype}, wanted u8, i32 or f32")
+        _SIZES[a.dtype] = size
+    _need(len(a.shape) == 1 and a.stride()[0] == 1 or _contiguous(a), "workspace: not contiguous")
     return n * size
 
 
@@ -198,10 +215,8 @@ class Rotary:
         self.lib = load_library()
         self.inv_freq = (C.c_double * len(inv_freq))(*[float(f) for f in inv_freq])
         self.pair_axis = (C.c_uint8 * len(pair_axis))(*[int(x) for x in pair_axis])
-        a = self.args = Rotary_()
-        a.pairs, a.adjacent, a.inverse = len(inv_freq), int(bool(adjacent)), int(bool(inverse))
-        a.inv_freq = C.cast(self.inv_freq, C.POINTER(C.c_double))
-        a.pair_axis = C.cast(self.pair_axis, C.POINTER(C.c_uint8))
+        self.flags = (len(inv_freq), int(bool(adjacent)), int(bool(inverse)))
+        self.host = (C.addressof(self.inv_freq), C.addressof(self.pair_axis))
 
     @classmethod
     def of(cls, sections: Sequence[int], theta: float = 10000.0, adjacent: bool = False, inverse: bool = False):
@@ -213,41 +228,45 @@ class Rotary:
         without them; pos int32 [batch][tokens][axes] or [tokens][axes]; tokens
         from lens[b] on are not written."""
         op = "rotary"
-        a = Rotary_.from_buffer_copy(self.args)
-        shape = tuple(q.shape)
-        _need(len(shape) == 4 and max(shape) < 2 ** 31, f"{op}: q is {shape}, wanted [batch][tokens][heads][width]")
-        a.dtype = dt = _type(q.dtype)
-        a.batch, a.tokens, a.q_heads, a.width = shape
-        _tokens(a.q, q, shape, dt, op, "q")
-        _tokens(a.q_out, q if q_out is None else q_out, shape, dt, op, "q_out")
+        shape = q.shape
+        _need(len(shape) == 4 and max(shape) < 2 ** 31, f"{op}: q is {tuple(shape)}, wanted [batch][tokens][heads][width]")
+        dt = _type(q.dtype)
+        if q_out is None:
+            q_out = q
+        arrays = _tokens(q, shape, dt, op, "q"), _tokens(q_out, shape, dt, op, "q_out")
+        k_arrays, k_heads = ((0, 0, 0, 0), (0, 0, 0, 0)), 0
         if k is not None:
-            ks = tuple(k.shape)
-            _need(len(ks) == 4 and ks[2] >= 1, f"{op}: k is {ks}, wanted [batch][tokens][heads][width]")
-            ks = (shape[0], shape[1], ks[2], shape[3])
-            a.k_heads = ks[2]
-            _tokens(a.k, k, ks, dt, op, "k")
-            _tokens(a.k_out, k if k_out is None else k_out, ks, dt, op, "k_out")
+            ks = k.shape
+            _need(len(ks) == 4 and 1 <= ks[2] < 2 ** 31, f"{op}: k is {tuple(ks)}, wanted [batch][tokens][heads][width]")
+            k_heads = ks[2]
+            ks = (shape[0], shape[1], k_heads, shape[3])
+            if k_out is None:
+                k_out = k
+            k_arrays = _tokens(k, ks, dt, op, "k"), _tokens(k_out, ks, dt, op, "k_out")
         else:
             _need(k_out is None, f"{op}: k_out without k")
-        ps, pstr = tuple(pos.shape), tuple(pos.stride())
-        a.axes = ps[-1] if ps else 0
-        _need(_is_int32(pos.dtype) and ps in (shape[1:2] + ps[-1:], shape[:2] + ps[-1:]),
+        ps, pstr = tuple(pos.shape), pos.stride()
+        _need(_is_int32(pos.dtype) and ps in ((shape[1],) + ps[-1:], (shape[0], shape[1]) + ps[-1:]),
               f"{op}: pos is {ps} of {pos.dtype}, wanted int32 [batch][tokens][axes] or [tokens][axes]")
         _need((pstr[-1] == 1 or ps[-1] == 1) and (pstr[-2] == ps[-1] or ps[-2] <= 1),
               f"{op}: the tokens and axes of pos are not adjacent")
-        a.pos, a.pos_batch = pos.data_ptr(), (pstr[0] if len(ps) == 3 else 0)
-        if lens is not None:
-            a.lens = _vector(lens, a.batch, op, "lens")
-        check(self.lib.s2s_rotary(C.byref(a), stream), op)
-        return (q if q_out is None else q_out) if k is None else (q if q_out is None else q_out, k if k_out is None else k_out)
+        args = _ROTARY.pack(dt, shape[0], shape[1], shape[2], k_heads, shape[3], min(ps[-1], 2 ** 31 - 1), *self.flags, *arrays[0],
+                            *k_arrays[0], *arrays[1], *k_arrays[1], pos.data_ptr(), pstr[0] if len(ps) == 3 else 0,
+                            _vector(lens, shape[0], op, "lens"), *self.host)
+        if self.lib.s2s_rotary(args, stream):
+            raise S2SError(f"{op}: {last_error()}")
+        return q_out if k is None else (q_out, k_out)
 
 
-def _rows(a, rows: int, cols: int, dtype: int, op: str, name: str):
-    s = a.stride()
-    if tuple(a.shape) != (rows, cols) or _type(a.dtype) != dtype or (s[1] != 1 and cols > 1):
-        raise S2SError(f"{op}: {name} is {tuple(a.shape)} of {a.dtype}, wanted [{rows}][{cols}] with adjacent columns "
+def _rows(a, shape, dtype: int, op: str, name: str):
+    """An array [rows][cols]: address and row stride; zeros for none."""
+    if a is None:
+        return 0, 0
+    r, c = a.stride()
+    if a.shape != shape or _type(a.dtype) != dtype or (c != 1 and shape[1] > 1):
+        raise S2SError(f"{op}: {name} is {tuple(a.shape)} of {a.dtype}, wanted {tuple(shape)} with adjacent columns "
                        "and the call's type")
-    return a.data_ptr(), s[0]
+    return a.data_ptr(), r
 
 
 def rms_norm(x, weight, out, eps: float = 1e-6, res=None, sum=None, scales=None, group: int = 0,
@@ -256,28 +275,25 @@ def rms_norm(x, weight, out, eps: float = 1e-6, res=None, sum=None, scales=None,
     x + res, with h in `sum`. x, res, sum [rows][cols] of one type, out of that type
     or e4m3 (then with `scales` f32 [rows][ceil(cols / group)], group 0 being the
     row); weight f32 [cols]."""
-    op = "rms_norm"
-    a = RmsNorm_()
-    _need(len(x.shape) == 2, f"{op}: x is {tuple(x.shape)}, wanted [rows][cols]")
-    rows, cols = x.shape
-    _need(cols < 2 ** 31 and abs(group) < 2 ** 31, f"{op}: columns or a group that are no 32-bit int")
-    a.rows, a.cols, a.eps, a.weight_offset, a.group = rows, cols, eps, weight_offset, group
-    a.dtype = dt = _type(x.dtype)
-    a.out_dtype = E4M3 if _type(out.dtype) == E4M3 else dt
-    a.x, a.x_stride = _rows(x, rows, cols, dt, op, "x")
-    if res is not None:
-        a.res, a.res_stride = _rows(res, rows, cols, dt, op, "res")
-    if sum is not None:
-        a.sum, a.sum_stride = _rows(sum, rows, cols, dt, op, "sum")
-    a.out, a.out_stride = _rows(out, rows, cols, a.out_dtype, op, "out")
-    _need(tuple(weight.shape) == (cols,) and _is_f32(weight.dtype) and _contiguous(weight),
+    op, shape = "rms_norm", x.shape
+    _need(len(shape) == 2, f"{op}: x is {tuple(shape)}, wanted [rows][cols]")
+    rows, cols = shape
+    _need(cols < 2 ** 31 and 0 <= group < 2 ** 31, f"{op}: columns or a group that are negative or no 32-bit int")
+    dt = _type(x.dtype)
+    odt = E4M3 if _type(out.dtype) == E4M3 else dt
+    xp, xs = _rows(x, shape, dt, op, "x")
+    rp, rs = _rows(res, shape, dt, op, "res")
+    sp, ss = _rows(sum, shape, dt, op, "sum")
+    op_, os_ = _rows(out, shape, odt, op, "out")
+    _need(weight.shape == (cols,) and _is_f32(weight.dtype) and (weight.stride()[0] == 1 or cols <= 1),
           f"{op}: weight is no f32 vector of {cols}")
-    a.weight = weight.data_ptr()
+    scale_ptr = 0
     if scales is not None:
-        _need(group >= 0, f"{op}: a negative group")
         n = -(-cols // group) if group else 1
-        _need(tuple(scales.shape) == (rows, n) and _is_f32(scales.dtype) and _contiguous(scales),
+        _need(scales.shape == (rows, n) and _is_f32(scales.dtype) and _contiguous(scales),
               f"{op}: scales is no contiguous f32 [{rows}][{n}]")
-        a.scales = scales.data_ptr()
-    check(load_library().s2s_rms_norm(C.byref(a), stream), op)
+        scale_ptr = scales.data_ptr()
+    args = _RMS.pack(dt, odt, rows, cols, xp, rp, sp, op_, xs, rs, ss, os_, weight.data_ptr(), weight_offset, eps, scale_ptr, group)
+    if load_library().s2s_rms_norm(args, stream):
+        raise S2SError(f"{op}: {last_error()}")
     return out

@@ -99,6 +99,11 @@ def scattered(g, c):
     return g.integers(-1, 4, (c["B"], c["Lq"])), g.integers(-1, 4, (c["B"], c["Lk"]))
 
 
+def scattered_blocks(g, c):
+    ids = np.repeat(g.integers(-1, 5, (c["B"], c["Lk"] // 50 + 1)), 50, 1)[:, :c["Lk"]]
+    return ids[:, :c["Lq"]], ids
+
+
 def far_apart(g, c):
     return np.full(c["Lq"], 3), np.full((c["B"], c["Lk"]), 5)
 
@@ -129,6 +134,11 @@ CASES = {
     "more_queries_than_keys": case("bf16", Lq=90, Lk=30, H=2, causal=True),
     "lengths": case("f16", B=5, Lq=33, Lk=70, H=2, q_lens=[0, 1, 33, 5, 40], k_lens=[70, 0, 1, -3, 64], causal=True),
     "documents": case("bf16", Lq=500, Lk=500, H=4, KV=2, docs=segments(130, 1, 64, 200)),
+    "documents_packed": case("bf16", Lq=2600, Lk=2600, H=2, KV=1, D=32, docs=segments(300, 900, 64, 1100, 200)),
+    "documents_backwards": case("f16", B=2, Lq=700, Lk=700, H=2, KV=1, D=64, docs=lambda g, c: (9 - np.arange(700) // 71, 9 - np.arange(700) // 71)),
+    "documents_lengths": case("f32", B=3, Lq=700, Lk=700, H=2, KV=2, D=32, docs=scattered_blocks, q_lens=[700, 1, 333], k_lens=[650, 700, 333]),
+    "rows_of_4_bytes": case("f16", B=2, Lq=40, Lk=150, H=2, KV=2, D=62, causal=True),
+    "rows_of_4_bytes_f32": case("f32", B=2, Lq=40, Lk=150, H=2, KV=1, D=97, causal=True, cap=20.0),
     "documents_causal": case("f16", Lq=300, Lk=300, H=2, KV=2, docs=segments(7, 100, 150), causal=True, slopes=True),
     "documents_scattered": case("f32", B=2, Lq=65, Lk=190, H=2, docs=scattered),
     "documents_empty": case("bf16", B=2, Lq=65, Lk=190, H=2, docs=far_apart),
@@ -150,6 +160,20 @@ CASES = {
 @pytest.mark.parametrize("name", CASES)
 def test_attention(pkg, name):
     check_attention(pkg, CASES[name])
+
+
+def test_attention_shared_rows(pkg):
+    """Strides of zero: one key and value row for all tokens, one batch entry for all."""
+    for dtype, Lk in (("bf16", 100), ("f32", 1), ("f16", 65)):
+        c = case(dtype, B=2, Lq=20, Lk=Lk, H=2, KV=2, D=64, causal=False)
+        q, k, v, more = inputs(c)
+        k[:], v[:] = k[:1, :1], v[:1, :1]
+        plan, ws, scale = make_plan(pkg, c)
+        want, bound, _ = R.attention(dtype, q, k, v, scale)
+        d, m = upload(pkg, c, q, k, v, more)
+        one = {n: pkg.ops.Array(d[n].array.ptr, (2, Lk, 2, 64), dtype, (0, 0, 64, 1)) for n in "kv"}
+        plan(d["q"].array, one["k"], one["v"], d["out"].array, workspace=ws.array)
+        assert (np.abs(d["out"].get() - want) <= bound).all()
 
 
 def masked_nan(c):

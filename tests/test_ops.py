@@ -124,6 +124,28 @@ def test_rms_norm_weight_refused(pkg):
         pkg.ops.rms_norm(arr(pkg, (4, 8), "f32"), arr(pkg, (9,), "f32"), arr(pkg, (4, 8), "f32", ptr=8192))
 
 
+@pytest.mark.parametrize("pack,name", [("_ATTENTION", "Attention_"), ("_ROTARY", "Rotary_"), ("_RMS", "RmsNorm_")])
+def test_argument_packs_are_the_c_structs(pkg, pack, name):
+    """The packs that the calls send are the C structs, field by field: distinct values packed
+    come back under the structs' names in order, nested ones flattened."""
+    import ctypes as C
+    packer, struct = getattr(pkg.ops, pack), getattr(pkg.abi, name)
+    assert packer.size == C.sizeof(struct)
+
+    def leaves(s):
+        for f, t in s._fields_:
+            v = getattr(s, f)
+            if isinstance(v, C.Structure):
+                yield from leaves(v)
+            elif isinstance(v, C._Pointer):
+                yield C.cast(v, C.c_void_p).value
+            else:
+                yield v
+    n = len(list(leaves(struct())))
+    data = packer.pack(*range(1, n + 1))
+    assert list(leaves(struct.from_buffer_copy(data))) == list(range(1, n + 1))
+
+
 def test_null_arguments_refused(pkg):
     lib = pkg.load_library()
     assert lib.s2s_attention_workspace(None, None) != 0 and b"null" in lib.s2s_last_error()
