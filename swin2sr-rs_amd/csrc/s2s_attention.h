@@ -100,7 +100,7 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = kAttnLog2e;
 
-enum { CAP = 1, SLOPES = 2, ANY = 4, GENERAL = 8 };
+enum { CAP = 1, SLOPES = 2, ANY = 4, DOCS = 8, GENERAL = 16 };
 
 template <typename T>
 struct Type;
@@ -304,15 +304,16 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 //  WK false: wave w has columns 16 NB w .. + 16 NB of the tile's 64 NB, all keys.
 //  WK true (at most 16 columns): every wave has all columns and a quarter of each
 //  key tile (one block of 16 keys of 64); the four sums meet in LDS at the end.
-//  MODE: CAP and SLOPES are known (0 to 3), or asked for in every tile (ANY), or these and
-//  what AttnScore::general stands for (GENERAL). Paths that a kernel might take and
-//  does not cost it registers, spilled around its loop, and copies where they meet.
+//  MODE: CAP and SLOPES are known (0 to 3), or asked for in every tile (ANY); documents
+//  (DOCS); or all of these and what AttnScore::general stands for (GENERAL). Paths that a
+//  kernel might take and does not cost it registers, spilled around its loop, and copies
+//  where they meet.
 // K and V tiles of TK keys are copied straight into LDS, two buffers each, the
 // next tile in flight while one is computed. ALIGN: bytes of one copy by the DMA
 // (16, or 4 for rows of 4-byte multiples), or 0: through registers, by elements.
 template <typename T, int DP, int NB, bool WK, int ALIGN, int MODE>
 struct Kernel {
-    static constexpr bool GEN = MODE == GENERAL;
+    static constexpr bool GEN = MODE == GENERAL, DOC = GEN || (MODE & DOCS), KNOWN = MODE < ANY;
     typedef Type<T> Ty;
     typedef typename Ty::V Vec;
     static constexpr bool F32 = sizeof(T) == 4;
@@ -369,11 +370,9 @@ struct Kernel {
             const int c = wc0 + nb * 16 + n16, i = L.by_group.of(c), h = kvh * a.group + (c - i * a.group);
             const bool ok = i < ql;
             lim[nb] = ok ? limit(i) : 0;
+            // (a column of no document computes what it may, and is zeroed at the end)
             doc[nb] = 0;
-            if (a.q_docs && ok) {
-                doc[nb] = a.q_docs[b * a.q_docs_b + i];
-                if (doc[nb] < 0) lim[nb] = 0;
-            }
+            if (DOC && a.q_docs && ok) doc[nb] = a.q_docs[b * a.q_docs_b + i];
             at[nb] = a.q_pos && ok ? a.q_pos[b * a.q_pos_b + i] : kl - ql + i;
             slope[nb] = a.slopes && ok ? a.slopes[h] * kLog2e : 0.f;
             tab[nb] = ok ? h * a.table_size : 0;
@@ -395,11 +394,24 @@ struct Kernel {
         const int w_first = min(ql - 1, L.by_group.of(wc0)), w_last = min(ql - 1, L.by_group.of(wc0 + 16 * NB - 1));
         const bool w_any = wc0 < ql * a.group;
         const int w_max = w_any ? limit(w_last) : 0, w_min = limit(w_first);
-        // documents of the workgroup's columns, where key tiles can be passed over
-        int q_lo = 0, q_hi = 0, q_min = 0;
-        if (L.meta) {
+        // documents of the workgroup's columns and of the wave's, where key tiles can be passed
+        // over
+        int q_lo = 0, q_hi = 0, w_lo = 0, w_hi = 0;
+        const bool summary = DOC && L.meta;
+        if (summary) {
             const int4 x = L.col_docs[b * L.tiles + ct];
-            q_lo = x.x, q_hi = x.y, q_min = x.z;
+            q_lo = x.x, q_hi = x.y;
+            w_lo = 0x7fffffff, w_hi = -1;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+                if (lim[nb] > 0 && doc[nb] >= 0) w_lo = min(w_lo, doc[nb]), w_hi = max(w_hi, doc[nb]);
+#pragma unroll
+            for (int m = 1; m < 16; m *= 2) {
+                w_lo = min(w_lo, __shfl_xor(w_lo, m));
+                w_hi = max(w_hi, __shfl_xor(w_hi, m));
+            }
+            w_lo = __builtin_amdgcn_readfirstlane(w_lo);
+            w_hi = __builtin_amdgcn_readfirstlane(w_hi);
         }
         const int nt = q_hi < 0 ? 0 : (wg_max + TK - 1) / TK;
         const int per = L.splits == 1 ? nt : (nt + L.splits - 1) / L.splits;
@@ -410,7 +422,7 @@ struct Kernel {
         unsigned long long live = 0, whole = 0;
         int live_at = -64;
         auto next = [&](int t) {
-            if (!L.meta) return t;
+            if (!summary) return t;
             while (t < t_end) {
                 if (t >= live_at + 64) {
                     live_at = t;
@@ -419,7 +431,7 @@ struct Kernel {
                     if (m < t_end) {
                         const int4 x = L.meta[(long long)b * L.meta_tiles + m];
                         l = x.x <= q_hi && x.y >= q_lo;
-                        w = x.z == x.y && q_min == q_hi && x.y == q_hi;
+                        w = x.z == x.y && q_lo == q_hi && x.y == q_hi;
                     }
                     live = __ballot(l);
                     whole = __ballot(w);
@@ -506,7 +518,7 @@ struct Kernel {
                            (F32 ? (n16 & 3) * 4 : (n16 & 1) * 8);
 
         Uniform u;
-        u.k_docs = a.k_docs ? a.k_docs + b * a.k_docs_b : nullptr;
+        u.k_docs = DOC && a.k_docs ? a.k_docs + b * a.k_docs_b : nullptr;
         u.k_pos = GEN && a.k_pos ? a.k_pos + b * a.k_pos_b : nullptr;
         u.table = GEN ? a.table : nullptr;
         u.half = a.table_size >> 1;
@@ -516,16 +528,36 @@ struct Kernel {
         u.general = GEN && L.score.general;
         u.sc = L.score;
 
+        // what is read per key, a lane each, and the tile's documents are read a tile ahead,
+        // by vector loads: a scalar load in flight would be waited for with the LDS reads, a
+        // vector load among the copies with the copies
+        int kdoc = -1, kdoc_next = -1;
+        int4 docs_next = {0, 0, 0, 0};
+        int zero = 0;
+        if (DOC) asm volatile("" : "+v"(zero));
+        auto fetch = [&](int t) {
+            if (DOC && u.k_docs) kdoc_next = u.k_docs[min(t * TK + (WK ? 16 * wave : 0) + min(lane, 16 * KB - 1), kl - 1)];
+            if (summary) docs_next = L.meta[(long long)b * L.meta_tiles + t + zero];
+        };
+
         int t = next(split * per), buf = 0;
         kp += (long long)t * kstep, vp += (long long)t * vstep;
-        if (t < t_end) stage(t, 0);
+        if (t < t_end) fetch(t), stage(t, 0);
         while (t < t_end) {
-            const bool one_doc = !a.q_docs || (L.meta && ((whole >> (t - live_at)) & 1));
+            const bool one_doc = !DOC || !u.k_docs || (summary && ((whole >> (t - live_at)) & 1));
             const int tn = next(t + 1);
             if constexpr (ALIGN > 0) WAIT_VMCNT(0);
             lds_sync();
+            bool mine = true, same = one_doc;  // whether the wave's columns have keys here, and all of one document
+            if (DOC) kdoc = kdoc_next;
+            if (summary) {
+                const int lo = __builtin_amdgcn_readfirstlane(docs_next.x), hi = __builtin_amdgcn_readfirstlane(docs_next.y),
+                          all = __builtin_amdgcn_readfirstlane(docs_next.z);
+                mine = lo <= w_hi && hi >= w_lo;
+                same = all == hi && w_lo == w_hi && hi == w_hi;
+            }
             kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
-            if (tn < t_end) stage(tn, buf ^ 1);
+            if (tn < t_end) fetch(tn), stage(tn, buf ^ 1);
             const int at_buf = buf * 2 * (int)kTile;
             if (!(t * TK + TK <= wg_min && one_doc) || (GEN && u.table)) {
                 // a masked key's weight is zero, and zero times an infinity is none: with
@@ -544,16 +576,23 @@ struct Kernel {
                 }
             }
             const int j0 = t * TK + (WK ? 16 * wave : 0);  // the wave's first key
-            if (j0 < w_max) {
-                const bool full = j0 + 16 * KB <= w_min && one_doc && !(GEN && u.table);
-                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, lim, doc, at, slope, tab, qf, o, m, l);
+            if (j0 < w_max && mine) {
+                const bool full = j0 + 16 * KB <= w_min && same && !(GEN && u.table);
+                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, kdoc, lim, doc, at, slope, tab, qf, o, m, l);
             }
             t = tn;
             buf ^= 1;
         }
 
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) l[nb] = col_sum(l[nb]);
+        for (int nb = 0; nb < NB; ++nb) {
+            l[nb] = col_sum(l[nb]);
+            if (DOC && doc[nb] < 0) {  // no document: no keys
+                m[nb] = -INFINITY, l[nb] = 0.f;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) o[db][nb] = f4v{0.f, 0.f, 0.f, 0.f};
+            }
+        }
         if constexpr (WK) {
             // the four waves' sums, rescaled to their largest reference
             __syncthreads();
@@ -653,7 +692,7 @@ struct Kernel {
 
     // The wave's keys of one tile: scores, softmax step, products with V.
     static __device__ __forceinline__ void tile(const Uniform &u, const lds_t *kl0, const lds_t *vl0, int j0,
-                                                bool full, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
+                                                bool full, int kdoc, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
                                                 const Vec (*qf)[KS], f4v (*o)[NB], float *m, float *l) {
         const int lane = threadIdx.x & 63, q = lane >> 4;
         // a lane per key for what is read per key
@@ -692,7 +731,7 @@ struct Kernel {
         // bias made it powers of two already
         const AttnScore &sc = u.sc;
         float unit = sc.c1;
-        if (MODE < ANY ? (MODE & CAP) != 0 : u.capped) {
+        if (KNOWN ? (MODE & CAP) != 0 : u.capped) {
             float big = 0.f;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
@@ -751,7 +790,7 @@ struct Kernel {
                         s[kb][nb][i] = x < -1e30f && x != -INFINITY ? -1e30f : x;
                     }
             unit = 1.f;
-        } else if (MODE < ANY ? (MODE & SLOPES) != 0 : u.slopes) {
+        } else if (KNOWN ? (MODE & SLOPES) != 0 : u.slopes) {
             // distances of neighbours differ by what the register says
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -774,8 +813,7 @@ struct Kernel {
                     for (int i = 0; i < 4; ++i)
                         if (16 * kb + i >= n) s[kb][nb][i] = -INFINITY;
             }
-            if (u.k_docs) {
-                const int kdoc = u.k_docs[jl];
+            if (DOC && u.k_docs) {
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -888,7 +926,7 @@ struct Kernel {
             const int r = (WK ? 16 * wave : 0) + jr;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                bool ok = j < lim[nb] && (!u.k_docs || u.k_docs[j] == doc[nb]);
+                bool ok = j < lim[nb] && (!DOC || !u.k_docs || (u.k_docs[j] == doc[nb] && doc[nb] >= 0));
                 if (GEN && ok && u.table) ok = entry(u, tab[nb], at[nb] - (u.k_pos ? u.k_pos[j] : j)) != -INFINITY;
                 if (!ok) continue;
 #pragma unroll
@@ -991,7 +1029,8 @@ template <typename T, int DP, bool WK>
 hipError_t launch_narrow(const AttnOpArgs &a, const AttnLaunch &L, int align, hipStream_t st) {
     if (align == 0) return launch<T, DP, 1, WK, 0, GENERAL>(a, L, st);
     if (align < 16) return launch<T, DP, 1, WK, 4, GENERAL>(a, L, st);
-    return L.score.general ? launch<T, DP, 1, WK, 16, GENERAL>(a, L, st) : launch<T, DP, 1, WK, 16, ANY>(a, L, st);
+    if (L.score.general) return launch<T, DP, 1, WK, 16, GENERAL>(a, L, st);
+    return a.k_docs ? launch<T, DP, 1, WK, 16, ANY | DOCS>(a, L, st) : launch<T, DP, 1, WK, 16, ANY>(a, L, st);
 }
 
 template <typename T, int DP>
@@ -1001,6 +1040,8 @@ hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, 
         e = launch_narrow<T, DP, true>(a, L, align, st);
     else if (c.nb == 1)
         e = launch_narrow<T, DP, false>(a, L, align, st);
+    else if (a.k_docs)
+        e = launch<T, DP, 2, false, 16, ANY | DOCS>(a, L, st);
     else if (a.cap > 0.f)
         e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES>(a, L, st) : launch<T, DP, 2, false, 16, CAP>(a, L, st);
     else
