@@ -156,7 +156,11 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
     L.out_vec = aligned_bytes(a.out, a.so, a.width, size) >= 4 * size;
     // (rows that overlap have no end that the copies' resource could tell: by elements)
     const int align = a.sk.t < a.width || a.sv.t < a.width ? 0 : al >= 16 ? 16 : al >= 4 ? 4 : 0;
-    const attn::Cut c = cut_of(dtype, a, align < 16 || L.score.general);
+    // Packed documents of narrow heads too: the fewer columns a workgroup has, the fewer lie
+    // across two documents and mask both's tiles (nine images, 11003 tokens, 12 heads: 64
+    // wide 153 us with waves of 32 and 127 with 16, 32 wide 132 and 105; 128 wide, 32 / 8
+    // heads, where a wave of 16 reads LDS twice as often for its products, 369 and 483).
+    const attn::Cut c = cut_of(dtype, a, align < 16 || L.score.general || (a.k_docs && a.width <= 64));
     L.cols = a.group * a.nq;
     L.tiles = c.tiles;
     L.splits = c.splits;
