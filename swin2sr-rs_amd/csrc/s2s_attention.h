@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "s2s_device.h"
 #include "s2s_kernels.h"
@@ -34,6 +35,11 @@ struct AttnScore {
     // fused operations where the exponential takes two transcendentals, and no
     // cancellation near zero. poly_max: the |x| that it holds for.
     float p0, p1, p2, p3, poly_max;
+    // A cap bounds the scores: with no bias and a type of f32's range, e^(s - ref) at one
+    // reference 2^20 below the cap's lies in 2^-125 to 2^20 for every score that a cap up to
+    // 50.2 leaves, and no maximum is looked for.
+    bool fixed;
+    float ref;
     bool general;  // a bias other than slopes by token distance
     void set(const AttnOpArgs &a) {
         // a negative or zero scale would turn masked minus infinities round: scores in
@@ -41,6 +47,8 @@ struct AttnScore {
         general = a.table || a.k_pos || (!(a.cap > 0.f) && !(a.scale > 1e-30f));
         c1 = a.scale * kAttnLog2e;
         capl = a.cap * kAttnLog2e;
+        fixed = a.cap > 0.f && !a.slopes && !a.table && 2.f * capl - 20.f <= 125.f;
+        ref = fixed ? capl - 20.f : 0.f;
         p0 = p1 = p2 = p3 = 0.f;
         poly_max = -1.f;
         if (a.cap > 0.f) {
@@ -100,7 +108,7 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = kAttnLog2e;
 
-enum { CAP = 1, SLOPES = 2, ANY = 4, DOCS = 8, GENERAL = 16 };
+enum { CAP = 1, SLOPES = 2, ANY = 8, DOCS = 16, GENERAL = 32, FIXED = 4 };
 
 template <typename T>
 struct Type;
@@ -305,7 +313,7 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 //  WK true (at most 16 columns): every wave has all columns and a quarter of each
 //  key tile (one block of 16 keys of 64); the four sums meet in LDS at the end.
 //  MODE: CAP and SLOPES are known (0 to 3), or asked for in every tile (ANY); documents
-//  (DOCS); or all of these and what AttnScore::general stands for (GENERAL). Paths that a
+//  (DOCS); a fixed reference of the softmax (FIXED, see AttnScore); or all but that and what AttnScore::general stands for (GENERAL). Paths that a
 //  kernel might take and does not cost it registers, spilled around its loop, and copies
 //  where they meet.
 // K and V tiles of TK keys are copied straight into LDS, two buffers each, the
@@ -394,6 +402,7 @@ struct Kernel {
         const int w_first = min(ql - 1, L.by_group.of(wc0)), w_last = min(ql - 1, L.by_group.of(wc0 + 16 * NB - 1));
         const bool w_any = wc0 < ql * a.group;
         const int w_max = w_any ? limit(w_last) : 0, w_min = limit(w_first);
+        const int w_at = kl - ql + w_first;  // the first place among the wave's queries
         // documents of the workgroup's columns and of the wave's, where key tiles can be passed
         // over
         int q_lo = 0, q_hi = 0, w_lo = 0, w_hi = 0;
@@ -499,12 +508,16 @@ struct Kernel {
             }
         };
 
+        // the sums of the weights: f32 per lane and key, over the lanes at the end; 16-bit types by
+        // the matrix cores, of the rounded weights (a product with ones, half the additions' time)
+        typedef typename std::conditional<F32, float, f4v>::type Sum;
         f4v o[DB][NB];
-        float m[NB], l[NB];
+        float m[NB];
+        Sum l[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            m[nb] = -INFINITY;
-            l[nb] = 0.f;
+            m[nb] = MODE & FIXED ? L.score.ref : -INFINITY;
+            l[nb] = Sum{};
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db][nb] = f4v{0.f, 0.f, 0.f, 0.f};
         }
@@ -578,17 +591,19 @@ struct Kernel {
             const int j0 = t * TK + (WK ? 16 * wave : 0);  // the wave's first key
             if (j0 < w_max && mine) {
                 const bool full = j0 + 16 * KB <= w_min && same && !(GEN && u.table);
-                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, kdoc, lim, doc, at, slope, tab, qf, o, m, l);
+                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, j0 + 16 * KB <= w_at + 1, kdoc, lim, doc, at, slope, tab, qf, o, m, l);
             }
             t = tn;
             buf ^= 1;
         }
 
+        float total[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            l[nb] = col_sum(l[nb]);
+            if constexpr (F32) total[nb] = col_sum(l[nb]);
+            else total[nb] = l[nb][0];
             if (DOC && doc[nb] < 0) {  // no document: no keys
-                m[nb] = -INFINITY, l[nb] = 0.f;
+                m[nb] = -INFINITY, total[nb] = 0.f;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) o[db][nb] = f4v{0.f, 0.f, 0.f, 0.f};
             }
@@ -600,7 +615,7 @@ struct Kernel {
             float *mine = jo + n16 * (DP + 4);
 #pragma unroll
             for (int db = 0; db < DB; ++db) *(f4v *)(mine + db * 16 + 4 * q) = o[db][0];
-            if (q == 0) mine[DP] = m[0], mine[DP + 1] = l[0];
+            if (q == 0) mine[DP] = m[0], mine[DP + 1] = total[0];
             __syncthreads();
             float top = -INFINITY;
 #pragma unroll
@@ -615,7 +630,7 @@ struct Kernel {
                 ls += p[1] == 0.f ? 0.f : f[w] * p[1];
             }
             m[0] = top;
-            l[0] = ls;
+            total[0] = ls;
             // wave w finishes channel blocks w, w + 4, ...
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
@@ -639,14 +654,14 @@ struct Kernel {
             if (splits > 1) {
                 const long long row = ((long long)bh * splits + split) * late->L.cols + c;
                 float *po = late->L.part_o + row * DP, *ml = late->L.part_ml + 2 * row;
-                if (q == 0 && (!WK || wave == 0)) ml[0] = m[nb], ml[1] = l[nb];
+                if (q == 0 && (!WK || wave == 0)) ml[0] = m[nb], ml[1] = total[nb];
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
                     if (!WK || (db & 3) == wave) *(f4v *)(po + db * 16 + 4 * q) = o[db][nb];
             } else {
                 const int h = kvh * group + (c - i * group);
                 T *row = (T *)late->a.out + b * late->a.so.b + (long long)i * late->a.so.t + h * late->a.so.h;
-                const float r = l[nb] == 0.f ? 0.f : 1.f / l[nb];
+                const float r = total[nb] == 0.f ? 0.f : 1.f / total[nb];
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
                     if (WK && (db & 3) != wave) continue;
@@ -692,24 +707,37 @@ struct Kernel {
 
     // The wave's keys of one tile: scores, softmax step, products with V.
     static __device__ __forceinline__ void tile(const Uniform &u, const lds_t *kl0, const lds_t *vl0, int j0,
-                                                bool full, int kdoc, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
-                                                const Vec (*qf)[KS], f4v (*o)[NB], float *m, float *l) {
+                                                bool full, bool behind, int kdoc, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
+                                                const Vec (*qf)[KS], f4v (*o)[NB], float *m,
+                                                typename std::conditional<F32, float, f4v>::type *l) {
         const int lane = threadIdx.x & 63, q = lane >> 4;
         // a lane per key for what is read per key
         const int jl = min(j0 + min(lane, 16 * KB - 1), u.kl - 1);
         // the table's entries on their way while the scores are made
-        int kpos = 0;
         float bias[GEN ? KB : 1][4][GEN ? NB : 1];
-        if (GEN && u.table) {
-            if (u.k_pos) kpos = u.k_pos[jl];
+        int place[GEN ? KB : 1][4];
+        if (GEN && u.general) {
+            if (u.k_pos) {
+                const int mine = u.k_pos[jl];
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+                for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int jr = 16 * kb + 4 * q + i, kp = u.k_pos ? __shfl(kpos, jr) : j0 + jr;
+                    for (int i = 0; i < 4; ++i) place[GEN ? kb : 0][i] = __shfl(mine, 16 * kb + 4 * q + i);
+            } else {
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) bias[GEN ? kb : 0][i][GEN ? nb : 0] = entry(u, tab[nb], at[nb] - kp);
-                }
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) place[GEN ? kb : 0][i] = j0 + 16 * kb + 4 * q + i;
+            }
+            if (u.table) {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                            bias[GEN ? kb : 0][i][GEN ? nb : 0] = entry(u, tab[nb], at[nb] - place[GEN ? kb : 0][i]);
+            }
         }
         f4v s[KB][NB];
 #pragma unroll
@@ -749,7 +777,7 @@ struct Kernel {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float e = __builtin_amdgcn_exp2f(s[kb][nb][i] * sc.c1);
-                            s[kb][nb][i] = fmaf(-2.f * sc.capl, __builtin_amdgcn_rcpf(e + 1.f), sc.capl);
+                            s[kb][nb][i] = fmaf(-2.f * sc.capl, __builtin_amdgcn_rcpf(e + 1.f), MODE & FIXED ? sc.capl - sc.ref : sc.capl);
                         }
             } else {
 #pragma unroll
@@ -759,47 +787,63 @@ struct Kernel {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float x = s[kb][nb][i], w = x * x;
-                            s[kb][nb][i] = x * fmaf(w, fmaf(w, fmaf(w, sc.p3, sc.p2), sc.p1), sc.p0);
+                            const float p = fmaf(w, fmaf(w, fmaf(w, sc.p3, sc.p2), sc.p1), sc.p0);
+                            s[kb][nb][i] = MODE & FIXED ? fmaf(x, p, -sc.ref) : x * p;
                         }
             }
             unit = 1.f;
         }
         if (GEN && u.general) {
-            if (u.slopes) {
-                if (u.k_pos && !u.table) kpos = u.k_pos[jl];
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int jr = 16 * kb + 4 * q + i, kp = u.k_pos ? __shfl(kpos, jr) : j0 + jr;
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
-                            s[kb][nb][i] = fmaf(-slope[nb], fabsf((float)(at[nb] - kp)), s[kb][nb][i] * unit);
-                    }
-                unit = 1.f;
-            }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        float x = s[kb][nb][i] * unit;
-                        if (u.table) x = add_bias(x, bias[GEN ? kb : 0][i][GEN ? nb : 0]);
-                        // lowest values stay numbers, so that a row of them is even
-                        s[kb][nb][i] = x < -1e30f && x != -INFINITY ? -1e30f : x;
-                    }
-            unit = 1.f;
-        } else if (KNOWN ? (MODE & SLOPES) != 0 : u.slopes) {
-            // distances of neighbours differ by what the register says
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const float d0 = (float)(at[nb] - j0 - 4 * q);
+                    for (int nb = 0; nb < NB; ++nb) s[kb][nb][i] *= unit;
+            if (u.slopes) {
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        s[kb][nb][i] = fmaf(-slope[nb], fabsf(d0 - (float)(16 * kb + i)), s[kb][nb][i] * unit);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                            s[kb][nb][i] = fmaf(-slope[nb], fabsf((float)(at[nb] - place[GEN ? kb : 0][i])), s[kb][nb][i]);
+            }
+            if (u.table) {
+                // a bias of minus infinity takes the key out; lower values than -1e30 count as
+                // that, so that a row of nothing but the type's lowest is even
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const float t = bias[GEN ? kb : 0][i][GEN ? nb : 0];
+                            const float x = __builtin_elementwise_maximum(fmaf(t, kLog2e, s[kb][nb][i]), -1e30f);
+                            s[kb][nb][i] = t == -INFINITY ? -INFINITY : x;
+                        }
+            }
+            unit = 1.f;
+        } else if (KNOWN ? (MODE & SLOPES) != 0 : u.slopes) {
+            // distances of neighbours differ by what the register says; keys that all lie
+            // behind the wave's queries, as under the causal mask, need no absolute value
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const float d0 = (float)(at[nb] - j0 - 4 * q);
+                if (behind) {
+                    const float b0 = -slope[nb] * d0;
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[kb][nb][i] = fmaf(s[kb][nb][i], unit, fmaf(slope[nb], (float)(16 * kb + i), b0));
+                } else {
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[kb][nb][i] = fmaf(s[kb][nb][i], unit, -slope[nb] * fabsf(d0 - (float)(16 * kb + i)));
+                }
             }
             unit = 1.f;
         }
@@ -826,26 +870,28 @@ struct Kernel {
             }
         }
         // the running reference: rescaled only where a score passes it by 2^kLazy
-        float top[NB];
-        bool grow = false;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            float x = s[0][nb][0];
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) x = max3(max3(x, s[kb][nb][0], s[kb][nb][1]), s[kb][nb][2], s[kb][nb][3]);
-            top[nb] = col_max(x) * unit;
-            grow |= top[nb] > m[nb] + Ty::kLazy;
-        }
-        if (__any(grow)) {
+        if constexpr (!(MODE & FIXED)) {
+            float top[NB];
+            bool grow = false;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                const float mn = fmaxf(m[nb], top[nb]);
-                // (no reference yet: sums of zero, or infinities of v that stay)
-                const float f = m[nb] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nb] - mn);
-                m[nb] = mn;
-                l[nb] *= f;
+                float x = s[0][nb][0];
 #pragma unroll
-                for (int db = 0; db < DB; ++db) o[db][nb] *= f;
+                for (int kb = 0; kb < KB; ++kb) x = max3(max3(x, s[kb][nb][0], s[kb][nb][1]), s[kb][nb][2], s[kb][nb][3]);
+                top[nb] = col_max(x) * unit;
+                grow |= top[nb] > m[nb] + Ty::kLazy;
+            }
+            if (__any(grow)) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const float mn = fmaxf(m[nb], top[nb]);
+                    // (no reference yet: sums of zero, or infinities of v that stay)
+                    const float f = m[nb] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nb] - mn);
+                    m[nb] = mn;
+                    l[nb] *= f;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) o[db][nb] *= f;
+                }
             }
         }
 #pragma unroll
@@ -856,25 +902,21 @@ struct Kernel {
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(s[kb][nb][i], unit, ref));
+                    const float p = __builtin_amdgcn_exp2f(MODE & FIXED ? s[kb][nb][i] : fmaf(s[kb][nb][i], unit, ref));
                     s[kb][nb][i] = p;
-                    sum[i] += p;
+                    if (F32) sum[i] += p;
                 }
-            l[nb] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if constexpr (F32) l[nb] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
-        products(vl0, s, o);
+        products(vl0, s, o, l);
     }
 
     static __device__ __forceinline__ float entry(const Uniform &u, int tab, int dist) {
         return u.table[tab + min(max(dist, -u.half), u.half) + u.half];
     }
-    // bias in powers of two; minus infinity takes the key out whatever its score
-    static __device__ __forceinline__ float add_bias(float x, float bias) {
-        return bias == -INFINITY ? -INFINITY : fmaxf(bias, -2e38f) * kLog2e + x;
-    }
-
     // O^T += V^T P^T
-    static __device__ __forceinline__ void products(const lds_t *vl0, const f4v (*s)[NB], f4v (*o)[NB]) {
+    static __device__ __forceinline__ void products(const lds_t *vl0, const f4v (*s)[NB], f4v (*o)[NB],
+                                                    typename std::conditional<F32, float, f4v>::type *l) {
         constexpr int J = F32 || WK ? KB : KB / 2;
         Vec p[J][NB];
 #pragma unroll
@@ -890,6 +932,15 @@ struct Kernel {
                     }
                 }
             }
+        if constexpr (!F32) {
+            Vec ones;
+#pragma unroll
+            for (int e = 0; e < E; ++e) ones[e] = (T)1.f;
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) l[nb] = mma(ones, p[j][nb], l[nb]);
+        }
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -1033,6 +1084,13 @@ hipError_t launch_narrow(const AttnOpArgs &a, const AttnLaunch &L, int align, hi
     return a.k_docs ? launch<T, DP, 1, WK, 16, ANY | DOCS>(a, L, st) : launch<T, DP, 1, WK, 16, ANY>(a, L, st);
 }
 
+// (f16 has not the range of a fixed reference)
+template <typename T, int DP>
+hipError_t launch_fixed(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
+    if constexpr (std::is_same<T, half_t>::value) return hipErrorInvalidValue;
+    else return launch<T, DP, 2, false, 16, CAP | FIXED>(a, L, st);
+}
+
 template <typename T, int DP>
 hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, int align, hipStream_t st) {
     hipError_t e;
@@ -1043,7 +1101,10 @@ hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, 
     else if (a.k_docs)
         e = launch<T, DP, 2, false, 16, ANY | DOCS>(a, L, st);
     else if (a.cap > 0.f)
-        e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES>(a, L, st) : launch<T, DP, 2, false, 16, CAP>(a, L, st);
+        e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES>(a, L, st)
+            : std::is_same<T, half_t>::value ? launch<T, DP, 2, false, 16, CAP>(a, L, st)
+            : L.score.fixed ? launch_fixed<T, DP>(a, L, st)
+                            : launch<T, DP, 2, false, 16, CAP>(a, L, st);
     else
         e = a.slopes ? launch<T, DP, 2, false, 16, SLOPES>(a, L, st) : launch<T, DP, 2, false, 16, 0>(a, L, st);
     if (e != hipSuccess || L.splits == 1) return e;

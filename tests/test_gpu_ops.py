@@ -157,6 +157,28 @@ CASES = {
 }
 
 
+# enough (batch entry, key head) pairs for the waves of 32 columns, in every kernel of theirs
+WIDE = dict(B=43, H=12, KV=12, Lq=70, Lk=90)
+CASES.update({
+    "wide_bf16": case("bf16", D=128, **WIDE),
+    "wide_causal_f16": case("f16", D=64, causal=True, **WIDE),
+    "wide_f32": case("f32", D=64, causal=True, **WIDE),
+    "wide_cap_bf16": case("bf16", D=128, causal=True, cap=50.0, spread=4.0, **WIDE),
+    "wide_cap_saturated_bf16": case("bf16", D=32, cap=50.0, spread=40.0, **WIDE),
+    "wide_cap_f32": case("f32", D=96, causal=True, cap=30.0, spread=8.0, **WIDE),
+    "wide_cap_running_bf16": case("bf16", D=64, causal=True, cap=80.0, spread=20.0, **WIDE),
+    "wide_cap_f16": case("f16", D=128, causal=True, cap=50.0, spread=10.0, **WIDE),
+    "wide_slopes_bf16": case("bf16", D=96, slopes=True, **WIDE),
+    "wide_slopes_causal_f16": case("f16", D=128, slopes=True, causal=True, **WIDE),
+    "wide_slopes_f32": case("f32", D=128, slopes=True, causal=True, **WIDE),
+    "wide_cap_slopes_bf16": case("bf16", D=64, slopes=True, causal=True, cap=50.0, **WIDE),
+    "wide_docs_bf16": case("bf16", D=128, docs=scattered, causal=True, cap=50.0, slopes=True, **WIDE),
+    "wide_docs_f32": case("f32", D=96, docs=scattered, **WIDE),
+    "wide_lengths_bf16": case("bf16", D=128, causal=True, cap=50.0, k_lens=[(7 * i) % 91 for i in range(43)],
+                              q_lens=[(5 * i) % 71 for i in range(43)], **WIDE),
+})
+
+
 @pytest.mark.parametrize("name", CASES)
 def test_attention(pkg, name):
     check_attention(pkg, CASES[name])
