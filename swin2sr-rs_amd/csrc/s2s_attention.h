@@ -96,6 +96,7 @@ struct AttnLaunch {
     int meta_tiles;
     const int4 *col_docs;  // [batch][tiles] the same of a column tile's queries, and its key tiles
     const int *order;      // [batch][tiles] column tiles with the most key tiles first, or null
+    int table_lds;  // the group's rows of the table fit LDS
     FastDiv by_pairs, by_tiles, by_hk, by_group;
     AttnScore score;
 };
@@ -105,6 +106,7 @@ namespace attn {
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
+typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = kAttnLog2e;
 
@@ -337,15 +339,19 @@ struct Kernel {
     static constexpr int UNIT = ALIGN ? ALIGN : 16, SUB = 16 / UNIT;  // the copies' units, per chunk
     static constexpr size_t kTile = (size_t)TK * CH * 16;
     static constexpr size_t kJoin = WK ? (size_t)4 * 16 * (DP + 4) * 4 : 0;
-    static constexpr size_t kLds = (4 * kTile > kJoin ? 4 * kTile : kJoin) + 16;  // (and four flags)
+    // two buffers of K and V (the join's sums afterwards), two of the keys' documents and
+    // places, four flags, and the table's rows
+    static constexpr int kIds = (int)(4 * kTile > kJoin ? 4 * kTile : kJoin), kPos = kIds + 512, kFlag = kPos + 512, kTab = kFlag + 16;
+    static constexpr int kTabEntries = 2048;
 
     // What a tile needs that is the same for all of the workgroup.
     struct Uniform {
         const int *k_docs, *k_pos;  // of this batch entry, or null
         const float *table;
         int half;  // the table's middle
+        const lds_t *tab0;  // the group's rows, in LDS
         int kl;
-        bool capped, slopes, general;
+        bool capped, slopes, general, table_lds;
         AttnScore sc;
     };
 
@@ -383,7 +389,7 @@ struct Kernel {
             if (DOC && a.q_docs && ok) doc[nb] = a.q_docs[b * a.q_docs_b + i];
             at[nb] = a.q_pos && ok ? a.q_pos[b * a.q_pos_b + i] : kl - ql + i;
             slope[nb] = a.slopes && ok ? a.slopes[h] * kLog2e : 0.f;
-            tab[nb] = ok ? h * a.table_size : 0;
+            tab[nb] = ok ? (L.table_lds ? c - i * a.group : h) * a.table_size : 0;
             const T *row = (const T *)a.q + b * a.sq.b + (long long)(ok ? i : 0) * a.sq.t + h * a.sq.h;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -429,7 +435,7 @@ struct Kernel {
         // the next tile from t on that holds a key some column's document has, and
         // whether all its keys and the columns are of one document
         unsigned long long live = 0, whole = 0;
-        int live_at = -64;
+        int live_at = -64, t_lo = 0, t_hi = 0, t_all = 0;
         auto next = [&](int t) {
             if (!summary) return t;
             while (t < t_end) {
@@ -439,6 +445,7 @@ struct Kernel {
                     bool l = false, w = false;
                     if (m < t_end) {
                         const int4 x = L.meta[(long long)b * L.meta_tiles + m];
+                        t_lo = x.x, t_hi = x.y, t_all = x.z;
                         l = x.x <= q_hi && x.y >= q_lo;
                         w = x.z == x.y && q_lo == q_hi && x.y == q_hi;
                     }
@@ -470,8 +477,14 @@ struct Kernel {
             voff[p] = vc < a.width ? (r * vst + vc) * (int)sizeof(T) : 0x60000000;
         }
         const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(const lds_t *)lds);
+        const int *doc_keys = DOC && a.k_docs ? a.k_docs + b * a.k_docs_b : nullptr;
+        const int *pos_keys = GEN && a.k_pos ? a.k_pos + b * a.k_pos_b : nullptr;
         auto stage = [&](int t, int buf) {
             const int left = min(kl - t * TK, TK);
+            if (DOC && doc_keys && wave == 0)
+                tile_dma<4>(tile_rsrc(doc_keys + t * TK, left * 4), lds0 + kIds + buf * 256, lane * 4);
+            if (GEN && pos_keys && wave == 1)
+                tile_dma<4>(tile_rsrc(pos_keys + t * TK, left * 4), lds0 + kPos + buf * 256, lane * 4);
             if constexpr (ALIGN > 0) {
                 const v4u kr = tile_rsrc(kp, ((left - 1) * kst + a.width) * (int)sizeof(T)),
                           vr = tile_rsrc(vp, ((left - 1) * vst + a.width) * (int)sizeof(T));
@@ -531,53 +544,59 @@ struct Kernel {
                            (F32 ? (n16 & 3) * 4 : (n16 & 1) * 8);
 
         Uniform u;
-        u.k_docs = DOC && a.k_docs ? a.k_docs + b * a.k_docs_b : nullptr;
-        u.k_pos = GEN && a.k_pos ? a.k_pos + b * a.k_pos_b : nullptr;
+        u.k_docs = doc_keys;
+        u.k_pos = pos_keys;
         u.table = GEN ? a.table : nullptr;
         u.half = a.table_size >> 1;
         u.kl = kl;
         u.capped = a.cap > 0.f;
         u.slopes = a.slopes != nullptr;
         u.general = GEN && L.score.general;
+        u.table_lds = GEN && L.table_lds;
+        u.tab0 = base + kTab;
         u.sc = L.score;
 
-        // what is read per key, a lane each, and the tile's documents are read a tile ahead,
-        // by vector loads: a scalar load in flight would be waited for with the LDS reads, a
-        // vector load among the copies with the copies
-        int kdoc = -1, kdoc_next = -1;
-        int4 docs_next = {0, 0, 0, 0};
-        int zero = 0;
-        if (DOC) asm volatile("" : "+v"(zero));
-        auto fetch = [&](int t) {
-            if (DOC && u.k_docs) kdoc_next = u.k_docs[min(t * TK + (WK ? 16 * wave : 0) + min(lane, 16 * KB - 1), kl - 1)];
-            if (summary) docs_next = L.meta[(long long)b * L.meta_tiles + t + zero];
+        if (GEN && u.table_lds)
+            for (int i = tid; i < a.group * a.table_size; i += 256)
+                *(__attribute__((address_space(3))) float *)((lds_t *)lds + kTab + 4 * i) = a.table[kvh * a.group * a.table_size + i];
+
+        // A found tile's documents: whether it and the workgroup's columns are of one, whether
+        // the wave's columns have keys in it, and whether those are of one
+        enum { ONE = 1, MINE = 2, SAME = 4 };
+        auto documents = [&](int t) {
+            if (!DOC || !doc_keys) return ONE | MINE | SAME;
+            if (!summary || t >= t_end) return (int)MINE;
+            const int at = t - live_at, lo = __builtin_amdgcn_readlane(t_lo, at), hi = __builtin_amdgcn_readlane(t_hi, at),
+                      all = __builtin_amdgcn_readlane(t_all, at);
+            return ((whole >> at) & 1 ? ONE : 0) | (lo <= w_hi && hi >= w_lo ? MINE : 0) |
+                   (all == hi && w_lo == w_hi && hi == w_hi ? SAME : 0);
         };
 
-        int t = next(split * per), buf = 0;
+        // the first two tiles set out together; then the next one's buffer is free when the one
+        // before has been computed
+        constexpr int W = 2 * LOADS * SUB;  // copies per thread and tile
+        int t = next(split * per), buf = 0, docs = documents(t);
         kp += (long long)t * kstep, vp += (long long)t * vstep;
-        if (t < t_end) fetch(t), stage(t, 0);
+        if (t < t_end) stage(t, 0);
+        int tn = t < t_end ? next(t + 1) : t_end, docs_n = documents(tn);
+        kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
+        bool ahead = DOC && tn < t_end;
+        if (ahead) stage(tn, 1);
         while (t < t_end) {
-            const bool one_doc = !DOC || !u.k_docs || (summary && ((whole >> (t - live_at)) & 1));
-            const int tn = next(t + 1);
-            if constexpr (ALIGN > 0) WAIT_VMCNT(0);
+            if constexpr (ALIGN > 0) {
+                if (ahead) WAIT_VMCNT(W < 63 ? W : 63);
+                else WAIT_VMCNT(0);
+            } else if (DOC) WAIT_VMCNT(0);
             lds_sync();
-            bool mine = true, same = one_doc;  // whether the wave's columns have keys here, and all of one document
-            if (DOC) kdoc = kdoc_next;
-            if (summary) {
-                const int lo = __builtin_amdgcn_readfirstlane(docs_next.x), hi = __builtin_amdgcn_readfirstlane(docs_next.y),
-                          all = __builtin_amdgcn_readfirstlane(docs_next.z);
-                mine = lo <= w_hi && hi >= w_lo;
-                same = all == hi && w_lo == w_hi && hi == w_hi;
-            }
-            kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
-            if (tn < t_end) fetch(tn), stage(tn, buf ^ 1);
+            if (!ahead && tn < t_end) stage(tn, buf ^ 1);
+            ahead = false;
             const int at_buf = buf * 2 * (int)kTile;
-            if (!(t * TK + TK <= wg_min && one_doc) || (GEN && u.table)) {
+            if (!(t * TK + TK <= wg_min && (docs & ONE)) || (GEN && u.table)) {
                 // a masked key's weight is zero, and zero times an infinity is none: with
                 // such values in the V of a tile that not every column reads whole, they are
                 // added by themselves to the columns that do read them, and taken out
                 lds_t *vd = (lds_t *)lds + at_buf + kTile;
-                auto *flag = (__attribute__((address_space(3))) int *)((lds_t *)lds + 4 * kTile);
+                auto *flag = (__attribute__((address_space(3))) int *)((lds_t *)lds + kFlag);
                 const bool w = __any(any_wild_chunk(vd));
                 if (lane == 0) flag[wave] = w;
                 lds_sync();
@@ -589,12 +608,16 @@ struct Kernel {
                 }
             }
             const int j0 = t * TK + (WK ? 16 * wave : 0);  // the wave's first key
-            if (j0 < w_max && mine) {
-                const bool full = j0 + 16 * KB <= w_min && same && !(GEN && u.table);
-                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, j0 + 16 * KB <= w_at + 1, kdoc, lim, doc, at, slope, tab, qf, o, m, l);
+            if (j0 < w_max && (docs & MINE)) {
+                const bool full = j0 + 16 * KB <= w_min && (docs & SAME) && !(GEN && u.table);
+                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, j0 + 16 * KB <= w_at + 1, base + kIds + buf * 256 + (WK ? 64 * wave : 0), lim, doc, at, slope, tab, qf, o, m, l);
             }
-            t = tn;
+            t = tn, docs = docs_n;
             buf ^= 1;
+            if (t < t_end) {
+                tn = next(t + 1), docs_n = documents(tn);
+                kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
+            }
         }
 
         float total[NB];
@@ -707,22 +730,21 @@ struct Kernel {
 
     // The wave's keys of one tile: scores, softmax step, products with V.
     static __device__ __forceinline__ void tile(const Uniform &u, const lds_t *kl0, const lds_t *vl0, int j0,
-                                                bool full, bool behind, int kdoc, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
+                                                bool full, bool behind, const lds_t *ids, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
                                                 const Vec (*qf)[KS], f4v (*o)[NB], float *m,
                                                 typename std::conditional<F32, float, f4v>::type *l) {
         const int lane = threadIdx.x & 63, q = lane >> 4;
-        // a lane per key for what is read per key
-        const int jl = min(j0 + min(lane, 16 * KB - 1), u.kl - 1);
         // the table's entries on their way while the scores are made
         float bias[GEN ? KB : 1][4][GEN ? NB : 1];
         int place[GEN ? KB : 1][4];
         if (GEN && u.general) {
             if (u.k_pos) {
-                const int mine = u.k_pos[jl];
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
+                for (int kb = 0; kb < KB; ++kb) {
+                    const i4 x = lds_read<i4>(ids + (kPos - kIds) + 16 * q, 64 * kb);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) place[GEN ? kb : 0][i] = __shfl(mine, 16 * kb + 4 * q + i);
+                    for (int i = 0; i < 4; ++i) place[GEN ? kb : 0][i] = x[i];
+                }
             } else {
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
@@ -859,14 +881,14 @@ struct Kernel {
             }
             if (DOC && u.k_docs) {
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
+                for (int kb = 0; kb < KB; ++kb) {
+                    const i4 x = lds_read<i4>(ids + 16 * q, 64 * kb);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int d = __shfl(kdoc, 16 * kb + 4 * q + i);
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)
-                            if (d != doc[nb]) s[kb][nb][i] = -INFINITY;
-                    }
+                            if (x[i] != doc[nb]) s[kb][nb][i] = -INFINITY;
+                }
             }
         }
         // the running reference: rescaled only where a score passes it by 2^kLazy
@@ -912,7 +934,8 @@ struct Kernel {
     }
 
     static __device__ __forceinline__ float entry(const Uniform &u, int tab, int dist) {
-        return u.table[tab + min(max(dist, -u.half), u.half) + u.half];
+        const int i = tab + min(max(dist, -u.half), u.half) + u.half;
+        return u.table_lds ? lds_read<float>(u.tab0 + 4 * i, 0) : u.table[i];
     }
     // O^T += V^T P^T
     static __device__ __forceinline__ void products(const lds_t *vl0, const f4v (*s)[NB], f4v (*o)[NB],
@@ -1067,10 +1090,13 @@ struct Cut {
 template <typename T, int DP, int NB, bool WK, int ALIGN, int MODE>
 hipError_t launch(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
     typedef Kernel<T, DP, NB, WK, ALIGN, MODE> K;
-    static_assert(K::kLds <= 163840, "LDS");
+    static_assert(K::kTab + 4 * K::kTabEntries <= 163840, "LDS");
+    AttnLaunch M = L;
+    M.table_lds = a.table && (long long)a.group * a.table_size <= K::kTabEntries;
+    const size_t lds = K::kTab + (M.table_lds ? (size_t)a.group * a.table_size * 4 : 0);
     const long long blocks = (long long)a.batch * a.hk * L.tiles * L.splits;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_attn<T, DP, NB, WK, ALIGN, MODE>), dim3((unsigned)blocks), dim3(256), K::kLds, st, a, L);
+    hipLaunchKernelGGL((k_attn<T, DP, NB, WK, ALIGN, MODE>), dim3((unsigned)blocks), dim3(256), lds, st, a, M);
     return hipGetLastError();
 }
 

@@ -289,9 +289,11 @@ int s2s_rotary(const s2s_rotary_args *a, void *stream) {
     k.lens = a->lens;
     for (int i = 0; i < a->pairs; ++i) {
         // inv_freq / 2 pi turns, its fraction in 64 bits (long double: 64-bit significand)
+        // inv_freq below 2^20 leaves whole turns that an int holds
         long double t = (long double)a->inv_freq[i] * 0.15915494309189533576888376337251436L;
-        t -= std::floor(t);
-        unsigned long long f = t >= 1.0L ? 0ULL : (unsigned long long)(t * 18446744073709551616.0L);
+        t -= (long double)(int)t;
+        if (t < 0) t += 1.0L;
+        const unsigned long long f = t >= 1.0L ? 0ULL : (unsigned long long)(t * 18446744073709551616.0L);
         k.freq[i] = a->inverse ? 0ULL - f : f;
         k.axis[i] = a->pair_axis[i];
     }
