@@ -89,7 +89,7 @@ struct AttnLaunch {
     int tiles;      // column tiles per (batch entry, key head)
     int splits;     // key ranges per column tile
     int vec;        // bytes of one element-wise access (unaligned arrays): 8, 4 or 2
-    int out_vec;    // the output takes 4 elements at once
+    int out_vec;    // elements that one store of the output takes: 4, 2 or 1
     float *part_o;  // splits > 1: [batch * hk][splits][cols][DP] unnormalised sums
     float *part_ml;  // [batch * hk][splits][cols][2]: reference and sum of the weights
     const int4 *meta;  // documents: [batch][key tiles] {smallest, largest id >= 0, smallest id, 0}
@@ -698,8 +698,12 @@ struct Kernel {
         VecOf<T, 4> y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) y.e[i] = (T)x[i];
-        if (vec) {
+        if (vec == 4) {
             if (c < width) *(VecOf<T, 4> *)(row + c) = y;
+        } else if (vec == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; i += 2)
+                if (c + i < width) *(VecOf<T, 2> *)(row + c + i) = VecOf<T, 2>{{y.e[i], y.e[i + 1]}};
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -1044,6 +1048,18 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnOpArgs a, AttnLaunch L) {
         ms = L.part_ml[2 * row];
         l = L.part_ml[2 * row + 1];
     }
+    // the first sums on their way while the weights are made
+    constexpr int N = 16;
+    const int d = tid % DP, g = tid / DP;
+    float x[N];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int s = s0 + k * G;
+            x[k] = g < G && s < L.splits ? L.part_o[(row0 + (long long)s * L.cols) * DP + d] : 0.f;
+        }
+    };
+    load(g);
     float top = half_max(ms);
 #pragma unroll
     for (int m = 1; m < 32; m *= 2) top = fmaxf(top, __shfl_xor(top, m));
@@ -1059,16 +1075,17 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnOpArgs a, AttnLaunch L) {
     if ((tid & 63) == 0) stat[4 + (tid >> 6)] = ls;
     __syncthreads();
     ls = (stat[4] + stat[5]) + (stat[6] + stat[7]);
-    const int d = tid % DP, g = tid / DP;
     float o = 0.f;
-    if (g < G) {
-#pragma unroll 4
-        for (int s = g; s < L.splits; s += G) {
-            const float w = weight[s], x = L.part_o[(row0 + (long long)s * L.cols) * DP + d];
-            o += w == 0.f ? 0.f : w * x;
+    for (int s0 = g; s0 < L.splits; s0 += N * G) {
+        if (s0 != g) load(s0);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int s = s0 + k * G;
+            const float w = s < L.splits ? weight[s] : 0.f;
+            o += w == 0.f ? 0.f : w * x[k];
         }
-        part[tid] = o;
     }
+    part[tid] = o;
     __syncthreads();
     if (tid < a.width) {
         o = 0.f;

@@ -153,7 +153,7 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
     int al = aligned_bytes(a.q, a.sq, a.width, size);
     if (a.nk > 0) al = std::min(al, std::min(aligned_bytes(a.k, a.sk, a.width, size), aligned_bytes(a.v, a.sv, a.width, size)));
     L.vec = std::min(al, 8);
-    L.out_vec = aligned_bytes(a.out, a.so, a.width, size) >= 4 * size;
+    L.out_vec = std::min(4, aligned_bytes(a.out, a.so, a.width, size) / size);
     // (rows that overlap have no end that the copies' resource could tell: by elements)
     const int align = a.sk.t < a.width || a.sv.t < a.width ? 0 : al >= 16 ? 16 : al >= 4 ? 4 : 0;
     // Packed documents of narrow heads too: the fewer columns a workgroup has, the fewer lie
