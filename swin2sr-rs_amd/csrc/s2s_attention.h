@@ -713,7 +713,7 @@ struct Kernel {
 
     // V^T's operand for channel block db (vl: the lane's address for it): the keys of
     // blocks 2 j and 2 j + 1 (f32: of block j, one key per lane group and register). With
-    // WK the wave's one block.
+    // WK the wave's one block, twice.
     static __device__ __forceinline__ Vec v_operand(const lds_t *vl, int j) {
         if constexpr (F32) {
             const int r = j * 16 * CH * 16;
@@ -725,7 +725,7 @@ struct Kernel {
                 Vec v;
             } u;
             u.h[0] = lds_read_tr(vl, j * 32 * CH * 16);
-            if constexpr (WK) u.h[1] = s4{0, 0, 0, 0};
+            if constexpr (WK) u.h[1] = u.h[0];
             else u.h[1] = lds_read_tr(vl, (j * 32 + 16) * CH * 16);
             return u.v;
         }
@@ -954,8 +954,12 @@ struct Kernel {
                 else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        p[j][nb][i] = (T)s[WK ? 0 : 2 * j][nb][i];
-                        p[j][nb][4 + i] = WK ? (T)0.f : (T)s[WK ? 0 : 2 * j + 1][nb][i];
+                        const float x = s[WK ? 0 : 2 * j][nb][i];
+                        const T hi = (T)x;
+                        p[j][nb][i] = hi;
+                        // with one block half the slots are free: what the rounding left of it
+                        // (2^-17 of it then; the caches' reads take longer than the products)
+                        p[j][nb][4 + i] = WK ? (T)(x - (float)hi) : (T)s[WK ? 0 : 2 * j + 1][nb][i];
                     }
                 }
             }

@@ -266,12 +266,12 @@ __global__ __launch_bounds__(256) void k_rms_norm_rows(RmsNormArgs a) {
 }
 
 // The rows of a workgroup in registers: TPR threads a row (256 / TPR rows at once), NC
-// chunks of V elements (16 bytes) a thread, so that x and the residual are read once and
+// chunks of V elements (16 or 8 bytes) a thread, so that x and the residual are read once and
 // nothing is read again; the weights stay in registers over the rows that the workgroup
 // walks. A group of the scales is a power of two of chunks, which neighbouring lanes hold.
-template <typename T, bool E4M3, int TPR, int NC>
+template <typename T, bool E4M3, int V, int TPR, int NC>
 __global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
-    constexpr int V = 16 / sizeof(T);
+    static_assert(V % 4 == 0, "codes are stored four and more at a time");
     typedef VecOf<T, V> Vec;
     const int tid = threadIdx.x, lane = tid & 63, r0 = tid / TPR, tr = tid % TPR;
     const int chunks = a.cols / V;
@@ -397,40 +397,54 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
     }
 }
 
-template <typename T, bool E4M3, int TPR, int NC>
+template <typename T, bool E4M3, int V, int TPR, int NC>
 hipError_t rms_launch(const RmsNormArgs &a, hipStream_t st) {
     const long long blocks = (a.rows + 256 / TPR - 1) / (256 / TPR);
     // at most 8 workgroups a CU, which then walk their rows with the weights at hand
     const long long most = 8LL * cu_count();
-    hipLaunchKernelGGL((k_rms_norm<T, E4M3, TPR, NC>), dim3((unsigned)std::min(blocks, most)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_rms_norm<T, E4M3, V, TPR, NC>), dim3((unsigned)std::min(blocks, most)), dim3(256), 0, st, a);
     return hipGetLastError();
+}
+
+// Whether rows of chunks of V elements can be taken: their places, their number, and the
+// scales' groups, which are a power of two of chunks.
+template <typename T, bool E4M3, int V>
+bool rms_takes(const RmsNormArgs &a, int most) {
+    auto fits = [](const void *p, long long stride, int size, int bytes) {
+        return !p || ((uintptr_t)p % bytes == 0 && stride * size % bytes == 0);
+    };
+    constexpr int B = V * sizeof(T);
+    const int gl = a.groups == 1 ? 1 : a.group / V;
+    return a.cols % V == 0 && a.cols <= most * V && fits(a.x, a.xs, sizeof(T), B) && fits(a.res, a.rs, sizeof(T), B) &&
+           fits(a.sum, a.ss, sizeof(T), B) && fits(a.out, a.os, E4M3 ? 1 : sizeof(T), E4M3 ? V : B) &&
+           fits(a.weight, 0, 4, 16) && (!E4M3 || a.groups == 1 || (a.group % V == 0 && (gl & (gl - 1)) == 0 && gl <= 64));
 }
 
 template <typename T, bool E4M3>
 hipError_t rms_type(const RmsNormArgs &a, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
-    auto fits = [](const void *p, long long stride, int size, int bytes) {
-        return !p || ((uintptr_t)p % bytes == 0 && stride * size % bytes == 0);
-    };
-    const int gl = a.groups == 1 ? 1 : a.group / V;
-    const bool vec = a.cols % V == 0 && a.cols <= 8 * 256 * V && fits(a.x, a.xs, sizeof(T), 16) &&
-                     fits(a.res, a.rs, sizeof(T), 16) && fits(a.sum, a.ss, sizeof(T), 16) &&
-                     fits(a.out, a.os, E4M3 ? 1 : sizeof(T), E4M3 ? V : 16) && fits(a.weight, 0, 4, 16) &&
-                     (!E4M3 || a.groups == 1 || (a.group % V == 0 && (gl & (gl - 1)) == 0 && gl <= 64));
-    if (!vec) {
-        hipLaunchKernelGGL((k_rms_norm_rows<T, E4M3>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
-        return hipGetLastError();
-    }
-    // a wave per row up to 2 chunks a lane, and up to 4 where there are rows for the chip
     const int chunks = a.cols / V;
-    const bool many = a.rows >= 16LL * cu_count();
-    if (chunks <= 64) return rms_launch<T, E4M3, 64, 1>(a, st);
-    if (chunks <= 128) return rms_launch<T, E4M3, 64, 2>(a, st);
-    if (chunks <= 256) return many ? rms_launch<T, E4M3, 64, 4>(a, st) : rms_launch<T, E4M3, 256, 1>(a, st);
-    if (chunks <= 512) return rms_launch<T, E4M3, 256, 2>(a, st);
-    if (chunks <= 768) return rms_launch<T, E4M3, 256, 3>(a, st);
-    if (chunks <= 1024) return rms_launch<T, E4M3, 256, 4>(a, st);
-    return rms_launch<T, E4M3, 256, 8>(a, st);
+    if (rms_takes<T, E4M3, V>(a, 8 * 256)) {
+        // a wave per row up to 2 chunks a lane, and up to 4 where there are rows for the chip
+        const bool many = a.rows >= 16LL * cu_count();
+        if (chunks <= 64) return rms_launch<T, E4M3, V, 64, 1>(a, st);
+        if (chunks <= 128) return rms_launch<T, E4M3, V, 64, 2>(a, st);
+        if (chunks <= 256) return many ? rms_launch<T, E4M3, V, 64, 4>(a, st) : rms_launch<T, E4M3, V, 256, 1>(a, st);
+        if (chunks <= 512) return rms_launch<T, E4M3, V, 256, 2>(a, st);
+        if (chunks <= 768) return rms_launch<T, E4M3, V, 256, 3>(a, st);
+        if (chunks <= 1024) return rms_launch<T, E4M3, V, 256, 4>(a, st);
+        return rms_launch<T, E4M3, V, 256, 8>(a, st);
+    }
+    // 16-bit rows of 8-byte multiples (180 or 60 columns): 45412 x 180 f16 to e4m3 took 74 us by
+    // rows read twice
+    if constexpr (sizeof(T) == 2) {
+        if (rms_takes<T, E4M3, 4>(a, 4 * 64)) {
+            if (a.cols <= 4 * 64) return rms_launch<T, E4M3, 4, 64, 1>(a, st);
+            return rms_launch<T, E4M3, 4, 64, 4>(a, st);
+        }
+    }
+    hipLaunchKernelGGL((k_rms_norm_rows<T, E4M3>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+    return hipGetLastError();
 }
 
 }  // namespace

@@ -485,6 +485,10 @@ def rms_case(pkg, dtype, rows, cols, res=True, sum_=True, e4m3=False, group=0, g
 RMS = {
     "one": dict(dtype="f32", rows=1, cols=1),
     "plane": dict(dtype="f32", rows=300, cols=180),
+    "plane_f16": dict(dtype="f16", rows=300, cols=180),
+    "plane_e4m3": dict(dtype="bf16", rows=300, cols=180, e4m3=True, group=128),
+    "plane_e4m3_row": dict(dtype="f16", rows=77, cols=60, e4m3=True),
+    "plane_720": dict(dtype="bf16", rows=77, cols=716, e4m3=True, group=32, alias=("sum",)),
     "narrow": dict(dtype="bf16", rows=70, cols=60, res=False, sum_=False),
     "odd": dict(dtype="f16", rows=9, cols=1023, gap=1, lead=1),
     "offset": dict(dtype="bf16", rows=5, cols=4096, offset=1.0),
