@@ -311,6 +311,282 @@ def test_attention_is_the_window_attention(pkg, heads, hd, shift):
     assert np.abs(got - want[at.ravel()]).max() <= 8 * (hd + 12) * 14 * 2.0 ** -24
 
 
+def test_attention_table_sizes(pkg):
+    """A table of the group's heads in LDS and one that is too large for it."""
+    for entries, heads in ((2047, 1), (4097, 2), (681, 6)):
+        check_attention(pkg, case("f16", B=2, Lq=70, Lk=190, H=heads, KV=1, D=32, table=entries))
+        check_attention(pkg, case("bf16", B=1, Lq=2, Lk=1300, H=heads, KV=1, D=64, table=entries, causal=True, order="cache"))
+
+
+def test_attention_lowest_bias_is_even(pkg):
+    """Every score at the type's lowest value: the weights are equal."""
+    for dtype, Lq in (("f32", 2), ("f32", 70), ("bf16", 70)):
+        c = case(dtype, Lq=Lq, Lk=80, H=2, KV=1, D=32, table=3)
+        q, k, v, more = inputs(c)
+        more["table"][:] = np.finfo(np.float32).min
+        plan, ws, _ = make_plan(pkg, c)
+        d, m = upload(pkg, c, q, k, v, more)
+        call(plan, ws, d, m)
+        want = v[:, :, 0].mean(1)[:, None, None, :]
+        tol = (80 + 8) * 2.0 ** -24 * np.abs(v).mean() * 2 + 2 * R.HALF[dtype] * (np.abs(want) + np.abs(v).mean())
+        assert (np.abs(d["out"].get() - want) <= tol).all()
+
+
+def test_attention_no_keys(pkg):
+    """No key at all gives zeros and reads nothing."""
+    for Lq in (1, 100):
+        plan = pkg.ops.Attention("bf16", 2, Lq, 0, 4, 2, 64, causal=True)
+        q, out = (R.Dev(pkg, np.full((2, Lq, 4, 64), 3.0), "bf16") for _ in range(2))
+        empty = pkg.ops.Array(0, (2, 0, 2, 64), "bf16")
+        ws = R.Dev(pkg, np.zeros(max(plan.workspace_bytes // 4, 1)), "f32")
+        plan(q.array, empty, empty, out.array, workspace=ws.array)
+        assert not out.get().any()
+
+
+def test_attention_is_deterministic(pkg):
+    """The same call gives the same bits, whatever order its workgroups come in."""
+    for c in (case("bf16", B=2, Lq=1500, Lk=1500, H=4, KV=2, D=64, docs=segments(400, 90, 700)),
+              case("f16", B=1, Lq=1, Lk=20000, H=8, KV=1, D=64, order="cache", causal=True),
+              case("f32", B=2, Lq=300, Lk=300, H=2, KV=2, D=30, docs=scattered)):
+        q, k, v, more = inputs(c)
+        plan, ws, _ = make_plan(pkg, c)
+        d, m = upload(pkg, c, q, k, v, more)
+        seen = set()
+        for _ in range(6):
+            call(plan, ws, d, m)
+            seen.add(d["out"].bits().tobytes())
+        assert len(seen) == 1
+
+
+@pytest.mark.parametrize("Lq", [1, 40])
+def test_attention_offsets_past_32_bits(pkg, Lq):
+    """A cache whose tokens lie 4 MiB apart: 8.8 GB from the first to the last, of which only the
+    tokens' own bytes are written."""
+    Lk, D, stride = 2100, 64, 1 << 21
+    g = np.random.default_rng(1)
+    q, k, v = (R.round_to(g.standard_normal(s), "bf16") for s in ((1, Lq, 2, D), (1, Lk, 1, D), (1, Lk, 1, D)))
+    buf = pkg.hip.DeviceBuffer((stride * (Lk - 1) + 2 * D + 1) // 2)
+    rows = np.concatenate([R.to_bits(k[0, :, 0], "bf16"), R.to_bits(v[0, :, 0], "bf16")], 1)
+    copy, vp = pkg.hip.rt().hipMemcpy, C.c_void_p
+    for j in range(Lk):
+        row = np.ascontiguousarray(rows[j])
+        assert copy(vp(buf.ptr + j * stride * 2), row.ctypes.data_as(vp), row.nbytes, 1) == 0
+    kd, vd = (pkg.ops.Array(buf.ptr + off, (1, Lk, 1, D), "bf16", (0, stride, 0, 1)) for off in (0, 2 * D))
+    qd, out = R.Dev(pkg, q, "bf16"), R.Dev(pkg, np.zeros(q.shape), "bf16")
+    plan = pkg.ops.Attention("bf16", 1, Lq, Lk, 2, 1, D, causal=True)
+    ws = R.Dev(pkg, np.zeros(max(plan.workspace_bytes // 4, 1)), "f32")
+    plan(qd.array, kd, vd, out.array, workspace=ws.array)
+    want, bound, _ = R.attention("bf16", q, k, v, np.float64(np.float32(D ** -0.5)), causal=True)
+    got = out.get()
+    buf.free()
+    assert (np.abs(got - want) <= bound).all()
+
+
+# ---- what a call refuses with a device at hand ---------------------------------------
+
+
+def refused(pkg, word, f):
+    with pytest.raises(pkg.S2SError, match=word):
+        f()
+
+
+def test_attention_refuses(pkg):
+    c = case("bf16", B=1, Lq=1, Lk=5000, H=8, KV=2, D=64)
+    q, k, v, more = inputs(c)
+    plan, ws, _ = make_plan(pkg, c)
+    d, m = upload(pkg, c, q, k, v, more)
+    A = pkg.ops.Array
+    a = {n: x.array for n, x in d.items()}
+    assert plan.workspace_bytes > 0
+    refused(pkg, "workspace", lambda: plan(**a))
+    refused(pkg, "workspace", lambda: plan(**a, workspace=A(ws.buf.ptr, (plan.workspace_bytes - 1,), "u8")))
+    refused(pkg, "workspace is not aligned", lambda: plan(**a, workspace=A(ws.buf.ptr + 4, (plan.workspace_bytes,), "u8")))
+    host = np.zeros(64, np.float32)
+    refused(pkg, "workspace is not device memory",
+            lambda: plan(**a, workspace=A(host.ctypes.data // 16 * 16, (plan.workspace_bytes,), "u8")))
+    w = dict(workspace=ws.array)
+    refused(pkg, "q is not device memory", lambda: plan(**{**a, "q": A(host.ctypes.data, (1, 1, 8, 64), "bf16")}, **w))
+    refused(pkg, "k_lens is not device memory", lambda: plan(**a, **w, k_lens=A(host.ctypes.data, (1,), "i32")))
+    refused(pkg, "k is null", lambda: plan(**{**a, "k": A(0, (1, 5000, 2, 64), "bf16")}, **w))
+    refused(pkg, "v is not aligned", lambda: plan(**{**a, "v": A(d["v"].array.ptr + 1, (1, 5000, 2, 64), "bf16")}, **w))
+    refused(pkg, "overlap", lambda: plan(**{**a, "out": A(d["out"].array.ptr, (1, 1, 8, 64), "bf16", (512, 512, 63, 1))}, **w))
+    refused(pkg, "out is an input", lambda: plan(**{**a, "out": a["q"]}, **w))
+    refused(pkg, "stride", lambda: plan(**{**a, "k": A(d["k"].array.ptr, (1, 5000, 2, 64), "bf16", (0, 1 << 23, 64, 1))}, **w))
+    refused(pkg, "stride", lambda: plan(**{**a, "k": A(d["k"].array.ptr, (1, 5000, 2, 64), "bf16", (0, -64, 64, 1))}, **w))
+    refused(pkg, "prefix without", lambda: plan(**a, **w, prefix=R.Dev(pkg, np.zeros(1, np.int32), "f32", whole=True).array))
+    # and nothing of these was run
+    assert np.all(d["out"].get() == 7.5)
+
+
+def test_rotary_and_norm_refuse(pkg):
+    A = pkg.ops.Array
+    x = R.Dev(pkg, np.ones((2, 4, 3, 16)), "bf16")
+    pos = R.Dev(pkg, np.zeros((2, 4, 1), np.int32), "f32", whole=True)
+    rot = pkg.ops.Rotary.of((8,))
+    p = x.array.ptr
+    refused(pkg, "in place", lambda: rot(x.array, pos.array, A(p, (2, 4, 3, 16), "bf16", (400, 48, 16, 1))))
+    refused(pkg, "overlap", lambda: rot(x.array, pos.array, A(p, (2, 4, 3, 16), "bf16", (0, 48, 16, 1))))
+    refused(pkg, "same array", lambda: rot(x.array, pos.array, x.array, x.array, x.array))
+    host = np.zeros(64, np.int32)
+    refused(pkg, "pos is not device memory", lambda: rot(x.array, A(host.ctypes.data, (2, 4, 1), "i32")))
+    y, w = R.Dev(pkg, np.ones((4, 32)), "f32"), R.Dev(pkg, np.ones(32), "f32")
+    out = R.Dev(pkg, np.zeros((4, 32)), "f32")
+    norm = pkg.ops.rms_norm
+    refused(pkg, "overlap", lambda: norm(y.array, w.array, A(out.array.ptr, (4, 32), "f32", (16, 1))))
+    refused(pkg, "not in its rows", lambda: norm(y.array, w.array, A(y.array.ptr, (4, 32), "f32", (64, 1))))
+    refused(pkg, "not in its rows", lambda: norm(y.array, w.array, A(y.array.ptr, (4, 32), "e4m3"), scales=A(out.array.ptr, (4, 1), "f32")))
+    refused(pkg, "same array", lambda: norm(y.array, w.array, out.array, sum=out.array))
+    refused(pkg, "weight is not device memory", lambda: norm(y.array, A(host.ctypes.data, (32,), "f32"), out.array))
+    assert not out.get().any()
+
+
+# ---- streams, graphs, the operators one after another --------------------------------------
+
+
+class Block:
+    """The front half of a transformer block on `tokens` image tokens: norm with the residual's
+    addition, a projection (made on the host beforehand: q, k, v are read from the norm's output
+    by strides), rotary positions, attention over documents and over a cache."""
+
+    def __init__(self, pkg, seed, tokens=700, heads=4, kv=2, D=32):
+        self.pkg, self.D = pkg, D
+        g = np.random.default_rng(seed)
+        cols = (heads + 2 * kv) * D
+        self.x, self.res = (R.round_to(g.standard_normal((tokens, cols)), "bf16") for _ in range(2))
+        self.weight = (1 + 0.1 * g.standard_normal(cols)).astype(np.float32)
+        self.pos = np.stack([np.arange(tokens) // 25, np.arange(tokens) % 25], 1)[None].astype(np.int32)
+        self.docs = np.where(np.arange(tokens) < 333, 0, np.where(np.arange(tokens) < 680, 1, -1)).astype(np.int32)
+        up = lambda v, t="bf16": R.Dev(pkg, v, t, whole=v.dtype == np.int32)  # noqa: E731
+        self.dx, self.dres, self.dw, self.dpos, self.ddocs = up(self.x), up(self.res), up(self.weight, "f32"), up(self.pos), up(self.docs)
+        self.h = up(np.zeros((tokens, cols)))
+        self.turned = up(np.zeros((1, tokens, heads + kv, D)))
+        self.out, self.last = up(np.zeros((1, tokens, heads, D))), up(np.zeros((1, 1, heads, D)))
+        self.rot = pkg.ops.Rotary.of((8, 8))
+        self.plan = pkg.ops.Attention("bf16", 1, tokens, tokens, heads, kv, D, cap=30.0)
+        self.step = pkg.ops.Attention("bf16", 1, 1, tokens, heads, kv, D, causal=True)
+        n = max(self.plan.workspace_bytes, self.step.workspace_bytes)
+        self.ws = R.Dev(pkg, np.zeros(n // 4 + 1), "f32")
+        self.tokens, self.heads, self.kv = tokens, heads, kv
+
+    def view(self, dev, first, n, width_heads):
+        ptr = dev.array.ptr + first * self.D * 2
+        return self.pkg.ops.Array(ptr, (1, self.tokens, n, self.D), "bf16", (0, width_heads * self.D, self.D, 1))
+
+    def run(self, stream=0):
+        H, KV = self.heads, self.kv
+        all_ = H + 2 * KV
+        self.pkg.ops.rms_norm(self.dx.array, self.dw.array, self.h.array, res=self.dres.array, stream=stream)
+        q, k, v = self.view(self.h, 0, H, all_), self.view(self.h, H, KV, all_), self.view(self.h, H + KV, KV, all_)
+        tq, tk = self.view(self.turned, 0, H, H + KV), self.view(self.turned, H, KV, H + KV)
+        self.rot(q, self.dpos.array, tq, k, tk, stream=stream)
+        self.plan(tq, tk, v, self.out.array, workspace=self.ws.array, stream=stream, q_docs=self.ddocs.array, k_docs=self.ddocs.array)
+        last = self.pkg.ops.Array(tq.ptr + (self.tokens - 1) * (H + KV) * self.D * 2, (1, 1, H, self.D), "bf16")
+        self.step(last, tk, v, self.last.array, workspace=self.ws.array, stream=stream)
+
+    def bits(self):
+        return self.h.bits().tobytes() + self.turned.bits().tobytes() + self.out.bits().tobytes() + self.last.bits().tobytes()
+
+
+def test_norm_rotary_attention(pkg):
+    """The three operators as they follow one another, each stage against 64 bits from what the
+    stage before left in memory."""
+    b = Block(pkg, 0)
+    b.run()
+    pkg.hip.synchronize()
+    H, KV, D, n = b.heads, b.kv, b.D, b.tokens
+    sum_ = b.x + b.res
+    y = sum_ / np.sqrt((sum_ * sum_).mean(1, keepdims=True) + 1e-6) * b.weight
+    h = b.h.get()
+    assert (np.abs(h - y) <= (40 * 2.0 ** -24 + R.HALF["bf16"]) * np.abs(y) + 1e-30).all()
+    qkv = h.reshape(1, n, H + 2 * KV, D)
+    axis, freq = np.array(b.rot.pair_axis[:]), np.array(b.rot.inv_freq[:])
+    turned = R.rotary(qkv[:, :, :H + KV], b.pos[..., axis] * freq, 16, False, False)
+    got = b.turned.get()
+    both = np.tile(np.abs(qkv[:, :, :H + KV, :16]) + np.abs(qkv[:, :, :H + KV, 16:]), 2)
+    assert (np.abs(got - turned) <= 6 * 2.0 ** -24 * both + R.HALF["bf16"] * np.abs(turned) + 1e-30).all()
+    scale = np.float64(np.float32(D ** -0.5))
+    want, bound, _ = R.attention("bf16", got[:, :, :H], got[:, :, H:], qkv[:, :, H + KV:], scale, 30.0, q_docs=b.docs, k_docs=b.docs)
+    assert (np.abs(b.out.get() - want) <= bound).all()
+    want, bound, _ = R.attention("bf16", got[:, -1:, :H], got[:, :, H:], qkv[:, :, H + KV:], scale, causal=True)
+    assert (np.abs(b.last.get() - want) <= bound).all()
+
+
+def new_stream(pkg):
+    h, st = pkg.hip.rt(), C.c_void_p()
+    h.hipStreamCreateWithFlags.argtypes = [C.POINTER(C.c_void_p), C.c_uint]
+    h.hipStreamDestroy.argtypes = [C.c_void_p]
+    assert h.hipStreamCreateWithFlags(C.byref(st), 1) == 0
+    return st
+
+
+def test_operators_on_streams(pkg):
+    """Two runs on streams of their own, at once, are each the run on the default stream."""
+    blocks = [Block(pkg, s) for s in (1, 2)]
+    want = []
+    for b in blocks:
+        b.run()
+        pkg.hip.synchronize()
+        want.append(b.bits())
+    streams = [new_stream(pkg) for _ in blocks]
+    for b in blocks:
+        for dev in (b.h, b.turned, b.out, b.last):
+            dev.buf.upload(np.zeros(dev.buf.n, np.float32))
+    pkg.hip.synchronize()
+    for _ in range(3):
+        for b, st in zip(blocks, streams):
+            b.run(stream=st.value)
+    for st in streams:
+        pkg.hip.stream_synchronize(st.value)
+    assert [b.bits() for b in blocks] == want
+    for st in streams:
+        pkg.hip.rt().hipStreamDestroy(st)
+
+
+def test_operators_captured(pkg):
+    """The run captured into a graph: every replay, with eager work between, is the eager run on
+    the inputs of the moment; a second graph has a workspace of its own."""
+    h, vp = pkg.hip.rt(), C.c_void_p
+    for name, args in {"hipStreamBeginCapture": [vp, C.c_int], "hipStreamEndCapture": [vp, C.POINTER(vp)],
+                       "hipGraphInstantiate": [C.POINTER(vp), vp, vp, vp, C.c_size_t], "hipGraphLaunch": [vp, vp],
+                       "hipGraphExecDestroy": [vp], "hipGraphDestroy": [vp]}.items():
+        getattr(h, name).argtypes = args
+    blocks, st = [Block(pkg, s) for s in (3, 4)], new_stream(pkg)
+    graphs, execs = [], []
+    for b in blocks:
+        assert h.hipStreamBeginCapture(st, 2) == 0
+        b.run(stream=st.value)
+        g, e = vp(), vp()
+        assert h.hipStreamEndCapture(st, C.byref(g)) == 0
+        assert h.hipGraphInstantiate(C.byref(e), g, None, None, 0) == 0
+        graphs.append(g)
+        execs.append(e)
+    other = Block(pkg, 5)
+    for turn in range(4):
+        for b in blocks:
+            b.x = R.round_to(np.random.default_rng(10 + turn).standard_normal(b.x.shape), "bf16")
+            raw = R.to_bits(b.x, "bf16").tobytes()
+            b.dx.buf.upload(np.frombuffer(raw, np.float32))
+            b.run()
+            pkg.hip.synchronize()
+            want = b.bits()
+            for dev in (b.h, b.turned, b.out, b.last):
+                dev.buf.upload(np.zeros(dev.buf.n, np.float32))
+            pkg.hip.synchronize()
+            assert h.hipGraphLaunch(execs[blocks.index(b)], st) == 0
+            other.run()
+            pkg.hip.stream_synchronize(st.value)
+            pkg.hip.synchronize()
+            assert b.bits() == want, turn
+        for e in execs:  # both at once: nothing shared
+            assert h.hipGraphLaunch(e, st) == 0
+        pkg.hip.stream_synchronize(st.value)
+        assert blocks[-1].bits() == want
+    for e, g in zip(execs, graphs):
+        h.hipGraphExecDestroy(e)
+        h.hipGraphDestroy(g)
+    h.hipStreamDestroy(st)
+
+
 # ---- rotary ---------------------------------------------------------------------
 
 
