@@ -328,7 +328,7 @@ struct Kernel {
     typedef typename Ty::V Vec;
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int E = Ty::kElems;
-    static constexpr int TK = F32 && !WK ? 32 : 64;
+    static constexpr int TK = F32 && !WK && DP > 64 ? 32 : 64;
     static constexpr int KB = WK ? 1 : TK / 16;          // key blocks per wave
     static constexpr int KS = DP / (4 * E);              // steps of four chunks
     static constexpr int DB = DP / 16;                   // channel blocks of the output

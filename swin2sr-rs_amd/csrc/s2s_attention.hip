@@ -16,7 +16,7 @@ attn::Cut cut_of(int dtype, const AttnOpArgs &a, bool narrow) {
     c.dp = round_up(std::max(a.width, 1), 32);
     c.wk = cols <= 16;
     c.nb = narrow || c.wk || cols <= 64 || (cols + 127) / 128 * pairs < 2 * cus ? 1 : 2;
-    c.tk = dtype == 0 && !c.wk ? 32 : 64;
+    c.tk = dtype == 0 && !c.wk && c.dp > 64 ? 32 : 64;
     const int per = c.wk ? 16 : 64 * c.nb;
     c.tiles = (int)((cols + per - 1) / per);
     // ranges of 4 tiles at least, workgroups for two per CU (four of the narrow ones) at most
