@@ -292,11 +292,14 @@ typedef struct s2s_tokens {
  *    minus infinity takes the key out.
  *  - a query with no key gives zeros. Queries from q_lens[b] on are not
  *    written. Lengths are taken as clamped to [0, tokens], prefix to k_lens.
- * (dy, dx) biases of an image's tokens: positions y * S + x with S at least
- * twice the width less one tell every (dy, dx) apart.
+ * Positions differ by less than 2^31. (dy, dx) biases of an image's tokens:
+ * positions y * S + x with S at least twice the width less one tell every
+ * (dy, dx) apart.
  * Width up to 128. Scores and sums are f32 (f32 arrays: f32 products too); for
  * f16 and bf16 the softmax's weights are rounded to that type before they
- * multiply v. `out` may not overlap an input. */
+ * multiply v, except where few queries share them (query tokens times heads per
+ * key head up to 16: a step), where what the rounding leaves is kept as well.
+ * `out` may not overlap an input. */
 typedef struct s2s_attention_args {
     int dtype; /* of q, k, v, out: S2S_F32, S2S_F16 or S2S_BF16 */
     int batch, q_tokens, k_tokens, q_heads, k_heads, width;

@@ -35,6 +35,7 @@ struct AttnScore {
     // fused operations where the exponential takes two transcendentals, and no
     // cancellation near zero. poly_max: the |x| that it holds for.
     float p0, p1, p2, p3, poly_max;
+    float z;  // scale / cap
     // A cap bounds the scores: with no bias and a type of f32's range, e^(s - ref) at one
     // reference 2^20 below the cap's lies in 2^-125 to 2^20 for every score that a cap up to
     // 50.2 leaves, and no maximum is looked for.
@@ -49,10 +50,11 @@ struct AttnScore {
         capl = a.cap * kAttnLog2e;
         fixed = a.cap > 0.f && !a.slopes && !a.table && 2.f * capl - 20.f <= 125.f;
         ref = fixed ? capl - 20.f : 0.f;
-        p0 = p1 = p2 = p3 = 0.f;
+        p0 = p1 = p2 = p3 = z = 0.f;
         poly_max = -1.f;
         if (a.cap > 0.f) {
-            const float z = a.scale / a.cap, w = z * z;
+            z = a.scale / a.cap;
+            const float w = z * z;
             c1 = z * (2.f * kAttnLog2e);
             // the coefficients and powers of x in the normal range
             if (std::fabs(z) > 1e-5f && std::fabs(z) < 1e5f && a.cap < 1e6f) {
@@ -795,15 +797,20 @@ struct Kernel {
                     big = max3(big, fabsf(s[kb][nb][2]), fabsf(s[kb][nb][3]));
                 }
             if (__any(!(big <= sc.poly_max))) {
-                // cap tanh(z) = cap (1 - 2 / (e^2z + 1))
+                // cap tanh(z) = cap (1 - 2 / (e^2z + 1)), and the polynomial for the scores among
+                // them that it holds for (the difference loses what z is smaller than one)
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
+                            const float t = s[kb][nb][i] * sc.z, w = t * t;
                             const float e = __builtin_amdgcn_exp2f(s[kb][nb][i] * sc.c1);
-                            s[kb][nb][i] = fmaf(-2.f * sc.capl, __builtin_amdgcn_rcpf(e + 1.f), MODE & FIXED ? sc.capl - sc.ref : sc.capl);
+                            const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
+                            const float near = t * fmaf(w, fmaf(w, fmaf(w, -0.04848728f, 0.13289726f), -0.33332333f), 1.f);
+                            const float x = fabsf(t) <= 0.375f ? near : far;
+                            s[kb][nb][i] = MODE & FIXED ? fmaf(x, sc.capl, -sc.ref) : x * sc.capl;
                         }
             } else {
 #pragma unroll

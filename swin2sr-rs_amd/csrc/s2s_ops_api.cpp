@@ -312,10 +312,10 @@ int s2s_rms_norm(const s2s_rms_norm_args *a, void *stream) {
     if (!(a->eps >= 0.f) || !std::isfinite(a->eps) || !std::isfinite(a->weight_offset))
         return refuse("%s: eps is negative, or eps or weight_offset not finite", op);
     if (!q8 && (a->scales || a->group)) return refuse("%s: scales or a group without an e4m3 output", op);
-    if (q8 && !a->scales) return refuse("%s: scales is null", op);
+    if (q8 && !a->scales && a->rows > 0) return refuse("%s: scales is null", op);
     if (a->group < 0 || a->group % 8) return refuse("%s: a group of %d is no multiple of 8", op, a->group);
-    if (!a->x || !a->out || !a->weight) return refuse("%s: x, out or weight is null", op);
     if (a->rows == 0) return 0;
+    if (!a->x || !a->out || !a->weight) return refuse("%s: x, out or weight is null", op);
     OnDevice on;
     const hipStream_t st = (hipStream_t)stream;
     hipError_t e = on.enter(st);

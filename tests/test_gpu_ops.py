@@ -151,6 +151,9 @@ CASES = {
     "group_33": case("f16", B=1, Lq=2, Lk=700, H=33, KV=1, D=32),
     "large_scores": case("bf16", Lq=64, Lk=300, H=2, D=64, spread=30.0),
     "large_scores_capped": case("f16", Lq=64, Lk=300, H=2, D=64, spread=30.0, cap=30.0),
+    "large_cap": case("f32", Lq=64, Lk=100, H=2, D=32, cap=30000.0, spread=3.0),
+    "huge_cap": case("bf16", Lq=3, Lk=100, H=2, D=32, cap=1e9, spread=3.0),
+    "mixed_cap": case("f32", Lq=64, Lk=300, H=2, D=64, spread=4.0, cap=8.0),
     "small_cap": case("f32", Lq=64, Lk=100, H=2, D=32, cap=0.5),
     "negative_scale": case("f32", Lq=20, Lk=100, H=2, D=32, scale=-0.3),
     "long_f16": case("f16", Lq=130, Lk=2000, H=2, KV=1, D=64, causal=True),

@@ -119,6 +119,15 @@ def test_rms_norm_refused(pkg, x, out, more, word):
         pkg.ops.rms_norm(arr(pkg, *x), arr(pkg, (x[0][1],), "f32"), arr(pkg, *out, ptr=8192), **more)
 
 
+def test_nothing_to_do(pkg):
+    """No row, no token: done without a device or an address."""
+    none = arr(pkg, (0, 8), "f32", ptr=0)
+    pkg.ops.rms_norm(none, arr(pkg, (8,), "f32"), none)
+    pkg.ops.rms_norm(none, arr(pkg, (8,), "f32"), arr(pkg, (0, 8), "e4m3", ptr=0), scales=arr(pkg, (0, 1), "f32", ptr=0))
+    for shape in ((0, 4, 2, 64), (2, 0, 2, 64)):
+        pkg.ops.Rotary.of((16, 16))(arr(pkg, shape, ptr=0), arr(pkg, shape[:2] + (2,), "i32", ptr=0))
+
+
 def test_rms_norm_weight_refused(pkg):
     with pytest.raises(pkg.S2SError, match="weight"):
         pkg.ops.rms_norm(arr(pkg, (4, 8), "f32"), arr(pkg, (9,), "f32"), arr(pkg, (4, 8), "f32", ptr=8192))
