@@ -1,6 +1,10 @@
 // s2s_ops.hip - rotary positions with several axes, and the root-mean-square
 // norm with the residual's addition and an e4m3 output. Both are bound by HBM:
-// every element is read once and written once.
+// every element is read once and written once. Measured on an MI355X, whose plain
+// copy of 1 GiB makes 5.05 TB/s: rotary of 16384 tokens, 32 + 8 bf16 heads of 128, 72 us
+// (4.65 TB/s); the norm of 16391 x 5120 bf16 with residual, sum and e4m3 groups of 128, 121 us
+// (4.86 TB/s). Steps (4 rows, 32 tokens) take 4 to 5 us, a launch and two or three reads that
+// wait for each other.
 #include <algorithm>
 #include <cmath>
 
@@ -43,8 +47,8 @@ __device__ __forceinline__ void sincos_turns(unsigned long long f, float &s, flo
 // LDS; then the threads walk the tokens' heads in memory order, a unit of V pairs (or of
 // V channels that are copied) at a time, neighbours next to each other across heads, so
 // that a wave's accesses are whole runs whatever the width. (A thread that kept its
-// angles in registers and looped over heads touched a run per head: 45 us for 2 x
-// 23400 tokens of 6 + 6 f32 heads of 30, of which every run is 120 bytes.)
+// angles in registers and looped over heads touched a run per head: 45 us against 37 for
+// 2 x 23400 tokens of 6 + 6 f32 heads of 30, of which every run is 120 bytes.)
 template <typename T, bool ADJ, int V, bool ALIGNED = true>
 __global__ __launch_bounds__(256) void k_rotary(RotaryArgs a, int tb, int per_head) {
     typedef VecOf<T, ADJ ? 2 * V : V, ALIGNED ? (ADJ ? 2 * V : V) : 1> Vec;
@@ -267,8 +271,8 @@ __global__ __launch_bounds__(256) void k_rms_norm_rows(RmsNormArgs a) {
 
 // The rows of a workgroup in registers: TPR threads a row (256 / TPR rows at once), NC
 // chunks of V elements (16 or 8 bytes) a thread, so that x and the residual are read once and
-// nothing is read again; the weights stay in registers over the rows that the workgroup
-// walks. A group of the scales is a power of two of chunks, which neighbouring lanes hold.
+// nothing is read again (rows read twice, k_rms_norm_rows: 450 us for the 16391 x 5120 above);
+// the weights stay in registers over the rows that the workgroup walks. A group of the scales is a power of two of chunks, which neighbouring lanes hold.
 template <typename T, bool E4M3, int V, int TPR, int NC>
 __global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
     static_assert(V % 4 == 0, "codes are stored four and more at a time");

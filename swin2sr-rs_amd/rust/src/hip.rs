@@ -41,6 +41,95 @@ pub struct S2sCtx {
     _p: [u8; 0],
 }
 
+/// `s2s_tokens`: a device array [batch][tokens][heads][width], strides in elements.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct S2sTokens {
+    pub data: *mut c_void,
+    pub batch: i64,
+    pub token: i64,
+    pub head: i64,
+}
+
+/// `s2s_attention_args`: one call of the attention operator.
+#[repr(C)]
+pub struct S2sAttentionArgs {
+    pub dtype: c_int,
+    pub batch: c_int,
+    pub q_tokens: c_int,
+    pub k_tokens: c_int,
+    pub q_heads: c_int,
+    pub k_heads: c_int,
+    pub width: c_int,
+    pub causal: c_int,
+    pub scale: f32,
+    pub cap: f32,
+    pub q: S2sTokens,
+    pub k: S2sTokens,
+    pub v: S2sTokens,
+    pub out: S2sTokens,
+    pub q_lens: *const i32,
+    pub k_lens: *const i32,
+    pub prefix: *const i32,
+    pub q_docs: *const i32,
+    pub k_docs: *const i32,
+    pub q_docs_batch: i64,
+    pub k_docs_batch: i64,
+    pub q_pos: *const i32,
+    pub k_pos: *const i32,
+    pub q_pos_batch: i64,
+    pub k_pos_batch: i64,
+    pub slopes: *const f32,
+    pub table: *const f32,
+    pub table_size: c_int,
+}
+
+/// `s2s_rotary_args`: one call of the rotary positions.
+#[repr(C)]
+pub struct S2sRotaryArgs {
+    pub dtype: c_int,
+    pub batch: c_int,
+    pub tokens: c_int,
+    pub q_heads: c_int,
+    pub k_heads: c_int,
+    pub width: c_int,
+    pub axes: c_int,
+    pub pairs: c_int,
+    pub adjacent: c_int,
+    pub inverse: c_int,
+    pub q: S2sTokens,
+    pub k: S2sTokens,
+    pub q_out: S2sTokens,
+    pub k_out: S2sTokens,
+    pub pos: *const i32,
+    pub pos_batch: i64,
+    pub lens: *const i32,
+    pub inv_freq: *const f64,
+    pub pair_axis: *const u8,
+}
+
+/// `s2s_rms_norm_args`: one call of the root-mean-square norm.
+#[repr(C)]
+pub struct S2sRmsNormArgs {
+    pub dtype: c_int,
+    pub out_dtype: c_int,
+    pub rows: i64,
+    pub cols: c_int,
+    pub x: *const c_void,
+    pub res: *const c_void,
+    pub sum: *mut c_void,
+    pub out: *mut c_void,
+    pub x_stride: i64,
+    pub res_stride: i64,
+    pub sum_stride: i64,
+    pub out_stride: i64,
+    pub weight: *const f32,
+    pub weight_offset: f32,
+    pub eps: f32,
+    pub scales: *mut f32,
+    pub group: c_int,
+}
+
 #[link(name = "swin2sr_hip")]
 extern "C" {
     pub fn s2s_create(arch: *const S2sArch, t: *const S2sTensor, n: usize, out: *mut *mut S2sCtx) -> c_int;
@@ -71,6 +160,10 @@ extern "C" {
     pub fn s2s_profile_enable(ctx: *mut S2sCtx, on: c_int) -> c_int;
     pub fn s2s_profile_reset(ctx: *mut S2sCtx) -> c_int;
     pub fn s2s_profile_report(ctx: *mut S2sCtx, wall_ms: f32) -> c_int;
+    pub fn s2s_attention_workspace(args: *const S2sAttentionArgs, bytes: *mut u64) -> c_int;
+    pub fn s2s_attention(args: *const S2sAttentionArgs, workspace: *mut c_void, bytes: u64, stream: *mut c_void) -> c_int;
+    pub fn s2s_rotary(args: *const S2sRotaryArgs, stream: *mut c_void) -> c_int;
+    pub fn s2s_rms_norm(args: *const S2sRmsNormArgs, stream: *mut c_void) -> c_int;
 }
 
 /// The library's message as the crate's `Result` error.

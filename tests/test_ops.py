@@ -155,6 +155,34 @@ def test_argument_packs_are_the_c_structs(pkg, pack, name):
     assert list(leaves(struct.from_buffer_copy(data))) == list(range(1, n + 1))
 
 
+@pytest.mark.parametrize("rust,c,py", [("S2sAttentionArgs", "s2s_attention_args", "Attention_"), ("S2sRotaryArgs", "s2s_rotary_args", "Rotary_"),
+                                       ("S2sRmsNormArgs", "s2s_rms_norm_args", "RmsNorm_"), ("S2sTokens", "s2s_tokens", "Tokens_")])
+def test_structs_are_the_headers(pkg, rust, c, py):
+    """The Rust and Python structs have the header's fields, in its order and of its sizes."""
+    import ctypes as C
+    import re
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (c, c), (root / "include" / "swin2sr_hip.h").read_text(), re.S).group(1)
+    fields = []
+    for decl in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"):
+        m = re.match(r"\s*((?:const )?\w+)\s+(.*)", decl.strip(), re.S)
+        if m:
+            for name in m.group(2).split(","):
+                name = name.strip()
+                fields.append((name.lstrip("*"), "pointer" if name.startswith("*") else m.group(1)))
+    rs = re.search(r"pub struct %s \{(.*?)\n\}" % rust, (root / "swin2sr-rs_amd" / "rust" / "src" / "hip.rs").read_text(), re.S).group(1)
+    rs = re.findall(r"pub (\w+): ([^,\n]+),", rs)
+    kinds = {"int": ("c_int", C.c_int), "float": ("f32", C.c_float), "int64_t": ("i64", C.c_int64), "s2s_tokens": ("S2sTokens", pkg.abi.Tokens_)}
+    assert [n for n, _ in rs] == [n for n, _ in fields] == [n for n, _ in getattr(pkg.abi, py)._fields_]
+    for (name, kind), (_, rt), (_, pt) in zip(fields, rs, getattr(pkg.abi, py)._fields_):
+        if kind == "pointer":
+            assert rt.startswith("*"), name
+            assert C.sizeof(pt) == 8, name
+        else:
+            assert (rt, pt) == kinds[kind], name
+
+
 def test_null_arguments_refused(pkg):
     lib = pkg.load_library()
     assert lib.s2s_attention_workspace(None, None) != 0 and b"null" in lib.s2s_last_error()
