@@ -273,8 +273,9 @@ int s2s_rstb_device(s2s_ctx *ctx, int stage, int hp, int wp, const float *d_in, 
 enum s2s_dtype { S2S_F32 = 0, S2S_F16 = 1, S2S_BF16 = 2, S2S_E4M3 = 3 };
 
 /* An array [batch][tokens][heads][width]: channels are adjacent, the other
- * strides are in elements. They may be any non-negative numbers (0 repeats an
- * input over that dimension); a written array's elements may not overlap. */
+ * strides are in elements. They may be any non-negative numbers up to 2^40 (0
+ * repeats an input over that dimension; k's and v's over the tokens of an attention
+ * up to 2^22); a written array's elements may not overlap. */
 typedef struct s2s_tokens {
     void *data;
     int64_t batch, token, head;
@@ -295,7 +296,8 @@ typedef struct s2s_tokens {
  * Positions differ by less than 2^31. (dy, dx) biases of an image's tokens:
  * positions y * S + x with S at least twice the width less one tell every
  * (dy, dx) apart.
- * Width up to 128. Scores and sums are f32 (f32 arrays: f32 products too); for
+ * Width up to 128, 2^30 k_tokens and 2^30 query tokens times heads of the batch, in
+ * 2^20 batch entries times key heads. Scores and sums are f32 (f32 arrays: f32 products too); for
  * f16 and bf16 the softmax's weights are rounded to that type before they
  * multiply v, except where few queries share them (query tokens times heads per
  * key head up to 16: a step), where what the rounding leaves is kept as well.
@@ -335,7 +337,7 @@ int s2s_attention(const s2s_attention_args *args, void *workspace, uint64_t work
  * on are copied. `inverse` turns the other way (the transpose: the gradient).
  * Angles are reduced in 64-bit fixed point, so far positions lose nothing.
  * Tokens from lens[b] on are not written. The outputs may be the inputs (with
- * the same strides) and may not overlap them otherwise. */
+ * the same strides; q_out q, k_out k) and may not overlap them otherwise. */
 typedef struct s2s_rotary_args {
     int dtype; /* S2S_F32, S2S_F16 or S2S_BF16 */
     int batch, tokens, q_heads, k_heads /* 0: no k */, width;

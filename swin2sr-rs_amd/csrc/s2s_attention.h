@@ -1134,8 +1134,7 @@ hipError_t launch(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
     AttnLaunch M = L;
     M.table_lds = a.table && (long long)a.group * a.table_size <= K::kTabEntries;
     const size_t lds = K::kTab + (M.table_lds ? (size_t)a.group * a.table_size * 4 : 0);
-    const long long blocks = (long long)a.batch * a.hk * L.tiles * L.splits;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    const long long blocks = (long long)a.batch * a.hk * L.tiles * L.splits;  // (below 2^24 by the entry's checks)
     hipLaunchKernelGGL((k_attn<T, DP, NB, WK, ALIGN, MODE>), dim3((unsigned)blocks), dim3(256), lds, st, a, M);
     return hipGetLastError();
 }
@@ -1174,8 +1173,7 @@ hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, 
     else
         e = a.slopes ? launch<T, DP, 2, false, 16, SLOPES>(a, L, st) : launch<T, DP, 2, false, 16, 0>(a, L, st);
     if (e != hipSuccess || L.splits == 1) return e;
-    const long long rows = (long long)a.batch * a.hk * L.cols;
-    if (rows > 0x7fffffffLL) return hipErrorInvalidValue;
+    const long long rows = (long long)a.batch * a.hk * L.cols;  // (few: the keys were split to fill the chip)
     hipLaunchKernelGGL((k_attn_join<T, DP>), dim3((unsigned)rows), dim3(256), 0, st, a, L);
     return hipGetLastError();
 }

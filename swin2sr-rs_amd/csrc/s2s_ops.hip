@@ -133,10 +133,9 @@ hipError_t rotary_of(const RotaryArgs &a, hipStream_t st) {
     // tokens per workgroup: 8 units a thread, fewer where that leaves CUs without work
     const long long units = (long long)(a.hq + a.hk) * per_head, all = (long long)a.batch * a.tokens;
     const long long fill = std::max(1LL, all / (4LL * cu_count()));
-    const int tb = (int)std::max(1LL, std::min({(2048 + units - 1) / units, fill, 16LL}));
-    const long long blocks = (all + tb - 1) / tb;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks);
+    // (a launch holds less than 2^24 workgroups of 256: of 2^30 tokens 65 each, 66 KB of LDS at most)
+    const int tb = (int)std::max({1LL, std::min({(2048 + units - 1) / units, fill, 16LL}), all / 0xffffff + 1});
+    const dim3 grid((unsigned)((all + tb - 1) / tb));
     const size_t lds = (size_t)tb * a.pairs * sizeof(float2);
     switch (v) {
         case 8:
@@ -202,70 +201,72 @@ __device__ __forceinline__ float e4m3_scale(float top) {
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;
 }
 
-// A workgroup per row, any width and alignment: the row is read for the sum of
+// A workgroup per row at a time, any width and alignment: the row is read for the sum of
 // squares and again for the output (and for the scales), from the caches the
 // second time where it fits.
 template <typename T, bool E4M3>
 __global__ __launch_bounds__(256) void k_rms_norm_rows(RmsNormArgs a) {
-    const long long row = blockIdx.x;
-    const T *x = (const T *)a.x + row * a.xs;
-    const T *res = a.res ? (const T *)a.res + row * a.rs : nullptr;
-    T *sum = a.sum ? (T *)a.sum + row * a.ss : nullptr;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __shared__ float part[4];
-    float ss = 0.f;
-    for (int c = tid; c < a.cols; c += 256) {
-        const float h = (float)x[c] + (res ? (float)res[c] : 0.f);
-        ss = fmaf(h, h, ss);
-    }
-    ss = wave_sum(ss);
-    if (lane == 0) part[wave] = ss;
-    __syncthreads();
-    const float mean = ((part[0] + part[1]) + (part[2] + part[3])) / (float)a.cols;
-    const float inv = 1.0f / sqrtf(mean + a.eps);
-    auto value = [&](int c) {
-        const float h = (float)x[c] + (res ? (float)res[c] : 0.f);
-        return h * inv * (a.weight[c] + a.offset);
-    };
-    if constexpr (!E4M3) {
-        T *out = (T *)a.out + row * a.os;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *x = (const T *)a.x + row * a.xs;
+        const T *res = a.res ? (const T *)a.res + row * a.rs : nullptr;
+        T *sum = a.sum ? (T *)a.sum + row * a.ss : nullptr;
+        float ss = 0.f;
         for (int c = tid; c < a.cols; c += 256) {
             const float h = (float)x[c] + (res ? (float)res[c] : 0.f);
-            if (sum) sum[c] = (T)h;
-            out[c] = (T)(h * inv * (a.weight[c] + a.offset));
+            ss = fmaf(h, h, ss);
         }
-    } else {
-        unsigned char *out = (unsigned char *)a.out + row * a.os;
-        float *scales = a.scales + row * a.groups;
-        if (a.groups == 1) {
-            float top = 0.f;
-            for (int c = tid; c < a.cols; c += 256) top = nan_max(top, fabsf(value(c)));
-            __syncthreads();
-#pragma unroll
-            for (int m = 1; m < 64; m *= 2) top = nan_max(top, __shfl_xor(top, m));
-            if (lane == 0) part[wave] = top;
-            __syncthreads();
-            top = nan_max(nan_max(part[0], part[1]), nan_max(part[2], part[3]));
-            const float s = e4m3_scale(top);
-            if (tid == 0) scales[0] = s;
-            for (int c = tid; c < a.cols; c += 256) out[c] = to_e4m3(value(c) / s);
+        ss = wave_sum(ss);
+        if (lane == 0) part[wave] = ss;
+        __syncthreads();
+        const float mean = ((part[0] + part[1]) + (part[2] + part[3])) / (float)a.cols;
+        const float inv = 1.0f / sqrtf(mean + a.eps);
+        auto value = [&](int c) {
+            const float h = (float)x[c] + (res ? (float)res[c] : 0.f);
+            return h * inv * (a.weight[c] + a.offset);
+        };
+        if constexpr (!E4M3) {
+            T *out = (T *)a.out + row * a.os;
+            for (int c = tid; c < a.cols; c += 256) {
+                const float h = (float)x[c] + (res ? (float)res[c] : 0.f);
+                if (sum) sum[c] = (T)h;
+                out[c] = (T)(h * inv * (a.weight[c] + a.offset));
+            }
         } else {
-            for (int g = wave; g < a.groups; g += 4) {  // a wave per group
-                const int c0 = g * a.group, c1 = min(a.cols, c0 + a.group);
+            unsigned char *out = (unsigned char *)a.out + row * a.os;
+            float *scales = a.scales + row * a.groups;
+            if (a.groups == 1) {
                 float top = 0.f;
-                for (int c = c0 + lane; c < c1; c += 64) top = nan_max(top, fabsf(value(c)));
+                for (int c = tid; c < a.cols; c += 256) top = nan_max(top, fabsf(value(c)));
+                __syncthreads();
 #pragma unroll
                 for (int m = 1; m < 64; m *= 2) top = nan_max(top, __shfl_xor(top, m));
+                if (lane == 0) part[wave] = top;
+                __syncthreads();
+                top = nan_max(nan_max(part[0], part[1]), nan_max(part[2], part[3]));
                 const float s = e4m3_scale(top);
-                if (lane == 0) scales[g] = s;
-                for (int c = c0 + lane; c < c1; c += 64) out[c] = to_e4m3(value(c) / s);
+                if (tid == 0) scales[0] = s;
+                for (int c = tid; c < a.cols; c += 256) out[c] = to_e4m3(value(c) / s);
+            } else {
+                for (int g = wave; g < a.groups; g += 4) {  // a wave per group
+                    const int c0 = g * a.group, c1 = min(a.cols, c0 + a.group);
+                    float top = 0.f;
+                    for (int c = c0 + lane; c < c1; c += 64) top = nan_max(top, fabsf(value(c)));
+#pragma unroll
+                    for (int m = 1; m < 64; m *= 2) top = nan_max(top, __shfl_xor(top, m));
+                    const float s = e4m3_scale(top);
+                    if (lane == 0) scales[g] = s;
+                    for (int c = c0 + lane; c < c1; c += 64) out[c] = to_e4m3(value(c) / s);
+                }
+            }
+            // the sum last: it may lie where x or res did
+            if (sum) {
+                __syncthreads();
+                for (int c = tid; c < a.cols; c += 256) sum[c] = (T)((float)x[c] + (res ? (float)res[c] : 0.f));
             }
         }
-        // the sum last: it may lie where x or res did
-        if (sum) {
-            __syncthreads();
-            for (int c = tid; c < a.cols; c += 256) sum[c] = (T)((float)x[c] + (res ? (float)res[c] : 0.f));
-        }
+        __syncthreads();  // the words of `part` are free
     }
 }
 
@@ -447,7 +448,7 @@ hipError_t rms_type(const RmsNormArgs &a, hipStream_t st) {
             return rms_launch<T, E4M3, 4, 64, 4>(a, st);
         }
     }
-    hipLaunchKernelGGL((k_rms_norm_rows<T, E4M3>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_rms_norm_rows<T, E4M3>), dim3((unsigned)std::min(a.rows, 1LL << 20)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

@@ -103,7 +103,11 @@ int check_array(const char *op, const char *name, const void *p, size_t align, i
     return check_memory(op, name, p, dev);
 }
 
-Strides strides(const s2s_tokens &t) { return Strides{t.batch, t.token, t.head}; }
+// The strides the kernels go by: that of a dimension of one counts for nothing, so that it
+// does not spoil the others' alignment either.
+Strides strides(const s2s_tokens &t, int batch, int tokens, int heads) {
+    return Strides{batch > 1 ? t.batch : 0, tokens > 1 ? t.token : 0, heads > 1 ? t.head : 0};
+}
 
 int attention_sizes(const char *op, const s2s_attention_args *a) {
     if (!is_real_type(a->dtype)) return refuse("%s: dtype %d is not f32, f16 or bf16", op, a->dtype);
@@ -116,6 +120,11 @@ int attention_sizes(const char *op, const s2s_attention_args *a) {
     if (a->k_tokens > (1 << 30) || (long long)a->q_tokens * a->q_heads > (1LL << 30))
         return refuse("%s: over 2^30 tokens, or query tokens times heads", op);
     if ((long long)a->batch * a->k_heads > (1 << 20)) return refuse("%s: over 2^20 batch entries times key heads", op);
+    // a workgroup takes 64 such pairs or more, of one batch entry and key head (a launch holds
+    // 2^24 of them)
+    const long long cols = (long long)a->q_tokens * (a->q_heads / a->k_heads);
+    if ((long long)a->batch * a->k_heads * ((cols + 63) / 64) >= (1 << 24))
+        return refuse("%s: over 2^30 query tokens times heads of the batch", op);
     return 0;
 }
 
@@ -135,10 +144,11 @@ AttnOpArgs attention_args(const s2s_attention_args *a) {
     k.k = a->k.data;
     k.v = a->v.data;
     k.out = a->out.data;
-    k.sq = strides(a->q);
-    k.sk = strides(a->k);
-    k.sv = strides(a->v);
-    k.so = strides(a->out);
+    k.sq = strides(a->q, a->batch, a->q_tokens, a->q_heads);
+    k.sk = strides(a->k, a->batch, a->k_tokens, a->k_heads);
+    k.sv = strides(a->v, a->batch, a->k_tokens, a->k_heads);
+    k.so = strides(a->out, a->batch, a->q_tokens, a->q_heads);
+    if (a->k_tokens <= 1) k.sk.t = k.sv.t = a->width;  // (a tile's rows past the last do not overlap it)
     k.q_lens = a->q_lens;
     k.k_lens = a->k_lens;
     k.prefix = a->prefix;
@@ -185,6 +195,9 @@ int s2s_attention(const s2s_attention_args *a, void *workspace, uint64_t workspa
         a->q_docs_batch > kMaxStride || a->k_docs_batch > kMaxStride || a->q_pos_batch > kMaxStride ||
         a->k_pos_batch > kMaxStride)
         return refuse("%s: a negative or impossible batch stride", op);
+    // (a wave per key tile, of 32 keys at least, makes the documents' summary)
+    if (a->k_docs && (long long)a->batch * ((a->k_tokens + 31LL) / 32) >= (1 << 26))
+        return refuse("%s: documents of over 2^31 keys of the batch", op);
     if (a->batch == 0 || a->q_tokens == 0) return 0;
     OnDevice on;
     const hipStream_t st = (hipStream_t)stream;
@@ -197,7 +210,7 @@ int s2s_attention(const s2s_attention_args *a, void *workspace, uint64_t workspa
         if (int rc = check_tokens(op, "k", a->k, a->dtype, on.dev)) return rc;
         if (int rc = check_tokens(op, "v", a->v, a->dtype, on.dev)) return rc;
         // 64 tokens of a tile are reached by 32-bit byte offsets from its first
-        if (a->k.token > (1 << 22) || a->v.token > (1 << 22))
+        if (a->k_tokens > 1 && (a->k.token > (1 << 22) || a->v.token > (1 << 22)))
             return refuse("%s: a token stride of k or v over 2^22 elements", op);
     }
     if (a->out.data == a->q.data || a->out.data == a->k.data || a->out.data == a->v.data)
@@ -242,6 +255,11 @@ int s2s_rotary(const s2s_rotary_args *a, void *stream) {
     }
     if (a->pos_batch < 0 || a->pos_batch > kMaxStride) return refuse("%s: a negative or impossible batch stride", op);
     if (a->batch == 0 || a->tokens == 0) return 0;
+    if (a->k_heads > 0 && a->q_out.data && a->k_out.data == a->q_out.data)
+        return refuse("%s: q_out and k_out are the same array", op);
+    // (other workgroups may not have read the other input yet)
+    if (a->k_heads > 0 && a->q_out.data && (a->q_out.data == a->k.data || a->k_out.data == a->q.data))
+        return refuse("%s: q's output is k, or k's is q", op);
     OnDevice on;
     const hipStream_t st = (hipStream_t)stream;
     hipError_t e = on.enter(st);
@@ -254,7 +272,6 @@ int s2s_rotary(const s2s_rotary_args *a, void *stream) {
         if (int rc = check_tokens(op, "k", a->k, a->dtype, on.dev)) return rc;
         if (int rc = check_tokens(op, "k_out", a->k_out, a->dtype, on.dev)) return rc;
         if (int rc = check_written(op, "k_out", a->k_out, a->batch, a->tokens, a->k_heads, a->width)) return rc;
-        if (a->k_out.data == a->q_out.data) return refuse("%s: q_out and k_out are the same array", op);
     }
     auto same = [](const s2s_tokens &x, const s2s_tokens &y) {
         return x.data != y.data || (x.batch == y.batch && x.token == y.token && x.head == y.head);
@@ -276,13 +293,13 @@ int s2s_rotary(const s2s_rotary_args *a, void *stream) {
     k.adjacent = a->adjacent != 0;
     k.q = a->q.data;
     k.qo = a->q_out.data;
-    k.sq = strides(a->q);
-    k.sqo = strides(a->q_out);
+    k.sq = strides(a->q, a->batch, a->tokens, a->q_heads);
+    k.sqo = strides(a->q_out, a->batch, a->tokens, a->q_heads);
     if (has_k) {
         k.k = a->k.data;
         k.ko = a->k_out.data;
-        k.sk = strides(a->k);
-        k.sko = strides(a->k_out);
+        k.sk = strides(a->k, a->batch, a->tokens, a->k_heads);
+        k.sko = strides(a->k_out, a->batch, a->tokens, a->k_heads);
     }
     k.pos = a->pos;
     k.pos_b = a->pos_batch;
@@ -341,7 +358,7 @@ int s2s_rms_norm(const s2s_rms_norm_args *a, void *stream) {
     for (int i = 2; i < 4; ++i)
         for (int j = 0; j < 2; ++j)
             if (arrays[i].p && arrays[i].p == arrays[j].p &&
-                (arrays[i].stride != arrays[j].stride || (i == 3 && q8)))
+                ((a->rows > 1 && arrays[i].stride != arrays[j].stride) || (i == 3 && q8)))
                 return refuse("%s: %s is %s but not in its rows' places", op, arrays[i].name, arrays[j].name);
     if (a->sum && a->sum == a->out) return refuse("%s: sum and out are the same array", op);
     if (int rc = check_array(op, "weight", a->weight, 4, on.dev)) return rc;
@@ -356,10 +373,11 @@ int s2s_rms_norm(const s2s_rms_norm_args *a, void *stream) {
     k.res = a->res;
     k.sum = a->sum;
     k.out = a->out;
-    k.xs = a->x_stride;
-    k.rs = a->res_stride;
-    k.ss = a->sum_stride;
-    k.os = a->out_stride;
+    const bool many = a->rows > 1;  // (one row's stride counts for nothing)
+    k.xs = many ? a->x_stride : 0;
+    k.rs = many ? a->res_stride : 0;
+    k.ss = many ? a->sum_stride : 0;
+    k.os = many ? a->out_stride : 0;
     k.weight = a->weight;
     k.offset = a->weight_offset;
     k.eps = a->eps;

@@ -76,6 +76,11 @@ def _need(ok, what: str):
         raise S2SError(what)
 
 
+def _f32(x) -> float:
+    """As a C float takes it: an infinity (which the library refuses) past its range."""
+    return C.c_float(x).value
+
+
 def _contiguous(a) -> bool:
     n = 1
     for d, s in zip(reversed(tuple(a.shape)), reversed(tuple(a.stride()))):
@@ -141,7 +146,7 @@ class Attention:
         self.lib = load_library()
         self.dtype = _type(dtype)
         self.head = (self.dtype, batch, q_tokens, k_tokens, q_heads, k_heads, width, int(bool(causal)),
-                     float(scale) if scale is not None else max(width, 1) ** -0.5, float(cap))
+                     _f32(scale) if scale is not None else max(width, 1) ** -0.5, _f32(cap))
         self.batch, self.q_tokens, self.k_tokens, self.q_heads = batch, q_tokens, k_tokens, q_heads
         self.q_shape, self.k_shape = (batch, q_tokens, q_heads, width), (batch, k_tokens, k_heads, width)
         a = Attention_(*self.head)
@@ -293,7 +298,8 @@ def rms_norm(x, weight, out, eps: float = 1e-6, res=None, sum=None, scales=None,
         _need(scales.shape == (rows, n) and _is_f32(scales.dtype) and _contiguous(scales),
               f"{op}: scales is no contiguous f32 [{rows}][{n}]")
         scale_ptr = scales.data_ptr()
-    args = _RMS.pack(dt, odt, rows, cols, xp, rp, sp, op_, xs, rs, ss, os_, weight.data_ptr(), weight_offset, eps, scale_ptr, group)
+    args = _RMS.pack(dt, odt, rows, cols, xp, rp, sp, op_, xs, rs, ss, os_, weight.data_ptr(), _f32(weight_offset), _f32(eps), scale_ptr,
+                     group)
     if load_library().s2s_rms_norm(args, stream):
         raise S2SError(f"{op}: {last_error()}")
     return out

@@ -807,3 +807,67 @@ def test_rms_norm_rows_apart(pkg, cols, e4m3):
         x[3], r[3] = x[3] * 1e-12, r[3] * 1e-12
     rms_case(pkg, "f32", 6, cols, e4m3=e4m3, group=0, change=change)
     rms_case(pkg, "f32", 6, cols, e4m3=e4m3, group=64 if e4m3 else 0, change=change)
+
+
+# ---- more rows than one launch holds, dimensions of one -------------------------------------
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_rms_norm_more_rows_than_workgroups(pkg, e4m3):
+    """2^24 + 5 rows of 3: every row the same (its stride is 0), so that each is the first one."""
+    rows, cols = 2 ** 24 + 5, 3
+    x, w = R.Dev(pkg, R.round_to(np.array([[1.5, -2.25, 0.125]]), "f16"), "f16"), R.Dev(pkg, np.array([1.0, 0.5, 2.0]), "f32")
+    out = pkg.hip.DeviceBuffer((rows * cols * (1 if e4m3 else 2) + 3) // 4)
+    out.upload(np.full(out.n, np.nan, np.float32))
+    scales = pkg.hip.DeviceBuffer(rows)
+    A = pkg.ops.Array
+    pkg.ops.rms_norm(A(x.array.ptr, (rows, cols), "f16", (0, 1)), w.array, A(out.ptr, (rows, cols), "e4m3" if e4m3 else "f16"),
+                     scales=A(scales.ptr, (rows, 1), "f32") if e4m3 else None)
+    pkg.hip.synchronize()
+    got = out.download().view(np.uint8 if e4m3 else np.float16)[:rows * cols].reshape(rows, cols)
+    h = np.array([1.5, -2.25, 0.125])
+    want = h / np.sqrt((h * h).mean() + np.float64(np.float32(1e-6))) * np.array([1.0, 0.5, 2.0])
+    # one rounding to f16 (one of e4m3 after the scale), and a dozen f32 ones before it
+    first = R.e4m3_values()[got[0]] * (np.abs(want).max() / 448) if e4m3 else got[0].astype(np.float64)
+    assert (np.abs(first - want) <= (2.0 ** -4 if e4m3 else 2.0 ** -11) * np.abs(want) + 24 * 2.0 ** -24 * np.abs(want)).all()
+    assert (got == got[0]).all()
+    if e4m3:
+        s = scales.download()
+        assert (s == s[0]).all() and abs(s[0] / (np.abs(want).max() / 448) - 1) <= 24 * 2.0 ** -24
+    out.free()
+    scales.free()
+
+
+def test_rotary_more_tokens_than_workgroups(pkg):
+    """2^28 + 2^14 tokens of one pair, the batch's entries all the same: each is the first one."""
+    batch, tokens = 2 ** 14 + 1, 2 ** 14
+    g = np.random.default_rng(3)
+    q = R.Dev(pkg, R.round_to(g.standard_normal((1, tokens, 1, 2)), "f16"), "f16")
+    pos = R.Dev(pkg, g.integers(0, 2 ** 31 - 1, (1, tokens, 1)).astype(np.int32), "f32", whole=True)
+    out, one = pkg.hip.DeviceBuffer(batch * tokens), R.Dev(pkg, np.zeros((1, tokens, 1, 2)), "f16")
+    rot, A = pkg.ops.Rotary([0.7], [0]), pkg.ops.Array
+    rot(q.array, pos.array, one.array)
+    rot(A(q.array.ptr, (batch, tokens, 1, 2), "f16", (0, 2, 2, 1)), A(pos.array.ptr, (tokens, 1), "i32"),
+        A(out.ptr, (batch, tokens, 1, 2), "f16"))
+    pkg.hip.synchronize()
+    want = one.bits().view(np.uint32).reshape(-1)[:tokens]
+    got = out.download().view(np.uint32).reshape(batch, tokens)
+    out.free()
+    assert (got == want).all()
+
+
+@pytest.mark.parametrize("Lq,Lk", [(1, 1), (1, 70), (5, 1)])
+def test_attention_strides_of_one(pkg, Lq, Lk):
+    """The stride of a dimension of one counts for nothing: odd, zero, or far past any array."""
+    c = case("bf16", Lq=Lq, Lk=Lk, H=2, KV=1, D=64)
+    q, k, v, more = inputs(c)
+    plan, ws, scale = make_plan(pkg, c)
+    d, m = upload(pkg, c, q, k, v, more)
+    want, bound, _ = R.attention("bf16", q, k, v, scale)
+    for odd in (0, 1, (1 << 23) + 1):
+        def moved(a, n):
+            b, t, h, w = a.stride()
+            return pkg.ops.Array(a.ptr, a.shape, a.dtype, (odd, odd if n == 1 else t, odd if a.shape[2] == 1 else h, w))
+        d["out"].buf.upload(np.zeros(d["out"].buf.n, np.float32))
+        plan(moved(d["q"].array, Lq), moved(d["k"].array, Lk), moved(d["v"].array, Lk), moved(d["out"].array, Lq), workspace=ws.array)
+        assert (np.abs(d["out"].get() - want) <= bound).all()

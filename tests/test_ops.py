@@ -119,6 +119,45 @@ def test_rms_norm_refused(pkg, x, out, more, word):
         pkg.ops.rms_norm(arr(pkg, *x), arr(pkg, (x[0][1],), "f32"), arr(pkg, *out, ptr=8192), **more)
 
 
+@pytest.mark.parametrize("more,fewer", [
+    (dict(batch=2 ** 10, q_tokens=2 ** 21, q_heads=1, k_heads=1), 2 ** 20 - 64),
+    (dict(batch=2 ** 19, q_tokens=2 ** 11 - 63, q_heads=2, k_heads=2), 2 ** 10 - 64),
+    (dict(batch=1, q_tokens=2 ** 30 - 63, q_heads=1, k_heads=1), 2 ** 30 - 64),
+])
+def test_attention_more_than_a_launch_refused(pkg, more, fewer):
+    """Query tokens times heads of the whole batch: a launch holds less than 2^24 tiles of 64."""
+    with pytest.raises(pkg.S2SError, match="of the batch"):
+        plan(pkg, **more)
+    assert plan(pkg, **{**more, "q_tokens": fewer}).workspace_bytes > 0
+
+
+def test_attention_more_documents_than_a_launch_refused(pkg):
+    b, nk = 2 ** 13, 2 ** 18
+    p = plan(pkg, batch=b, k_tokens=nk, q_heads=2, k_heads=2, q_tokens=1)
+    a = [arr(pkg, (b, n, 2, 64)) for n in (1, nk, nk, 1)]
+    with pytest.raises(pkg.S2SError, match="documents"):
+        p(*a, q_docs=arr(pkg, (1,), "i32"), k_docs=arr(pkg, (nk,), "i32"))
+
+
+@pytest.mark.parametrize("big", [1e39, -1e39, 1e300])
+def test_numbers_past_a_float_refused(pkg, big):
+    for more in (dict(scale=big), dict(cap=big)):
+        with pytest.raises(pkg.S2SError, match="scale|cap"):
+            plan(pkg, **more)(**tensors(pkg))
+    for more in (dict(eps=big), dict(weight_offset=big)):
+        with pytest.raises(pkg.S2SError, match="eps"):
+            pkg.ops.rms_norm(arr(pkg, (4, 8), "f32"), arr(pkg, (8,), "f32"), arr(pkg, (4, 8), "f32"), **more)
+
+
+@pytest.mark.parametrize("name", ["q_out", "k_out"])
+def test_rotary_across_refused(pkg, name):
+    """q's output where k lies, or k's where q lies: read by other workgroups still."""
+    q, k, o = (arr(pkg, (1, 4, 2, 64), ptr=4096 * (1 + i)) for i in range(3))
+    out = dict(q_out=k, k_out=o) if name == "q_out" else dict(q_out=o, k_out=q)
+    with pytest.raises(pkg.S2SError, match="q's output is k"):
+        pkg.ops.Rotary.of((16, 16))(q, arr(pkg, (1, 4, 2), "i32"), k=k, **out)
+
+
 def test_nothing_to_do(pkg):
     """No row, no token: done without a device or an address."""
     none = arr(pkg, (0, 8), "f32", ptr=0)
