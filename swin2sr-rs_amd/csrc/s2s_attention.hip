@@ -6,9 +6,18 @@ namespace {
 
 int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
-// Columns of at most 16 share one set of waves that split each key tile; more take
-// waves of 16 or 32 columns. Where that leaves CUs without work the keys are cut
-// into ranges whose sums a second kernel joins. `narrow`: waves of 16 only.
+// Columns of at most 16 share one set of waves that split each key tile (f32 64 wide,
+// one query of 8192 keys, 32 / 8 heads: 13.6 us against 18.8 by waves of 16 of which one works; 16-bit
+// types are as fast either way, and keep what the weights' rounding leaves). More take waves
+// of 16 columns, or of 32 where those give every CU two workgroups: a key tile's LDS reads then serve
+// two products (2 x 4096 causal bf16, 32 / 8 heads: 128 wide 278 us against 366 by waves of 16,
+// 64 wide 167 and 200; 2048 tokens of 16 / 4 heads, too few, 103 and 43). `narrow`: waves of 16 only.
+// Where few columns leave CUs without work the keys are cut into ranges whose sums a second
+// kernel joins, up to two workgroups a CU (four: nothing for one query, 32 us against 15 for 64
+// sequences of 4 queries and 512 keys, by the join). Ranges of four tiles at least; of two, and up to 16
+// of one, for columns of at most 16, whose rows to join are few: one query of 32 / 8 bf16 heads of 128 over 512,
+// 1024, 2048 and 4096 keys takes 9.1, 9.1, 9.9 and 10.5 us against 11.4 to 11.7, but over 256 keys
+// 9.0 against 8.1 uncut; 64 queries of 8 sequences over 256 keys 20 against 9.5.
 attn::Cut cut_of(int dtype, const AttnOpArgs &a, bool narrow) {
     attn::Cut c;
     const long long cols = (long long)a.group * a.nq, pairs = (long long)a.batch * a.hk;
@@ -19,10 +28,9 @@ attn::Cut cut_of(int dtype, const AttnOpArgs &a, bool narrow) {
     c.tk = dtype == 0 && !c.wk && c.dp > 64 ? 32 : 64;
     const int per = c.wk ? 16 : 64 * c.nb;
     c.tiles = (int)((cols + per - 1) / per);
-    // ranges of 4 tiles at least, workgroups for two per CU (four of the narrow ones) at most
-    const long long blocks = std::max(1LL, pairs * c.tiles), want = (c.wk && c.dp <= 64 ? 4LL : 2LL) * cus;
-    const long long nt = ((long long)a.nk + c.tk - 1) / c.tk;
-    c.splits = (int)std::max(1LL, std::min({want / blocks, nt / 4, 256LL}));
+    const long long blocks = std::max(1LL, pairs * c.tiles), nt = ((long long)a.nk + c.tk - 1) / c.tk;
+    const long long ranges = c.wk && nt > 4 ? std::max({nt / 4, std::min(nt / 2, 32LL), std::min(nt, 16LL)}) : nt / 4;
+    c.splits = (int)std::max(1LL, std::min({2LL * cus / blocks, ranges, 256LL}));
     return c;
 }
 

@@ -1,9 +1,9 @@
 // s2s_ops.hip - rotary positions with several axes, and the root-mean-square
 // norm with the residual's addition and an e4m3 output. Both are bound by HBM:
 // every element is read once and written once. Measured on an MI355X, whose plain
-// copy of 1 GiB makes 5.05 TB/s: rotary of 16384 tokens, 32 + 8 bf16 heads of 128, 72 us
-// (4.65 TB/s); the norm of 16391 x 5120 bf16 with residual, sum and e4m3 groups of 128, 121 us
-// (4.86 TB/s). Steps (4 rows, 32 tokens) take 4 to 5 us, a launch and two or three reads that
+// copy of 1 GiB makes 5.05 TB/s: rotary of 16384 tokens, 32 + 8 bf16 heads of 128, 64 us
+// (5.2 TB/s); the norm of 16391 x 5120 bf16 with residual, sum and e4m3 groups of 128, 115 us
+// (5.1 TB/s). Steps (4 rows, 32 tokens) take 4 to 5 us, a launch and two or three reads that
 // wait for each other.
 #include <algorithm>
 #include <cmath>
@@ -47,7 +47,7 @@ __device__ __forceinline__ void sincos_turns(unsigned long long f, float &s, flo
 // LDS; then the threads walk the tokens' heads in memory order, a unit of V pairs (or of
 // V channels that are copied) at a time, neighbours next to each other across heads, so
 // that a wave's accesses are whole runs whatever the width. (A thread that kept its
-// angles in registers and looped over heads touched a run per head: 45 us against 37 for
+// angles in registers and looped over heads touched a run per head: 45 us against 38 for
 // 2 x 23400 tokens of 6 + 6 f32 heads of 30, of which every run is 120 bytes.)
 template <typename T, bool ADJ, int V, bool ALIGNED = true>
 __global__ __launch_bounds__(256) void k_rotary(RotaryArgs a, int tb, int per_head) {
@@ -130,11 +130,14 @@ hipError_t rotary_of(const RotaryArgs &a, hipStream_t st) {
     while (v > 1 && (a.pairs % v || (a.width - 2 * a.pairs) % v)) v /= 2;
     v = std::max(v, 1);
     const int per_head = (a.pairs + a.width - 2 * a.pairs) / v;
-    // tokens per workgroup: 8 units a thread, fewer where that leaves CUs without work
+    // tokens per workgroup: a unit for every thread and 128 sines at least, since the threads past
+    // them idle there; fewer where that leaves CUs without work. (16384 tokens, 32 + 8 bf16 heads of 128:
+    // 64 us, 72 by 8 units a thread; 2 x 23400, 6 + 6 f32 heads of 30, whose tokens have 15 sines:
+    // 38 and 37 us, 42 by a unit a thread alone. Reading a unit's channels ahead of the sines, 55 and 73.)
     const long long units = (long long)(a.hq + a.hk) * per_head, all = (long long)a.batch * a.tokens;
     const long long fill = std::max(1LL, all / (4LL * cu_count()));
     // (a launch holds less than 2^24 workgroups of 256: of 2^30 tokens 65 each, 66 KB of LDS at most)
-    const int tb = (int)std::max({1LL, std::min({(2048 + units - 1) / units, fill, 16LL}), all / 0xffffff + 1});
+    const int tb = (int)std::max({1LL, std::min({std::max((256 + units - 1) / units, (128LL + a.pairs - 1) / a.pairs), fill, 16LL}), all / 0xffffff + 1});
     const dim3 grid((unsigned)((all + tb - 1) / tb));
     const size_t lds = (size_t)tb * a.pairs * sizeof(float2);
     switch (v) {
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(256) void k_rms_norm_rows(RmsNormArgs a) {
 
 // The rows of a workgroup in registers: TPR threads a row (256 / TPR rows at once), NC
 // chunks of V elements (16 or 8 bytes) a thread, so that x and the residual are read once and
-// nothing is read again (rows read twice, k_rms_norm_rows: 450 us for the 16391 x 5120 above);
+// nothing is read again (rows read twice, k_rms_norm_rows: 493 us for the 16391 x 5120 above);
 // the weights stay in registers over the rows that the workgroup walks. A group of the scales is a power of two of chunks, which neighbouring lanes hold.
 template <typename T, bool E4M3, int V, int TPR, int NC>
 __global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
@@ -389,10 +392,14 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
                 const int i = n * TPR + tr;
-                const float s = e4m3_scale(top[n]), r = 1.0f / s;
+                // h / s as h times 1 / s in two words: with the reciprocal's own rounding more values
+                // land on the other side of a code's border (31925 x 720 bf16, groups of 64: 3.2e-5 of the
+                // values away from a division's codes, 1.8e-5 so; no time)
+                const float s = e4m3_scale(top[n]), r = 1.0f / s, low = r == 0.f ? 0.f : fmaf(-r, s, 1.f) * r;
+                auto code_of = [&](float v) { return fmaf(v, r, v * low); };
                 VecOf<unsigned, V / 4> code;
 #pragma unroll
-                for (int e = 0; e < V; e += 4) code.e[e / 4] = to_e4m3x4(h[n][e] * r, h[n][e + 1] * r, h[n][e + 2] * r, h[n][e + 3] * r);
+                for (int e = 0; e < V; e += 4) code.e[e / 4] = to_e4m3x4(code_of(h[n][e]), code_of(h[n][e + 1]), code_of(h[n][e + 2]), code_of(h[n][e + 3]));
                 if (i < chunks) {
                     *(VecOf<unsigned, V / 4> *)(out + i * V) = code;
                     if (a.groups == 1 ? i == 0 : (lane & (gl - 1)) == 0) scales[a.groups == 1 ? 0 : i / gl] = s;
@@ -405,8 +412,9 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
 template <typename T, bool E4M3, int V, int TPR, int NC>
 hipError_t rms_launch(const RmsNormArgs &a, hipStream_t st) {
     const long long blocks = (a.rows + 256 / TPR - 1) / (256 / TPR);
-    // at most 8 workgroups a CU, which then walk their rows with the weights at hand
-    const long long most = 8LL * cu_count();
+    // at most 32 workgroups a CU, which then walk their rows with the weights at hand (16391 x 5120
+    // bf16 to e4m3: 117 us, 122 with 8, 120 with 64)
+    const long long most = 32LL * cu_count();
     hipLaunchKernelGGL((k_rms_norm<T, E4M3, V, TPR, NC>), dim3((unsigned)std::min(blocks, most)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
@@ -430,17 +438,18 @@ hipError_t rms_type(const RmsNormArgs &a, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
     const int chunks = a.cols / V;
     if (rms_takes<T, E4M3, V>(a, 8 * 256)) {
-        // a wave per row up to 2 chunks a lane, and up to 4 where there are rows for the chip
-        const bool many = a.rows >= 16LL * cu_count();
+        // a wave per row up to 2 chunks a lane (16384 x 1024 bf16 to e4m3: 22 us, 28 by a workgroup per
+        // row), where there are rows for the chip (64 rows: 4.4 us, 3.4 by a workgroup each); 4 chunks
+        // a lane (65536 x 2048: 183 us, 179 by a workgroup per row) gain nothing
         if (chunks <= 64) return rms_launch<T, E4M3, V, 64, 1>(a, st);
-        if (chunks <= 128) return rms_launch<T, E4M3, V, 64, 2>(a, st);
-        if (chunks <= 256) return many ? rms_launch<T, E4M3, V, 64, 4>(a, st) : rms_launch<T, E4M3, V, 256, 1>(a, st);
+        if (chunks <= 128 && a.rows >= 4LL * cu_count()) return rms_launch<T, E4M3, V, 64, 2>(a, st);
+        if (chunks <= 256) return rms_launch<T, E4M3, V, 256, 1>(a, st);
         if (chunks <= 512) return rms_launch<T, E4M3, V, 256, 2>(a, st);
         if (chunks <= 768) return rms_launch<T, E4M3, V, 256, 3>(a, st);
         if (chunks <= 1024) return rms_launch<T, E4M3, V, 256, 4>(a, st);
         return rms_launch<T, E4M3, V, 256, 8>(a, st);
     }
-    // 16-bit rows of 8-byte multiples (180 or 60 columns): 45412 x 180 f16 to e4m3 took 74 us by
+    // 16-bit rows of 8-byte multiples (180 or 60 columns): 45412 x 180 f16 to e4m3 21 us, 74 us by
     // rows read twice
     if constexpr (sizeof(T) == 2) {
         if (rms_takes<T, E4M3, 4>(a, 4 * 64)) {
