@@ -871,3 +871,23 @@ def test_attention_strides_of_one(pkg, Lq, Lk):
         d["out"].buf.upload(np.zeros(d["out"].buf.n, np.float32))
         plan(moved(d["q"].array, Lq), moved(d["k"].array, Lk), moved(d["v"].array, Lk), moved(d["out"].array, Lq), workspace=ws.array)
         assert (np.abs(d["out"].get() - want) <= bound).all()
+
+
+# ---- key ranges joined column by column -----------------------------------------------------
+
+JOIN = {
+    "bf16_128": case("bf16", Lq=140, Lk=1500, H=8, KV=8, D=128, causal=True),
+    "f16_96": case("f16", Lq=140, Lk=1500, H=8, KV=4, D=96, cap=20.0),
+    "f32_64": case("f32", Lq=140, Lk=900, H=8, KV=8, D=64, slopes=True, causal=True),
+    "f32_32": case("f32", Lq=260, Lk=800, H=6, KV=6, D=30, order="cache", gap=2),
+    "odd": case("bf16", Lq=140, Lk=1100, H=8, KV=2, D=17, gap=1, lead=1, causal=True),
+    "two": case("f16", Lq=140, Lk=1300, H=8, KV=8, D=34, gap=2),
+    "lengths": case("bf16", B=4, Lq=70, Lk=1024, H=8, KV=4, D=80, causal=True, q_lens=[70, 0, 33, 70], k_lens=[1024, 900, 20, 0]),
+    "prefix": case("bf16", B=2, Lq=90, Lk=1024, H=8, KV=8, D=64, causal=True, prefix=[1000, 0], cap=50.0),
+    "step": case("bf16", B=40, Lq=1, Lk=512, H=32, KV=8, D=128, order="cache", causal=True, k_lens=[1 + 13 * i for i in range(40)]),
+}
+
+
+@pytest.mark.parametrize("name", JOIN)
+def test_attention_few_ranges(pkg, name):
+    check_attention(pkg, JOIN[name])
