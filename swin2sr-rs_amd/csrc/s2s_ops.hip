@@ -206,7 +206,8 @@ __device__ __forceinline__ float e4m3_scale(float top) {
 
 // A workgroup per row at a time, any width and alignment: the row is read for the sum of
 // squares and again for the output (and for the scales), from the caches the
-// second time where it fits.
+// second time where it fits. (45412 x 177 f16 38 us, to e4m3 75; with its elements one by one
+// in registers, 32 a thread, a row of 5121 took twice as long: 278 us for 16391 of them, 599 so.)
 template <typename T, bool E4M3>
 __global__ __launch_bounds__(256) void k_rms_norm_rows(RmsNormArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;

@@ -891,3 +891,38 @@ JOIN = {
 @pytest.mark.parametrize("name", JOIN)
 def test_attention_few_ranges(pkg, name):
     check_attention(pkg, JOIN[name])
+
+
+# ---- rows of odd widths and addresses ------------------------------------------------
+
+ODD = {
+    "wave": dict(dtype="f16", rows=2001, cols=177, gap=1, lead=1),
+    "wave_row": dict(dtype="bf16", rows=1501, cols=177, e4m3=True, lead=1),
+    "wave_groups": dict(dtype="f16", rows=1030, cols=1023, e4m3=True, group=128, gap=1),
+    "wave_group_8": dict(dtype="f32", rows=1027, cols=333, e4m3=True, group=8, alias=("sum",)),
+    "wave_group_24": dict(dtype="bf16", rows=1025, cols=1024, e4m3=True, group=24),
+    "wave_group_past_row": dict(dtype="bf16", rows=1025, cols=77, e4m3=True, group=80),
+    "in_place": dict(dtype="f32", rows=1100, cols=61, alias=("sum", "out")),
+    "widest": dict(dtype="bf16", rows=5, cols=8191, lead=1),
+    "widest_groups": dict(dtype="bf16", rows=5, cols=8191, lead=1, e4m3=True, group=8),
+    "group_1000": dict(dtype="f32", rows=9, cols=8192, e4m3=True, group=1000),
+    "past": dict(dtype="f16", rows=5, cols=8193, e4m3=True, group=200),
+}
+
+
+@pytest.mark.parametrize("name", ODD)
+def test_rms_norm_odd_rows(pkg, name):
+    rms_case(pkg, **ODD[name])
+
+
+@pytest.mark.parametrize("cols,rows", [(179, 1030), (4095, 6)])
+@pytest.mark.parametrize("group", [0, 64])
+def test_rms_norm_odd_rows_apart(pkg, cols, rows, group):
+    """Rows of zeros, of NaN, of the largest and of tiny values: each its own."""
+    def change(x, r):
+        x[0], r[0] = 0, 0
+        x[1, 3] = np.nan
+        x[2], r[2] = x[2] * 1e15, r[2] * 1e15
+        x[3], r[3] = x[3] * 1e-12, r[3] * 1e-12
+    rms_case(pkg, "f32", rows, cols, e4m3=True, group=group, change=change)
+    rms_case(pkg, "f32", rows, cols, change=change)
