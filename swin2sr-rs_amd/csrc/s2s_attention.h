@@ -361,6 +361,9 @@ struct Kernel {
     typedef typename Ty::V Vec;
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int E = Ty::kElems;
+    // keys per tile: 64, so that the barriers and the softmax's steps across lanes come half as often
+    // (2048 f32 tokens, 64 wide, 147 us against 160 with 32; windows of 16 x 16, 57 and 73); 32 for f32 rows
+    // over 64 wide, whose two buffers of 64 would fill 128 KB and leave a CU one workgroup
     static constexpr int TK = F32 && !WK && DP > 64 ? 32 : 64;
     static constexpr int KB = WK ? 1 : TK / 16;          // key blocks per wave
     static constexpr int KS = DP / (4 * E);              // steps of four chunks
