@@ -94,7 +94,8 @@ __global__ __launch_bounds__(256) void k_doc_columns(AttnOpArgs a, int tk, int k
 }
 
 // Column tiles by falling number of key tiles, to 256 steps: a workgroup per batch
-// entry. (Tiles of one step come in any order; no result goes by it.)
+// entry. (Tiles of one step come in any order; no result goes by it. Nine images of different sizes, 11003
+// tokens: 120 us, 165 in the tokens' order.)
 __global__ __launch_bounds__(256) void k_doc_order(int tiles, const int4 *col, int *order) {
     __shared__ int bin[256], most;
     const int tid = threadIdx.x;
@@ -121,6 +122,80 @@ __global__ __launch_bounds__(256) void k_doc_order(int tiles, const int4 *col, i
     bin[tid] = n;
     __syncthreads();
     for (int t = tid; t < tiles; t += 256) order[atomicAdd(&bin[of(t)], 1)] = t;
+}
+
+// The three above in one launch, a workgroup of 16 waves per batch entry, for up to 64 key and
+// 64 column tiles: 16 lanes a tile for the ids, a wave per column tile for its live key tiles. (12 bf16
+// heads of 64: 1000 tokens 29 us, 33 by the three; 3000 61 and 65; with more tiles one workgroup
+// takes longer than the launches, 11003 tokens 161 and 158, 65536 885 and 750.)
+constexpr int kDocTiles = 64;
+__global__ __launch_bounds__(1024) void k_doc_all(AttnOpArgs a, int tk, int key_tiles, int per, int tiles, int4 *meta, int4 *col,
+                                                  int *order) {
+    __shared__ int2 keys[kDocTiles];
+    __shared__ int4 cols[kDocTiles];
+    __shared__ int bin[256], most;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = tid & 15, b = blockIdx.x;
+    meta += (long long)b * key_tiles, col += (long long)b * tiles;
+    const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.nk) : a.nk;
+    const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
+    const int *kd = a.k_docs + b * a.k_docs_b, *qd = a.q_docs + b * a.q_docs_b;
+    // {smallest id >= 0, largest, smallest of all} of ids[first .. last], in all 16 lanes
+    auto ids = [&](const int *p, int first, int last) {
+        int lo = 0x7fffffff, hi = -1, all = 0x7fffffff;
+        for (int i = first + sub; i <= last; i += 16) {
+            const int d = p[i];
+            all = min(all, d);
+            if (d >= 0) lo = min(lo, d), hi = max(hi, d);
+        }
+#pragma unroll
+        for (int m = 1; m < 16; m *= 2) {
+            lo = min(lo, __shfl_xor(lo, m));
+            hi = max(hi, __shfl_xor(hi, m));
+            all = min(all, __shfl_xor(all, m));
+        }
+        return make_int4(lo, hi, all, 0);
+    };
+    const int t = tid >> 4;
+    if (t < key_tiles) {
+        const int4 x = ids(kd, t * tk, min(kl, t * tk + tk) - 1);
+        if (sub == 0) meta[t] = x, keys[t] = make_int2(x.x, x.y);
+    }
+    if (t < tiles) {
+        const int4 x = ids(qd, t * per / a.group, min(ql - 1, (t * per + per - 1) / a.group));
+        if (sub == 0) cols[t] = x;
+    }
+    if (tid < 256) bin[tid] = 0;
+    if (tid == 0) most = 1;
+    __syncthreads();
+    for (int t = wave; t < tiles; t += 16) {
+        int4 x = cols[t];
+        const int2 y = keys[min(lane, key_tiles - 1)];
+        x.w = __popcll(__ballot(lane < key_tiles && y.x <= x.y && y.y >= x.x));
+        if (lane == 0) col[t] = cols[t] = x, atomicMax(&most, x.w);
+    }
+    if (!order) return;  // (all of the workgroup)
+    order += (long long)b * tiles;
+    __syncthreads();
+    const float step = 255.f / (float)most;
+    auto of = [&](int t) { return 255 - min(255, (int)((float)cols[t].w * step)); };
+    if (tid < tiles) atomicAdd(&bin[of(tid)], 1);
+    __syncthreads();
+    if (wave == 0) {  // four bins a lane to the sums before them
+        int n[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n[i] = bin[4 * lane + i], sum += n[i];
+        int before = sum;
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) {
+            const int x = __shfl_up(before, m);
+            if (lane >= m) before += x;
+        }
+        before -= sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bin[4 * lane + i] = before, before += n[i];
+    }
+    __syncthreads();
+    if (tid < tiles) order[atomicAdd(&bin[of(tid)], 1)] = tid;
 }
 
 // The largest power of two in bytes, up to 16, that an array's address, strides
@@ -192,12 +267,15 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
         L.meta_tiles = mt;
         L.col_docs = col;
         const long long nk = (long long)a.batch * mt, nc = (long long)a.batch * c.tiles;
-        hipLaunchKernelGGL(k_doc_tiles, dim3((unsigned)((nk + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, meta);
-        hipLaunchKernelGGL(k_doc_columns, dim3((unsigned)((nc + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, per, c.tiles, meta, col);
         // documents of different sizes make column tiles of different work; the longest first
-        if (c.tiles >= 8) {
-            L.order = order;
-            hipLaunchKernelGGL(k_doc_order, dim3((unsigned)a.batch), dim3(256), 0, st, c.tiles, col, order);
+        if (c.tiles >= 8) L.order = order;
+        if (mt <= kDocTiles && c.tiles <= kDocTiles) {
+            hipLaunchKernelGGL(k_doc_all, dim3((unsigned)a.batch), dim3(1024), 0, st, a, c.tk, mt, per, c.tiles, meta, col,
+                               c.tiles >= 8 ? order : nullptr);
+        } else {
+            hipLaunchKernelGGL(k_doc_tiles, dim3((unsigned)((nk + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, meta);
+            hipLaunchKernelGGL(k_doc_columns, dim3((unsigned)((nc + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, per, c.tiles, meta, col);
+            if (c.tiles >= 8) hipLaunchKernelGGL(k_doc_order, dim3((unsigned)a.batch), dim3(256), 0, st, c.tiles, col, order);
         }
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;

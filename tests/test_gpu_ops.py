@@ -926,3 +926,28 @@ def test_rms_norm_odd_rows_apart(pkg, cols, rows, group):
         x[3], r[3] = x[3] * 1e-12, r[3] * 1e-12
     rms_case(pkg, "f32", rows, cols, e4m3=True, group=group, change=change)
     rms_case(pkg, "f32", rows, cols, change=change)
+
+
+# ---- documents' summaries: in one launch up to 64 tiles of keys and of columns, in three past them
+
+
+def doc_lengths(g, c):
+    ids = np.sort(g.integers(0, 9, (c["B"], c["Lk"])), 1)
+    ids[:, -c["Lk"] // 20:] = -1
+    return ids[:, :c["Lq"]], ids
+
+
+DOCS = {
+    "five_tiles": case("bf16", B=3, Lq=300, Lk=300, H=2, KV=2, D=32, docs=doc_lengths, q_lens=[300, 0, 123], k_lens=[300, 300, 123]),
+    "64_tiles": case("f16", Lq=4096, Lk=4096, H=1, KV=1, D=16, docs=doc_lengths),
+    "65_tiles": case("f16", Lq=4097, Lk=4097, H=1, KV=1, D=16, docs=doc_lengths),
+    "65_columns": case("bf16", B=2, Lq=1100, Lk=1100, H=4, KV=1, D=40, docs=doc_lengths, causal=True),
+    "few_columns": case("bf16", B=2, Lq=2, Lk=4000, H=4, KV=1, D=64, docs=scattered, order="cache"),
+    "half_tiles": case("f32", B=2, Lq=1500, Lk=1500, H=1, KV=1, D=100, docs=doc_lengths),
+    "none": case("f32", B=2, Lq=500, Lk=500, H=1, KV=1, D=24, docs=lambda g, c: (np.full(500, -1), np.full(500, -1))),
+}
+
+
+@pytest.mark.parametrize("name", DOCS)
+def test_attention_document_summaries(pkg, name):
+    check_attention(pkg, DOCS[name])
