@@ -17,11 +17,12 @@
 //
 // What bounds it, measured on an MI355X. Prompts: instruction issue, since MFMA and
 // other VALU instructions do not overlap here: on 2 x 4096 causal bf16 tokens, 32 query and 8
-// key heads of 128, capped, 40% of the cycles are MFMA and 41% VALU, at the 2.06 GHz that power
-// leaves (313 us, 882 TFLOP/s of the pairs that the mask leaves); 12001 f16 tokens with
-// slopes 38% and 43% (680 us, 867 TFLOP/s); no LDS bank conflicts. Hence the tile's path
-// counts its instructions: a polynomial for small capped scores, no maximum where the cap
-// bounds them, sums by MFMA, slopes in two operations, max by v_maximum3. Steps: HBM (32
+// key heads of 128, capped, 341 us, 810 TFLOP/s of the pairs that the mask leaves; 12001 f16 tokens with
+// slopes 38% MFMA and 43% VALU (680 us, 867 TFLOP/s); no LDS bank conflicts. Hence the tile's path
+// counts its instructions: a polynomial for small capped scores, sums by MFMA, slopes in two
+// operations, max by v_maximum3. (The maximum is looked for under a cap too: one reference for all
+// of a call's rows, below the cap, gave 315 us, but left a row whose scores are all far below it
+// weights of 2^-124, whose products with v are no normal numbers.) Steps: HBM (32
 // sequences of up to 8192 keys, 8 x 128 bf16: 135 us, 5.07 TB/s). Small windows (1089
 // of 64 f32 tokens, 6 heads of 30, table and bands): the 733 VALU and 584 scalar instructions of a
 // wave for 16 columns, 79 us.
@@ -47,11 +48,6 @@ struct AttnScore {
     // cancellation near zero. poly_max: the |x| that it holds for.
     float p0, p1, p2, p3, poly_max;
     float z;  // scale / cap
-    // A cap bounds the scores: with no bias and a type of f32's range, e^(s - ref) at one
-    // reference 2^20 below the cap's lies in 2^-125 to 2^20 for every score that a cap up to
-    // 50.2 leaves, and no maximum is looked for.
-    bool fixed;
-    float ref;
     bool general;  // a bias other than slopes by token distance
     void set(const AttnOpArgs &a) {
         // a negative or zero scale would turn masked minus infinities round: scores in
@@ -59,8 +55,6 @@ struct AttnScore {
         general = a.table || a.k_pos || (!(a.cap > 0.f) && !(a.scale > 1e-30f));
         c1 = a.scale * kAttnLog2e;
         capl = a.cap * kAttnLog2e;
-        fixed = a.cap > 0.f && !a.slopes && !a.table && 2.f * capl - 20.f <= 125.f;
-        ref = fixed ? capl - 20.f : 0.f;
         p0 = p1 = p2 = p3 = z = 0.f;
         poly_max = -1.f;
         if (a.cap > 0.f) {
@@ -123,7 +117,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = kAttnLog2e;
 
-enum { CAP = 1, SLOPES = 2, ANY = 8, DOCS = 16, GENERAL = 32, FIXED = 4 };
+enum { CAP = 1, SLOPES = 2, ANY = 8, DOCS = 16, GENERAL = 32 };
 
 template <typename T>
 struct Type;
@@ -347,7 +341,7 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 //  WK true (at most 16 columns): every wave has all columns and a quarter of each
 //  key tile (one block of 16 keys of 64); the four sums meet in LDS at the end.
 //  MODE: CAP and SLOPES are known (0 to 3), or asked for in every tile (ANY); documents
-//  (DOCS); a fixed reference of the softmax (FIXED, see AttnScore); or all but that and what AttnScore::general stands for (GENERAL). Paths that a
+//  (DOCS); or all of that and what AttnScore::general stands for (GENERAL). Paths that a
 //  kernel might take and does not cost it registers, spilled around its loop, and copies
 //  where they meet.
 // K and V tiles of TK keys are copied straight into LDS, two buffers each (three and four
@@ -565,7 +559,7 @@ struct Kernel {
         Sum l[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            m[nb] = MODE & FIXED ? L.score.ref : -INFINITY;
+            m[nb] = -INFINITY;
             l[nb] = Sum{};
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db][nb] = f4v{0.f, 0.f, 0.f, 0.f};
@@ -827,7 +821,7 @@ struct Kernel {
                             const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
                             const float near = t * fmaf(w, fmaf(w, fmaf(w, -0.04848728f, 0.13289726f), -0.33332333f), 1.f);
                             const float x = fabsf(t) <= 0.375f ? near : far;
-                            s[kb][nb][i] = MODE & FIXED ? fmaf(x, sc.capl, -sc.ref) : x * sc.capl;
+                            s[kb][nb][i] = x * sc.capl;
                         }
             } else {
 #pragma unroll
@@ -837,8 +831,7 @@ struct Kernel {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float x = s[kb][nb][i], w = x * x;
-                            const float p = fmaf(w, fmaf(w, fmaf(w, sc.p3, sc.p2), sc.p1), sc.p0);
-                            s[kb][nb][i] = MODE & FIXED ? fmaf(x, p, -sc.ref) : x * p;
+                            s[kb][nb][i] = x * fmaf(w, fmaf(w, fmaf(w, sc.p3, sc.p2), sc.p1), sc.p0);
                         }
             }
             unit = 1.f;
@@ -920,28 +913,26 @@ struct Kernel {
             }
         }
         // the running reference: rescaled only where a score passes it by 2^kLazy
-        if constexpr (!(MODE & FIXED)) {
-            float top[NB];
-            bool grow = false;
+        float top[NB];
+        bool grow = false;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            float x = s[0][nb][0];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) x = max3(max3(x, s[kb][nb][0], s[kb][nb][1]), s[kb][nb][2], s[kb][nb][3]);
+            top[nb] = col_max(x) * unit;
+            grow |= top[nb] > m[nb] + Ty::kLazy;
+        }
+        if (__any(grow)) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                float x = s[0][nb][0];
+                const float mn = fmaxf(m[nb], top[nb]);
+                // (no reference yet: sums of zero, or infinities of v that stay)
+                const float f = m[nb] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nb] - mn);
+                m[nb] = mn;
+                l[nb] *= f;
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) x = max3(max3(x, s[kb][nb][0], s[kb][nb][1]), s[kb][nb][2], s[kb][nb][3]);
-                top[nb] = col_max(x) * unit;
-                grow |= top[nb] > m[nb] + Ty::kLazy;
-            }
-            if (__any(grow)) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const float mn = fmaxf(m[nb], top[nb]);
-                    // (no reference yet: sums of zero, or infinities of v that stay)
-                    const float f = m[nb] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nb] - mn);
-                    m[nb] = mn;
-                    l[nb] *= f;
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) o[db][nb] *= f;
-                }
+                for (int db = 0; db < DB; ++db) o[db][nb] *= f;
             }
         }
 #pragma unroll
@@ -952,7 +943,7 @@ struct Kernel {
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(MODE & FIXED ? s[kb][nb][i] : fmaf(s[kb][nb][i], unit, ref));
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[kb][nb][i], unit, ref));
                     s[kb][nb][i] = p;
                     if (F32) sum[i] += p;
                 }
@@ -1195,13 +1186,6 @@ hipError_t launch_narrow(const AttnOpArgs &a, const AttnLaunch &L, int align, hi
     return a.k_docs ? launch<T, DP, 1, WK, 16, ANY | DOCS>(a, L, st) : launch<T, DP, 1, WK, 16, ANY>(a, L, st);
 }
 
-// (f16 has not the range of a fixed reference)
-template <typename T, int DP>
-hipError_t launch_fixed(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
-    if constexpr (std::is_same<T, half_t>::value) return hipErrorInvalidValue;
-    else return launch<T, DP, 2, false, 16, CAP | FIXED>(a, L, st);
-}
-
 template <typename T, int DP>
 hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, int align, hipStream_t st) {
     hipError_t e;
@@ -1212,10 +1196,7 @@ hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, 
     else if (a.k_docs)
         e = launch<T, DP, 2, false, 16, ANY | DOCS>(a, L, st);
     else if (a.cap > 0.f)
-        e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES>(a, L, st)
-            : std::is_same<T, half_t>::value ? launch<T, DP, 2, false, 16, CAP>(a, L, st)
-            : L.score.fixed ? launch_fixed<T, DP>(a, L, st)
-                            : launch<T, DP, 2, false, 16, CAP>(a, L, st);
+        e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES>(a, L, st) : launch<T, DP, 2, false, 16, CAP>(a, L, st);
     else
         e = a.slopes ? launch<T, DP, 2, false, 16, SLOPES>(a, L, st) : launch<T, DP, 2, false, 16, 0>(a, L, st);
     if (e != hipSuccess || L.splits == 1) return e;
