@@ -28,3 +28,73 @@ def test_attention_values_under_a_cap(pkg, dtype, scale):
     """Scores of a cap's size either way leave the values' precision alone, however small or large they
     are: a row whose keys all score -50 has the same result as one whose keys all score 50."""
     T.check_attention(pkg, T.case(dtype, D=64, causal=True, cap=50.0, **T.WIDE), saturated(scale))
+
+
+# ---- calls that the documentation allows ------------------------------------------------
+
+
+@pytest.mark.parametrize("mode", [0, 1])
+def test_operators_captured_in_every_mode(pkg, mode):
+    """Capture in the global and the thread's own mode, which refuse calls that a capture cannot hold: a call makes none.
+    Replays, with eager work between them, are the eager run."""
+    import ctypes as C
+    h, vp = pkg.hip.rt(), C.c_void_p
+    for name, args in {"hipStreamBeginCapture": [vp, C.c_int], "hipStreamEndCapture": [vp, C.POINTER(vp)],
+                       "hipGraphInstantiate": [C.POINTER(vp), vp, vp, vp, C.c_size_t], "hipGraphLaunch": [vp, vp],
+                       "hipGraphExecDestroy": [vp], "hipGraphDestroy": [vp]}.items():
+        getattr(h, name).argtypes = args
+    b, other, st = T.Block(pkg, 7), T.Block(pkg, 8), T.new_stream(pkg)
+    b.run()
+    pkg.hip.synchronize()
+    want = b.bits()
+    g, e = vp(), vp()
+    assert h.hipStreamBeginCapture(st, mode) == 0
+    b.run(stream=st.value)
+    assert h.hipStreamEndCapture(st, C.byref(g)) == 0
+    assert h.hipGraphInstantiate(C.byref(e), g, None, None, 0) == 0
+    for _ in range(4):
+        for dev in (b.h, b.turned, b.out, b.last):
+            dev.buf.upload(np.zeros(dev.buf.n, np.float32))
+        other.run()
+        pkg.hip.synchronize()
+        assert h.hipGraphLaunch(e, st) == 0
+        pkg.hip.stream_synchronize(st.value)
+        assert b.bits() == want
+    h.hipGraphExecDestroy(e)
+    h.hipGraphDestroy(g)
+    h.hipStreamDestroy(st)
+
+
+# ---- hidden keys in the kernels of large calls --------------------------------------------
+
+HIDDEN = {
+    "f16": dict(dtype="f16", D=128),
+    "bf16": dict(dtype="bf16", D=64),
+    "f32": dict(dtype="f32", D=64),
+    "cap_bf16": dict(dtype="bf16", D=128, cap=50.0, spread=4.0),
+    "cap_f32": dict(dtype="f32", D=32, cap=50.0, spread=4.0),
+    "slopes_bf16": dict(dtype="bf16", D=64, slopes=True),
+    "slopes_f32": dict(dtype="f32", D=128, slopes=True),
+    "cap_slopes_f16": dict(dtype="f16", D=96, slopes=True, cap=30.0),
+    "documents_bf16": dict(dtype="bf16", D=128, docs=T.scattered, cap=50.0),
+    "documents_f32": dict(dtype="f32", D=96, docs=T.scattered, slopes=True),
+}
+
+
+@pytest.mark.parametrize("where,name", [(w, n) for w in ("future", "past_the_length", "documents") for n in HIDDEN
+                                        if w != "documents" or "docs" in HIDDEN[n]])
+def test_attention_hidden_keys_of_large_calls(pkg, name, where):
+    """NaN and infinities in keys that some or all of the queries do not see, by the causal mask, the
+    lengths or the documents: as they are not there for those, and are for the others."""
+    more = dict(causal=True) if where == "future" else dict(k_lens=[90 - i for i in range(43)]) if where == "past_the_length" else {}
+
+    def change(q, k, v, extra):
+        if where == "future":
+            v[:, 89, 0, 5], v[:, 88, 3, 2], k[:, 89, 4, 0], v[:, 60, 5, 7] = np.nan, np.inf, np.nan, -np.inf
+        elif where == "past_the_length":
+            for b in range(43):
+                k[b, 90 - b:], v[b, 90 - b:] = np.nan, (np.inf, -np.inf, np.nan)[b % 3]
+        else:
+            k[:, 80:], v[:, 70:75], v[:, 75:] = np.inf, np.nan, -np.inf
+            extra["k_docs"][:, 70:] = np.where(np.arange(20) % 2, -1, 7)
+    T.check_attention(pkg, T.case(**HIDDEN[name], **more, **T.WIDE), change)
