@@ -121,10 +121,11 @@ enum { CAP = 1, SLOPES = 2, ANY = 8, DOCS = 16, GENERAL = 32 };
 
 template <typename T>
 struct Type;
-// V: 16 bytes of elements. kShift: weights are 2^kShift times e^(s - max), so that f16's
-// smallest normal number, 2^-14, is 2^-24 of a row's largest weight and a long row of small
-// weights is not lost below it. kLazy: how many powers of two a score may pass the
-// reference before sums are rescaled (2^(kShift + kLazy) stays below f16's 65504).
+// V: 16 bytes of elements. kLazy: how many powers of two a score may pass the reference before
+// sums are rescaled. kShift: weights are 2^kShift times e^(s - reference). For f16 10, so that its
+// smallest normal number, 2^-14, is 2^-24 of a row's largest weight and a long row of small weights
+// is not lost below it (2^(kShift + kLazy) stays below its 65504). For the types of f32's range
+// -kLazy: no weight is above one, so that no product with a finite v passes what v has.
 template <>
 struct Type<half_t> {
     typedef h8 V;
@@ -135,13 +136,13 @@ template <>
 struct Type<bfloat_t> {
     typedef b8 V;
     static constexpr int kElems = 8;
-    static constexpr float kShift = 0.f, kLazy = 8.f;
+    static constexpr float kShift = -8.f, kLazy = 8.f;
 };
 template <>
 struct Type<float> {
     typedef f4v V;
     static constexpr int kElems = 4;
-    static constexpr float kShift = 0.f, kLazy = 8.f;
+    static constexpr float kShift = -8.f, kLazy = 8.f;
 };
 
 __device__ __forceinline__ f4v mma(h8 a, h8 b, f4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }

@@ -30,6 +30,19 @@ def test_attention_values_under_a_cap(pkg, dtype, scale):
     T.check_attention(pkg, T.case(dtype, D=64, causal=True, cap=50.0, **T.WIDE), saturated(scale))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [dict(Lq=1, Lk=130, H=2), dict(Lq=80, Lk=130, H=2), T.WIDE])
+def test_attention_values_near_the_largest(pkg, dtype, shape):
+    """Values of 2e37 whose weighted mean is no larger: one key scores 5 above the others, in a tile behind
+    theirs."""
+    def change(q, k, v, more):
+        q[...], k[...] = 1.0, 0.0
+        k[:, 70] = 0.625  # times 64 / 8
+        v *= 2e37 / 8
+        v[...] = T.R.round_to(v, "bf16")
+    T.check_attention(pkg, T.case(dtype, D=64, **shape), change)
+
+
 # ---- calls that the documentation allows ------------------------------------------------
 
 
