@@ -289,8 +289,9 @@ typedef struct s2s_tokens {
  *    Whatever other keys' k and v hold (NaN and infinities too) has no effect.
  *  - the score is scale q.k, capped if cap > 0; then - slopes[h] |d| and
  *    + table[h][clamp(d + table_size / 2, 0, table_size - 1)] are added, d =
- *    q_pos[b][i] - k_pos[b][j] or, without positions, P(i) - j. A bias of
- *    minus infinity takes the key out.
+ *    q_pos[b][i] - k_pos[b][j] or, without positions, P(i) - j. An entry of
+ *    minus infinity takes the key out. Slopes are taken as clamped to
+ *    [-10^20, 10^20]: with a larger one a row sees its nearest keys alone.
  *  - a query with no key gives zeros. Queries from q_lens[b] on are not
  *    written. Lengths are taken as clamped to [0, tokens], prefix to k_lens.
  * Positions differ by less than 2^31. (dy, dx) biases of an image's tokens:

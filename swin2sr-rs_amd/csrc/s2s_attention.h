@@ -419,7 +419,7 @@ struct Kernel {
             doc[nb] = 0;
             if (DOC && a.q_docs && ok) doc[nb] = a.q_docs[b * a.q_docs_b + i];
             at[nb] = a.q_pos && ok ? a.q_pos[b * a.q_pos_b + i] : kl - ql + i;
-            slope[nb] = a.slopes && ok ? a.slopes[h] * kLog2e : 0.f;
+            slope[nb] = a.slopes && ok ? slope_of(a.slopes[h]) : 0.f;
             tab[nb] = ok ? (L.table_lds ? c - i * a.group : h) * a.table_size : 0;
             const T *row = (const T *)a.q + b * a.sq.b + (long long)(ok ? i : 0) * a.sq.t + h * a.sq.h;
 #pragma unroll
@@ -953,6 +953,12 @@ struct Kernel {
         products(vl0, s, o, l);
     }
 
+    // A head's slope in powers of two, up to 10^20: its product with a distance, and the differences
+    // of such products, are finite then (2^30 tokens are 1.5e29), and 10^20 between neighbours takes
+    // all but a row's nearest keys out as well as more would. (NaN stays.)
+    static __device__ __forceinline__ float slope_of(float x) {
+        return (x > 1e20f ? 1e20f : x < -1e20f ? -1e20f : x) * kLog2e;
+    }
     static __device__ __forceinline__ float entry(const Uniform &u, int tab, int dist) {
         const int i = tab + min(max(dist, -u.half), u.half) + u.half;
         return u.table_lds ? lds_read<float>(u.tab0 + 4 * i, 0) : u.table[i];

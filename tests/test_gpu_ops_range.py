@@ -43,6 +43,31 @@ def test_attention_values_near_the_largest(pkg, dtype, shape):
     T.check_attention(pkg, T.case(dtype, D=64, **shape), change)
 
 
+# ---- slopes past what a product with a distance holds -----------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [dict(Lq=1, Lk=200, H=8), dict(Lq=90, Lk=200, H=8, KV=2), dict(T.WIDE, H=12)])
+@pytest.mark.parametrize("mask", ["causal", "all", "positions", "cap"])
+def test_attention_steep_slopes(pkg, dtype, shape, mask):
+    """However steep the slopes, infinite ones too, the key in the query's own place scores without a bias: it is
+    all that the row sees."""
+    c = T.case(dtype, D=64, causal=mask in ("causal", "cap"), cap=30.0 if mask == "cap" else 0.0, slopes=True,
+               pos=(lambda g, c: (np.arange(c["Lq"]) + 1000, np.arange(c["Lk"]) + 1000)) if mask == "positions" else None, **shape)
+    q, k, v, more = T.inputs(c)
+    steep = np.array([1e21, 1e30, 5e36, 1e37, 1e38, 3e38, np.inf, 2.0], np.float32)
+    more["slopes"] = steep[np.arange(c["H"]) % 8]
+    plan, ws, _ = T.make_plan(pkg, c)
+    d, m = T.upload(pkg, c, q, k, v, more)
+    T.call(plan, ws, d, m)
+    got = d["out"].get()
+    first = 0 if mask == "positions" else c["Lk"] - c["Lq"]
+    for h in np.flatnonzero(more["slopes"] > 1e20):
+        want = v[:, first:first + c["Lq"], h // (c["H"] // c["KV"])]
+        # one weight, which the sum divides away: a product and a division in f32, and the type's rounding
+        assert (np.abs(got[:, :, h] - want) <= (T.R.HALF[dtype] + 4 * 2.0 ** -24) * np.abs(want)).all(), h
+
+
 # ---- calls that the documentation allows ------------------------------------------------
 
 
