@@ -1179,8 +1179,7 @@ hipError_t launch(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
     M.table_lds = a.table && (long long)a.group * a.table_size <= K::kTabEntries;
     const size_t lds = K::kTab + (M.table_lds ? (size_t)a.group * a.table_size * 4 : 0);
     const long long blocks = (long long)a.batch * a.hk * L.tiles * L.splits;  // (below 2^24 by the entry's checks)
-    hipLaunchKernelGGL((k_attn<T, DP, NB, WK, ALIGN, MODE>), dim3((unsigned)blocks), dim3(256), lds, st, a, M);
-    return hipGetLastError();
+    return enqueue(k_attn<T, DP, NB, WK, ALIGN, MODE>, dim3((unsigned)blocks), dim3(256), lds, st, a, M);
 }
 
 // Arrays that are not of 16-byte multiples and general biases take the kernels of 16
@@ -1213,10 +1212,8 @@ hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, 
     // 1024 keys) 20.3 against 19.6
     constexpr int N = 256 / (DP / 4);
     if (L.splits <= kFewRanges && rows >= 4 * cu_count())
-        hipLaunchKernelGGL((k_attn_join_few<T, DP>), dim3((unsigned)((rows + N - 1) / N)), dim3(256), 0, st, a, L, (int)rows);
-    else
-        hipLaunchKernelGGL((k_attn_join<T, DP>), dim3((unsigned)rows), dim3(256), 0, st, a, L);
-    return hipGetLastError();
+        return enqueue(k_attn_join_few<T, DP>, dim3((unsigned)((rows + N - 1) / N)), dim3(256), 0, st, a, L, (int)rows);
+    return enqueue(k_attn_join<T, DP>, dim3((unsigned)rows), dim3(256), 0, st, a, L);
 }
 
 template <typename T>

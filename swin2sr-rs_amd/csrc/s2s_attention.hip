@@ -269,15 +269,17 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
         const long long nk = (long long)a.batch * mt, nc = (long long)a.batch * c.tiles;
         // documents of different sizes make column tiles of different work; the longest first
         if (c.tiles >= 8) L.order = order;
+        hipError_t e;
         if (mt <= kDocTiles && c.tiles <= kDocTiles) {
-            hipLaunchKernelGGL(k_doc_all, dim3((unsigned)a.batch), dim3(1024), 0, st, a, c.tk, mt, per, c.tiles, meta, col,
-                               c.tiles >= 8 ? order : nullptr);
+            e = enqueue(k_doc_all, dim3((unsigned)a.batch), dim3(1024), 0, st, a, c.tk, mt, per, c.tiles, meta, col,
+                        c.tiles >= 8 ? order : nullptr);
         } else {
-            hipLaunchKernelGGL(k_doc_tiles, dim3((unsigned)((nk + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, meta);
-            hipLaunchKernelGGL(k_doc_columns, dim3((unsigned)((nc + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, per, c.tiles, meta, col);
-            if (c.tiles >= 8) hipLaunchKernelGGL(k_doc_order, dim3((unsigned)a.batch), dim3(256), 0, st, c.tiles, col, order);
+            e = enqueue(k_doc_tiles, dim3((unsigned)((nk + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, meta);
+            if (e == hipSuccess)
+                e = enqueue(k_doc_columns, dim3((unsigned)((nc + 3) / 4)), dim3(256), 0, st, a, c.tk, mt, per, c.tiles, meta, col);
+            if (e == hipSuccess && c.tiles >= 8)
+                e = enqueue(k_doc_order, dim3((unsigned)a.batch), dim3(256), 0, st, c.tiles, col, order);
         }
-        const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     switch (dtype) {

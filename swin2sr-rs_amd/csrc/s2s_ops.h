@@ -7,6 +7,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 struct Strides {
     long long b, t, h;
 };
@@ -60,6 +62,14 @@ template <typename T, int N, int A = N>
 struct alignas(sizeof(T) * A) VecOf {
     T e[N];
 };
+
+// Enqueues a kernel and returns that launch's own error: hipGetLastError would return any
+// earlier one that the caller has not taken.
+template <typename... P>
+hipError_t enqueue(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t st, std::common_type_t<P>... args) {
+    void *ptrs[] = {&args...};
+    return hipLaunchKernel((const void *)kernel, grid, block, ptrs, lds, st);
+}
 
 size_t attn_op_workspace(int dtype, const AttnOpArgs &a);
 hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStream_t st);

@@ -142,27 +142,15 @@ hipError_t rotary_of(const RotaryArgs &a, hipStream_t st) {
     const size_t lds = (size_t)tb * a.pairs * sizeof(float2);
     switch (v) {
         case 8:
-            if constexpr (!ADJ && sizeof(T) == 2) {
-                hipLaunchKernelGGL((k_rotary<T, ADJ, 8>), grid, dim3(256), lds, st, a, tb, per_head);
-                break;
-            }
+            if constexpr (!ADJ && sizeof(T) == 2) return enqueue(k_rotary<T, ADJ, 8>, grid, dim3(256), lds, st, a, tb, per_head);
             return hipErrorInvalidValue;
         case 4:
-            if constexpr (!(ADJ && sizeof(T) == 4)) {
-                hipLaunchKernelGGL((k_rotary<T, ADJ, 4>), grid, dim3(256), lds, st, a, tb, per_head);
-                break;
-            }
+            if constexpr (!(ADJ && sizeof(T) == 4)) return enqueue(k_rotary<T, ADJ, 4>, grid, dim3(256), lds, st, a, tb, per_head);
             return hipErrorInvalidValue;
-        case 2:
-            hipLaunchKernelGGL((k_rotary<T, ADJ, 2>), grid, dim3(256), lds, st, a, tb, per_head);
-            break;
-        default:
-            if (ADJ && w < 2)
-                hipLaunchKernelGGL((k_rotary<T, ADJ, 1, false>), grid, dim3(256), lds, st, a, tb, per_head);
-            else
-                hipLaunchKernelGGL((k_rotary<T, ADJ, 1>), grid, dim3(256), lds, st, a, tb, per_head);
+        case 2: return enqueue(k_rotary<T, ADJ, 2>, grid, dim3(256), lds, st, a, tb, per_head);
     }
-    return hipGetLastError();
+    if (ADJ && w < 2) return enqueue(k_rotary<T, ADJ, 1, false>, grid, dim3(256), lds, st, a, tb, per_head);
+    return enqueue(k_rotary<T, ADJ, 1>, grid, dim3(256), lds, st, a, tb, per_head);
 }
 
 template <typename T>
@@ -416,8 +404,7 @@ hipError_t rms_launch(const RmsNormArgs &a, hipStream_t st) {
     // at most 32 workgroups a CU, which then walk their rows with the weights at hand (16391 x 5120
     // bf16 to e4m3: 117 us, 122 with 8, 120 with 64)
     const long long most = 32LL * cu_count();
-    hipLaunchKernelGGL((k_rms_norm<T, E4M3, V, TPR, NC>), dim3((unsigned)std::min(blocks, most)), dim3(256), 0, st, a);
-    return hipGetLastError();
+    return enqueue(k_rms_norm<T, E4M3, V, TPR, NC>, dim3((unsigned)std::min(blocks, most)), dim3(256), 0, st, a);
 }
 
 // Whether rows of chunks of V elements can be taken: their places, their number, and the
@@ -458,8 +445,7 @@ hipError_t rms_type(const RmsNormArgs &a, hipStream_t st) {
             return rms_launch<T, E4M3, 4, 64, 4>(a, st);
         }
     }
-    hipLaunchKernelGGL((k_rms_norm_rows<T, E4M3>), dim3((unsigned)std::min(a.rows, 1LL << 20)), dim3(256), 0, st, a);
-    return hipGetLastError();
+    return enqueue(k_rms_norm_rows<T, E4M3>, dim3((unsigned)std::min(a.rows, 1LL << 20)), dim3(256), 0, st, a);
 }
 
 }  // namespace

@@ -71,6 +71,29 @@ def test_attention_steep_slopes(pkg, dtype, shape, mask):
 # ---- calls that the documentation allows ------------------------------------------------
 
 
+def test_operators_after_an_error_of_the_callers(pkg):
+    """A failed call of the caller's own to the runtime, whose error nobody has taken, is no error of the operators."""
+    h = pkg.hip.rt()
+    c = T.case("bf16", Lq=3, Lk=70, H=2, KV=1)
+    q, k, v, more = T.inputs(c)
+    plan, ws, scale = T.make_plan(pkg, c)
+    want, bound, _ = T.R.attention("bf16", q, k, v, scale)
+    d, m = T.upload(pkg, c, q, k, v, more)
+    pos = T.R.Dev(pkg, np.zeros((1, 3, 1), np.int32), "f32", whole=True)
+    x, w, out = (T.R.Dev(pkg, a, "f32") for a in (np.ones((4, 32)), np.ones(32), np.zeros((4, 32))))
+    rot = pkg.ops.Rotary.of((8,))
+    assert h.hipSetDevice(9999) != 0
+    T.call(plan, ws, d, m)
+    assert h.hipSetDevice(9999) != 0
+    rot(d["q"].array, pos.array)
+    assert h.hipSetDevice(9999) != 0
+    pkg.ops.rms_norm(x.array, w.array, out.array)
+    h.hipGetLastError()
+    pkg.hip.synchronize()
+    assert (np.abs(d["out"].get() - want) <= bound).all()
+    assert (np.abs(out.get() - 1) <= 1e-6).all()
+
+
 @pytest.mark.parametrize("mode", [0, 1])
 def test_operators_captured_in_every_mode(pkg, mode):
     """Capture in the global and the thread's own mode, which refuse calls that a capture cannot hold: a call makes none.
