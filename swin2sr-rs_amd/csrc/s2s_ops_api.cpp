@@ -273,10 +273,11 @@ int s2s_rotary(const s2s_rotary_args *a, void *stream) {
         if (int rc = check_tokens(op, "k_out", a->k_out, a->dtype, on.dev)) return rc;
         if (int rc = check_written(op, "k_out", a->k_out, a->batch, a->tokens, a->k_heads, a->width)) return rc;
     }
-    auto same = [](const s2s_tokens &x, const s2s_tokens &y) {
-        return x.data != y.data || (x.batch == y.batch && x.token == y.token && x.head == y.head);
+    auto same = [&](const s2s_tokens &x, const s2s_tokens &y, int heads) {
+        const Strides s = strides(x, a->batch, a->tokens, heads), t = strides(y, a->batch, a->tokens, heads);
+        return x.data != y.data || (s.b == t.b && s.t == t.t && s.h == t.h);
     };
-    if (!same(a->q, a->q_out) || (has_k && !same(a->k, a->k_out)))
+    if (!same(a->q, a->q_out, a->q_heads) || (has_k && !same(a->k, a->k_out, a->k_heads)))
         return refuse("%s: in place, the output's strides must be the input's", op);
     if (!a->pos) return refuse("%s: pos is null", op);
     if (int rc = check_array(op, "pos", a->pos, 4, on.dev)) return rc;

@@ -94,6 +94,17 @@ def test_operators_after_an_error_of_the_callers(pkg):
     assert (np.abs(out.get() - 1) <= 1e-6).all()
 
 
+def test_rotary_in_place_strides_of_one(pkg):
+    """In place the strides have to be the same, but that of a dimension of one counts for nothing."""
+    x = np.random.default_rng(0).standard_normal((1, 1, 1, 16))
+    d, one = T.R.Dev(pkg, x, "f32"), T.R.Dev(pkg, x, "f32")
+    pos = T.R.Dev(pkg, np.full((1, 1, 1), 3, np.int32), "f32", whole=True)
+    rot, A = pkg.ops.Rotary.of((8,)), pkg.ops.Array
+    rot(one.array, pos.array)
+    rot(A(d.array.ptr, (1, 1, 1, 16), "f32", (5, 7, 9, 1)), pos.array, A(d.array.ptr, (1, 1, 1, 16), "f32", (64, 16, 16, 1)))
+    assert np.array_equal(d.get(), one.get())
+
+
 @pytest.mark.parametrize("mode", [0, 1])
 def test_operators_captured_in_every_mode(pkg, mode):
     """Capture in the global and the thread's own mode, which refuse calls that a capture cannot hold: a call makes none.
