@@ -152,12 +152,13 @@ AttnOpArgs attention_args(const s2s_attention_args *a) {
     k.q_lens = a->q_lens;
     k.k_lens = a->k_lens;
     k.prefix = a->prefix;
-    k.q_docs = a->q_docs;
-    k.k_docs = a->k_docs;
+    // (without keys the row is zeros whatever else is given)
+    k.q_docs = a->k_tokens > 0 ? a->q_docs : nullptr;
+    k.k_docs = a->k_tokens > 0 ? a->k_docs : nullptr;
     k.q_docs_b = a->q_docs_batch;
     k.k_docs_b = a->k_docs_batch;
-    k.q_pos = a->q_pos;
-    k.k_pos = a->k_pos;
+    k.q_pos = a->k_tokens > 0 ? a->q_pos : nullptr;
+    k.k_pos = a->k_tokens > 0 ? a->k_pos : nullptr;
     k.q_pos_b = a->q_pos_batch;
     k.k_pos_b = a->k_pos_batch;
     k.slopes = a->slopes;
@@ -185,8 +186,10 @@ int s2s_attention(const s2s_attention_args *a, void *workspace, uint64_t workspa
     if (!(a->cap >= 0.f) || !std::isfinite(a->cap)) return refuse("%s: the cap is negative or not finite", op);
     if (a->cap > 0.f && a->cap < 1e-6f) return refuse("%s: a cap below 1e-6", op);
     if (a->prefix && !a->causal) return refuse("%s: a prefix without the causal mask", op);
-    if (!a->q_docs != !a->k_docs) return refuse("%s: documents of queries and keys come together", op);
-    if (!a->q_pos != !a->k_pos) return refuse("%s: positions of queries and keys come together", op);
+    // (an array of no elements may have no address, or one that is nobody's)
+    const bool keys = a->k_tokens > 0, some = keys && a->batch > 0 && a->q_tokens > 0;
+    if (some && !a->q_docs != !a->k_docs) return refuse("%s: documents of queries and keys come together", op);
+    if (some && !a->q_pos != !a->k_pos) return refuse("%s: positions of queries and keys come together", op);
     if (a->q_pos && !a->slopes && !a->table) return refuse("%s: positions without slopes or table", op);
     if (a->table && (a->table_size < 1 || a->table_size % 2 == 0 || a->table_size > (1 << 24)))
         return refuse("%s: a table of %d entries: an odd number up to 2^24 is wanted", op, a->table_size);
@@ -206,20 +209,26 @@ int s2s_attention(const s2s_attention_args *a, void *workspace, uint64_t workspa
     if (int rc = check_tokens(op, "q", a->q, a->dtype, on.dev)) return rc;
     if (int rc = check_tokens(op, "out", a->out, a->dtype, on.dev)) return rc;
     if (int rc = check_written(op, "out", a->out, a->batch, a->q_tokens, a->q_heads, a->width)) return rc;
-    if (a->k_tokens > 0) {
+    if (keys) {
         if (int rc = check_tokens(op, "k", a->k, a->dtype, on.dev)) return rc;
         if (int rc = check_tokens(op, "v", a->v, a->dtype, on.dev)) return rc;
         // 64 tokens of a tile are reached by 32-bit byte offsets from its first
         if (a->k_tokens > 1 && (a->k.token > (1 << 22) || a->v.token > (1 << 22)))
             return refuse("%s: a token stride of k or v over 2^22 elements", op);
     }
-    if (a->out.data == a->q.data || a->out.data == a->k.data || a->out.data == a->v.data)
+    if (a->out.data == a->q.data || (keys && (a->out.data == a->k.data || a->out.data == a->v.data)))
         return refuse("%s: out is an input", op);
     const struct {
         const char *name;
         const void *p;
-    } arrays[] = {{"q_lens", a->q_lens}, {"k_lens", a->k_lens}, {"prefix", a->prefix}, {"q_docs", a->q_docs},
-                  {"k_docs", a->k_docs}, {"q_pos", a->q_pos},   {"k_pos", a->k_pos},   {"slopes", a->slopes},
+    } arrays[] = {{"q_lens", a->q_lens},
+                  {"k_lens", a->k_lens},
+                  {"prefix", a->prefix},
+                  {"q_docs", a->q_docs},
+                  {"k_docs", keys ? a->k_docs : nullptr},
+                  {"q_pos", a->q_pos},
+                  {"k_pos", keys ? a->k_pos : nullptr},
+                  {"slopes", a->slopes},
                   {"table", a->table}};
     for (const auto &x : arrays)
         if (x.p)

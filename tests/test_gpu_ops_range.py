@@ -105,6 +105,27 @@ def test_rotary_in_place_strides_of_one(pkg):
     assert np.array_equal(d.get(), one.get())
 
 
+@pytest.mark.parametrize("Lq", [2, 100])
+def test_attention_no_keys_with_documents_and_positions(pkg, Lq):
+    """No key: the keys' documents and positions are arrays of nothing, whose address may be zero."""
+    plan = pkg.ops.Attention("bf16", 2, Lq, 0, 4, 2, 64)
+    q, out = (T.R.Dev(pkg, np.full((2, Lq, 4, 64), 3.0), "bf16") for _ in range(2))
+    empty, none = pkg.ops.Array(0, (2, 0, 2, 64), "bf16"), pkg.ops.Array(0, (2, 0), "i32")
+    ids = T.R.Dev(pkg, np.zeros((2, Lq), np.int32), "f32", whole=True)
+    slopes = T.R.Dev(pkg, np.ones(4), "f32")
+    ws = T.R.Dev(pkg, np.zeros(max(plan.workspace_bytes // 4, 1)), "f32")
+    plan(q.array, empty, empty, out.array, workspace=ws.array, q_docs=ids.array, k_docs=none)
+    assert not out.get().any()
+    out.buf.upload(np.ones(out.buf.n, np.float32))
+    plan(q.array, empty, empty, out.array, workspace=ws.array, q_pos=ids.array, k_pos=none, slopes=slopes.array)
+    assert not out.get().any()
+    # nor does the address of nothing say anything: here the output's, and one past every array
+    out.buf.upload(np.ones(out.buf.n, np.float32))
+    at_out, past = pkg.ops.Array(out.array.ptr, (2, 0, 2, 64), "bf16"), pkg.ops.Array(8, (2, 0), "i32")
+    plan(q.array, at_out, at_out, out.array, workspace=ws.array, q_docs=ids.array, k_docs=past, q_pos=ids.array, k_pos=past, slopes=slopes.array)
+    assert not out.get().any()
+
+
 @pytest.mark.parametrize("mode", [0, 1])
 def test_operators_captured_in_every_mode(pkg, mode):
     """Capture in the global and the thread's own mode, which refuse calls that a capture cannot hold: a call makes none.
