@@ -377,7 +377,7 @@ int s2s_rms_norm(const s2s_rms_norm_args *a, void *stream) {
     RmsNormArgs k{};
     k.rows = a->rows;
     k.cols = a->cols;
-    k.group = a->group ? a->group : a->cols;
+    k.group = a->group > 0 && a->group < a->cols ? a->group : a->cols;
     k.groups = (a->cols + k.group - 1) / k.group;
     k.x = a->x;
     k.res = a->res;

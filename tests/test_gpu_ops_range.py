@@ -126,6 +126,12 @@ def test_attention_no_keys_with_documents_and_positions(pkg, Lq):
     assert not out.get().any()
 
 
+@pytest.mark.parametrize("cols", [100, 4096])
+def test_rms_norm_largest_group(pkg, cols):
+    """A group far past the row is the row."""
+    T.rms_case(pkg, "bf16", 5, cols, e4m3=True, group=2 ** 31 - 8)
+
+
 @pytest.mark.parametrize("mode", [0, 1])
 def test_operators_captured_in_every_mode(pkg, mode):
     """Capture in the global and the thread's own mode, which refuse calls that a capture cannot hold: a call makes none.
