@@ -267,11 +267,10 @@ def _rows(a, shape, dtype: int, op: str, name: str):
     """An array [rows][cols]: address and row stride; zeros for none."""
     if a is None:
         return 0, 0
-    r, c = a.stride()
-    if a.shape != shape or _type(a.dtype) != dtype or (c != 1 and shape[1] > 1):
+    if a.shape != shape or _type(a.dtype) != dtype or (a.stride()[1] != 1 and shape[1] > 1):
         raise S2SError(f"{op}: {name} is {tuple(a.shape)} of {a.dtype}, wanted {tuple(shape)} with adjacent columns "
                        "and the call's type")
-    return a.data_ptr(), r
+    return a.data_ptr(), a.stride()[0]
 
 
 def rms_norm(x, weight, out, eps: float = 1e-6, res=None, sum=None, scales=None, group: int = 0,

@@ -9,3 +9,13 @@ def test_attention_of_no_batch_entry_with_documents(pkg):
     p = plan(pkg, batch=0)
     p(arr(pkg, (0, 5, 4, 64)), arr(pkg, (0, 7, 2, 64)), arr(pkg, (0, 7, 2, 64)), arr(pkg, (0, 5, 4, 64)),
       q_docs=arr(pkg, (5,), "i32"), k_docs=arr(pkg, (0, 7), "i32", ptr=0))
+
+
+@pytest.mark.parametrize("name", ["res", "sum", "out", "x"])
+@pytest.mark.parametrize("shape", [(4,), (1, 4, 8), ()])
+def test_rms_norm_dimensions_refused(pkg, name, shape):
+    """Arrays that are no rows and columns raise the library's error, as other wrong shapes do."""
+    a = dict(x=arr(pkg, (4, 8), "f32"), out=arr(pkg, (4, 8), "f32", ptr=8192))
+    a[name] = arr(pkg, shape, "f32", ptr=16384)
+    with pytest.raises(pkg.S2SError, match=name):
+        pkg.ops.rms_norm(weight=arr(pkg, (8,), "f32"), **a)
