@@ -307,8 +307,8 @@ typedef struct s2s_attention_args {
     int dtype; /* of q, k, v, out: S2S_F32, S2S_F16 or S2S_BF16 */
     int batch, q_tokens, k_tokens, q_heads, k_heads, width;
     int causal;
-    float scale;
-    float cap; /* 0: none */
+    float scale; /* up to 10^30 either way */
+    float cap;   /* 0: none; else 10^-6 to 10^30 */
     s2s_tokens q, k, v, out;
     const int32_t *q_lens, *k_lens; /* [batch], or NULL: all tokens */
     const int32_t *prefix;          /* [batch], or NULL; only with causal */

@@ -185,6 +185,9 @@ int s2s_attention(const s2s_attention_args *a, void *workspace, uint64_t workspa
     if (!std::isfinite(a->scale)) return refuse("%s: the scale is not finite", op);
     if (!(a->cap >= 0.f) || !std::isfinite(a->cap)) return refuse("%s: the cap is negative or not finite", op);
     if (a->cap > 0.f && a->cap < 1e-6f) return refuse("%s: a cap below 1e-6", op);
+    // (their products with log2(e), and the quotient of the two, are finite)
+    if (std::fabs(a->scale) > 1e30f) return refuse("%s: the scale is past 10^30", op);
+    if (a->cap > 1e30f) return refuse("%s: the cap is past 10^30", op);
     if (a->prefix && !a->causal) return refuse("%s: a prefix without the causal mask", op);
     // (an array of no elements may have no address, or one that is nobody's)
     const bool keys = a->k_tokens > 0, some = keys && a->batch > 0 && a->q_tokens > 0;

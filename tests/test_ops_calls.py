@@ -19,3 +19,11 @@ def test_rms_norm_dimensions_refused(pkg, name, shape):
     a[name] = arr(pkg, shape, "f32", ptr=16384)
     with pytest.raises(pkg.S2SError, match=name):
         pkg.ops.rms_norm(weight=arr(pkg, (8,), "f32"), **a)
+
+
+@pytest.mark.parametrize("big", [1.1e30, 3e38, -3e38])
+def test_attention_numbers_past_their_products_refused(pkg, big):
+    """A scale or cap whose product with log2(e) or with a score of one overflows would give NaN."""
+    for more, word in ((dict(scale=big), "the scale"), (dict(cap=abs(big)), "the cap")):
+        with pytest.raises(pkg.S2SError, match=word):
+            plan(pkg, **more)(**tensors(pkg))
