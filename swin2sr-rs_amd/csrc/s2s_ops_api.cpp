@@ -201,8 +201,9 @@ int s2s_attention(const s2s_attention_args *a, void *workspace, uint64_t workspa
         a->q_docs_batch > kMaxStride || a->k_docs_batch > kMaxStride || a->q_pos_batch > kMaxStride ||
         a->k_pos_batch > kMaxStride)
         return refuse("%s: a negative or impossible batch stride", op);
-    // (a wave per key tile, of 32 keys at least, makes the documents' summary)
-    if (a->k_docs && (long long)a->batch * ((a->k_tokens + 31LL) / 32) >= (1 << 26))
+    // (a wave per key tile, of 32 keys at least, makes the documents' summary, four a workgroup, of which
+    // a launch holds less than 2^24)
+    if (a->k_docs && ((long long)a->batch * ((a->k_tokens + 31LL) / 32) + 3) / 4 >= (1 << 24))
         return refuse("%s: documents of over 2^31 keys of the batch", op);
     if (a->batch == 0 || a->q_tokens == 0) return 0;
     OnDevice on;

@@ -27,3 +27,13 @@ def test_attention_numbers_past_their_products_refused(pkg, big):
     for more, word in ((dict(scale=big), "the scale"), (dict(cap=abs(big)), "the cap")):
         with pytest.raises(pkg.S2SError, match=word):
             plan(pkg, **more)(**tensors(pkg))
+
+
+def test_attention_document_tiles_past_a_launch_refused(pkg):
+    """The last counts of key tiles below 2^26, whose last workgroup would be the launch's 2^24th."""
+    b, nk = 24573, 32 * 2731
+    assert b * (nk // 32) == 2 ** 26 - 1
+    p = plan(pkg, dtype="f32", batch=b, q_tokens=17, k_tokens=nk, q_heads=1, k_heads=1, width=100)
+    a = [arr(pkg, (b, n, 1, 100), "f32", strides=(0, 100, 100, 1)) for n in (17, nk, nk, 17)]
+    with pytest.raises(pkg.S2SError, match="documents"):
+        p(*a, q_docs=arr(pkg, (17,), "i32"), k_docs=arr(pkg, (nk,), "i32"))
