@@ -15,10 +15,12 @@
 // the transposing LDS read (16-bit types) or by plain reads (f32, whose MFMA takes
 // one key per lane group). Nothing of the scores passes through LDS or HBM.
 //
-// What bounds it, measured on an MI355X. Prompts: instruction issue, since MFMA and
-// other VALU instructions do not overlap here: on 2 x 4096 causal bf16 tokens, 32 query and 8
-// key heads of 128, capped, 341 us, 810 TFLOP/s of the pairs that the mask leaves; 12001 f16 tokens with
-// slopes 38% MFMA and 43% VALU (680 us, 867 TFLOP/s); no LDS bank conflicts. Hence the tile's path
+// What bounds it, measured on an MI355X. Prompts: instructions, at the clock that power
+// leaves: on 2 x 4096 causal bf16 tokens, 32 query and 8 key heads of 128, capped, the matrix
+// cores are busy in 37% of the cycles and the other VALU instructions take 48%, at 2.04 GHz (341 us,
+// 810 TFLOP/s of the pairs that the mask leaves); 12001 f16 tokens with slopes 38% and 43%, at 1.99
+// GHz (680 us, 867 TFLOP/s); no LDS bank conflicts. (How far two waves of a SIMD could run the two at
+// the same time is not known; fewer of either have made every kernel here faster.) Hence the tile's path
 // counts its instructions: a polynomial for small capped scores, sums by MFMA, slopes in two
 // operations, max by v_maximum3. (The maximum is looked for under a cap too: one reference for all
 // of a call's rows, below the cap, gave 315 us, but left a row whose scores are all far below it

@@ -13,8 +13,11 @@ int round_up(int v, int m) { return (v + m - 1) / m * m; }
 // two products (2 x 4096 causal bf16, 32 / 8 heads: 128 wide 278 us against 366 by waves of 16,
 // 64 wide 167 and 200; 2048 tokens of 16 / 4 heads, too few, 103 and 43). `narrow`: waves of 16 only.
 // Where few columns leave CUs without work the keys are cut into ranges whose sums a second
-// kernel joins, up to two workgroups a CU (four: nothing for one query, 32 us against 15 for 64
-// sequences of 4 queries and 512 keys, by the join). Ranges of four tiles at least; of two, and up to 16
+// kernel joins, at most two workgroups a CU (four: nothing for one query, 32 us against 15 for 64
+// sequences of 4 queries and 512 keys, by the join). Column tiles of more than one a CU and less than two
+// are not cut, since the quotient is rounded down: 376 of them, 3000 f32 tokens of 8 heads of 32, take 91 us
+// causal and 125 over all keys, 71 and 97 in two ranges; the same of bf16 heads of 128, 58 and 66 against
+// 52 and 79. Ranges of four tiles at least; of two, and up to 16
 // of one, for columns of at most 16, whose rows to join are few: one query of 32 / 8 bf16 heads of 128 over 512,
 // 1024, 2048 and 4096 keys takes 9.1, 9.1, 9.9 and 10.5 us against 11.4 to 11.7, but over 256 keys
 // 9.0 against 8.1 uncut; 64 queries of 8 sequences over 256 keys 20 against 9.5.

@@ -323,7 +323,9 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
         }
         ss = wave_sum(ss);
         if constexpr (TPR == 256) {
-            // two sets of words in turn: a row's are read before the next but one writes them
+            // part[0] is the squares' sum, part[1] the largest magnitude (e4m3): a barrier lies between a
+            // row's last reading of either and the next row's writing, here the one behind the outputs, or
+            // the one behind the largest magnitudes
             if (lane == 0) part[0][tid >> 6] = ss;
             __syncthreads();
             ss = (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]);
