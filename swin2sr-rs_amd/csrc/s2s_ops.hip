@@ -187,6 +187,21 @@ __device__ __forceinline__ float nan_max(float m, float v) {
     return v > m || v != v ? v : m;
 }
 
+// 1 / sqrt(mean of n squares + eps) from the squares' sum. Where that lies past an f32's range, or
+// (with so small an eps) where its precision ends, it is made again of the row times 2^-80 or
+// 2^80: `again(factor)`, which all threads of the row call or none. (Squares of f16 lie within 2^-48
+// and 2^34, and 2^24 of them within both ends.)
+template <typename T, typename F>
+__device__ __forceinline__ float inverse_root(float ss, int n, float eps, const F &again) {
+    constexpr bool F16 = std::is_same<T, half_t>::value;
+    const bool far = !F16 && ss > 0x1p127f, near = !F16 && ss < 0x1p-100f && eps < 0x1p-100f;
+    if (__builtin_expect(far || near, 0)) {
+        const float f = far ? 0x1p-80f : 0x1p80f;
+        return f / sqrtf(again(f) / (float)n + eps * f * f);
+    }
+    return 1.0f / sqrtf(ss / (float)n + eps);
+}
+
 __device__ __forceinline__ float e4m3_scale(float top) {
     const float s = top / 448.f;
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;
@@ -204,16 +219,21 @@ __global__ __launch_bounds__(256) void k_rms_norm_rows(RmsNormArgs a) {
         const T *x = (const T *)a.x + row * a.xs;
         const T *res = a.res ? (const T *)a.res + row * a.rs : nullptr;
         T *sum = a.sum ? (T *)a.sum + row * a.ss : nullptr;
-        float ss = 0.f;
-        for (int c = tid; c < a.cols; c += 256) {
-            const float h = (float)x[c] + (res ? (float)res[c] : 0.f);
-            ss = fmaf(h, h, ss);
-        }
-        ss = wave_sum(ss);
-        if (lane == 0) part[wave] = ss;
-        __syncthreads();
-        const float mean = ((part[0] + part[1]) + (part[2] + part[3])) / (float)a.cols;
-        const float inv = 1.0f / sqrtf(mean + a.eps);
+        auto squares = [&](float f) {
+            float ss = 0.f;
+            for (int c = tid; c < a.cols; c += 256) {
+                const float h = ((float)x[c] + (res ? (float)res[c] : 0.f)) * f;
+                ss = fmaf(h, h, ss);
+            }
+            ss = wave_sum(ss);
+            if (lane == 0) part[wave] = ss;
+            __syncthreads();
+            return (part[0] + part[1]) + (part[2] + part[3]);
+        };
+        const float inv = inverse_root<T>(squares(1.f), a.cols, a.eps, [&](float f) {
+            __syncthreads();  // `part` has been read
+            return squares(f);
+        });
         auto value = [&](int c) {
             const float h = (float)x[c] + (res ? (float)res[c] : 0.f);
             return h * inv * (a.weight[c] + a.offset);
@@ -305,11 +325,27 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
 #pragma unroll
             for (int e = 0; e < V; ++e) h[n][e] = (float)u.e[e] + (float)v.e[e];
         }
-        float ss = 0.f;
+        auto squares = [&](float f) {
+            float ss = 0.f;
 #pragma unroll
-        for (int n = 0; n < NC; ++n)
+            for (int n = 0; n < NC; ++n)
 #pragma unroll
-            for (int e = 0; e < V; ++e) ss = fmaf(h[n][e], h[n][e], ss);
+                for (int e = 0; e < V; ++e) ss = fmaf(h[n][e] * f, h[n][e] * f, ss);
+            return ss;
+        };
+        // part[0] is the squares' sum, part[1] the largest magnitude (e4m3): a barrier lies between a
+        // row's last reading of either and the next row's writing, here the one behind the outputs, or
+        // the one behind the largest magnitudes
+        auto of_row = [&](float ss) {
+            ss = wave_sum(ss);
+            if constexpr (TPR == 256) {
+                if (lane == 0) part[0][tid >> 6] = ss;
+                __syncthreads();
+                ss = (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]);
+            }
+            return ss;
+        };
+        const float own = squares(1.f);
         if (a.sum) {
             T *sum = (T *)a.sum + row * a.ss;
 #pragma unroll
@@ -321,16 +357,10 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
                 if (i < chunks) *(Vec *)(sum + i * V) = u;
             }
         }
-        ss = wave_sum(ss);
-        if constexpr (TPR == 256) {
-            // part[0] is the squares' sum, part[1] the largest magnitude (e4m3): a barrier lies between a
-            // row's last reading of either and the next row's writing, here the one behind the outputs, or
-            // the one behind the largest magnitudes
-            if (lane == 0) part[0][tid >> 6] = ss;
-            __syncthreads();
-            ss = (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]);
-        }
-        const float inv = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+        const float inv = inverse_root<T>(of_row(own), a.cols, a.eps, [&](float f) {
+            if constexpr (TPR == 256) __syncthreads();  // `part` has been read
+            return of_row(squares(f));
+        });
 #pragma unroll
         for (int n = 0; n < NC; ++n)
 #pragma unroll

@@ -197,3 +197,23 @@ def test_attention_hidden_keys_of_large_calls(pkg, name, where):
             k[:, 80:], v[:, 70:75], v[:, 75:] = np.inf, np.nan, -np.inf
             extra["k_docs"][:, 70:] = np.where(np.arange(20) % 2, -1, 7)
     T.check_attention(pkg, T.case(**HIDDEN[name], **more, **T.WIDE), change)
+
+
+# ---- rows whose squares pass an f32 --------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [60, 180, 177, 4096, 16400])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_rms_norm_rows_far_from_one(pkg, dtype, cols, e4m3):
+    """Rows of 1e19 to 1e37 and, without eps, of 1e-19 to 1e-30: their squares' mean is past what an f32 holds, or below
+    its precision, and the norm is not."""
+    def change(x, r):
+        for n, s in enumerate((1e19, 1e25, 1e37, 1.0, 1e-19, 1e-25, 1e-30)):
+            x[n] *= s
+            r[n] *= s
+    for group in (0, 64) if e4m3 else (0,):
+        T.rms_case(pkg, dtype, 8, cols, e4m3=e4m3, group=group, change=change, eps=0.0)
+    def large(x, r):
+        x[1:4], r[1:4] = x[1:4] * 1e30, r[1:4] * 1e30
+    T.rms_case(pkg, dtype, 8, cols, e4m3=e4m3, change=large, alias=("sum",))
