@@ -1,5 +1,7 @@
 """The attention operator over the range of its values, on the GPU: values far from one, and
 keys that a mask hides, in every kernel that large calls take."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -136,7 +138,6 @@ def test_rms_norm_largest_group(pkg, cols):
 def test_operators_captured_in_every_mode(pkg, mode):
     """Capture in the global and the thread's own mode, which refuse calls that a capture cannot hold: a call makes none.
     Replays, with eager work between them, are the eager run."""
-    import ctypes as C
     h, vp = pkg.hip.rt(), C.c_void_p
     for name, args in {"hipStreamBeginCapture": [vp, C.c_int], "hipStreamEndCapture": [vp, C.POINTER(vp)],
                        "hipGraphInstantiate": [C.POINTER(vp), vp, vp, vp, C.c_size_t], "hipGraphLaunch": [vp, vp],
@@ -214,6 +215,7 @@ def test_rms_norm_rows_far_from_one(pkg, dtype, cols, e4m3):
             r[n] *= s
     for group in (0, 64) if e4m3 else (0,):
         T.rms_case(pkg, dtype, 8, cols, e4m3=e4m3, group=group, change=change, eps=0.0)
+
     def large(x, r):
         x[1:4], r[1:4] = x[1:4] * 1e30, r[1:4] * 1e30
     T.rms_case(pkg, dtype, 8, cols, e4m3=e4m3, change=large, alias=("sum",))
