@@ -354,6 +354,22 @@ typedef struct s2s_rotary_args {
 
 int s2s_rotary(const s2s_rotary_args *args, void *stream);
 
+/* The rotation of `rotary` of heads that are normed first, each by itself: channel c of
+ * a head x is x[c] / sqrt(mean over the width of x^2 + eps) * (weight[h][c] +
+ * weight_offset), channels past the pairs included, and the pairs of these are
+ * turned as above. The weights of q (and k) are f32, [width] for all heads (a head
+ * stride of 0) or a row for each head. (A head divided by its length, as for cosine
+ * attention: weights of 1 / sqrt(width), times the head's own scale.) `rotary`'s rules on
+ * arrays hold; the weights may not overlap the outputs. */
+typedef struct s2s_norm_rotary_args {
+    s2s_rotary_args rotary;
+    const float *q_weight, *k_weight; /* k_weight only with k */
+    int64_t q_weight_head, k_weight_head; /* head strides, in elements */
+    float weight_offset, eps;
+} s2s_norm_rotary_args;
+
+int s2s_norm_rotary(const s2s_norm_rotary_args *args, void *stream);
+
 /* out = h / sqrt(mean(h^2) + eps) * (weight + weight_offset) for every row of
  * h = x + res, the sum stored in `sum` too if that is not NULL. out_dtype is
  * dtype, or S2S_E4M3: then every `group` columns (0: the row; else a multiple of

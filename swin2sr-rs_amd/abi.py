@@ -67,6 +67,12 @@ class Rotary_(C.Structure):
                 ("inv_freq", C.POINTER(C.c_double)), ("pair_axis", C.POINTER(C.c_uint8))]
 
 
+class NormRotary_(C.Structure):
+    _fields_ = [("rotary", Rotary_), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p),
+                ("q_weight_head", C.c_int64), ("k_weight_head", C.c_int64),
+                ("weight_offset", C.c_float), ("eps", C.c_float)]
+
+
 class RmsNorm_(C.Structure):
     _fields_ = [("dtype", C.c_int), ("out_dtype", C.c_int), ("rows", C.c_int64), ("cols", C.c_int),
                 ("x", C.c_void_p), ("res", C.c_void_p), ("sum", C.c_void_p), ("out", C.c_void_p),
@@ -112,6 +118,7 @@ EXPORTS = {
     "s2s_attention_workspace": (C.c_int, [C.POINTER(Attention_), C.POINTER(C.c_uint64)]),
     "s2s_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
     "s2s_rotary": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "s2s_norm_rotary": (C.c_int, [C.c_void_p, C.c_void_p]),
     "s2s_rms_norm": (C.c_int, [C.c_void_p, C.c_void_p]),
     "s2s_test_window_map": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int32),
                                       C.POINTER(C.c_uint8)]),

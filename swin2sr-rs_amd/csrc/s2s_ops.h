@@ -42,6 +42,14 @@ struct RotaryArgs {
     unsigned char axis[128];
 };
 
+// Rotary positions behind a norm of every head.
+struct NormRotaryArgs {
+    RotaryArgs r;
+    const float *qw, *kw;
+    long long qw_head, kw_head;  // the weights' head strides (0: one row for all heads)
+    float offset, eps;
+};
+
 struct RmsNormArgs {
     long long rows;
     int cols, group, groups;  // group: columns per scale
@@ -74,4 +82,5 @@ hipError_t enqueue(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipS
 size_t attn_op_workspace(int dtype, const AttnOpArgs &a);
 hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStream_t st);
 hipError_t launch_rotary_op(int dtype, const RotaryArgs &a, hipStream_t st);
+hipError_t launch_norm_rotary_op(int dtype, const NormRotaryArgs &a, hipStream_t st);
 hipError_t launch_rms_norm_op(int dtype, bool e4m3, const RmsNormArgs &a, hipStream_t st);

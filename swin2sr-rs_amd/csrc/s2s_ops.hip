@@ -14,6 +14,13 @@
 
 namespace {
 
+__device__ __forceinline__ float wave_sum(float v) {
+    v = row16_sum(v);
+    float w = v;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+    return half_sum(v + w);
+}
+
 // ---- rotary ------------------------------------------------------------------
 
 // sin and cos of a whole turn times f / 2^64. The angle arrives in turns as a
@@ -159,13 +166,6 @@ hipError_t rotary_type(const RotaryArgs &a, hipStream_t st) {
 }
 
 // ---- root-mean-square norm ------------------------------------------------------
-
-__device__ __forceinline__ float wave_sum(float v) {
-    v = row16_sum(v);
-    float w = v;
-    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(w));
-    return half_sum(v + w);
-}
 
 // The nearest e4m3 (OCP, ties to even) of v clamped to +-448; NaN stays NaN.
 __device__ __forceinline__ unsigned char to_e4m3(float v) {
@@ -480,7 +480,65 @@ hipError_t rms_type(const RmsNormArgs &a, hipStream_t st) {
     return enqueue(k_rms_norm_rows<T, E4M3>, dim3((unsigned)std::min(a.rows, 1LL << 20)), dim3(256), 0, st, a);
 }
 
+// ---- norms of heads with the rotation ----------------------------------------------
+
+// A wave per token and head, any width and alignment: the head is read for the sum of squares
+// and, pair by pair, again for the output, with a pair's angle made where it is used.
+template <typename T>
+__global__ __launch_bounds__(256) void k_norm_rotary_heads(NormRotaryArgs a) {
+    const RotaryArgs &r = a.r;
+    const int lane = threadIdx.x & 63, heads = r.hq + r.hk;
+    const long long items = (long long)r.batch * r.tokens * heads;
+    for (long long it = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += (long long)gridDim.x * 4) {
+        const long long tok = it / heads;
+        const int hh = (int)(it - tok * heads);
+        const int b = (int)(tok / r.tokens), at = (int)(tok - (long long)b * r.tokens);
+        if (r.lens && at >= r.lens[b]) continue;
+        const bool isq = hh < r.hq;
+        const int h = isq ? hh : hh - r.hq;
+        const Strides &si = isq ? r.sq : r.sk, &so = isq ? r.sqo : r.sko;
+        const T *x = (const T *)(isq ? r.q : r.k) + b * si.b + at * si.t + h * si.h;
+        T *y = (T *)(isq ? r.qo : r.ko) + b * so.b + at * so.t + h * so.h;
+        const float *w = isq ? a.qw + h * a.qw_head : a.kw + h * a.kw_head;
+        const int *pos = r.pos + b * r.pos_b + (long long)at * r.axes;
+        auto squares = [&](float f) {
+            float ss = 0.f;
+            for (int c = lane; c < r.width; c += 64) {
+                const float v = (float)x[c] * f;
+                ss = fmaf(v, v, ss);
+            }
+            return wave_sum(ss);
+        };
+        const float inv = inverse_root<T>(squares(1.f), r.width, a.eps, squares);
+        auto value = [&](int c) { return (float)x[c] * inv * (w[c] + a.offset); };
+        for (int p = lane; p < r.pairs; p += 64) {
+            const int c0 = r.adjacent ? 2 * p : p, c1 = r.adjacent ? c0 + 1 : c0 + r.pairs;
+            const float u = value(c0), v = value(c1);
+            float s, c;
+            sincos_turns((unsigned long long)(long long)pos[r.axis[p]] * r.freq[p], s, c);
+            y[c0] = (T)fmaf(u, c, -v * s);
+            y[c1] = (T)fmaf(u, s, v * c);
+        }
+        for (int c = 2 * r.pairs + lane; c < r.width; c += 64) y[c] = (T)value(c);
+    }
+}
+
+template <typename T>
+hipError_t norm_rotary_type(const NormRotaryArgs &a, hipStream_t st) {
+    const long long items = (long long)a.r.batch * a.r.tokens * (a.r.hq + a.r.hk);
+    return enqueue(k_norm_rotary_heads<T>, dim3((unsigned)std::min((items + 3) / 4, 1LL << 20)), dim3(256), 0, st, a);
+}
+
 }  // namespace
+
+hipError_t launch_norm_rotary_op(int dtype, const NormRotaryArgs &a, hipStream_t st) {
+    switch (dtype) {
+        case 0: return norm_rotary_type<float>(a, st);
+        case 1: return norm_rotary_type<half_t>(a, st);
+        case 2: return norm_rotary_type<bfloat_t>(a, st);
+    }
+    return hipErrorInvalidValue;
+}
 
 hipError_t launch_rotary_op(int dtype, const RotaryArgs &a, hipStream_t st) {
     switch (dtype) {

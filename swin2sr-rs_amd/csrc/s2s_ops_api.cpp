@@ -167,6 +167,109 @@ AttnOpArgs attention_args(const s2s_attention_args *a) {
     return k;
 }
 
+// Rotary positions, behind a norm of the heads if `n` is not null (`a` is its part then).
+int rotary_call(const char *op, const s2s_rotary_args *a, const s2s_norm_rotary_args *n, void *stream) {
+    if (!is_real_type(a->dtype)) return refuse("%s: dtype %d is not f32, f16 or bf16", op, a->dtype);
+    if (a->batch < 0 || a->tokens < 0 || a->q_heads < 1 || a->k_heads < 0)
+        return refuse("%s: negative sizes, or no query head", op);
+    if (a->width < 2 || a->width > 65536) return refuse("%s: width %d is not in 2 to 65536", op, a->width);
+    if (a->axes < 1 || a->axes > 4) return refuse("%s: %d axes: 1 to 4 are wanted", op, a->axes);
+    if (a->pairs < 1 || a->pairs > 128 || 2 * a->pairs > a->width)
+        return refuse("%s: %d pairs: 1 to 128 that fit the width are wanted", op, a->pairs);
+    if ((long long)a->batch * a->tokens > (1 << 30) || a->q_heads > 65535 || a->k_heads > 65535)
+        return refuse("%s: over 2^30 tokens or 65535 heads", op);
+    if (!a->inv_freq || !a->pair_axis) return refuse("%s: inv_freq or pair_axis is null", op);
+    for (int i = 0; i < a->pairs; ++i) {
+        if (!(std::fabs(a->inv_freq[i]) < 1048576.0)) return refuse("%s: inv_freq[%d] is not below 2^20", op, i);
+        if (a->pair_axis[i] >= a->axes) return refuse("%s: pair_axis[%d] is no axis", op, i);
+    }
+    if (a->pos_batch < 0 || a->pos_batch > kMaxStride) return refuse("%s: a negative or impossible batch stride", op);
+    if (n) {
+        if (!(n->eps >= 0.f) || !std::isfinite(n->eps) || !std::isfinite(n->weight_offset))
+            return refuse("%s: eps is negative, or eps or weight_offset not finite", op);
+        if (n->q_weight_head < 0 || n->k_weight_head < 0 || n->q_weight_head > kMaxStride || n->k_weight_head > kMaxStride)
+            return refuse("%s: a negative or impossible head stride of the weights", op);
+    }
+    if (a->batch == 0 || a->tokens == 0) return 0;
+    if (a->k_heads > 0 && a->q_out.data && a->k_out.data == a->q_out.data)
+        return refuse("%s: q_out and k_out are the same array", op);
+    // (other workgroups may not have read the other input yet)
+    if (a->k_heads > 0 && a->q_out.data && (a->q_out.data == a->k.data || a->k_out.data == a->q.data))
+        return refuse("%s: q's output is k, or k's is q", op);
+    OnDevice on;
+    const hipStream_t st = (hipStream_t)stream;
+    hipError_t e = on.enter(st);
+    if (e != hipSuccess) return refuse_hip(op, "the stream's device", e);
+    const bool has_k = a->k_heads > 0;
+    if (int rc = check_tokens(op, "q", a->q, a->dtype, on.dev)) return rc;
+    if (int rc = check_tokens(op, "q_out", a->q_out, a->dtype, on.dev)) return rc;
+    if (int rc = check_written(op, "q_out", a->q_out, a->batch, a->tokens, a->q_heads, a->width)) return rc;
+    if (has_k) {
+        if (int rc = check_tokens(op, "k", a->k, a->dtype, on.dev)) return rc;
+        if (int rc = check_tokens(op, "k_out", a->k_out, a->dtype, on.dev)) return rc;
+        if (int rc = check_written(op, "k_out", a->k_out, a->batch, a->tokens, a->k_heads, a->width)) return rc;
+    }
+    auto same = [&](const s2s_tokens &x, const s2s_tokens &y, int heads) {
+        const Strides s = strides(x, a->batch, a->tokens, heads), t = strides(y, a->batch, a->tokens, heads);
+        return x.data != y.data || (s.b == t.b && s.t == t.t && s.h == t.h);
+    };
+    if (!same(a->q, a->q_out, a->q_heads) || (has_k && !same(a->k, a->k_out, a->k_heads)))
+        return refuse("%s: in place, the output's strides must be the input's", op);
+    if (!a->pos) return refuse("%s: pos is null", op);
+    if (int rc = check_array(op, "pos", a->pos, 4, on.dev)) return rc;
+    if (a->lens)
+        if (int rc = check_array(op, "lens", a->lens, 4, on.dev)) return rc;
+    if (n) {
+        if (!n->q_weight || (has_k && !n->k_weight)) return refuse("%s: q_weight or k_weight is null", op);
+        if (int rc = check_array(op, "q_weight", n->q_weight, 4, on.dev)) return rc;
+        if (has_k)
+            if (int rc = check_array(op, "k_weight", n->k_weight, 4, on.dev)) return rc;
+    }
+    NormRotaryArgs m{};
+    RotaryArgs &k = m.r;
+    k.batch = a->batch;
+    k.tokens = a->tokens;
+    k.hq = a->q_heads;
+    k.hk = a->k_heads;
+    k.width = a->width;
+    k.axes = a->axes;
+    k.pairs = a->pairs;
+    k.adjacent = a->adjacent != 0;
+    k.q = a->q.data;
+    k.qo = a->q_out.data;
+    k.sq = strides(a->q, a->batch, a->tokens, a->q_heads);
+    k.sqo = strides(a->q_out, a->batch, a->tokens, a->q_heads);
+    if (has_k) {
+        k.k = a->k.data;
+        k.ko = a->k_out.data;
+        k.sk = strides(a->k, a->batch, a->tokens, a->k_heads);
+        k.sko = strides(a->k_out, a->batch, a->tokens, a->k_heads);
+    }
+    k.pos = a->pos;
+    k.pos_b = a->pos_batch;
+    k.lens = a->lens;
+    for (int i = 0; i < a->pairs; ++i) {
+        // inv_freq / 2 pi turns, its fraction in 64 bits (long double: 64-bit significand)
+        // inv_freq below 2^20 leaves whole turns that an int holds
+        long double t = (long double)a->inv_freq[i] * 0.15915494309189533576888376337251436L;
+        t -= (long double)(int)t;
+        if (t < 0) t += 1.0L;
+        const unsigned long long f = t >= 1.0L ? 0ULL : (unsigned long long)(t * 18446744073709551616.0L);
+        k.freq[i] = a->inverse ? 0ULL - f : f;
+        k.axis[i] = a->pair_axis[i];
+    }
+    if (n) {
+        m.qw = n->q_weight;
+        m.kw = n->k_weight;
+        m.qw_head = a->q_heads > 1 ? n->q_weight_head : 0;
+        m.kw_head = a->k_heads > 1 ? n->k_weight_head : 0;
+        m.offset = n->weight_offset;
+        m.eps = n->eps;
+    }
+    e = n ? launch_norm_rotary_op(a->dtype, m, st) : launch_rotary_op(a->dtype, k, st);
+    return e == hipSuccess ? 0 : refuse_hip(op, "the launch", e);
+}
+
 }  // namespace
 
 extern "C" {
@@ -252,84 +355,13 @@ int s2s_attention(const s2s_attention_args *a, void *workspace, uint64_t workspa
 int s2s_rotary(const s2s_rotary_args *a, void *stream) {
     const char *op = "s2s_rotary";
     if (!a) return refuse("%s: null argument", op);
-    if (!is_real_type(a->dtype)) return refuse("%s: dtype %d is not f32, f16 or bf16", op, a->dtype);
-    if (a->batch < 0 || a->tokens < 0 || a->q_heads < 1 || a->k_heads < 0)
-        return refuse("%s: negative sizes, or no query head", op);
-    if (a->width < 2 || a->width > 65536) return refuse("%s: width %d is not in 2 to 65536", op, a->width);
-    if (a->axes < 1 || a->axes > 4) return refuse("%s: %d axes: 1 to 4 are wanted", op, a->axes);
-    if (a->pairs < 1 || a->pairs > 128 || 2 * a->pairs > a->width)
-        return refuse("%s: %d pairs: 1 to 128 that fit the width are wanted", op, a->pairs);
-    if ((long long)a->batch * a->tokens > (1 << 30) || a->q_heads > 65535 || a->k_heads > 65535)
-        return refuse("%s: over 2^30 tokens or 65535 heads", op);
-    if (!a->inv_freq || !a->pair_axis) return refuse("%s: inv_freq or pair_axis is null", op);
-    for (int i = 0; i < a->pairs; ++i) {
-        if (!(std::fabs(a->inv_freq[i]) < 1048576.0)) return refuse("%s: inv_freq[%d] is not below 2^20", op, i);
-        if (a->pair_axis[i] >= a->axes) return refuse("%s: pair_axis[%d] is no axis", op, i);
-    }
-    if (a->pos_batch < 0 || a->pos_batch > kMaxStride) return refuse("%s: a negative or impossible batch stride", op);
-    if (a->batch == 0 || a->tokens == 0) return 0;
-    if (a->k_heads > 0 && a->q_out.data && a->k_out.data == a->q_out.data)
-        return refuse("%s: q_out and k_out are the same array", op);
-    // (other workgroups may not have read the other input yet)
-    if (a->k_heads > 0 && a->q_out.data && (a->q_out.data == a->k.data || a->k_out.data == a->q.data))
-        return refuse("%s: q's output is k, or k's is q", op);
-    OnDevice on;
-    const hipStream_t st = (hipStream_t)stream;
-    hipError_t e = on.enter(st);
-    if (e != hipSuccess) return refuse_hip(op, "the stream's device", e);
-    const bool has_k = a->k_heads > 0;
-    if (int rc = check_tokens(op, "q", a->q, a->dtype, on.dev)) return rc;
-    if (int rc = check_tokens(op, "q_out", a->q_out, a->dtype, on.dev)) return rc;
-    if (int rc = check_written(op, "q_out", a->q_out, a->batch, a->tokens, a->q_heads, a->width)) return rc;
-    if (has_k) {
-        if (int rc = check_tokens(op, "k", a->k, a->dtype, on.dev)) return rc;
-        if (int rc = check_tokens(op, "k_out", a->k_out, a->dtype, on.dev)) return rc;
-        if (int rc = check_written(op, "k_out", a->k_out, a->batch, a->tokens, a->k_heads, a->width)) return rc;
-    }
-    auto same = [&](const s2s_tokens &x, const s2s_tokens &y, int heads) {
-        const Strides s = strides(x, a->batch, a->tokens, heads), t = strides(y, a->batch, a->tokens, heads);
-        return x.data != y.data || (s.b == t.b && s.t == t.t && s.h == t.h);
-    };
-    if (!same(a->q, a->q_out, a->q_heads) || (has_k && !same(a->k, a->k_out, a->k_heads)))
-        return refuse("%s: in place, the output's strides must be the input's", op);
-    if (!a->pos) return refuse("%s: pos is null", op);
-    if (int rc = check_array(op, "pos", a->pos, 4, on.dev)) return rc;
-    if (a->lens)
-        if (int rc = check_array(op, "lens", a->lens, 4, on.dev)) return rc;
-    RotaryArgs k{};
-    k.batch = a->batch;
-    k.tokens = a->tokens;
-    k.hq = a->q_heads;
-    k.hk = a->k_heads;
-    k.width = a->width;
-    k.axes = a->axes;
-    k.pairs = a->pairs;
-    k.adjacent = a->adjacent != 0;
-    k.q = a->q.data;
-    k.qo = a->q_out.data;
-    k.sq = strides(a->q, a->batch, a->tokens, a->q_heads);
-    k.sqo = strides(a->q_out, a->batch, a->tokens, a->q_heads);
-    if (has_k) {
-        k.k = a->k.data;
-        k.ko = a->k_out.data;
-        k.sk = strides(a->k, a->batch, a->tokens, a->k_heads);
-        k.sko = strides(a->k_out, a->batch, a->tokens, a->k_heads);
-    }
-    k.pos = a->pos;
-    k.pos_b = a->pos_batch;
-    k.lens = a->lens;
-    for (int i = 0; i < a->pairs; ++i) {
-        // inv_freq / 2 pi turns, its fraction in 64 bits (long double: 64-bit significand)
-        // inv_freq below 2^20 leaves whole turns that an int holds
-        long double t = (long double)a->inv_freq[i] * 0.15915494309189533576888376337251436L;
-        t -= (long double)(int)t;
-        if (t < 0) t += 1.0L;
-        const unsigned long long f = t >= 1.0L ? 0ULL : (unsigned long long)(t * 18446744073709551616.0L);
-        k.freq[i] = a->inverse ? 0ULL - f : f;
-        k.axis[i] = a->pair_axis[i];
-    }
-    e = launch_rotary_op(a->dtype, k, st);
-    return e == hipSuccess ? 0 : refuse_hip(op, "the launch", e);
+    return rotary_call(op, a, nullptr, stream);
+}
+
+int s2s_norm_rotary(const s2s_norm_rotary_args *a, void *stream) {
+    const char *op = "s2s_norm_rotary";
+    if (!a) return refuse("%s: null argument", op);
+    return rotary_call(op, &a->rotary, a, stream);
 }
 
 int s2s_rms_norm(const s2s_rms_norm_args *a, void *stream) {

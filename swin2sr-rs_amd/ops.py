@@ -104,6 +104,7 @@ def _tokens(a, shape, dtype: int, op: str, name: str):
 # ctypes take as long as the call): the C structs' layout, null pointers as 0.
 _ATTENTION = struct.Struct("@8i2f 4q4q4q4q 3P 2P2q 2P2q 2Pi0q")
 _ROTARY = struct.Struct("@10i 4q4q4q4q Pq3P")
+_NORM_ROTARY = struct.Struct(_ROTARY.format + "2P2q2f")
 _RMS = struct.Struct("@2iqi4P4qP2fPi0q")
 
 
@@ -232,7 +233,13 @@ class Rotary:
         """q (and k) [batch][tokens][heads][width] into q_out (and k_out), in place
         without them; pos int32 [batch][tokens][axes] or [tokens][axes]; tokens
         from lens[b] on are not written."""
-        op = "rotary"
+        args, q_out, k_out = self._arrays("rotary", q, pos, q_out, k, k_out, lens)
+        if self.lib.s2s_rotary(_ROTARY.pack(*args), stream):
+            raise S2SError(f"rotary: {last_error()}")
+        return q_out if k is None else (q_out, k_out)
+
+    def _arrays(self, op, q, pos, q_out, k, k_out, lens):
+        """The struct's fields, and the outputs."""
         shape = q.shape
         _need(len(shape) == 4 and max(shape) < 2 ** 31, f"{op}: q is {tuple(shape)}, wanted [batch][tokens][heads][width]")
         dt = _type(q.dtype)
@@ -255,12 +262,53 @@ class Rotary:
               f"{op}: pos is {ps} of {pos.dtype}, wanted int32 [batch][tokens][axes] or [tokens][axes]")
         _need((pstr[-1] == 1 or ps[-1] == 1) and (pstr[-2] == ps[-1] or ps[-2] <= 1),
               f"{op}: the tokens and axes of pos are not adjacent")
-        args = _ROTARY.pack(dt, shape[0], shape[1], shape[2], k_heads, shape[3], min(ps[-1], 2 ** 31 - 1), *self.flags, *arrays[0],
-                            *k_arrays[0], *arrays[1], *k_arrays[1], pos.data_ptr(), pstr[0] if len(ps) == 3 else 0,
-                            _vector(lens, shape[0], op, "lens"), *self.host)
-        if self.lib.s2s_rotary(args, stream):
+        return (dt, shape[0], shape[1], shape[2], k_heads, shape[3], min(ps[-1], 2 ** 31 - 1), *self.flags, *arrays[0],
+                *k_arrays[0], *arrays[1], *k_arrays[1], pos.data_ptr(), pstr[0] if len(ps) == 3 else 0,
+                _vector(lens, shape[0], op, "lens"), *self.host), q_out, k_out
+
+
+class NormRotary(Rotary):
+    """Rotary positions of heads that are normed first: a head is divided by the root of
+    its mean square (plus eps) and multiplied by weight + weight_offset before its pairs are turned.
+
+        turn = ops.NormRotary.of((32, 32), eps=1e-6)
+        turn(q, pos, q_weight, k=k, k_weight=k_weight, stream=stream)
+    """
+
+    def __init__(self, inv_freq: Sequence[float], pair_axis: Sequence[int], eps: float = 1e-6, weight_offset: float = 0.0,
+                 adjacent: bool = False, inverse: bool = False):
+        super().__init__(inv_freq, pair_axis, adjacent=adjacent, inverse=inverse)
+        self.numbers = (_f32(weight_offset), _f32(eps))
+
+    @classmethod
+    def of(cls, sections: Sequence[int], theta: float = 10000.0, eps: float = 1e-6, weight_offset: float = 0.0,
+           adjacent: bool = False, inverse: bool = False):
+        return cls([theta ** (-i / n) for n in sections for i in range(n)],
+                   [a for a, n in enumerate(sections) for _ in range(n)], eps=eps, weight_offset=weight_offset,
+                   adjacent=adjacent, inverse=inverse)
+
+    def __call__(self, q, pos, q_weight, q_out=None, k=None, k_weight=None, k_out=None, lens=None, stream: int = 0):
+        """As `Rotary`'s call, with f32 weights [width] or [heads][width] of q (and k)."""
+        op = "norm_rotary"
+        args, q_out, k_out = self._arrays(op, q, pos, q_out, k, k_out, lens)
+        qw, qs = _head_weight(q_weight, q.shape, op, "q_weight")
+        kw = ks = 0
+        if k is not None:
+            _need(k_weight is not None, f"{op}: k without k_weight")
+            kw, ks = _head_weight(k_weight, k.shape, op, "k_weight")
+        else:
+            _need(k_weight is None, f"{op}: k_weight without k")
+        if self.lib.s2s_norm_rotary(_NORM_ROTARY.pack(*args, qw, kw, qs, ks, *self.numbers), stream):
             raise S2SError(f"{op}: {last_error()}")
         return q_out if k is None else (q_out, k_out)
+
+
+def _head_weight(w, shape, op: str, name: str):
+    """f32 [width], or [heads][width] with adjacent channels: address and head stride."""
+    ws = tuple(w.shape)
+    _need(_is_f32(w.dtype) and ws in (tuple(shape[3:]), tuple(shape[2:])) and (w.stride()[-1] == 1 or shape[3] == 1),
+          f"{op}: {name} is {ws} of {w.dtype}, wanted f32 [{shape[3]}] or [{shape[2]}][{shape[3]}] with adjacent channels")
+    return w.data_ptr(), (w.stride()[0] if len(ws) == 2 else 0)
 
 
 def _rows(a, shape, dtype: int, op: str, name: str):

@@ -108,6 +108,18 @@ pub struct S2sRotaryArgs {
     pub pair_axis: *const u8,
 }
 
+/// `s2s_norm_rotary_args`: one call of the heads' norms with the rotation.
+#[repr(C)]
+pub struct S2sNormRotaryArgs {
+    pub rotary: S2sRotaryArgs,
+    pub q_weight: *const f32,
+    pub k_weight: *const f32,
+    pub q_weight_head: i64,
+    pub k_weight_head: i64,
+    pub weight_offset: f32,
+    pub eps: f32,
+}
+
 /// `s2s_rms_norm_args`: one call of the root-mean-square norm.
 #[repr(C)]
 pub struct S2sRmsNormArgs {
@@ -163,6 +175,7 @@ extern "C" {
     pub fn s2s_attention_workspace(args: *const S2sAttentionArgs, bytes: *mut u64) -> c_int;
     pub fn s2s_attention(args: *const S2sAttentionArgs, workspace: *mut c_void, bytes: u64, stream: *mut c_void) -> c_int;
     pub fn s2s_rotary(args: *const S2sRotaryArgs, stream: *mut c_void) -> c_int;
+    pub fn s2s_norm_rotary(args: *const S2sNormRotaryArgs, stream: *mut c_void) -> c_int;
     pub fn s2s_rms_norm(args: *const S2sRmsNormArgs, stream: *mut c_void) -> c_int;
 }
 

@@ -203,3 +203,23 @@ def rotary(x, angle, pairs, adjacent, inverse):
     a, b = x[..., i], x[..., j]
     y[..., i], y[..., j] = a * c - b * s, a * s + b * c
     return y
+
+
+def norm_rotary(dtype, x, weight, offset, eps, angle, pairs, adjacent, inverse):
+    """(out, bound): heads x [B][L][H][D] (values of `dtype`) normed, times weight [D] or [H][D] plus
+    offset, and turned by angle [B][L][pairs], in 64 bits, and what a 32-bit evaluation may be off.
+
+    The bound, with u = 2^-24: the squares' sum is a chain of at most max(16, D / 64) additions in
+    a lane and 6 across lanes, halved by the root; the mean and eps (2 u, halved), root, reciprocal
+    and three roundings of the product with the weight (whose own sum is one): max(16, D / 64) / 2
+    + 9 u of the normed channel. Sin and cos are off by 3 u, two products and a sum: 6 u of the pair's
+    magnitudes. The result is rounded once."""
+    u, D = 2.0 ** -24, x.shape[-1]
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        y = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * (np.asarray(weight, np.float64) + offset)
+        out = rotary(y, angle, pairs, adjacent, inverse)
+        mag = np.abs(y)
+        i, j = (slice(0, 2 * pairs, 2), slice(1, 2 * pairs, 2)) if adjacent else (slice(0, pairs), slice(pairs, 2 * pairs))
+        both = mag[..., i] + mag[..., j]
+        mag[..., i], mag[..., j] = both, both
+        return out, (max(16, D / 64) / 2 + 15) * u * mag + np.maximum(HALF[dtype] * np.abs(out), TINY[dtype] / 2)

@@ -1,0 +1,125 @@
+"""Heads' norms with the rotation, attention with a sliding window and attention of a batch that
+shares a prefix, without a GPU: every refusal that needs no device, and the plain implementations."""
+import ctypes as C
+import re
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+import ops_ref as R
+from test_ops import arr
+
+# ---- heads' norms with the rotation ------------------------------------------------
+
+
+def turn(pkg, q=(2, 5, 4, 64), k=None, qw=(64,), kw=None, sections=(16, 16), plan=None, **more):
+    p = plan or pkg.ops.NormRotary.of(sections)
+    p(arr(pkg, q), arr(pkg, (q[0], q[1], len(sections)), "i32"), arr(pkg, qw, "f32"), k=arr(pkg, k, ptr=8192) if k else None,
+      k_weight=arr(pkg, kw, "f32") if kw else None, **more)
+
+
+@pytest.mark.parametrize("call,word", [
+    (dict(qw=(63,)), "q_weight"), (dict(qw=(3, 64)), "q_weight"), (dict(qw=(2, 5, 64)), "q_weight"),
+    (dict(k=(2, 5, 2, 64)), "k without k_weight"), (dict(kw=(64,)), "k_weight without k"),
+    (dict(k=(2, 5, 2, 64), kw=(4, 64)), "k_weight"), (dict(k=(2, 4, 2, 64), kw=(64,)), "k is"),
+    (dict(sections=(16, 17)), "pairs"), (dict(sections=(8,) * 5), "axes"), (dict(q=(5, 4, 64)), "wanted"),
+])
+def test_norm_rotary_refused(pkg, call, word):
+    with pytest.raises(pkg.S2SError, match=word):
+        turn(pkg, **call)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_norm_rotary_weight_type_refused(pkg, dtype):
+    p = pkg.ops.NormRotary.of((16, 16))
+    with pytest.raises(pkg.S2SError, match="q_weight"):
+        p(arr(pkg, (2, 5, 4, 64)), arr(pkg, (2, 5, 2), "i32"), arr(pkg, (64,), dtype))
+    with pytest.raises(pkg.S2SError, match="q_weight"):
+        p(arr(pkg, (2, 5, 4, 64)), arr(pkg, (2, 5, 2), "i32"), arr(pkg, (4, 64), "f32", strides=(128, 2)))
+
+
+@pytest.mark.parametrize("number", [-1.0, float("nan"), float("inf"), 1e39])
+def test_norm_rotary_eps_refused(pkg, number):
+    with pytest.raises(pkg.S2SError, match="eps"):
+        turn(pkg, plan=pkg.ops.NormRotary.of((16, 16), eps=number))
+    if number != -1.0:
+        with pytest.raises(pkg.S2SError, match="weight_offset"):
+            turn(pkg, plan=pkg.ops.NormRotary.of((16, 16), weight_offset=number))
+
+
+def test_norm_rotary_nothing_to_do(pkg):
+    for shape in ((0, 4, 2, 64), (2, 0, 2, 64)):
+        pkg.ops.NormRotary.of((16, 16))(arr(pkg, shape, ptr=0), arr(pkg, shape[:2] + (2,), "i32", ptr=0), arr(pkg, (64,), "f32", ptr=0))
+
+
+def test_norm_rotary_across_refused(pkg):
+    q, k, o = (arr(pkg, (1, 4, 2, 64), ptr=4096 * (1 + i)) for i in range(3))
+    w = arr(pkg, (64,), "f32")
+    with pytest.raises(pkg.S2SError, match="q's output is k"):
+        pkg.ops.NormRotary.of((16, 16))(q, arr(pkg, (1, 4, 2), "i32"), w, q_out=k, k=k, k_weight=w, k_out=o)
+
+
+# ---- the C interface ------------------------------------------------------------------
+
+STRUCTS = [("S2sNormRotaryArgs", "s2s_norm_rotary_args", "NormRotary_", "_NORM_ROTARY")]
+RUST = {"s2s_rotary_args": "S2sRotaryArgs", "s2s_attention_args": "S2sAttentionArgs", "s2s_tokens": "S2sTokens", "int": "c_int",
+        "float": "f32", "int64_t": "i64"}
+
+
+@pytest.mark.parametrize("rust,c,py,pack", STRUCTS)
+def test_structs_are_the_headers(pkg, rust, c, py, pack):
+    """The Rust and Python structs have the header's fields, in its order and of its types, and the pack that a call sends is
+    the struct: distinct values packed come back under the fields, nested ones flattened."""
+    root = Path(__file__).resolve().parent.parent
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (c, c), (root / "include" / "swin2sr_hip.h").read_text(), re.S).group(1)
+    fields = []
+    for decl in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"):
+        m = re.match(r"\s*((?:const )?\w+)\s+(.*)", decl.strip(), re.S)
+        if m:
+            for name in m.group(2).split(","):
+                fields.append((name.strip().lstrip("*"), "pointer" if name.strip().startswith("*") else m.group(1)))
+    rs = re.search(r"pub struct %s \{(.*?)\n\}" % rust, (root / "swin2sr-rs_amd" / "rust" / "src" / "hip.rs").read_text(), re.S).group(1)
+    rs = re.findall(r"pub (\w+): ([^,\n]+),", rs)
+    struct = getattr(pkg.abi, py)
+    assert [n for n, _ in rs] == [n for n, _ in fields] == [n for n, _ in struct._fields_]
+    for (name, kind), (_, rt), (_, pt) in zip(fields, rs, struct._fields_):
+        if kind == "pointer":
+            assert rt.startswith("*") and C.sizeof(pt) == 8, name
+        else:
+            assert rt == RUST[kind], name
+            assert pt in {"int": [C.c_int], "float": [C.c_float], "int64_t": [C.c_int64], "s2s_tokens": [pkg.abi.Tokens_],
+                          "s2s_rotary_args": [pkg.abi.Rotary_], "s2s_attention_args": [pkg.abi.Attention_]}[kind], name
+    packer = getattr(pkg.ops, pack)
+    assert packer.size == C.sizeof(struct)
+
+    def leaves(s):
+        for f, t in s._fields_:
+            v = getattr(s, f)
+            if isinstance(v, C.Structure):
+                yield from leaves(v)
+            elif isinstance(v, C._Pointer):
+                yield C.cast(v, C.c_void_p).value
+            else:
+                yield v
+    n = len(list(leaves(struct())))
+    assert list(leaves(struct.from_buffer_copy(packer.pack(*range(1, n + 1))))) == list(range(1, n + 1))
+
+
+def test_null_arguments_refused(pkg):
+    lib = pkg.load_library()
+    assert lib.s2s_norm_rotary(None, None) != 0 and b"null" in lib.s2s_last_error()
+
+
+# ---- the plain implementations ----------------------------------------------------------
+
+
+def test_plain_norm_rotary():
+    """A head of equal channels has the weights, turned, whatever its size."""
+    x = np.full((1, 2, 1, 6), 7.0)
+    w = np.arange(1.0, 7.0)
+    for adjacent in (False, True):
+        y, bound = R.norm_rotary("f32", x, w, 0.0, 0.0, np.full((1, 2, 2), np.pi / 2), 2, adjacent, False)
+        i, j = ([0, 2], [1, 3]) if adjacent else ([0, 1], [2, 3])
+        assert np.allclose(y[..., i], -w[j]) and np.allclose(y[..., j], w[i]) and np.allclose(y[..., 4:], w[4:])
+        assert (bound > 0).all() and (bound < 1e-4).all()
