@@ -332,6 +332,18 @@ int s2s_attention_workspace(const s2s_attention_args *args, uint64_t *bytes);
  * need no preparation and are left undefined. */
 int s2s_attention(const s2s_attention_args *args, void *workspace, uint64_t workspace_bytes, void *stream);
 
+/* The same with a sliding window and sinks. Of the keys that take part by the rules
+ * above, a query sees j > P(i) - window (the `window` last ones up to its own place,
+ * under `causal`) and the entry's first keys, j < sinks; without `causal`, of
+ * both only j < P(i) + window. P(i) goes by tokens, also where positions are given for the
+ * biases. Tiles of keys that no query of a workgroup sees are neither read nor
+ * counted. With documents, sinks have to be 0 (they would be the entry's first keys
+ * and not each document's). window and sinks up to 2^30; the workspace goes by
+ * them and `causal` too. */
+int s2s_window_attention_workspace(const s2s_attention_args *args, int window, int sinks, uint64_t *bytes);
+int s2s_window_attention(const s2s_attention_args *args, int window, int sinks, void *workspace, uint64_t workspace_bytes,
+                         void *stream);
+
 /* Rotary positions with up to four axes: the pair p of every head of q (and k)
  * is turned by the angle pos[b][token][pair_axis[p]] * inv_freq[p]. Pairs are
  * channels (p, p + pairs), or (2p, 2p + 1) if `adjacent`; channels from 2 pairs

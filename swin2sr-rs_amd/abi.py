@@ -117,6 +117,8 @@ EXPORTS = {
     "s2s_rstb_device": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
     "s2s_attention_workspace": (C.c_int, [C.POINTER(Attention_), C.POINTER(C.c_uint64)]),
     "s2s_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "s2s_window_attention_workspace": (C.c_int, [C.POINTER(Attention_), C.c_int, C.c_int, C.POINTER(C.c_uint64)]),
+    "s2s_window_attention": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_uint64, C.c_void_p]),
     "s2s_rotary": (C.c_int, [C.c_void_p, C.c_void_p]),
     "s2s_norm_rotary": (C.c_int, [C.c_void_p, C.c_void_p]),
     "s2s_rms_norm": (C.c_int, [C.c_void_p, C.c_void_p]),

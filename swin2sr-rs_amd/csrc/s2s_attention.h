@@ -119,7 +119,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = kAttnLog2e;
 
-enum { CAP = 1, SLOPES = 2, ANY = 8, DOCS = 16, GENERAL = 32 };
+enum { CAP = 1, SLOPES = 2, ANY = 8, DOCS = 16, GENERAL = 32, WINDOW = 64 };
 
 template <typename T>
 struct Type;
@@ -345,7 +345,8 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 //  WK true (at most 16 columns): every wave has all columns and a quarter of each
 //  key tile (one block of 16 keys of 64); the four sums meet in LDS at the end.
 //  MODE: CAP and SLOPES are known (0 to 3), or asked for in every tile (ANY); documents
-//  (DOCS); or all of that and what AttnScore::general stands for (GENERAL). Paths that a
+//  (DOCS); or all of that and what AttnScore::general stands for (GENERAL); each with a
+//  sliding window or without (WINDOW). Paths that a
 //  kernel might take and does not cost it registers, spilled around its loop, and copies
 //  where they meet.
 // K and V tiles of TK keys are copied straight into LDS, two buffers each (three and four
@@ -354,7 +355,7 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 // (16, or 4 for rows of 4-byte multiples), or 0: through registers, by elements.
 template <typename T, int DP, int NB, bool WK, int ALIGN, int MODE>
 struct Kernel {
-    static constexpr bool GEN = MODE == GENERAL, DOC = GEN || (MODE & DOCS), KNOWN = MODE < ANY;
+    static constexpr bool WIN = MODE & WINDOW, GEN = (MODE & ~WINDOW) == GENERAL, DOC = GEN || (MODE & DOCS), KNOWN = (MODE & ~WINDOW) < ANY;
     typedef Type<T> Ty;
     typedef typename Ty::V Vec;
     static constexpr bool F32 = sizeof(T) == 4;
@@ -384,7 +385,7 @@ struct Kernel {
         const float *table;
         int half;  // the table's middle
         const lds_t *tab0;  // the group's rows, in LDS
-        int kl;
+        int kl, sinks;
         bool capped, slopes, general, table_lds;
         AttnScore sc;
     };
@@ -405,11 +406,16 @@ struct Kernel {
         const int c0 = ct * COLS;
         if (c0 >= ql * a.group) return;  // (the whole workgroup; ql * group <= 2^30)
         const int pre = a.prefix ? a.prefix[b] : 0;
-        auto limit = [&](int i) { return a.causal ? min(kl, max(max(kl - ql + i + 1, pre), 0)) : kl; };
+        auto limit = [&](int i) {
+            if (WIN && !a.causal) return min(kl, max(kl - ql + i + a.window, 0));
+            return a.causal ? min(kl, max(max(kl - ql + i + 1, pre), 0)) : kl;
+        };
+        // the first key of a query's window; before it lie only sinks that it reads
+        auto start = [&](int i) { return WIN ? max(kl - ql + i + 1 - a.window, 0) : 0; };
 
         // the columns of this lane
         const int wc0 = WK ? c0 : c0 + wave * 16 * NB;
-        int lim[NB], doc[NB], at[NB];
+        int lim[NB], low[NB], doc[NB], at[NB];
         int tab[NB];  // the head's row of the table
         float slope[NB];
         Vec qf[NB][KS];
@@ -418,6 +424,7 @@ struct Kernel {
             const int c = wc0 + nb * 16 + n16, i = L.by_group.of(c), h = kvh * a.group + (c - i * a.group);
             const bool ok = i < ql;
             lim[nb] = ok ? limit(i) : 0;
+            low[nb] = ok ? start(i) : 0;
             // (a column of no document computes what it may, and is zeroed at the end)
             doc[nb] = 0;
             if (DOC && a.q_docs && ok) doc[nb] = a.q_docs[b * a.q_docs_b + i];
@@ -443,6 +450,8 @@ struct Kernel {
         const bool w_any = wc0 < ql * a.group;
         const int w_max = w_any ? limit(w_last) : 0, w_min = limit(w_first);
         const int w_at = kl - ql + w_first;  // the first place among the wave's queries
+        // what all columns' windows hold begins here, and what any holds
+        const int wg_from = start(i_last), w_from = start(w_last), w_low = start(w_first);
         // documents of the workgroup's columns and of the wave's, where key tiles can be passed
         // over
         int q_lo = 0, q_hi = 0, w_lo = 0, w_hi = 0;
@@ -463,14 +472,20 @@ struct Kernel {
             w_hi = __builtin_amdgcn_readfirstlane(w_hi);
         }
         const int nt = q_hi < 0 ? 0 : (wg_max + TK - 1) / TK;
-        const int per = L.splits == 1 ? nt : (nt + L.splits - 1) / L.splits;
-        const int t_end = min(nt, (split + 1) * per);
+        // under a window the tiles between the sinks' and its first one are passed over
+        const int t_sinks = WIN ? min((a.sinks + TK - 1) / TK, nt) : 0;
+        const int t_win = WIN ? max(t_sinks, min(start(L.by_group.of(c0)) / TK, nt)) : 0;
+        const int live_tiles = nt - (t_win - t_sinks);
+        const int per = L.splits == 1 ? live_tiles : (live_tiles + L.splits - 1) / L.splits;
+        auto tile_of = [&](int n) { return WIN && n >= t_sinks ? n + (t_win - t_sinks) : n; };
+        const int t_end = min(nt, tile_of((split + 1) * per));
 
         // the next tile from t on that holds a key some column's document has, and
         // whether all its keys and the columns are of one document
         unsigned long long live = 0, whole = 0;
         int live_at = -64, t_lo = 0, t_hi = 0, t_all = 0;
         auto next = [&](int t) {
+            if (WIN && t >= t_sinks && t < t_win) t = t_win;
             if (!summary) return t;
             while (t < t_end) {
                 if (t >= live_at + 64) {
@@ -487,7 +502,12 @@ struct Kernel {
                     whole = __ballot(w);
                 }
                 const unsigned long long m = live >> (t - live_at);
-                if (m) return t + (int)__builtin_ctzll(m);
+                if (m) {
+                    t += (int)__builtin_ctzll(m);
+                    if (!WIN || t < t_sinks || t >= t_win) return t;
+                    t = t_win;
+                    continue;
+                }
                 t = live_at + 64;
             }
             return t_end;
@@ -583,6 +603,7 @@ struct Kernel {
         u.table = GEN ? a.table : nullptr;
         u.half = a.table_size >> 1;
         u.kl = kl;
+        u.sinks = WIN ? a.sinks : 0;
         u.capped = a.cap > 0.f;
         u.slopes = a.slopes != nullptr;
         u.general = GEN && L.score.general;
@@ -609,7 +630,7 @@ struct Kernel {
         // the first two tiles set out together; then the next one's buffer is free when the one
         // before has been computed
         constexpr int W = 2 * LOADS * SUB;  // copies per thread and tile
-        int t = next(split * per), buf = 0, docs = documents(t);
+        int t = next(tile_of(split * per)), buf = 0, docs = documents(t);
         kp += (long long)t * kstep, vp += (long long)t * vstep;
         if (t < t_end) stage(t, 0);
         int tn = t < t_end ? next(t + 1) : t_end, docs_n = documents(tn);
@@ -625,7 +646,8 @@ struct Kernel {
             if (!ahead && tn < t_end) stage(tn, buf ^ 1);
             ahead = false;
             const int at_buf = buf * 2 * (int)kTile;
-            if (!(t * TK + TK <= wg_min && (docs & ONE)) || (GEN && u.table)) {
+            const bool inside = !WIN || t * TK >= wg_from || t * TK + TK <= a.sinks;
+            if (!(t * TK + TK <= wg_min && (docs & ONE) && inside) || (GEN && u.table)) {
                 // a masked key's weight is zero, and zero times an infinity is none: with
                 // such values in the V of a tile that not every column reads whole, they are
                 // added by themselves to the columns that do read them, and taken out
@@ -635,16 +657,17 @@ struct Kernel {
                 if (lane == 0) flag[wave] = w;
                 lds_sync();
                 if (__builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3])) {
-                    wild_products(u, vd, t * TK + (WK ? 16 * wave : 0), lim, doc, at, tab, o);
+                    wild_products(u, vd, t * TK + (WK ? 16 * wave : 0), lim, low, doc, at, tab, o);
                     lds_sync();
                     remove_wild(vd);
                     lds_sync();
                 }
             }
             const int j0 = t * TK + (WK ? 16 * wave : 0);  // the wave's first key
-            if (j0 < w_max && (docs & MINE)) {
-                const bool full = j0 + 16 * KB <= w_min && (docs & SAME) && !(GEN && u.table);
-                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, j0 + 16 * KB <= w_at + 1, base + kIds + buf * 256 + (WK ? 64 * wave : 0), lim, doc, at, slope, tab, qf, o, m, l);
+            if (j0 < w_max && (docs & MINE) && (!WIN || j0 + 16 * KB > w_low || j0 < a.sinks)) {
+                const bool all = !WIN || j0 >= w_from || j0 + 16 * KB <= a.sinks;
+                const bool full = j0 + 16 * KB <= w_min && all && (docs & SAME) && !(GEN && u.table);
+                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, j0 + 16 * KB <= w_at + 1, base + kIds + buf * 256 + (WK ? 64 * wave : 0), lim, low, doc, at, slope, tab, qf, o, m, l);
             }
             t = tn, docs = docs_n;
             buf ^= 1;
@@ -751,7 +774,7 @@ struct Kernel {
 
     // The wave's keys of one tile: scores, softmax step, products with V.
     static __device__ __forceinline__ void tile(const Uniform &u, const lds_t *kl0, const lds_t *vl0, int j0,
-                                                bool full, bool behind, const lds_t *ids, const int *lim, const int *doc, const int *at, const float *slope, const int *tab,
+                                                bool full, bool behind, const lds_t *ids, const int *lim, const int *low, const int *doc, const int *at, const float *slope, const int *tab,
                                                 const Vec (*qf)[KS], f4v (*o)[NB], float *m,
                                                 typename std::conditional<F32, float, f4v>::type *l) {
         const int lane = threadIdx.x & 63, q = lane >> 4;
@@ -903,6 +926,14 @@ struct Kernel {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (16 * kb + i >= n) s[kb][nb][i] = -INFINITY;
+                if (WIN) {
+                    const int from = low[nb] - j0 - 4 * q, sinks = u.sinks - j0 - 4 * q;
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (16 * kb + i < from && 16 * kb + i >= sinks) s[kb][nb][i] = -INFINITY;
+                }
             }
             if (DOC && u.k_docs) {
 #pragma unroll
@@ -1023,7 +1054,7 @@ struct Kernel {
     }
 
     // The infinities and NaN of the tile's v, added to the columns that read their key.
-    static __device__ __forceinline__ void wild_products(const Uniform &u, const lds_t *vd, int j0, const int *lim,
+    static __device__ __forceinline__ void wild_products(const Uniform &u, const lds_t *vd, int j0, const int *lim, const int *low,
                                                          const int *doc, const int *at, const int *tab, f4v (*o)[NB]) {
         const int lane = threadIdx.x & 63, q = lane >> 4, wave = wave_of();
 #pragma unroll 1
@@ -1033,7 +1064,7 @@ struct Kernel {
             const int r = (WK ? 16 * wave : 0) + jr;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                bool ok = j < lim[nb] && (!DOC || !u.k_docs || (u.k_docs[j] == doc[nb] && doc[nb] >= 0));
+                bool ok = j < lim[nb] && (!WIN || j >= low[nb] || j < u.sinks) && (!DOC || !u.k_docs || (u.k_docs[j] == doc[nb] && doc[nb] >= 0));
                 if (GEN && ok && u.table) ok = entry(u, tab[nb], at[nb] - (u.k_pos ? u.k_pos[j] : j)) != -INFINITY;
                 if (!ok) continue;
 #pragma unroll
@@ -1186,29 +1217,17 @@ hipError_t launch(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
 }
 
 // Arrays that are not of 16-byte multiples and general biases take the kernels of 16
-// columns a wave.
-template <typename T, int DP, bool WK>
+// columns a wave. (W: WINDOW or 0)
+template <typename T, int DP, bool WK, int W>
 hipError_t launch_narrow(const AttnOpArgs &a, const AttnLaunch &L, int align, hipStream_t st) {
-    if (align == 0) return launch<T, DP, 1, WK, 0, GENERAL>(a, L, st);
-    if (align < 16) return launch<T, DP, 1, WK, 4, GENERAL>(a, L, st);
-    if (L.score.general) return launch<T, DP, 1, WK, 16, GENERAL>(a, L, st);
-    return a.k_docs ? launch<T, DP, 1, WK, 16, ANY | DOCS>(a, L, st) : launch<T, DP, 1, WK, 16, ANY>(a, L, st);
+    if (align == 0) return launch<T, DP, 1, WK, 0, GENERAL | W>(a, L, st);
+    if (align < 16) return launch<T, DP, 1, WK, 4, GENERAL | W>(a, L, st);
+    if (L.score.general) return launch<T, DP, 1, WK, 16, GENERAL | W>(a, L, st);
+    return a.k_docs ? launch<T, DP, 1, WK, 16, ANY | DOCS | W>(a, L, st) : launch<T, DP, 1, WK, 16, ANY | W>(a, L, st);
 }
 
 template <typename T, int DP>
-hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, int align, hipStream_t st) {
-    hipError_t e;
-    if (c.wk)
-        e = launch_narrow<T, DP, true>(a, L, align, st);
-    else if (c.nb == 1)
-        e = launch_narrow<T, DP, false>(a, L, align, st);
-    else if (a.k_docs)
-        e = launch<T, DP, 2, false, 16, ANY | DOCS>(a, L, st);
-    else if (a.cap > 0.f)
-        e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES>(a, L, st) : launch<T, DP, 2, false, 16, CAP>(a, L, st);
-    else
-        e = a.slopes ? launch<T, DP, 2, false, 16, SLOPES>(a, L, st) : launch<T, DP, 2, false, 16, 0>(a, L, st);
-    if (e != hipSuccess || L.splits == 1) return e;
+hipError_t join(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
     const long long rows = (long long)a.batch * a.hk * L.cols;  // (few: the keys were split to fill the chip)
     // few ranges of many columns: 8 causal bf16 heads of 128 over 512, 1024 and 2048 tokens 15, 26
     // and 40 us against 21, 39 and 62 by a workgroup per column; 512 columns of 4 ranges (16 steps over
@@ -1219,13 +1238,29 @@ hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, 
     return enqueue(k_attn_join<T, DP>, dim3((unsigned)rows), dim3(256), 0, st, a, L);
 }
 
-template <typename T>
+template <typename T, int DP, int W>
+hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, int align, hipStream_t st) {
+    hipError_t e;
+    if (c.wk)
+        e = launch_narrow<T, DP, true, W>(a, L, align, st);
+    else if (c.nb == 1)
+        e = launch_narrow<T, DP, false, W>(a, L, align, st);
+    else if (a.k_docs)
+        e = launch<T, DP, 2, false, 16, ANY | DOCS | W>(a, L, st);
+    else if (a.cap > 0.f)
+        e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES | W>(a, L, st) : launch<T, DP, 2, false, 16, CAP | W>(a, L, st);
+    else
+        e = a.slopes ? launch<T, DP, 2, false, 16, SLOPES | W>(a, L, st) : launch<T, DP, 2, false, 16, W>(a, L, st);
+    return e != hipSuccess || L.splits == 1 ? e : join<T, DP>(a, L, st);
+}
+
+template <typename T, int W>
 hipError_t launch_type(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, int align, hipStream_t st) {
     switch (c.dp) {
-        case 32: return launch_width<T, 32>(a, L, c, align, st);
-        case 64: return launch_width<T, 64>(a, L, c, align, st);
-        case 96: return launch_width<T, 96>(a, L, c, align, st);
-        default: return launch_width<T, 128>(a, L, c, align, st);
+        case 32: return launch_width<T, 32, W>(a, L, c, align, st);
+        case 64: return launch_width<T, 64, W>(a, L, c, align, st);
+        case 96: return launch_width<T, 96, W>(a, L, c, align, st);
+        default: return launch_width<T, 128, W>(a, L, c, align, st);
     }
 }
 
@@ -1234,3 +1269,6 @@ hipError_t launch_type(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, i
 hipError_t launch_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
 hipError_t launch_attention_f16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
 hipError_t launch_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_window_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_window_attention_f16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_window_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);

@@ -31,7 +31,11 @@ attn::Cut cut_of(int dtype, const AttnOpArgs &a, bool narrow) {
     c.tk = dtype == 0 && !c.wk && c.dp > 64 ? 32 : 64;
     const int per = c.wk ? 16 : 64 * c.nb;
     c.tiles = (int)((cols + per - 1) / per);
-    const long long blocks = std::max(1LL, pairs * c.tiles), nt = ((long long)a.nk + c.tk - 1) / c.tk;
+    const long long blocks = std::max(1LL, pairs * c.tiles);
+    long long nt = ((long long)a.nk + c.tk - 1) / c.tk;
+    // of a window the tiles that a column tile's queries and the sinks lie in
+    if (a.window)
+        nt = std::min(nt, ((long long)(a.causal ? 1 : 2) * a.window + per / a.group + c.tk) / c.tk + 1 + ((long long)a.sinks + c.tk - 1) / c.tk);
     const long long ranges = c.wk && nt > 4 ? std::max({nt / 4, std::min(nt / 2, 32LL), std::min(nt, 16LL)}) : nt / 4;
     c.splits = (int)std::max(1LL, std::min({2LL * cus / blocks, ranges, 256LL}));
     return c;
@@ -285,6 +289,11 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
         }
         if (e != hipSuccess) return e;
     }
+    if (a.window) switch (dtype) {
+            case 0: return launch_window_attention_f32(a, L, c, align, st);
+            case 1: return launch_window_attention_f16(a, L, c, align, st);
+            case 2: return launch_window_attention_bf16(a, L, c, align, st);
+        }
     switch (dtype) {
         case 0: return launch_attention_f32(a, L, c, align, st);
         case 1: return launch_attention_f16(a, L, c, align, st);

@@ -2,5 +2,5 @@
 #include "s2s_attention.h"
 
 hipError_t launch_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st) {
-    return attn::launch_type<float>(a, L, c, align, st);
+    return attn::launch_type<float, 0>(a, L, c, align, st);
 }

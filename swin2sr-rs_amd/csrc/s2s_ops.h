@@ -27,6 +27,7 @@ struct AttnOpArgs {
     long long q_pos_b, k_pos_b;
     const float *slopes, *table;
     int table_size;
+    int window, sinks;  // window 0: none
 };
 
 struct RotaryArgs {

@@ -128,8 +128,16 @@ int attention_sizes(const char *op, const s2s_attention_args *a) {
     return 0;
 }
 
-AttnOpArgs attention_args(const s2s_attention_args *a) {
+int window_sizes(const char *op, const s2s_attention_args *a, int window, int sinks) {
+    if (window < 1 || window > (1 << 30)) return refuse("%s: a window of %d keys is not in 1 to 2^30", op, window);
+    if (sinks < 0 || sinks > (1 << 30)) return refuse("%s: %d sinks are not in 0 to 2^30", op, sinks);
+    return 0;
+}
+
+AttnOpArgs attention_args(const s2s_attention_args *a, int window = 0, int sinks = 0) {
     AttnOpArgs k{};
+    k.window = window;
+    k.sinks = sinks;
     k.batch = a->batch;
     k.nq = a->q_tokens;
     k.nk = a->k_tokens;
@@ -165,6 +173,76 @@ AttnOpArgs attention_args(const s2s_attention_args *a) {
     k.table = a->table;
     k.table_size = a->table_size;
     return k;
+}
+
+// A call whose sizes have been checked; window 0: none.
+int attention_call(const char *op, const s2s_attention_args *a, int window, int sinks, void *workspace, uint64_t workspace_bytes,
+                   void *stream) {
+    if (!std::isfinite(a->scale)) return refuse("%s: the scale is not finite", op);
+    if (!(a->cap >= 0.f) || !std::isfinite(a->cap)) return refuse("%s: the cap is negative or not finite", op);
+    if (a->cap > 0.f && a->cap < 1e-6f) return refuse("%s: a cap below 1e-6", op);
+    // (their products with log2(e), and the quotient of the two, are finite)
+    if (std::fabs(a->scale) > 1e30f) return refuse("%s: the scale is past 10^30", op);
+    if (a->cap > 1e30f) return refuse("%s: the cap is past 10^30", op);
+    if (a->prefix && !a->causal) return refuse("%s: a prefix without the causal mask", op);
+    // (an array of no elements may have no address, or one that is nobody's)
+    const bool keys = a->k_tokens > 0, some = keys && a->batch > 0 && a->q_tokens > 0;
+    if (some && !a->q_docs != !a->k_docs) return refuse("%s: documents of queries and keys come together", op);
+    if (some && !a->q_pos != !a->k_pos) return refuse("%s: positions of queries and keys come together", op);
+    if (a->q_pos && !a->slopes && !a->table) return refuse("%s: positions without slopes or table", op);
+    if (a->table && (a->table_size < 1 || a->table_size % 2 == 0 || a->table_size > (1 << 24)))
+        return refuse("%s: a table of %d entries: an odd number up to 2^24 is wanted", op, a->table_size);
+    if (a->table && (long long)a->q_heads * a->table_size > (1 << 30)) return refuse("%s: a table over 2^30 entries", op);
+    if (a->q_docs_batch < 0 || a->k_docs_batch < 0 || a->q_pos_batch < 0 || a->k_pos_batch < 0 ||
+        a->q_docs_batch > kMaxStride || a->k_docs_batch > kMaxStride || a->q_pos_batch > kMaxStride ||
+        a->k_pos_batch > kMaxStride)
+        return refuse("%s: a negative or impossible batch stride", op);
+    // (a wave per key tile, of 32 keys at least, makes the documents' summary, four a workgroup, of which
+    // a launch holds less than 2^24)
+    if (a->k_docs && ((long long)a->batch * ((a->k_tokens + 31LL) / 32) + 3) / 4 >= (1 << 24))
+        return refuse("%s: documents of over 2^31 keys of the batch", op);
+    if (a->batch == 0 || a->q_tokens == 0) return 0;
+    OnDevice on;
+    const hipStream_t st = (hipStream_t)stream;
+    hipError_t e = on.enter(st);
+    if (e != hipSuccess) return refuse_hip(op, "the stream's device", e);
+    if (int rc = check_tokens(op, "q", a->q, a->dtype, on.dev)) return rc;
+    if (int rc = check_tokens(op, "out", a->out, a->dtype, on.dev)) return rc;
+    if (int rc = check_written(op, "out", a->out, a->batch, a->q_tokens, a->q_heads, a->width)) return rc;
+    if (keys) {
+        if (int rc = check_tokens(op, "k", a->k, a->dtype, on.dev)) return rc;
+        if (int rc = check_tokens(op, "v", a->v, a->dtype, on.dev)) return rc;
+        // 64 tokens of a tile are reached by 32-bit byte offsets from its first
+        if (a->k_tokens > 1 && (a->k.token > (1 << 22) || a->v.token > (1 << 22)))
+            return refuse("%s: a token stride of k or v over 2^22 elements", op);
+    }
+    if (a->out.data == a->q.data || (keys && (a->out.data == a->k.data || a->out.data == a->v.data)))
+        return refuse("%s: out is an input", op);
+    const struct {
+        const char *name;
+        const void *p;
+    } arrays[] = {{"q_lens", a->q_lens},
+                  {"k_lens", a->k_lens},
+                  {"prefix", a->prefix},
+                  {"q_docs", a->q_docs},
+                  {"k_docs", keys ? a->k_docs : nullptr},
+                  {"q_pos", a->q_pos},
+                  {"k_pos", keys ? a->k_pos : nullptr},
+                  {"slopes", a->slopes},
+                  {"table", a->table}};
+    for (const auto &x : arrays)
+        if (x.p)
+            if (int rc = check_array(op, x.name, x.p, 4, on.dev)) return rc;
+    const AttnOpArgs k = attention_args(a, window, sinks);
+    const size_t need = attn_op_workspace(a->dtype, k);
+    if (need) {
+        if (!workspace || workspace_bytes < need)
+            return refuse("%s: a workspace of %zu bytes is needed, %llu are given", op, need,
+                          workspace ? (unsigned long long)workspace_bytes : 0ULL);
+        if (int rc = check_array(op, "workspace", workspace, 16, on.dev)) return rc;
+    }
+    e = launch_attention_op(a->dtype, k, workspace, st);
+    return e == hipSuccess ? 0 : refuse_hip(op, "the launch", e);
 }
 
 // Rotary positions, behind a norm of the heads if `n` is not null (`a` is its part then).
@@ -285,71 +363,27 @@ int s2s_attention(const s2s_attention_args *a, void *workspace, uint64_t workspa
     const char *op = "s2s_attention";
     if (!a) return refuse("%s: null argument", op);
     if (int rc = attention_sizes(op, a)) return rc;
-    if (!std::isfinite(a->scale)) return refuse("%s: the scale is not finite", op);
-    if (!(a->cap >= 0.f) || !std::isfinite(a->cap)) return refuse("%s: the cap is negative or not finite", op);
-    if (a->cap > 0.f && a->cap < 1e-6f) return refuse("%s: a cap below 1e-6", op);
-    // (their products with log2(e), and the quotient of the two, are finite)
-    if (std::fabs(a->scale) > 1e30f) return refuse("%s: the scale is past 10^30", op);
-    if (a->cap > 1e30f) return refuse("%s: the cap is past 10^30", op);
-    if (a->prefix && !a->causal) return refuse("%s: a prefix without the causal mask", op);
-    // (an array of no elements may have no address, or one that is nobody's)
-    const bool keys = a->k_tokens > 0, some = keys && a->batch > 0 && a->q_tokens > 0;
-    if (some && !a->q_docs != !a->k_docs) return refuse("%s: documents of queries and keys come together", op);
-    if (some && !a->q_pos != !a->k_pos) return refuse("%s: positions of queries and keys come together", op);
-    if (a->q_pos && !a->slopes && !a->table) return refuse("%s: positions without slopes or table", op);
-    if (a->table && (a->table_size < 1 || a->table_size % 2 == 0 || a->table_size > (1 << 24)))
-        return refuse("%s: a table of %d entries: an odd number up to 2^24 is wanted", op, a->table_size);
-    if (a->table && (long long)a->q_heads * a->table_size > (1 << 30)) return refuse("%s: a table over 2^30 entries", op);
-    if (a->q_docs_batch < 0 || a->k_docs_batch < 0 || a->q_pos_batch < 0 || a->k_pos_batch < 0 ||
-        a->q_docs_batch > kMaxStride || a->k_docs_batch > kMaxStride || a->q_pos_batch > kMaxStride ||
-        a->k_pos_batch > kMaxStride)
-        return refuse("%s: a negative or impossible batch stride", op);
-    // (a wave per key tile, of 32 keys at least, makes the documents' summary, four a workgroup, of which
-    // a launch holds less than 2^24)
-    if (a->k_docs && ((long long)a->batch * ((a->k_tokens + 31LL) / 32) + 3) / 4 >= (1 << 24))
-        return refuse("%s: documents of over 2^31 keys of the batch", op);
-    if (a->batch == 0 || a->q_tokens == 0) return 0;
-    OnDevice on;
-    const hipStream_t st = (hipStream_t)stream;
-    hipError_t e = on.enter(st);
-    if (e != hipSuccess) return refuse_hip(op, "the stream's device", e);
-    if (int rc = check_tokens(op, "q", a->q, a->dtype, on.dev)) return rc;
-    if (int rc = check_tokens(op, "out", a->out, a->dtype, on.dev)) return rc;
-    if (int rc = check_written(op, "out", a->out, a->batch, a->q_tokens, a->q_heads, a->width)) return rc;
-    if (keys) {
-        if (int rc = check_tokens(op, "k", a->k, a->dtype, on.dev)) return rc;
-        if (int rc = check_tokens(op, "v", a->v, a->dtype, on.dev)) return rc;
-        // 64 tokens of a tile are reached by 32-bit byte offsets from its first
-        if (a->k_tokens > 1 && (a->k.token > (1 << 22) || a->v.token > (1 << 22)))
-            return refuse("%s: a token stride of k or v over 2^22 elements", op);
-    }
-    if (a->out.data == a->q.data || (keys && (a->out.data == a->k.data || a->out.data == a->v.data)))
-        return refuse("%s: out is an input", op);
-    const struct {
-        const char *name;
-        const void *p;
-    } arrays[] = {{"q_lens", a->q_lens},
-                  {"k_lens", a->k_lens},
-                  {"prefix", a->prefix},
-                  {"q_docs", a->q_docs},
-                  {"k_docs", keys ? a->k_docs : nullptr},
-                  {"q_pos", a->q_pos},
-                  {"k_pos", keys ? a->k_pos : nullptr},
-                  {"slopes", a->slopes},
-                  {"table", a->table}};
-    for (const auto &x : arrays)
-        if (x.p)
-            if (int rc = check_array(op, x.name, x.p, 4, on.dev)) return rc;
-    const AttnOpArgs k = attention_args(a);
-    const size_t need = attn_op_workspace(a->dtype, k);
-    if (need) {
-        if (!workspace || workspace_bytes < need)
-            return refuse("%s: a workspace of %zu bytes is needed, %llu are given", op, need,
-                          workspace ? (unsigned long long)workspace_bytes : 0ULL);
-        if (int rc = check_array(op, "workspace", workspace, 16, on.dev)) return rc;
-    }
-    e = launch_attention_op(a->dtype, k, workspace, st);
-    return e == hipSuccess ? 0 : refuse_hip(op, "the launch", e);
+    return attention_call(op, a, 0, 0, workspace, workspace_bytes, stream);
+}
+
+int s2s_window_attention_workspace(const s2s_attention_args *a, int window, int sinks, uint64_t *bytes) {
+    const char *op = "s2s_window_attention_workspace";
+    if (!a || !bytes) return refuse("%s: null argument", op);
+    if (int rc = attention_sizes(op, a)) return rc;
+    if (int rc = window_sizes(op, a, window, sinks)) return rc;
+    *bytes = attn_op_workspace(a->dtype, attention_args(a, window, sinks));
+    return 0;
+}
+
+int s2s_window_attention(const s2s_attention_args *a, int window, int sinks, void *workspace, uint64_t workspace_bytes,
+                         void *stream) {
+    const char *op = "s2s_window_attention";
+    if (!a) return refuse("%s: null argument", op);
+    if (int rc = attention_sizes(op, a)) return rc;
+    if (int rc = window_sizes(op, a, window, sinks)) return rc;
+    // (a document's own first keys are not known)
+    if (sinks > 0 && (a->q_docs || a->k_docs)) return refuse("%s: sinks with documents", op);
+    return attention_call(op, a, window, sinks, workspace, workspace_bytes, stream);
 }
 
 int s2s_rotary(const s2s_rotary_args *a, void *stream) {

@@ -130,7 +130,9 @@ class Attention:
     """A plan of `s2s_attention` for one set of sizes.
 
     `dtype` ("f32", "f16", "bf16") is the type of q, k, v and out; `scale` is
-    1 / sqrt(width) by default, `cap` 0 for none. `workspace_bytes` of device
+    1 / sqrt(width) by default, `cap` 0 for none, `window` 0 for none: with one, a
+    query sees the `window` last keys up to its own place (not `causal`: those less than
+    `window` away either way) and the first `sinks` ones. `workspace_bytes` of device
     memory go with every call: one buffer serves all calls of a stream, calls
     that may overlap on the device (other streams, replays of captured graphs)
     need one each.
@@ -141,8 +143,8 @@ class Attention:
     """
 
     def __init__(self, dtype, batch: int, q_tokens: int, k_tokens: int, q_heads: int, k_heads: int, width: int,
-                 scale: Optional[float] = None, cap: float = 0.0, causal: bool = False):
-        sizes = (batch, q_tokens, k_tokens, q_heads, k_heads, width)
+                 scale: Optional[float] = None, cap: float = 0.0, causal: bool = False, window: int = 0, sinks: int = 0):
+        sizes = (batch, q_tokens, k_tokens, q_heads, k_heads, width, window, sinks)
         _need(all(-2 ** 31 <= n < 2 ** 31 for n in sizes), "attention: a size that is no 32-bit int")
         self.lib = load_library()
         self.dtype = _type(dtype)
@@ -152,7 +154,12 @@ class Attention:
         self.q_shape, self.k_shape = (batch, q_tokens, q_heads, width), (batch, k_tokens, k_heads, width)
         a = Attention_(*self.head)
         n = C.c_uint64()
-        check(self.lib.s2s_attention_workspace(C.byref(a), C.byref(n)), "attention")
+        self.window = (window, sinks)
+        if window:
+            check(self.lib.s2s_window_attention_workspace(C.byref(a), window, sinks, C.byref(n)), "attention")
+        else:
+            _need(sinks == 0, "attention: sinks without a window")
+            check(self.lib.s2s_attention_workspace(C.byref(a), C.byref(n)), "attention")
         self.workspace_bytes = n.value
 
     def __call__(self, q, k, v, out, workspace=None, stream: int = 0, q_lens=None, k_lens=None, prefix=None,
@@ -184,7 +191,7 @@ class Attention:
             _need(entries < 2 ** 31, f"{op}: a table of {entries} entries")
         args = _ATTENTION.pack(*self.head, *arrays, *lens, *docs, *pos, slope_ptr, table_ptr, entries)
         ws, n = (None, 0) if workspace is None else (workspace.data_ptr(), _bytes(workspace))
-        if self.lib.s2s_attention(args, ws, n, stream):
+        if self.lib.s2s_window_attention(args, *self.window, ws, n, stream) if self.window[0] else self.lib.s2s_attention(args, ws, n, stream):
             raise S2SError(f"{op}: {last_error()}")
         return out
 

@@ -174,6 +174,15 @@ extern "C" {
     pub fn s2s_profile_report(ctx: *mut S2sCtx, wall_ms: f32) -> c_int;
     pub fn s2s_attention_workspace(args: *const S2sAttentionArgs, bytes: *mut u64) -> c_int;
     pub fn s2s_attention(args: *const S2sAttentionArgs, workspace: *mut c_void, bytes: u64, stream: *mut c_void) -> c_int;
+    pub fn s2s_window_attention_workspace(args: *const S2sAttentionArgs, window: c_int, sinks: c_int, bytes: *mut u64) -> c_int;
+    pub fn s2s_window_attention(
+        args: *const S2sAttentionArgs,
+        window: c_int,
+        sinks: c_int,
+        workspace: *mut c_void,
+        bytes: u64,
+        stream: *mut c_void,
+    ) -> c_int;
     pub fn s2s_rotary(args: *const S2sRotaryArgs, stream: *mut c_void) -> c_int;
     pub fn s2s_norm_rotary(args: *const S2sNormRotaryArgs, stream: *mut c_void) -> c_int;
     pub fn s2s_rms_norm(args: *const S2sRmsNormArgs, stream: *mut c_void) -> c_int;

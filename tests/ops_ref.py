@@ -104,7 +104,7 @@ class Dev:
 
 
 def attention(dtype, q, k, v, scale, cap=0.0, causal=False, q_lens=None, k_lens=None, prefix=None, q_docs=None,
-              k_docs=None, q_pos=None, k_pos=None, slopes=None, table=None):
+              k_docs=None, q_pos=None, k_pos=None, slopes=None, table=None, window=0, sinks=0):
     """(out, bound, written): the result in 64 bits for inputs that are values of
     `dtype`, the error a 32-bit evaluation may have, and which rows are written.
 
@@ -134,6 +134,11 @@ def attention(dtype, q, k, v, scale, cap=0.0, causal=False, q_lens=None, k_lens=
             ok = j <= n - m + i
             if prefix is not None:
                 ok |= j < int(prefix[b])
+        if window:
+            place = n - m + i
+            ok = ok & ((j > place - window) | (j < sinks))
+            if not causal:
+                ok = ok & (j < place + window)
         if q_docs is not None:
             dq, dk = at2(q_docs, b)[:m, None], at2(k_docs, b)[None, :n]
             ok = ok & (dq == dk) & (dq >= 0)

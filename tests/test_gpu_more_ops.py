@@ -138,3 +138,159 @@ def test_norm_rotary_refuses(pkg):
     T.refused(pkg, "k_weight is not aligned", lambda: rot(x.array, pos.array, w.array, out.array, k=k.array, k_weight=A(w.array.ptr + 2, (16,), "f32")))
     T.refused(pkg, "stride", lambda: rot(x.array, pos.array, A(w.array.ptr, (3, 16), "f32", (-16, 1))))
     assert (x.get() == 1).all()
+
+
+# ---- attention with a sliding window ------------------------------------------------------
+
+
+def wcase(dtype="bf16", window=16, sinks=0, **more):
+    return dict(T.case(dtype, **more), window=window, sinks=sinks)
+
+
+def window_plan(pkg, c):
+    scale = c["D"] ** -0.5 if c["scale"] is None else c["scale"]
+    p = pkg.ops.Attention(c["dtype"], c["B"], c["Lq"], c["Lk"], c["H"], c["KV"], c["D"], scale=scale, cap=c["cap"],
+                          causal=c["causal"], window=c["window"], sinks=c["sinks"])
+    ws = R.Dev(pkg, np.full(max(p.workspace_bytes // 4, 1), np.nan), "f32")
+    return p, ws, np.float64(np.float32(scale))
+
+
+def check_window(pkg, c, change=None):
+    q, k, v, more = T.inputs(c)
+    if change:
+        change(q, k, v, more)
+    p, ws, scale = window_plan(pkg, c)
+    want, bound, written = R.attention(c["dtype"], q, k, v, scale, np.float64(np.float32(c["cap"])), c["causal"], window=c["window"],
+                                       sinks=c["sinks"], **{n: x.astype(np.float64) if x.dtype == np.float32 else x for n, x in more.items()})
+    d, m = T.upload(pkg, c, q, k, v, more)
+    T.call(p, ws, d, m)
+    pkg.hip.synchronize()
+    got = d["out"].get()
+    assert d["out"].gaps_kept()
+    w = written[:, :, None, None] & np.ones(got.shape, bool)
+    assert np.all(got[~w] == 7.5), "rows past the sequence were written"
+    got, want, bound = got[w], want[w], bound[w]
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    fine = np.isfinite(want)
+    worst = (np.abs(got[fine] - want[fine]) / np.maximum(bound[fine], 1e-300)).max(initial=0.0)
+    assert worst <= 1.0, worst
+    # (infinities of the same sign too)
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+
+
+WINDOWS = {
+    "one": wcase(Lq=1, Lk=1, H=1, window=1),
+    "one_key": wcase("f32", Lq=9, Lk=200, H=2, causal=True, window=1),
+    "one_key_both_ways": wcase("f16", Lq=90, Lk=200, H=2, window=1),
+    "sinks_alone": wcase("f32", Lq=9, Lk=200, H=2, causal=True, window=1, sinks=1),
+    "step": wcase("bf16", B=4, Lq=1, Lk=3000, H=8, KV=2, D=128, order="cache", causal=True, window=500, sinks=4, k_lens=[3000, 1, 333, 0]),
+    "step_f16_slopes": wcase("f16", Lq=1, Lk=5003, H=16, KV=2, order="cache", causal=True, slopes=True, window=1000, sinks=130),
+    "step_f32": wcase("f32", B=2, Lq=1, Lk=1500, H=4, KV=4, D=64, order="cache", causal=True, table=63, window=300, sinks=3),
+    "step_f32_128": wcase("f32", B=2, Lq=1, Lk=1700, H=4, KV=2, D=128, order="cache", causal=True, window=900),
+    "step_4": wcase("bf16", B=2, Lq=4, Lk=2100, H=8, KV=2, D=128, order="cache", causal=True, window=777, sinks=1, cap=30.0),
+    "step_short": wcase("f16", B=2, Lq=1, Lk=900, H=4, KV=1, order="cache", causal=True, window=5, sinks=2),
+    "step_window_past_all": wcase("f16", B=2, Lq=1, Lk=900, H=4, KV=1, order="cache", causal=True, window=2 ** 30, sinks=2 ** 30),
+    "sinks_past_all": wcase("bf16", Lq=100, Lk=300, H=2, causal=True, window=7, sinks=1000),
+    "sinks_meet_window": wcase("bf16", Lq=300, Lk=300, H=2, causal=True, window=64, sinks=65),
+    "prompt": wcase("bf16", Lq=700, Lk=700, H=4, KV=2, D=128, causal=True, window=100, sinks=4),
+    "prompt_f16": wcase("f16", Lq=513, Lk=513, H=4, KV=1, D=64, causal=True, window=64, sinks=64),
+    "prompt_f32": wcase("f32", Lq=400, Lk=400, H=2, KV=2, D=128, causal=True, window=33, sinks=1, slopes=True),
+    "both_ways": wcase("f32", Lq=500, Lk=500, H=6, KV=6, D=30, window=50),
+    "both_ways_sinks": wcase("bf16", Lq=500, Lk=500, H=2, KV=1, D=96, window=70, sinks=9, cap=20.0),
+    "table": wcase("f32", B=2, Lq=256, Lk=256, H=6, KV=6, D=30, table=225, pos=T.grid, window=40),
+    "documents": wcase("bf16", Lq=1200, Lk=1200, H=4, KV=2, docs=T.segments(130, 1, 64, 700, 200), causal=True, window=90),
+    "documents_both_ways": wcase("f16", Lq=1200, Lk=1200, H=2, KV=2, docs=T.segments(130, 1, 64, 700, 200), window=90),
+    "documents_scattered": wcase("f32", B=2, Lq=65, Lk=790, H=2, docs=T.scattered, window=30),
+    "documents_blocks": wcase("f32", B=3, Lq=700, Lk=700, H=2, KV=2, D=32, docs=T.scattered_blocks, window=200, causal=True, q_lens=[700, 1, 333], k_lens=[650, 700, 333]),
+    "documents_step": wcase("f16", B=2, Lq=2, Lk=9100, H=4, KV=2, D=96, order="cache", docs=T.scattered_blocks, window=3000, causal=True),
+    "prefix": wcase("bf16", B=3, Lq=150, Lk=150, H=4, KV=2, causal=True, prefix=[0, 37, 1000], window=20, sinks=2),
+    "lengths": wcase("f16", B=5, Lq=33, Lk=70, H=2, q_lens=[0, 1, 33, 5, 40], k_lens=[70, 0, 1, -3, 64], causal=True, window=3, sinks=1),
+    "lengths_both_ways": wcase("f16", B=5, Lq=33, Lk=170, H=2, q_lens=[0, 1, 33, 5, 40], k_lens=[170, 0, 1, -3, 64], window=3),
+    "more_queries_than_keys": wcase("bf16", Lq=190, Lk=30, H=2, causal=True, window=10, sinks=2),
+    "more_queries_than_keys_both_ways": wcase("bf16", Lq=190, Lk=30, H=2, window=10, sinks=2),
+    "odd_address": wcase("f16", B=2, Lq=40, Lk=277, H=4, KV=2, D=64, gap=3, lead=1, causal=True, window=50, sinks=5),
+    "rows_of_4_bytes": wcase("f16", B=2, Lq=40, Lk=350, H=2, KV=2, D=62, causal=True, window=50, sinks=5),
+    "odd_step": wcase("bf16", B=2, Lq=1, Lk=2277, H=4, KV=2, D=63, gap=3, lead=1, causal=True, window=1050, sinks=5),
+    "group_33": wcase("f16", Lq=2, Lk=700, H=33, KV=1, D=32, causal=True, window=80, sinks=3),
+    "ranges": wcase("bf16", Lq=140, Lk=3500, H=8, KV=8, D=128, causal=True, window=1500, sinks=4),
+    "ranges_f32": wcase("f32", Lq=260, Lk=1800, H=6, KV=6, D=30, order="cache", gap=2, window=700, sinks=70),
+    "negative_scale": wcase("f32", Lq=20, Lk=100, H=2, D=32, scale=-0.3, window=20, causal=True),
+    "large_scores": wcase("bf16", Lq=64, Lk=300, H=2, D=64, spread=30.0, window=100, sinks=3, causal=True),
+}
+WIDE = dict(B=23, H=12, KV=12, Lq=170, Lk=190)
+WINDOWS.update({
+    "wide_bf16": wcase("bf16", D=128, window=30, sinks=3, causal=True, **WIDE),
+    "wide_f16": wcase("f16", D=64, window=70, **WIDE),
+    "wide_f32": wcase("f32", D=64, window=33, sinks=1, causal=True, **WIDE),
+    "wide_f32_128": wcase("f32", D=128, window=65, sinks=1, causal=True, **WIDE),
+    "wide_cap_bf16": wcase("bf16", D=96, window=64, sinks=64, cap=50.0, spread=4.0, causal=True, **WIDE),
+    "wide_slopes_bf16": wcase("bf16", D=64, window=100, slopes=True, **WIDE),
+    "wide_cap_slopes_f16": wcase("f16", D=32, window=100, slopes=True, cap=30.0, causal=True, **WIDE),
+    "wide_docs_bf16": wcase("bf16", D=128, window=20, docs=T.scattered, causal=True, cap=50.0, slopes=True, **WIDE),
+    "wide_lengths_bf16": wcase("bf16", D=128, window=20, sinks=2, causal=True, k_lens=[(17 * i) % 191 for i in range(23)],
+                               q_lens=[(13 * i) % 171 for i in range(23)], **WIDE),
+})
+
+
+@pytest.mark.parametrize("name", WINDOWS)
+def test_window(pkg, name):
+    check_window(pkg, WINDOWS[name])
+
+
+HIDDEN = {
+    "step": wcase("bf16", Lq=1, Lk=900, H=4, KV=2, D=128, causal=True, window=300, sinks=4),
+    "steps_f32": wcase("f32", Lq=3, Lk=900, H=4, KV=2, causal=True, window=300, sinks=4),
+    "prompt_f16": wcase("f16", Lq=300, Lk=900, H=4, KV=2, causal=True, window=300, sinks=4),
+    "prompt_f32": wcase("f32", Lq=300, Lk=900, H=2, D=100, causal=True, window=300, sinks=4),
+    "table": wcase("bf16", Lq=300, Lk=900, H=4, KV=2, causal=True, window=300, sinks=4, table=63),
+    "wide": wcase("bf16", causal=True, window=20, sinks=4, **WIDE),
+    "wide_f32": wcase("f32", causal=True, window=20, sinks=4, D=96, **WIDE),
+}
+
+
+@pytest.mark.parametrize("name", HIDDEN)
+def test_window_hides_what_keys_hold(pkg, name):
+    """NaN and infinities in keys that have left some or all of the windows: as if they were not there for the queries
+    that do not see them, and there for those that do; the same in a sink."""
+    c = HIDDEN[name]
+    first = c["Lk"] - c["Lq"] - c["window"] + 1  # the first key of the first query's window
+
+    def gone(q, k, v, more):
+        k[:, 4:max(first, 4)], v[:, 4:max(first, 4)] = np.nan, np.inf
+        if c["Lq"] > 20:
+            v[:, first + 5 if first > 0 else 7, 0, 3] = np.inf  # seen by the first few queries
+            k[:, first + 9 if first > 0 else 9, -1, 2] = np.nan
+    check_window(pkg, c, gone)
+
+    def sink(q, k, v, more):
+        v[:, 2, 0, 3] = -np.inf
+        v[:, 3, -1, 1] = np.nan
+    check_window(pkg, c, sink)
+
+
+def test_window_past_all_is_no_window(pkg):
+    """A window of all keys gives the attention without one."""
+    for c in (wcase("bf16", Lq=300, Lk=300, H=4, KV=2, D=128, causal=True, window=300),
+              wcase("f32", Lq=1, Lk=1300, H=4, KV=2, causal=True, window=1300), wcase("f16", **dict(WIDE, B=30), D=64, window=2 ** 30)):
+        q, k, v, more = T.inputs(c)
+        d, m = T.upload(pkg, c, q, k, v, more)
+        p, ws, scale = window_plan(pkg, c)
+        T.call(p, ws, d, m)
+        got = d["out"].get()
+        p, ws, scale = T.make_plan(pkg, c)
+        T.call(p, ws, d, m)
+        want, bound, _ = R.attention(c["dtype"], q, k, v, scale, causal=c["causal"])
+        assert (np.abs(got - d["out"].get()) <= 2 * bound).all()
+
+
+def test_window_refuses(pkg):
+    c = wcase("bf16", Lq=1, Lk=9000, H=8, KV=2, causal=True, window=5000, sinks=4)
+    q, k, v, more = T.inputs(c)
+    p, ws, _ = window_plan(pkg, c)
+    d, m = T.upload(pkg, c, q, k, v, more)
+    a = {n: x.array for n, x in d.items()}
+    assert p.workspace_bytes > 0
+    T.refused(pkg, "workspace", lambda: p(**a))
+    T.refused(pkg, "workspace", lambda: p(**a, workspace=pkg.ops.Array(ws.buf.ptr, (p.workspace_bytes - 1,), "u8")))
+    T.refused(pkg, "out is an input", lambda: p(**{**a, "out": a["q"]}, workspace=ws.array))
+    assert np.all(d["out"].get() == 7.5)

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import ops_ref as R
-from test_ops import arr
+from test_ops import arr, plan, tensors
 
 # ---- heads' norms with the rotation ------------------------------------------------
 
@@ -60,6 +60,42 @@ def test_norm_rotary_across_refused(pkg):
         pkg.ops.NormRotary.of((16, 16))(q, arr(pkg, (1, 4, 2), "i32"), w, q_out=k, k=k, k_weight=w, k_out=o)
 
 
+# ---- attention with a sliding window ---------------------------------------------------
+
+
+@pytest.mark.parametrize("more,word", [
+    (dict(window=-1), "a window of -1"), (dict(window=2 ** 30 + 1), "window"), (dict(window=8, sinks=-1), "sinks"),
+    (dict(window=8, sinks=2 ** 30 + 1), "sinks"), (dict(sinks=4), "sinks without"), (dict(window=2 ** 31), "int"),
+    (dict(window=8, width=129), "width"), (dict(window=8, q_heads=3), "multiple"),
+])
+def test_window_sizes_refused(pkg, more, word):
+    with pytest.raises(pkg.S2SError, match=word):
+        plan(pkg, **more)
+
+
+def test_window_calls_refused(pkg):
+    """Sinks with documents: the entry's first keys are not each document's."""
+    with pytest.raises(pkg.S2SError, match="sinks with documents"):
+        plan(pkg, window=3, sinks=1)(**tensors(pkg), q_docs=arr(pkg, (2, 5), "i32"), k_docs=arr(pkg, (2, 7), "i32"))
+    with pytest.raises(pkg.S2SError, match="scale"):
+        plan(pkg, window=3, scale=float("nan"))(**tensors(pkg))
+    with pytest.raises(pkg.S2SError, match="prefix without"):
+        plan(pkg, window=3)(**tensors(pkg), prefix=arr(pkg, (2,), "i32"))
+
+
+def test_window_nothing_to_do(pkg):
+    for more in (dict(batch=0), dict(q_tokens=0)):
+        b, n = more.get("batch", 2), more.get("q_tokens", 5)
+        plan(pkg, window=4, **more)(arr(pkg, (b, n, 4, 64)), arr(pkg, (b, 7, 2, 64)), arr(pkg, (b, 7, 2, 64)), arr(pkg, (b, n, 4, 64)))
+
+
+def test_window_workspace_goes_by_the_window(pkg):
+    """A step over a long cache needs ranges for its whole length, one over a short window few or none."""
+    sizes = dict(batch=1, q_tokens=1, k_tokens=100000, q_heads=4, k_heads=1)
+    assert plan(pkg, window=64, **sizes).workspace_bytes < plan(pkg, window=4096, **sizes).workspace_bytes < plan(pkg, **sizes).workspace_bytes
+    assert plan(pkg, window=2 ** 30, **sizes).workspace_bytes == plan(pkg, **sizes).workspace_bytes
+
+
 # ---- the C interface ------------------------------------------------------------------
 
 STRUCTS = [("S2sNormRotaryArgs", "s2s_norm_rotary_args", "NormRotary_", "_NORM_ROTARY")]
@@ -109,6 +145,8 @@ def test_structs_are_the_headers(pkg, rust, c, py, pack):
 def test_null_arguments_refused(pkg):
     lib = pkg.load_library()
     assert lib.s2s_norm_rotary(None, None) != 0 and b"null" in lib.s2s_last_error()
+    assert lib.s2s_window_attention_workspace(None, 1, 0, None) != 0 and b"null" in lib.s2s_last_error()
+    assert lib.s2s_window_attention(None, 1, 0, None, 0, None) != 0 and b"null" in lib.s2s_last_error()
 
 
 # ---- the plain implementations ----------------------------------------------------------
@@ -123,3 +161,21 @@ def test_plain_norm_rotary():
         i, j = ([0, 2], [1, 3]) if adjacent else ([0, 1], [2, 3])
         assert np.allclose(y[..., i], -w[j]) and np.allclose(y[..., j], w[i]) and np.allclose(y[..., 4:], w[4:])
         assert (bound > 0).all() and (bound < 1e-4).all()
+
+
+def test_plain_window():
+    """Uniform weights average the window and the sinks; not causal, what lies less than the window away."""
+    g = np.random.default_rng(1)
+    k, v = g.standard_normal((1, 9, 1, 4)), g.standard_normal((1, 9, 1, 4))
+    q = np.zeros((1, 9, 2, 4))
+    out, _, _ = R.attention("f32", q, k, v, 1.0, causal=True, window=3, sinks=2)
+    for i in range(9):
+        seen = sorted(set(range(max(0, i - 2), i + 1)) | set(range(min(2, i + 1))))
+        assert np.allclose(out[0, i, 1], v[0, seen, 0].mean(0))
+    out, _, _ = R.attention("f32", q, k, v, 1.0, window=3, sinks=2)
+    for i in range(9):
+        seen = sorted(set(range(max(0, i - 2), min(9, i + 3))) | {0, 1})
+        assert np.allclose(out[0, i, 1], v[0, seen, 0].mean(0))
+    # more queries than keys: the first ones have no key
+    out, _, _ = R.attention("f32", q, k[:, :4], v[:, :4], 1.0, causal=True, window=2, sinks=1)
+    assert not out[0, :5].any() and np.allclose(out[0, 5, 0], v[0, 0, 0])
