@@ -21,6 +21,22 @@ __device__ __forceinline__ float wave_sum(float v) {
     return half_sum(v + w);
 }
 
+// Over G neighbouring lanes (a power of two), every lane receiving the total.
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v) {
+    if constexpr (G >= 2) v = DPP_ADD(v, 0xB1);
+    if constexpr (G >= 4) v = DPP_ADD(v, 0x4E);
+    if constexpr (G >= 8) v = DPP_ADD(v, 0x141);
+    if constexpr (G >= 16) v = DPP_ADD(v, 0x140);
+    if constexpr (G >= 32) {
+        float w = v;
+        asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+        v += w;
+    }
+    if constexpr (G >= 64) v = half_sum(v);
+    return v;
+}
+
 // ---- rotary ------------------------------------------------------------------
 
 // sin and cos of a whole turn times f / 2^64. The angle arrives in turns as a
@@ -523,9 +539,177 @@ __global__ __launch_bounds__(256) void k_norm_rotary_heads(NormRotaryArgs a) {
     }
 }
 
+// A head in the registers of G lanes (a power of two): lane g holds V pairs, or V channels that are
+// not turned, reads them once, and the squares' sum is made across the lanes. The sines of the
+// workgroup's `tb` tokens are made once, in LDS; a lane keeps its channels' weights while it goes
+// from head to head, neighbouring lanes' heads side by side in memory.
+template <typename T, bool ADJ, int V, int G>
+__global__ __launch_bounds__(256) void k_norm_rotary(NormRotaryArgs a, int tb, int per_head) {
+    typedef VecOf<T, V> Part;
+    const RotaryArgs &r = a.r;
+    extern __shared__ float2 turn[];  // [tb][pairs]
+    const int tid = threadIdx.x, heads = r.hq + r.hk, rot = r.pairs / V, g = tid % G;
+    const unsigned tok0 = blockIdx.x * (unsigned)tb, all = (unsigned)r.batch * (unsigned)r.tokens;  // (at most 2^30)
+    const int n_tok = (int)min((unsigned)tb, all - tok0);
+    for (int i = tid; i < n_tok * r.pairs; i += 256) {
+        const unsigned t = (unsigned)i / (unsigned)r.pairs, p = i - t * r.pairs, b = (tok0 + t) / (unsigned)r.tokens;
+        const int pos = r.pos[b * r.pos_b + (long long)(tok0 + t - b * r.tokens) * r.axes + r.axis[p]];
+        float2 x;
+        sincos_turns((unsigned long long)(long long)pos * r.freq[p], x.y, x.x);
+        turn[i] = x;
+    }
+    // this lane's channels: two runs of V (ADJ: one of 2 V), or one of V that is not turned
+    const bool turns = g < rot, there = g < per_head;
+    const int c0 = !there ? 0 : turns ? (ADJ ? 2 * V : V) * g : 2 * r.pairs + (g - rot) * V;
+    const int c1 = turns ? (ADJ ? c0 + V : c0 + r.pairs) : c0;
+    float wt[2][2][V];  // [k][run]
+    auto weights = [&](const float *w, float (*to)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[0][i] = w[c0 + i] + a.offset, to[1][i] = w[c1 + i] + a.offset;
+    };
+    if (!a.qw_head) weights(a.qw, wt[0]);
+    if (!a.kw_head && r.hk) weights(a.kw, wt[1]);
+    __syncthreads();
+    constexpr int STEP = 256 / G;
+    int h = tid / G, t = 0, b = (int)(tok0 / (unsigned)r.tokens), at = (int)(tok0 - (unsigned)b * r.tokens);
+    auto wrap = [&] {
+        while (h >= heads) {
+            h -= heads, ++t;
+            if (++at == r.tokens) at = 0, ++b;
+        }
+    };
+    wrap();
+    // (a wave's lanes all stay to its end: the sums are made across them)
+    for (int left = n_tok * heads - (tid / 64) * (64 / G); left > 0; left -= STEP) {
+        const bool isq = h < r.hq;
+        const int hh = isq ? h : h - r.hq;
+        const bool ok = t < n_tok && there && (!r.lens || at < r.lens[b]);
+        const Strides si = isq ? r.sq : r.sk, so = isq ? r.sqo : r.sko;
+        const T *src = (const T *)(isq ? r.q : r.k) + b * si.b + at * si.t + hh * si.h;
+        T *dst = (T *)(isq ? r.qo : r.ko) + b * so.b + at * so.t + hh * so.h;
+        Part x{}, y{};
+        if (ok) {
+            if (ADJ && turns) {
+                const VecOf<T, 2 * V> z = *(const VecOf<T, 2 * V> *)(src + c0);
+#pragma unroll
+                for (int i = 0; i < V; ++i) x.e[i] = z.e[i], y.e[i] = z.e[V + i];
+            } else {
+                x = *(const Part *)(src + c0);
+                if (turns) y = *(const Part *)(src + c1);
+            }
+        }
+        float u[2][V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) u[0][i] = (float)x.e[i], u[1][i] = (float)y.e[i];
+        auto squares = [&](float f) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float p = u[0][i] * f, q = u[1][i] * f;
+                ss = fmaf(p, p, fmaf(q, q, ss));
+            }
+            return lanes_sum<G>(ss);
+        };
+        const float ss = squares(1.f);
+        float inv = 1.0f / sqrtf(ss / (float)r.width + a.eps);
+        if constexpr (!std::is_same<T, half_t>::value) {
+            // heads whose squares pass an f32's range, either way (as of a row of the norm)
+            const bool far = ss > 0x1p127f, near = ss < 0x1p-100f && a.eps < 0x1p-100f;
+            if (__builtin_expect(__any(far || near), 0)) {
+                const float f = far ? 0x1p-80f : near ? 0x1p80f : 1.f;
+                inv = f / sqrtf(squares(f) / (float)r.width + a.eps * f * f);
+            }
+        }
+        if (ok) {
+            float w[2][V];
+            if (isq ? a.qw_head : a.kw_head) weights(isq ? a.qw + hh * a.qw_head : a.kw + hh * a.kw_head, w);
+            else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) w[0][i] = isq ? wt[0][0][i] : wt[1][0][i], w[1][i] = isq ? wt[0][1][i] : wt[1][1][i];
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) u[0][i] = u[0][i] * inv * w[0][i], u[1][i] = u[1][i] * inv * w[1][i];
+            if (turns) {
+                const float2 *cs = turn + t * r.pairs + g * V;
+                if (ADJ) {
+                    VecOf<T, 2 * V> z;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float p = u[2 * i / V][2 * i % V], q = u[(2 * i + 1) / V][(2 * i + 1) % V];
+                        z.e[2 * i] = (T)fmaf(p, cs[i].x, -q * cs[i].y);
+                        z.e[2 * i + 1] = (T)fmaf(p, cs[i].y, q * cs[i].x);
+                    }
+                    *(VecOf<T, 2 * V> *)(dst + c0) = z;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        x.e[i] = (T)fmaf(u[0][i], cs[i].x, -u[1][i] * cs[i].y);
+                        y.e[i] = (T)fmaf(u[0][i], cs[i].y, u[1][i] * cs[i].x);
+                    }
+                    *(Part *)(dst + c0) = x;
+                    *(Part *)(dst + c1) = y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) x.e[i] = (T)u[0][i];
+                *(Part *)(dst + c0) = x;
+            }
+        }
+        h += STEP;
+        wrap();
+    }
+}
+
+template <typename T, bool ADJ, int V, int G>
+hipError_t norm_rotary_launch(const NormRotaryArgs &a, int per_head, hipStream_t st) {
+    const RotaryArgs &r = a.r;
+    const long long all = (long long)r.batch * r.tokens;
+    const int heads = r.hq + r.hk;
+    const long long fill = std::max(1LL, all / (4LL * cu_count()));
+    const int tb = (int)std::max({1LL, std::min({std::max((256LL + heads * G - 1) / (heads * G), (128LL + r.pairs - 1) / r.pairs), fill, 16LL}), all / 0xffffff + 1});
+    return enqueue(k_norm_rotary<T, ADJ, V, G>, dim3((unsigned)((all + tb - 1) / tb)), dim3(256), (size_t)tb * r.pairs * sizeof(float2), st, a,
+                   tb, per_head);
+}
+
+template <typename T, bool ADJ, int V>
+hipError_t norm_rotary_of(const NormRotaryArgs &a, hipStream_t st) {
+    const int per_head = (a.r.width - a.r.pairs) / V;
+    if (per_head <= 4) return norm_rotary_launch<T, ADJ, V, 4>(a, per_head, st);
+    if (per_head <= 8) return norm_rotary_launch<T, ADJ, V, 8>(a, per_head, st);
+    if (per_head <= 16) return norm_rotary_launch<T, ADJ, V, 16>(a, per_head, st);
+    if (per_head <= 32) return norm_rotary_launch<T, ADJ, V, 32>(a, per_head, st);
+    return norm_rotary_launch<T, ADJ, V, 64>(a, per_head, st);
+}
+
 template <typename T>
 hipError_t norm_rotary_type(const NormRotaryArgs &a, hipStream_t st) {
-    const long long items = (long long)a.r.batch * a.r.tokens * (a.r.hq + a.r.hk);
+    constexpr int size = sizeof(T);
+    const RotaryArgs &r = a.r;
+    int v = std::min(aligned_elements(r.q, r.sq, size), aligned_elements(r.qo, r.sqo, size));
+    if (r.hk) v = std::min(v, std::min(aligned_elements(r.k, r.sk, size), aligned_elements(r.ko, r.sko, size)));
+    const int most = v;
+    // V pairs a lane, as in k_rotary
+    if (r.adjacent) v /= 2;
+    while (v > 1 && (r.pairs % v || (r.width - 2 * r.pairs) % v)) v /= 2;
+    // (adjacent pairs of odd addresses, and heads of more than a wave's lanes, element by element)
+    if (most >= (r.adjacent ? 2 : 1) && (r.width - r.pairs) / v <= 64) {
+        if (r.adjacent) switch (v) {
+                case 4:
+                    if constexpr (size == 2) return norm_rotary_of<T, true, 4>(a, st);
+                    break;
+                case 2: return norm_rotary_of<T, true, 2>(a, st);
+                case 1: return norm_rotary_of<T, true, 1>(a, st);
+            }
+        else switch (v) {
+                case 8:
+                    if constexpr (size == 2) return norm_rotary_of<T, false, 8>(a, st);
+                    break;
+                case 4: return norm_rotary_of<T, false, 4>(a, st);
+                case 2: return norm_rotary_of<T, false, 2>(a, st);
+                case 1: return norm_rotary_of<T, false, 1>(a, st);
+            }
+    }
+    const long long items = (long long)r.batch * r.tokens * (r.hq + r.hk);
     return enqueue(k_norm_rotary_heads<T>, dim3((unsigned)std::min((items + 3) / 4, 1LL << 20)), dim3(256), 0, st, a);
 }
 
