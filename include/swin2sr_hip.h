@@ -344,6 +344,25 @@ int s2s_window_attention_workspace(const s2s_attention_args *args, int window, i
 int s2s_window_attention(const s2s_attention_args *args, int window, int sinks, void *workspace, uint64_t workspace_bytes,
                          void *stream);
 
+/* The attention of a batch whose entries all begin with the same keys, which lie in
+ * memory once and are read once for all of them: entry b's keys are the shared ones
+ * j < shared_lens[b], and behind them its own. The query's place is P(i) =
+ * shared_lens[b] + k_lens[b] - q_lens[b] + i; masks (`causal`, lengths), cap and slopes are as
+ * above. `own` holds the call's sizes (k_tokens of each entry's own keys, 0
+ * allowed), arrays and masks; its prefix, documents, positions and table have to be
+ * NULL. Lengths are taken as clamped to the tokens. Up to 2^30 shared and own
+ * tokens, 2^26 query tokens times heads of the batch. The workspace goes by dtype
+ * and the seven sizes. */
+typedef struct s2s_shared_attention_args {
+    s2s_attention_args own;
+    int shared_tokens;
+    s2s_tokens shared_k, shared_v; /* their batch strides count for nothing */
+    const int32_t *shared_lens;    /* [batch], or NULL: all shared tokens */
+} s2s_shared_attention_args;
+
+int s2s_shared_attention_workspace(const s2s_shared_attention_args *args, uint64_t *bytes);
+int s2s_shared_attention(const s2s_shared_attention_args *args, void *workspace, uint64_t workspace_bytes, void *stream);
+
 /* Rotary positions with up to four axes: the pair p of every head of q (and k)
  * is turned by the angle pos[b][token][pair_axis[p]] * inv_freq[p]. Pairs are
  * channels (p, p + pairs), or (2p, 2p + 1) if `adjacent`; channels from 2 pairs

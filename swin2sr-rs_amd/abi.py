@@ -58,6 +58,11 @@ class Attention_(C.Structure):
                 ("slopes", C.c_void_p), ("table", C.c_void_p), ("table_size", C.c_int)]
 
 
+class SharedAttention_(C.Structure):
+    _fields_ = [("own", Attention_), ("shared_tokens", C.c_int), ("shared_k", Tokens_), ("shared_v", Tokens_),
+                ("shared_lens", C.c_void_p)]
+
+
 class Rotary_(C.Structure):
     _fields_ = [("dtype", C.c_int), ("batch", C.c_int), ("tokens", C.c_int), ("q_heads", C.c_int),
                 ("k_heads", C.c_int), ("width", C.c_int), ("axes", C.c_int), ("pairs", C.c_int),
@@ -119,6 +124,8 @@ EXPORTS = {
     "s2s_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
     "s2s_window_attention_workspace": (C.c_int, [C.POINTER(Attention_), C.c_int, C.c_int, C.POINTER(C.c_uint64)]),
     "s2s_window_attention": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "s2s_shared_attention_workspace": (C.c_int, [C.POINTER(SharedAttention_), C.POINTER(C.c_uint64)]),
+    "s2s_shared_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
     "s2s_rotary": (C.c_int, [C.c_void_p, C.c_void_p]),
     "s2s_norm_rotary": (C.c_int, [C.c_void_p, C.c_void_p]),
     "s2s_rms_norm": (C.c_int, [C.c_void_p, C.c_void_p]),

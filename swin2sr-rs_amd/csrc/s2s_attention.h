@@ -105,8 +105,12 @@ struct AttnLaunch {
     int meta_tiles;
     const int4 *col_docs;  // [batch][tiles] the same of a column tile's queries, and its key tiles
     const int *order;      // [batch][tiles] column tiles with the most key tiles first, or null
+    int join;       // the ranges' sums are joined behind this launch
     int table_lds;  // the group's rows of the table fit LDS
-    FastDiv by_pairs, by_tiles, by_hk, by_group;
+    FastDiv by_pairs, by_tiles, by_hk, by_group, by_nq;
+    // the ranges of the keys that the batch shares: their sums, number and columns (of all entries)
+    float *shared_o, *shared_ml;
+    int shared_splits, shared_cols;
     AttnScore score;
 };
 
@@ -119,7 +123,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = kAttnLog2e;
 
-enum { CAP = 1, SLOPES = 2, ANY = 8, DOCS = 16, GENERAL = 32, WINDOW = 64 };
+enum { CAP = 1, SLOPES = 2, ANY = 8, DOCS = 16, GENERAL = 32, WINDOW = 64, SHARED = 128 };
 
 template <typename T>
 struct Type;
@@ -346,7 +350,8 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 //  key tile (one block of 16 keys of 64); the four sums meet in LDS at the end.
 //  MODE: CAP and SLOPES are known (0 to 3), or asked for in every tile (ANY); documents
 //  (DOCS); or all of that and what AttnScore::general stands for (GENERAL); each with a
-//  sliding window or without (WINDOW). Paths that a
+//  sliding window or without (WINDOW); or for the columns of all batch entries over keys that
+//  they share (SHARED: k and v are the shared ones, and the sums go to the ranges' join). Paths that a
 //  kernel might take and does not cost it registers, spilled around its loop, and copies
 //  where they meet.
 // K and V tiles of TK keys are copied straight into LDS, two buffers each (three and four
@@ -355,7 +360,9 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 // (16, or 4 for rows of 4-byte multiples), or 0: through registers, by elements.
 template <typename T, int DP, int NB, bool WK, int ALIGN, int MODE>
 struct Kernel {
-    static constexpr bool WIN = MODE & WINDOW, GEN = (MODE & ~WINDOW) == GENERAL, DOC = GEN || (MODE & DOCS), KNOWN = (MODE & ~WINDOW) < ANY;
+    static constexpr bool WIN = MODE & WINDOW, SHARE = MODE & SHARED;
+    static constexpr int KIND = MODE & ~(WINDOW | SHARED);
+    static constexpr bool GEN = KIND == GENERAL, DOC = GEN || (KIND & DOCS), KNOWN = KIND < ANY;
     typedef Type<T> Ty;
     typedef typename Ty::V Vec;
     static constexpr bool F32 = sizeof(T) == 4;
@@ -397,12 +404,12 @@ struct Kernel {
         // tile-major, so that with a multiple of 8 (batch, key head) pairs one XCD
         // keeps a pair's keys in its L2, and the tiles with the most keys (the last
         // ones, under the causal mask) start first
-        const int rest = L.by_pairs.of(blockIdx.x), bh = blockIdx.x - rest * (a.batch * a.hk);
+        const int rest = L.by_pairs.of(blockIdx.x), bh = blockIdx.x - rest * (SHARE ? a.hk : a.batch * a.hk);
         const int split = L.by_tiles.of(rest), rank = rest - split * L.tiles;
-        const int b = L.by_hk.of(bh), kvh = bh - b * a.hk;
+        const int b = SHARE ? 0 : L.by_hk.of(bh), kvh = SHARE ? bh : bh - b * a.hk;
         const int ct = L.order ? L.order[b * L.tiles + rank] : L.tiles - 1 - rank;
-        const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
-        const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.nk) : a.nk;
+        const int ql = SHARE ? a.batch * a.nq : a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
+        int kl = !SHARE && a.k_lens ? min(max(a.k_lens[b], 0), a.nk) : a.nk;
         const int c0 = ct * COLS;
         if (c0 >= ql * a.group) return;  // (the whole workgroup; ql * group <= 2^30)
         const int pre = a.prefix ? a.prefix[b] : 0;
@@ -422,16 +429,29 @@ struct Kernel {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int c = wc0 + nb * 16 + n16, i = L.by_group.of(c), h = kvh * a.group + (c - i * a.group);
-            const bool ok = i < ql;
+            bool ok = i < ql;
+            const T *row;
+            if constexpr (SHARE) {
+                // the entry's lengths and the query's place behind its part of the shared keys
+                const int e = ok ? L.by_nq.of(i) : 0, ie = i - e * a.nq;
+                const int n = a.q_lens ? min(max(a.q_lens[e], 0), a.nq) : a.nq, own = a.k_lens ? min(max(a.k_lens[e], 0), a.own_nk) : a.own_nk;
+                const int mine = a.shared_lens ? min(max(a.shared_lens[e], 0), a.nk) : a.nk;
+                ok = ok && ie < n;
+                at[nb] = mine + own - n + ie;
+                lim[nb] = !ok ? -1 : a.causal ? min(mine, max(at[nb] + 1, 0)) : mine;
+                low[nb] = doc[nb] = tab[nb] = 0;
+                row = (const T *)a.q + e * a.sq.b + (long long)ie * a.sq.t + h * a.sq.h;
+            } else {
             lim[nb] = ok ? limit(i) : 0;
             low[nb] = ok ? start(i) : 0;
             // (a column of no document computes what it may, and is zeroed at the end)
             doc[nb] = 0;
             if (DOC && a.q_docs && ok) doc[nb] = a.q_docs[b * a.q_docs_b + i];
             at[nb] = a.q_pos && ok ? a.q_pos[b * a.q_pos_b + i] : kl - ql + i;
-            slope[nb] = a.slopes && ok ? slope_of(a.slopes[h]) : 0.f;
             tab[nb] = ok ? (L.table_lds ? c - i * a.group : h) * a.table_size : 0;
-            const T *row = (const T *)a.q + b * a.sq.b + (long long)(ok ? i : 0) * a.sq.t + h * a.sq.h;
+            row = (const T *)a.q + b * a.sq.b + (long long)(ok ? i : 0) * a.sq.t + h * a.sq.h;
+            }
+            slope[nb] = a.slopes && ok ? slope_of(a.slopes[h]) : 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const int c = (4 * ks + q) * E;
@@ -445,11 +465,39 @@ struct Kernel {
         }
         // keys that any column of the workgroup (of the wave) may read, and that all may
         const int i_last = min(ql - 1, L.by_group.of(c0 + COLS - 1));
-        const int wg_max = limit(i_last), wg_min = limit(L.by_group.of(c0));
+        int wg_max = 0, wg_min = 0;
         const int w_first = min(ql - 1, L.by_group.of(wc0)), w_last = min(ql - 1, L.by_group.of(wc0 + 16 * NB - 1));
         const bool w_any = wc0 < ql * a.group;
-        const int w_max = w_any ? limit(w_last) : 0, w_min = limit(w_first);
-        const int w_at = kl - ql + w_first;  // the first place among the wave's queries
+        int w_max = 0, w_min = 0, w_at = 0;  // (w_at: the first place among the wave's queries)
+        if constexpr (SHARE) {
+            // the limits in no order: over the wave's columns (those of no query aside), then the workgroup's
+            w_min = w_at = 0x7fffffff;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+                if (lim[nb] >= 0) w_max = max(w_max, lim[nb]), w_min = min(w_min, lim[nb]), w_at = min(w_at, at[nb]);
+#pragma unroll
+            for (int m = 1; m < 16; m *= 2) {
+                w_max = max(w_max, __shfl_xor(w_max, m));
+                w_min = min(w_min, __shfl_xor(w_min, m));
+                w_at = min(w_at, __shfl_xor(w_at, m));
+            }
+            w_max = __builtin_amdgcn_readfirstlane(w_max);
+            w_min = __builtin_amdgcn_readfirstlane(w_min);
+            w_at = __builtin_amdgcn_readfirstlane(w_at);
+            w_at = w_at == 0x7fffffff ? 0 : w_at;
+            if (lane == 0) ((int2 *)lds)[wave] = make_int2(w_max, w_min);
+            __syncthreads();
+            wg_min = 0x7fffffff;
+            for (int w = 0; w < 4; ++w) wg_max = max(wg_max, ((int2 *)lds)[w].x), wg_min = min(wg_min, ((int2 *)lds)[w].y);
+            __syncthreads();
+            wg_max = __builtin_amdgcn_readfirstlane(wg_max);
+            wg_min = __builtin_amdgcn_readfirstlane(wg_min);
+            kl = wg_max;
+        } else {
+            wg_max = limit(i_last), wg_min = limit(L.by_group.of(c0));
+            w_max = w_any ? limit(w_last) : 0, w_min = limit(w_first);
+            w_at = kl - ql + w_first;
+        }
         // what all columns' windows hold begins here, and what any holds
         const int wg_from = start(i_last), w_from = start(w_last), w_low = start(w_first);
         // documents of the workgroup's columns and of the wave's, where key tiles can be passed
@@ -730,8 +778,8 @@ struct Kernel {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int c = wc0 + nb * 16 + n16, i = (int)((__umulhi((unsigned)c, late->L.by_group.m) + (unsigned)c) >> late->L.by_group.s);
-            if (i >= ql) continue;
-            if (splits > 1) {
+            if (SHARE ? lim[nb] < 0 : i >= ql) continue;
+            if (SHARE || late->L.part_o) {
                 const long long row = ((long long)bh * splits + split) * late->L.cols + c;
                 float *po = late->L.part_o + row * DP, *ml = late->L.part_ml + 2 * row;
                 if (q == 0 && (!WK || wave == 0)) ml[0] = m[nb], ml[1] = total[nb];
@@ -1091,7 +1139,24 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnOpArgs a, AttnLaunch L) {
 // The key ranges' sums of one column: a workgroup each, its threads over the ranges
 // for their weights and then over (channel, every 256 / DP-th range), so that the
 // reads of all ranges are in flight together.
-template <typename T, int DP>
+// Where range s of a column has its sums: among its entry's own, or (SHARE) behind those
+// among the shared keys'.
+template <bool SHARE>
+struct Ranges {
+    const AttnLaunch &L;
+    long long own, shared;
+    __device__ Ranges(const AttnOpArgs &a, const AttnLaunch &L, int b, int kvh, int c)
+        : L(L), own((long long)(b * a.hk + kvh) * L.splits * L.cols + c),
+          shared(SHARE ? (long long)kvh * L.shared_splits * L.shared_cols + (long long)b * L.cols + c : 0) {}
+    __device__ int count() const { return L.splits + (SHARE ? L.shared_splits : 0); }
+    __device__ bool mine(int s) const { return !SHARE || s < L.splits; }
+    __device__ long long row(int s) const { return mine(s) ? own + (long long)s * L.cols : shared + (long long)(s - L.splits) * L.shared_cols; }
+    __device__ const float *ml(int s) const { return (mine(s) ? L.part_ml : L.shared_ml) + 2 * row(s); }
+    template <int DP>
+    __device__ const float *o(int s) const { return (mine(s) ? L.part_o : L.shared_o) + row(s) * DP; }
+};
+
+template <typename T, int DP, bool SHARE>
 __global__ __launch_bounds__(256) void k_attn_join(AttnOpArgs a, AttnLaunch L) {
     constexpr int G = 256 / DP;
     const int tid = threadIdx.x;
@@ -1100,13 +1165,14 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnOpArgs a, AttnLaunch L) {
     const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
     const int i = c / a.group;
     if (i >= ql) return;
-    const long long row0 = (long long)bh * L.splits * L.cols + c;
+    const Ranges<SHARE> at(a, L, b, kvh, c);
+    const int count = at.count();
     __shared__ float weight[256], part[256], stat[8];
     float ms = -INFINITY, l = 0.f;
-    if (tid < L.splits) {
-        const long long row = row0 + (long long)tid * L.cols;
-        ms = L.part_ml[2 * row];
-        l = L.part_ml[2 * row + 1];
+    if (tid < count) {
+        const float *ml = at.ml(tid);
+        ms = ml[0];
+        l = ml[1];
     }
     // the first sums on their way while the weights are made
     constexpr int N = 16;
@@ -1116,7 +1182,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnOpArgs a, AttnLaunch L) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int s = s0 + k * G;
-            x[k] = g < G && s < L.splits ? L.part_o[(row0 + (long long)s * L.cols) * DP + d] : 0.f;
+            x[k] = g < G && s < count ? at.template o<DP>(s)[d] : 0.f;
         }
     };
     load(g);
@@ -1136,12 +1202,12 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnOpArgs a, AttnLaunch L) {
     __syncthreads();
     ls = (stat[4] + stat[5]) + (stat[6] + stat[7]);
     float o = 0.f;
-    for (int s0 = g; s0 < L.splits; s0 += N * G) {
+    for (int s0 = g; s0 < count; s0 += N * G) {
         if (s0 != g) load(s0);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int s = s0 + k * G;
-            const float w = s < L.splits ? weight[s] : 0.f;
+            const float w = s < count ? weight[s] : 0.f;
             o += w == 0.f ? 0.f : w * x[k];
         }
     }
@@ -1160,7 +1226,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnOpArgs a, AttnLaunch L) {
 // The same for up to kFewRanges ranges of many columns: four channels a thread, 256 / (DP / 4)
 // columns a workgroup, all ranges' sums on their way at once.
 constexpr int kFewRanges = 8;
-template <typename T, int DP>
+template <typename T, int DP, bool SHARE>
 __global__ __launch_bounds__(256) void k_attn_join_few(AttnOpArgs a, AttnLaunch L, int rows) {
     constexpr int R = DP / 4, N = 256 / R;
     const int tid = threadIdx.x, id = blockIdx.x * N + tid / R, d = tid % R * 4;
@@ -1169,17 +1235,18 @@ __global__ __launch_bounds__(256) void k_attn_join_few(AttnOpArgs a, AttnLaunch 
     const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
     const int i = L.by_group.of(c);
     if (i >= ql) return;
-    const long long row0 = (long long)bh * L.splits * L.cols + c;
+    const Ranges<SHARE> at(a, L, b, kvh, c);
+    const int count = at.count();
     f4v x[kFewRanges];
     float ms[kFewRanges], l[kFewRanges], top = -INFINITY;
 #pragma unroll
     for (int s = 0; s < kFewRanges; ++s) {
         x[s] = f4v{0.f, 0.f, 0.f, 0.f};
         ms[s] = -INFINITY, l[s] = 0.f;
-        if (s < L.splits) {
-            const long long row = row0 + (long long)s * L.cols;
-            ms[s] = L.part_ml[2 * row], l[s] = L.part_ml[2 * row + 1];
-            x[s] = *(const f4v *)(L.part_o + row * DP + d);
+        if (s < count) {
+            const float *ml = at.ml(s);
+            ms[s] = ml[0], l[s] = ml[1];
+            x[s] = *(const f4v *)(at.template o<DP>(s) + d);
         }
     }
 #pragma unroll
@@ -1212,7 +1279,7 @@ hipError_t launch(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
     AttnLaunch M = L;
     M.table_lds = a.table && (long long)a.group * a.table_size <= K::kTabEntries;
     const size_t lds = K::kTab + (M.table_lds ? (size_t)a.group * a.table_size * 4 : 0);
-    const long long blocks = (long long)a.batch * a.hk * L.tiles * L.splits;  // (below 2^24 by the entry's checks)
+    const long long blocks = (long long)((MODE & SHARED) ? 1 : a.batch) * a.hk * L.tiles * L.splits;  // (below 2^24 by the entry's checks)
     return enqueue(k_attn<T, DP, NB, WK, ALIGN, MODE>, dim3((unsigned)blocks), dim3(256), lds, st, a, M);
 }
 
@@ -1223,19 +1290,21 @@ hipError_t launch_narrow(const AttnOpArgs &a, const AttnLaunch &L, int align, hi
     if (align == 0) return launch<T, DP, 1, WK, 0, GENERAL | W>(a, L, st);
     if (align < 16) return launch<T, DP, 1, WK, 4, GENERAL | W>(a, L, st);
     if (L.score.general) return launch<T, DP, 1, WK, 16, GENERAL | W>(a, L, st);
-    return a.k_docs ? launch<T, DP, 1, WK, 16, ANY | DOCS | W>(a, L, st) : launch<T, DP, 1, WK, 16, ANY | W>(a, L, st);
+    if constexpr (W != SHARED)
+        if (a.k_docs) return launch<T, DP, 1, WK, 16, ANY | DOCS | W>(a, L, st);
+    return launch<T, DP, 1, WK, 16, ANY | W>(a, L, st);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool SHARE = false>
 hipError_t join(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
     const long long rows = (long long)a.batch * a.hk * L.cols;  // (few: the keys were split to fill the chip)
     // few ranges of many columns: 8 causal bf16 heads of 128 over 512, 1024 and 2048 tokens 15, 26
     // and 40 us against 21, 39 and 62 by a workgroup per column; 512 columns of 4 ranges (16 steps over
     // 1024 keys) 20.3 against 19.6
     constexpr int N = 256 / (DP / 4);
-    if (L.splits <= kFewRanges && rows >= 4 * cu_count())
-        return enqueue(k_attn_join_few<T, DP>, dim3((unsigned)((rows + N - 1) / N)), dim3(256), 0, st, a, L, (int)rows);
-    return enqueue(k_attn_join<T, DP>, dim3((unsigned)rows), dim3(256), 0, st, a, L);
+    if (L.splits + (SHARE ? L.shared_splits : 0) <= kFewRanges && rows >= 4 * cu_count())
+        return enqueue(k_attn_join_few<T, DP, SHARE>, dim3((unsigned)((rows + N - 1) / N)), dim3(256), 0, st, a, L, (int)rows);
+    return enqueue(k_attn_join<T, DP, SHARE>, dim3((unsigned)rows), dim3(256), 0, st, a, L);
 }
 
 template <typename T, int DP, int W>
@@ -1251,7 +1320,27 @@ hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, 
         e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES | W>(a, L, st) : launch<T, DP, 2, false, 16, CAP | W>(a, L, st);
     else
         e = a.slopes ? launch<T, DP, 2, false, 16, SLOPES | W>(a, L, st) : launch<T, DP, 2, false, 16, W>(a, L, st);
-    return e != hipSuccess || L.splits == 1 ? e : join<T, DP>(a, L, st);
+    return e != hipSuccess || !L.join ? e : join<T, DP>(a, L, st);
+}
+
+// The columns of all entries over the shared keys (`s`, cut by `c`); then each entry's own keys' sums
+// are there already, and all are joined by `own`.
+template <typename T, int DP>
+hipError_t launch_shared_width(const AttnOpArgs &s, const AttnLaunch &L, const Cut &c, int align, const AttnOpArgs &own, const AttnLaunch &J, hipStream_t st) {
+    hipError_t e;
+    if (c.nb == 2) e = launch<T, DP, 2, false, 16, ANY | SHARED>(s, L, st);
+    else e = c.wk ? launch_narrow<T, DP, true, SHARED>(s, L, align, st) : launch_narrow<T, DP, false, SHARED>(s, L, align, st);
+    return e != hipSuccess ? e : join<T, DP, true>(own, J, st);
+}
+
+template <typename T>
+hipError_t launch_shared_type(const AttnOpArgs &s, const AttnLaunch &L, const Cut &c, int align, const AttnOpArgs &own, const AttnLaunch &J, hipStream_t st) {
+    switch (c.dp) {
+        case 32: return launch_shared_width<T, 32>(s, L, c, align, own, J, st);
+        case 64: return launch_shared_width<T, 64>(s, L, c, align, own, J, st);
+        case 96: return launch_shared_width<T, 96>(s, L, c, align, own, J, st);
+        default: return launch_shared_width<T, 128>(s, L, c, align, own, J, st);
+    }
 }
 
 template <typename T, int W>
@@ -1272,3 +1361,9 @@ hipError_t launch_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const
 hipError_t launch_window_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
 hipError_t launch_window_attention_f16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
 hipError_t launch_window_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_shared_attention_f32(const AttnOpArgs &s, const AttnLaunch &L, const attn::Cut &c, int align, const AttnOpArgs &own,
+                                        const AttnLaunch &J, hipStream_t st);
+hipError_t launch_shared_attention_f16(const AttnOpArgs &s, const AttnLaunch &L, const attn::Cut &c, int align, const AttnOpArgs &own,
+                                        const AttnLaunch &J, hipStream_t st);
+hipError_t launch_shared_attention_bf16(const AttnOpArgs &s, const AttnLaunch &L, const attn::Cut &c, int align, const AttnOpArgs &own,
+                                        const AttnLaunch &J, hipStream_t st);

@@ -236,16 +236,42 @@ size_t attn_op_workspace(int dtype, const AttnOpArgs &a) {
     return most;
 }
 
+namespace {
+
+// The copies' size that a call's arrays allow: 16, or 4, or 0 for element by element.
+int copies_of(const AttnOpArgs &a, int al) {
+    // (rows that overlap have no end that the copies' resource could tell: by elements)
+    return a.sk.t < a.width || a.sv.t < a.width ? 0 : al >= 16 ? 16 : al >= 4 ? 4 : 0;
+}
+int aligned_inputs(const AttnOpArgs &a, int size) {
+    const int al = aligned_bytes(a.q, a.sq, a.width, size);
+    return a.nk > 0 ? std::min(al, std::min(aligned_bytes(a.k, a.sk, a.width, size), aligned_bytes(a.v, a.sv, a.width, size))) : al;
+}
+
+hipError_t launch_of(int dtype, const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st) {
+    if (a.window) switch (dtype) {
+            case 0: return launch_window_attention_f32(a, L, c, align, st);
+            case 1: return launch_window_attention_f16(a, L, c, align, st);
+            case 2: return launch_window_attention_bf16(a, L, c, align, st);
+        }
+    switch (dtype) {
+        case 0: return launch_attention_f32(a, L, c, align, st);
+        case 1: return launch_attention_f16(a, L, c, align, st);
+        case 2: return launch_attention_bf16(a, L, c, align, st);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
 hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStream_t st) {
     const int size = dtype == 0 ? 4 : 2;
     AttnLaunch L{};
     L.score.set(a);
-    int al = aligned_bytes(a.q, a.sq, a.width, size);
-    if (a.nk > 0) al = std::min(al, std::min(aligned_bytes(a.k, a.sk, a.width, size), aligned_bytes(a.v, a.sv, a.width, size)));
+    const int al = aligned_inputs(a, size);
     L.vec = std::min(al, 8);
     L.out_vec = std::min(4, aligned_bytes(a.out, a.so, a.width, size) / size);
-    // (rows that overlap have no end that the copies' resource could tell: by elements)
-    const int align = a.sk.t < a.width || a.sv.t < a.width ? 0 : al >= 16 ? 16 : al >= 4 ? 4 : 0;
+    const int align = copies_of(a, al);
     // Packed documents of narrow heads too: the fewer columns a workgroup has, the fewer lie
     // across two documents and mask both's tiles (nine images, 11003 tokens, 12 heads: 64
     // wide 153 us with waves of 32 and 127 with 16, 32 wide 132 and 105; 128 wide, 32 / 8
@@ -264,6 +290,7 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
         const size_t rows = (size_t)a.batch * a.hk * c.splits * L.cols;
         L.part_o = (float *)(w + doc_bytes(c, a));
         L.part_ml = L.part_o + rows * c.dp;
+        L.join = 1;
     }
     // a summary of few tiles would skip nothing
     if (a.k_docs && mt > 4) {
@@ -289,15 +316,86 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
         }
         if (e != hipSuccess) return e;
     }
-    if (a.window) switch (dtype) {
-            case 0: return launch_window_attention_f32(a, L, c, align, st);
-            case 1: return launch_window_attention_f16(a, L, c, align, st);
-            case 2: return launch_window_attention_bf16(a, L, c, align, st);
-        }
+    return launch_of(dtype, a, L, c, align, st);
+}
+
+// ---- a batch that shares a prefix ---------------------------------------------------
+
+namespace {
+
+// How the columns of all entries go over the shared keys.
+attn::Cut shared_cut(int dtype, const AttnOpArgs &s, bool narrow) {
+    AttnOpArgs one = s;
+    one.nq = s.batch * s.nq;
+    one.batch = 1;
+    attn::Cut c = cut_of(dtype, one, narrow);
+    c.splits = std::min(c.splits, 128);  // (the join takes 256 ranges)
+    return c;
+}
+attn::Cut own_cut(int dtype, const AttnOpArgs &a, bool narrow) {
+    attn::Cut c = cut_of(dtype, a, narrow);
+    c.splits = std::min(c.splits, 128);
+    return c;
+}
+
+size_t sums_bytes(const attn::Cut &c, size_t columns) { return columns * c.splits * ((size_t)c.dp * 4 + 8); }
+
+}  // namespace
+
+size_t shared_attn_op_workspace(int dtype, const AttnOpArgs &s, const AttnOpArgs &a) {
+    size_t own = 0, shared = 0;
+    const size_t columns = (size_t)a.batch * a.nq * a.hq;
+    for (const bool narrow : {false, true}) {
+        own = std::max(own, sums_bytes(own_cut(dtype, a, narrow), columns));
+        shared = std::max(shared, sums_bytes(shared_cut(dtype, s, narrow), columns));
+    }
+    return round16(own) + shared;
+}
+
+hipError_t launch_shared_attention_op(int dtype, const AttnOpArgs &s, const AttnOpArgs &a, void *ws, hipStream_t st) {
+    const int size = dtype == 0 ? 4 : 2;
+    const size_t columns = (size_t)a.batch * a.nq * a.hq;
+    auto fill = [&](const AttnOpArgs &x, const attn::Cut &c, int al, float *sums) {
+        AttnLaunch L{};
+        L.score.set(x);
+        L.vec = std::min(al, 8);
+        L.out_vec = std::min(4, aligned_bytes(a.out, a.so, a.width, size) / size);
+        L.tiles = c.tiles;
+        L.splits = c.splits;
+        L.by_tiles.set(c.tiles);
+        L.by_hk.set(a.hk);
+        L.by_group.set(a.group);
+        L.by_nq.set(a.nq);
+        L.part_o = sums;
+        L.part_ml = sums + columns * c.splits * c.dp;
+        return L;
+    };
+    // each entry's own keys
+    const int own_al = aligned_inputs(a, size), own_align = copies_of(a, own_al);
+    AttnScore score;
+    score.set(a);
+    const attn::Cut oc = own_cut(dtype, a, own_align < 16 || score.general);
+    AttnLaunch O = fill(a, oc, own_al, (float *)ws);
+    O.cols = a.group * a.nq;
+    O.by_pairs.set(a.batch * a.hk);
+    hipError_t e = launch_of(dtype, a, O, oc, own_align, st);
+    if (e != hipSuccess) return e;
+    // the shared ones, and the join
+    const int al = aligned_inputs(s, size), align = copies_of(s, al);
+    const attn::Cut sc = shared_cut(dtype, s, align < 16 || score.general);
+    size_t own_most = 0;
+    for (const bool narrow : {false, true}) own_most = std::max(own_most, sums_bytes(own_cut(dtype, a, narrow), columns));
+    AttnLaunch S = fill(s, sc, al, (float *)((char *)ws + round16(own_most)));
+    S.cols = a.group * a.nq * a.batch;
+    S.by_pairs.set(a.hk);
+    O.shared_o = S.part_o;
+    O.shared_ml = S.part_ml;
+    O.shared_splits = sc.splits;
+    O.shared_cols = S.cols;
     switch (dtype) {
-        case 0: return launch_attention_f32(a, L, c, align, st);
-        case 1: return launch_attention_f16(a, L, c, align, st);
-        case 2: return launch_attention_bf16(a, L, c, align, st);
+        case 0: return launch_shared_attention_f32(s, S, sc, align, a, O, st);
+        case 1: return launch_shared_attention_f16(s, S, sc, align, a, O, st);
+        case 2: return launch_shared_attention_bf16(s, S, sc, align, a, O, st);
     }
     return hipErrorInvalidValue;
 }

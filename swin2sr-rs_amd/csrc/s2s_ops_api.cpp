@@ -175,9 +175,33 @@ AttnOpArgs attention_args(const s2s_attention_args *a, int window = 0, int sinks
     return k;
 }
 
-// A call whose sizes have been checked; window 0: none.
-int attention_call(const char *op, const s2s_attention_args *a, int window, int sinks, void *workspace, uint64_t workspace_bytes,
-                   void *stream) {
+int shared_sizes(const char *op, const s2s_shared_attention_args *s) {
+    const s2s_attention_args *a = &s->own;
+    if (s->shared_tokens < 0) return refuse("%s: negative shared tokens", op);
+    if ((long long)s->shared_tokens + a->k_tokens > (1 << 30)) return refuse("%s: over 2^30 shared and own tokens", op);
+    // the columns of all entries are an int, and the join has one part of a workgroup for each
+    if ((long long)a->batch * a->q_tokens * a->q_heads > (1 << 26))
+        return refuse("%s: over 2^26 query tokens times heads of the batch", op);
+    return 0;
+}
+
+// The shared keys' part of a call whose own part is `own`.
+AttnOpArgs shared_args(const s2s_shared_attention_args *s, const AttnOpArgs &own) {
+    AttnOpArgs k = own;
+    k.k = s->shared_k.data;
+    k.v = s->shared_v.data;
+    k.sk = strides(s->shared_k, 1, s->shared_tokens, s->own.k_heads);
+    k.sv = strides(s->shared_v, 1, s->shared_tokens, s->own.k_heads);
+    if (s->shared_tokens <= 1) k.sk.t = k.sv.t = own.width;
+    k.nk = s->shared_tokens;
+    k.own_nk = own.nk;
+    k.shared_lens = s->shared_lens;
+    return k;
+}
+
+// A call whose sizes have been checked; window 0: none; `s`: the call whose own part `a` is, or null.
+int attention_call(const char *op, const s2s_attention_args *a, int window, int sinks, const s2s_shared_attention_args *s,
+                   void *workspace, uint64_t workspace_bytes, void *stream) {
     if (!std::isfinite(a->scale)) return refuse("%s: the scale is not finite", op);
     if (!(a->cap >= 0.f) || !std::isfinite(a->cap)) return refuse("%s: the cap is negative or not finite", op);
     if (a->cap > 0.f && a->cap < 1e-6f) return refuse("%s: a cap below 1e-6", op);
@@ -216,7 +240,15 @@ int attention_call(const char *op, const s2s_attention_args *a, int window, int 
         if (a->k_tokens > 1 && (a->k.token > (1 << 22) || a->v.token > (1 << 22)))
             return refuse("%s: a token stride of k or v over 2^22 elements", op);
     }
-    if (a->out.data == a->q.data || (keys && (a->out.data == a->k.data || a->out.data == a->v.data)))
+    const bool shared = s && s->shared_tokens > 0;
+    if (shared) {
+        if (int rc = check_tokens(op, "shared_k", s->shared_k, a->dtype, on.dev)) return rc;
+        if (int rc = check_tokens(op, "shared_v", s->shared_v, a->dtype, on.dev)) return rc;
+        if (s->shared_tokens > 1 && (s->shared_k.token > (1 << 22) || s->shared_v.token > (1 << 22)))
+            return refuse("%s: a token stride of shared_k or shared_v over 2^22 elements", op);
+    }
+    if (a->out.data == a->q.data || (keys && (a->out.data == a->k.data || a->out.data == a->v.data)) ||
+        (shared && (a->out.data == s->shared_k.data || a->out.data == s->shared_v.data)))
         return refuse("%s: out is an input", op);
     const struct {
         const char *name;
@@ -229,19 +261,21 @@ int attention_call(const char *op, const s2s_attention_args *a, int window, int 
                   {"q_pos", a->q_pos},
                   {"k_pos", keys ? a->k_pos : nullptr},
                   {"slopes", a->slopes},
-                  {"table", a->table}};
+                  {"table", a->table},
+                  {"shared_lens", s ? s->shared_lens : nullptr}};
     for (const auto &x : arrays)
         if (x.p)
             if (int rc = check_array(op, x.name, x.p, 4, on.dev)) return rc;
     const AttnOpArgs k = attention_args(a, window, sinks);
-    const size_t need = attn_op_workspace(a->dtype, k);
+    const AttnOpArgs ks = s ? shared_args(s, k) : k;
+    const size_t need = s ? shared_attn_op_workspace(a->dtype, ks, k) : attn_op_workspace(a->dtype, k);
     if (need) {
         if (!workspace || workspace_bytes < need)
             return refuse("%s: a workspace of %zu bytes is needed, %llu are given", op, need,
                           workspace ? (unsigned long long)workspace_bytes : 0ULL);
         if (int rc = check_array(op, "workspace", workspace, 16, on.dev)) return rc;
     }
-    e = launch_attention_op(a->dtype, k, workspace, st);
+    e = s ? launch_shared_attention_op(a->dtype, ks, k, workspace, st) : launch_attention_op(a->dtype, k, workspace, st);
     return e == hipSuccess ? 0 : refuse_hip(op, "the launch", e);
 }
 
@@ -363,7 +397,7 @@ int s2s_attention(const s2s_attention_args *a, void *workspace, uint64_t workspa
     const char *op = "s2s_attention";
     if (!a) return refuse("%s: null argument", op);
     if (int rc = attention_sizes(op, a)) return rc;
-    return attention_call(op, a, 0, 0, workspace, workspace_bytes, stream);
+    return attention_call(op, a, 0, 0, nullptr, workspace, workspace_bytes, stream);
 }
 
 int s2s_window_attention_workspace(const s2s_attention_args *a, int window, int sinks, uint64_t *bytes) {
@@ -383,7 +417,28 @@ int s2s_window_attention(const s2s_attention_args *a, int window, int sinks, voi
     if (int rc = window_sizes(op, a, window, sinks)) return rc;
     // (a document's own first keys are not known)
     if (sinks > 0 && (a->q_docs || a->k_docs)) return refuse("%s: sinks with documents", op);
-    return attention_call(op, a, window, sinks, workspace, workspace_bytes, stream);
+    return attention_call(op, a, window, sinks, nullptr, workspace, workspace_bytes, stream);
+}
+
+int s2s_shared_attention_workspace(const s2s_shared_attention_args *s, uint64_t *bytes) {
+    const char *op = "s2s_shared_attention_workspace";
+    if (!s || !bytes) return refuse("%s: null argument", op);
+    if (int rc = attention_sizes(op, &s->own)) return rc;
+    if (int rc = shared_sizes(op, s)) return rc;
+    const AttnOpArgs k = attention_args(&s->own);
+    *bytes = shared_attn_op_workspace(s->own.dtype, shared_args(s, k), k);
+    return 0;
+}
+
+int s2s_shared_attention(const s2s_shared_attention_args *s, void *workspace, uint64_t workspace_bytes, void *stream) {
+    const char *op = "s2s_shared_attention";
+    if (!s) return refuse("%s: null argument", op);
+    const s2s_attention_args *a = &s->own;
+    if (int rc = attention_sizes(op, a)) return rc;
+    if (int rc = shared_sizes(op, s)) return rc;
+    if (a->prefix || a->q_docs || a->k_docs || a->q_pos || a->k_pos || a->table)
+        return refuse("%s: prefix, documents, positions and table are not taken", op);
+    return attention_call(op, a, 0, 0, s, workspace, workspace_bytes, stream);
 }
 
 int s2s_rotary(const s2s_rotary_args *a, void *stream) {

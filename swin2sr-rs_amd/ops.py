@@ -17,7 +17,7 @@ import ctypes as C
 import struct
 from typing import Optional, Sequence
 
-from .abi import Attention_, S2SError, check, last_error, load_library
+from .abi import Attention_, S2SError, SharedAttention_, check, last_error, load_library
 
 F32, F16, BF16, E4M3 = 0, 1, 2, 3
 _NAMES = {"f32": F32, "float32": F32, "f16": F16, "float16": F16, "bf16": BF16, "bfloat16": BF16,
@@ -103,6 +103,7 @@ def _tokens(a, shape, dtype: int, op: str, name: str):
 # The argument structs as one pack each (a call's fields set one by one through
 # ctypes take as long as the call): the C structs' layout, null pointers as 0.
 _ATTENTION = struct.Struct("@8i2f 4q4q4q4q 3P 2P2q 2P2q 2Pi0q")
+_SHARED = struct.Struct(_ATTENTION.format + "i4q4qP")
 _ROTARY = struct.Struct("@10i 4q4q4q4q Pq3P")
 _NORM_ROTARY = struct.Struct(_ROTARY.format + "2P2q2f")
 _RMS = struct.Struct("@2iqi4P4qP2fPi0q")
@@ -194,6 +195,63 @@ class Attention:
         if self.lib.s2s_window_attention(args, *self.window, ws, n, stream) if self.window[0] else self.lib.s2s_attention(args, ws, n, stream):
             raise S2SError(f"{op}: {last_error()}")
         return out
+
+
+class SharedAttention:
+    """A plan of `s2s_shared_attention`: every entry's keys are the shared ones, which lie in
+    memory once, and behind them its own `k_tokens`. Arguments and workspace as
+    `Attention`'s.
+
+        plan = ops.SharedAttention("bf16", batch, 1, shared_tokens, k_tokens, q_heads, k_heads, width, causal=True)
+        plan(q, shared_k, shared_v, k, v, out, workspace=ws, stream=stream, k_lens=lens)
+    """
+
+    def __init__(self, dtype, batch: int, q_tokens: int, shared_tokens: int, k_tokens: int, q_heads: int, k_heads: int,
+                 width: int, scale: Optional[float] = None, cap: float = 0.0, causal: bool = False):
+        sizes = (batch, q_tokens, shared_tokens, k_tokens, q_heads, k_heads, width)
+        _need(all(-2 ** 31 <= n < 2 ** 31 for n in sizes), "shared_attention: a size that is no 32-bit int")
+        self.lib = load_library()
+        self.dtype = _type(dtype)
+        self.head = (self.dtype, batch, q_tokens, k_tokens, q_heads, k_heads, width, int(bool(causal)),
+                     _f32(scale) if scale is not None else max(width, 1) ** -0.5, _f32(cap))
+        self.batch, self.q_heads, self.shared_tokens = batch, q_heads, shared_tokens
+        self.q_shape, self.k_shape = (batch, q_tokens, q_heads, width), (batch, k_tokens, k_heads, width)
+        self.shared_shape = (shared_tokens, k_heads, width)
+        a = SharedAttention_(Attention_(*self.head), shared_tokens)
+        n = C.c_uint64()
+        check(self.lib.s2s_shared_attention_workspace(C.byref(a), C.byref(n)), "shared_attention")
+        self.workspace_bytes = n.value
+
+    def __call__(self, q, shared_k, shared_v, k, v, out, workspace=None, stream: int = 0, shared_lens=None, q_lens=None,
+                 k_lens=None, slopes=None):
+        """out [batch][q_tokens][q_heads][width] from q (the same shape), shared_k and shared_v
+        [shared_tokens][k_heads][width], k and v [batch][k_tokens][k_heads][width]; lengths int32
+        [batch]; slopes f32 [q_heads]."""
+        op, dt, batch = "shared_attention", self.dtype, self.batch
+        arrays = (*_tokens(q, self.q_shape, dt, op, "q"), *_tokens(k, self.k_shape, dt, op, "k"),
+                  *_tokens(v, self.k_shape, dt, op, "v"), *_tokens(out, self.q_shape, dt, op, "out"))
+        slope_ptr = 0
+        if slopes is not None:
+            _need(slopes.shape == (self.q_heads,) and _is_f32(slopes.dtype) and _contiguous(slopes),
+                  f"{op}: slopes is no f32 vector of {self.q_heads}")
+            slope_ptr = slopes.data_ptr()
+        args = _SHARED.pack(*self.head, *arrays, _vector(q_lens, batch, op, "q_lens"), _vector(k_lens, batch, op, "k_lens"),
+                            0, 0, 0, 0, 0, 0, 0, 0, 0, slope_ptr, 0, 0, self.shared_tokens,
+                            *self._shared(shared_k, "shared_k"), *self._shared(shared_v, "shared_v"),
+                            _vector(shared_lens, batch, op, "shared_lens"))
+        ws, n = (None, 0) if workspace is None else (workspace.data_ptr(), _bytes(workspace))
+        if self.lib.s2s_shared_attention(args, ws, n, stream):
+            raise S2SError(f"{op}: {last_error()}")
+        return out
+
+    def _shared(self, a, name: str):
+        """An array [shared_tokens][k_heads][width] as its C struct's fields."""
+        if a.shape != self.shared_shape or _type(a.dtype) != self.dtype:
+            raise S2SError(f"shared_attention: {name} is {tuple(a.shape)} of {a.dtype}, wanted {self.shared_shape} of the call's type")
+        t, h, d = a.stride()
+        if d != 1 and self.shared_shape[2] > 1:
+            raise S2SError(f"shared_attention: the channels of {name} are not adjacent")
+        return a.data_ptr(), 0, t, h
 
 
 _SIZES = {}

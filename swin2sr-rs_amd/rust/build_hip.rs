@@ -22,7 +22,8 @@ fn build_hip() {
     let arch = std::env::var("SWIN2SR_HIP_ARCH").unwrap_or_else(|_| "gfx950".into());
     let srcs = ["s2s_kernels.hip", "s2s_split.hip", "s2s_attention.hip", "s2s_attention_f32.hip",
                 "s2s_attention_f16.hip", "s2s_attention_bf16.hip", "s2s_attention_window_f32.hip",
-                "s2s_attention_window_f16.hip", "s2s_attention_window_bf16.hip", "s2s_ops.hip", "s2s_ops_api.cpp",
+                "s2s_attention_window_f16.hip", "s2s_attention_window_bf16.hip", "s2s_attention_shared_f32.hip",
+                "s2s_attention_shared_f16.hip", "s2s_attention_shared_bf16.hip", "s2s_ops.hip", "s2s_ops_api.cpp",
                 "s2s_api.cpp", "s2s_test_api.cpp", "s2s_selftest.cpp"];
     let status = Command::new(&hipcc)
         .arg(format!("--offload-arch={arch}"))

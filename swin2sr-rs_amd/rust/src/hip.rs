@@ -84,6 +84,16 @@ pub struct S2sAttentionArgs {
     pub table_size: c_int,
 }
 
+/// `s2s_shared_attention_args`: one call of the attention of a batch that shares its first keys.
+#[repr(C)]
+pub struct S2sSharedAttentionArgs {
+    pub own: S2sAttentionArgs,
+    pub shared_tokens: c_int,
+    pub shared_k: S2sTokens,
+    pub shared_v: S2sTokens,
+    pub shared_lens: *const i32,
+}
+
 /// `s2s_rotary_args`: one call of the rotary positions.
 #[repr(C)]
 pub struct S2sRotaryArgs {
@@ -183,6 +193,8 @@ extern "C" {
         bytes: u64,
         stream: *mut c_void,
     ) -> c_int;
+    pub fn s2s_shared_attention_workspace(args: *const S2sSharedAttentionArgs, bytes: *mut u64) -> c_int;
+    pub fn s2s_shared_attention(args: *const S2sSharedAttentionArgs, workspace: *mut c_void, bytes: u64, stream: *mut c_void) -> c_int;
     pub fn s2s_rotary(args: *const S2sRotaryArgs, stream: *mut c_void) -> c_int;
     pub fn s2s_norm_rotary(args: *const S2sNormRotaryArgs, stream: *mut c_void) -> c_int;
     pub fn s2s_rms_norm(args: *const S2sRmsNormArgs, stream: *mut c_void) -> c_int;

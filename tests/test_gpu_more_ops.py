@@ -294,3 +294,166 @@ def test_window_refuses(pkg):
     T.refused(pkg, "workspace", lambda: p(**a, workspace=pkg.ops.Array(ws.buf.ptr, (p.workspace_bytes - 1,), "u8")))
     T.refused(pkg, "out is an input", lambda: p(**{**a, "out": a["q"]}, workspace=ws.array))
     assert np.all(d["out"].get() == 7.5)
+
+
+# ---- attention of a batch that shares its first keys ---------------------------------------
+
+
+def scase(dtype="bf16", S=100, shared_lens=None, shared_order="cache", **more):
+    return dict(T.case(dtype, **more), S=S, shared_lens=shared_lens, shared_order=shared_order)
+
+
+def shared_inputs(c):
+    q, k, v, more = T.inputs(c)
+    g = np.random.default_rng(c["seed"] + 1000)
+    sk, sv = (R.round_to(g.standard_normal((c["S"], c["KV"], c["D"])), c["dtype"]) for _ in range(2))
+    if c["shared_lens"] is not None:
+        more["shared_lens"] = np.array(c["shared_lens"], np.int32)
+    return q, k, v, sk, sv, more
+
+
+def shared_want(c, q, k, v, sk, sv, more, scale):
+    """Entry by entry, the entry's shared keys ahead of its own."""
+    outs = []
+    for b in range(c["B"]):
+        n = int(np.clip(more["shared_lens"][b], 0, c["S"])) if "shared_lens" in more else c["S"]
+        own = int(np.clip(more["k_lens"][b], 0, c["Lk"])) if "k_lens" in more else c["Lk"]
+        kk, vv = (np.concatenate((x[:n], y[b, :own]))[None] for x, y in ((sk, k), (sv, v)))
+        extra = {"q_lens": more["q_lens"][b:b + 1]} if "q_lens" in more else {}
+        if "slopes" in more:
+            extra["slopes"] = more["slopes"].astype(np.float64)
+        outs.append(R.attention(c["dtype"], q[b:b + 1], kk, vv, scale, np.float64(np.float32(c["cap"])), c["causal"], **extra))
+    return [np.concatenate(x) for x in zip(*outs)]
+
+
+def shared_setup(pkg, c, arrays):
+    q, k, v, sk, sv, more = arrays
+    scale = c["D"] ** -0.5 if c["scale"] is None else c["scale"]
+    p = pkg.ops.SharedAttention(c["dtype"], c["B"], c["Lq"], c["S"], c["Lk"], c["H"], c["KV"], c["D"], scale=scale, cap=c["cap"], causal=c["causal"])
+    ws = R.Dev(pkg, np.full(max(p.workspace_bytes // 4, 1), np.nan), "f32")
+    d, m = T.upload(pkg, c, q, k, v, more)
+    order = (1, 0, 2) if c["shared_order"] == "cache" else (0, 1, 2)
+    d["shared_k"], d["shared_v"] = (R.Dev(pkg, x, c["dtype"], order, c["gap"], c["lead"], np.nan) for x in (sk, sv))
+    return p, ws, d, m, np.float64(np.float32(scale))
+
+
+def shared_call(p, ws, d, m, stream=0):
+    p(*(d[n].array for n in ("q", "shared_k", "shared_v", "k", "v", "out")), workspace=ws.array, stream=stream, **{n: x.array for n, x in m.items()})
+
+
+def check_shared(pkg, c, change=None):
+    arrays = shared_inputs(c)
+    if change:
+        change(*arrays)
+    p, ws, d, m, scale = shared_setup(pkg, c, arrays)
+    want, bound, written = shared_want(c, *arrays, scale)
+    # the ranges' weights and their sum: a rescaling and an addition each, f32
+    bound = bound + 8 * 2.0 ** -24 * np.abs(want)
+    shared_call(p, ws, d, m)
+    pkg.hip.synchronize()
+    got = d["out"].get()
+    assert d["out"].gaps_kept()
+    w = written[:, :, None, None] & np.ones(got.shape, bool)
+    assert np.all(got[~w] == 7.5), "rows past the sequence were written"
+    got, want, bound = got[w], want[w], bound[w]
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    fine = np.isfinite(want)
+    worst = (np.abs(got[fine] - want[fine]) / np.maximum(bound[fine], 1e-300)).max(initial=0.0)
+    assert worst <= 1.0, worst
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+
+
+SHARED = {
+    "one": scase(S=1, Lq=1, Lk=1, H=1),
+    "step": scase("bf16", S=900, B=5, Lq=1, Lk=70, H=8, KV=2, D=128, causal=True, k_lens=[70, 1, 33, 64, 0]),
+    "step_many": scase("bf16", S=2000, B=40, Lq=1, Lk=130, H=16, KV=4, D=128, causal=True, k_lens=[1 + 3 * i for i in range(40)]),
+    "step_f16": scase("f16", S=1501, B=16, Lq=1, Lk=20, H=8, KV=8, D=64, causal=True, cap=20.0),
+    "step_f32": scase("f32", S=700, B=16, Lq=1, Lk=20, H=8, KV=2, D=64, causal=True, slopes=True),
+    "step_f32_128": scase("f32", S=300, B=30, Lq=1, Lk=20, H=8, KV=2, D=128, causal=True),
+    "step_few": scase("f16", S=2700, B=2, Lq=1, Lk=500, H=4, KV=2, D=96, causal=True, slopes=True, order="cache"),
+    "step_long_own": scase("bf16", S=64, B=3, Lq=1, Lk=3000, H=8, KV=2, D=128, causal=True, order="cache"),
+    "steps_of_4": scase("bf16", S=800, B=7, Lq=4, Lk=100, H=8, KV=2, D=64, causal=True, k_lens=[100, 4, 50, 2, 0, 99, 7], q_lens=[4, 4, 3, 2, 0, 1, 4]),
+    "parts": scase("bf16", S=500, B=6, Lq=1, Lk=40, H=8, KV=2, D=64, causal=True, shared_lens=[0, 1, 64, 333, 500, 1000]),
+    "parts_none": scase("f16", S=500, B=6, Lq=2, Lk=40, H=2, KV=2, D=64, causal=True, shared_lens=[0, -5, 0, 0, 0, 0]),
+    "parts_f32_slopes": scase("f32", S=500, B=6, Lq=3, Lk=40, H=4, KV=2, D=32, causal=True, slopes=True, shared_lens=[0, 1, 64, 333, 500, 499], k_lens=[40, 3, 2, 0, 1, 30], q_lens=[3, 3, 2, 0, 3, 3]),
+    "nothing": scase("bf16", S=50, B=3, Lq=2, Lk=40, H=2, D=64, causal=True, shared_lens=[0, 0, 50], k_lens=[0, 40, 0]),
+    "more_queries_than_keys": scase("f32", S=20, B=3, Lq=90, Lk=30, H=2, D=32, causal=True, shared_lens=[20, 0, 7], slopes=True),
+    "tail": scase("bf16", S=700, B=4, Lq=130, Lk=130, H=8, KV=2, D=128, causal=True),
+    "tail_f16": scase("f16", S=333, B=3, Lq=257, Lk=257, H=4, KV=4, D=64, causal=True, cap=30.0, k_lens=[257, 100, 31], q_lens=[257, 100, 31]),
+    "tail_f32": scase("f32", S=333, B=3, Lq=100, Lk=150, H=4, KV=2, D=128, causal=True, slopes=True),
+    "all": scase("f32", S=289, B=9, Lq=64, Lk=64, H=6, KV=6, D=30),
+    "all_bf16": scase("bf16", S=400, B=4, Lq=33, Lk=70, H=4, KV=2, D=80, shared_lens=[400, 17, 0, 399]),
+    "no_own": scase("bf16", S=400, B=4, Lq=3, Lk=0, H=4, KV=2, D=64),
+    "no_shared": scase("bf16", S=0, B=4, Lq=3, Lk=90, H=4, KV=2, D=64, causal=True),
+    "odd_address": scase("f16", S=277, B=3, Lq=5, Lk=40, H=4, KV=2, D=64, gap=3, lead=1, causal=True),
+    "rows_of_4_bytes": scase("f16", S=350, B=3, Lq=5, Lk=40, H=2, KV=2, D=62, causal=True),
+    "odd_width": scase("bf16", S=350, B=20, Lq=5, Lk=40, H=2, KV=1, D=17, causal=True, shared_order="packed"),
+    "packed": scase("bf16", S=350, B=20, Lq=2, Lk=40, H=4, KV=2, D=64, causal=True, shared_order="packed", order="cache"),
+    "negative_scale": scase("f32", S=90, B=3, Lq=20, Lk=30, H=2, D=32, scale=-0.3, causal=True),
+    "large_scores": scase("bf16", S=300, B=3, Lq=40, Lk=100, H=2, D=64, spread=30.0, causal=True),
+    "group_33": scase("f16", S=500, B=2, Lq=2, Lk=70, H=33, KV=1, D=32, causal=True),
+    "batch_of_one": scase("bf16", S=500, B=1, Lq=1, Lk=70, H=8, KV=2, D=128, causal=True),
+    "wide": scase("bf16", S=190, B=40, Lq=40, Lk=50, H=12, KV=12, D=128, causal=True),
+    "wide_f32": scase("f32", S=190, B=40, Lq=40, Lk=50, H=12, KV=12, D=64, slopes=True, causal=True),
+    "wide_cap_f16": scase("f16", S=190, B=40, Lq=40, Lk=50, H=12, KV=12, D=96, cap=50.0, spread=4.0),
+}
+
+
+@pytest.mark.parametrize("name", SHARED)
+def test_shared(pkg, name):
+    check_shared(pkg, SHARED[name])
+
+
+SHARED_HIDDEN = {
+    "step": scase("bf16", S=300, B=5, Lq=1, Lk=40, H=8, KV=2, D=128, causal=True, shared_lens=[0, 200, 100, 1, 250]),
+    "steps_f32": scase("f32", S=300, B=5, Lq=3, Lk=40, H=4, KV=2, D=64, causal=True, shared_lens=[0, 200, 100, 1, 250]),
+    "few_f16": scase("f16", S=300, B=2, Lq=1, Lk=40, H=4, KV=2, D=64, causal=True, shared_lens=[0, 200]),
+    "tail": scase("bf16", S=300, B=4, Lq=100, Lk=100, H=4, KV=2, D=64, causal=True, shared_lens=[0, 200, 100, 250]),
+    "all_f32": scase("f32", S=300, B=4, Lq=100, Lk=100, H=4, KV=2, D=100, shared_lens=[0, 200, 100, 250]),
+    "wide_f16": scase("f16", S=300, B=40, Lq=40, Lk=50, H=12, KV=12, D=64, causal=True, shared_lens=[(7 * i) % 260 for i in range(40)]),
+}
+
+
+@pytest.mark.parametrize("name", SHARED_HIDDEN)
+def test_shared_hides_what_keys_hold(pkg, name):
+    """NaN and infinities in shared keys that no entry, or only some, have a part of."""
+    def past(q, k, v, sk, sv, more):
+        sk[260:], sv[260:] = np.nan, np.inf
+        sv[150, 0, 3], sv[151, 1, 5], sk[180, 1, 0] = np.inf, np.nan, np.nan  # seen where the part is longer
+    check_shared(pkg, SHARED_HIDDEN[name], past)
+
+
+def test_shared_is_the_attention_of_whole_keys(pkg):
+    """The same batch with every entry's keys laid out whole, through the attention without sharing."""
+    c = scase("bf16", S=600, B=6, Lq=3, Lk=50, H=8, KV=2, D=64, causal=True)
+    arrays = shared_inputs(c)
+    p, ws, d, m, scale = shared_setup(pkg, c, arrays)
+    shared_call(p, ws, d, m)
+    got = d["out"].get()
+    q, k, v, sk, sv, _ = arrays
+    whole = {n: np.concatenate((np.broadcast_to(s, (6,) + s.shape), x), 1) for n, s, x in (("k", sk, k), ("v", sv, v))}
+    big = T.case("bf16", B=6, Lq=3, Lk=650, H=8, KV=2, D=64, causal=True)
+    plan, ws2, _ = T.make_plan(pkg, big)
+    d2, m2 = T.upload(pkg, big, q, whole["k"], whole["v"], {})
+    T.call(plan, ws2, d2, m2)
+    _, bound, _ = R.attention("bf16", q, whole["k"], whole["v"], scale, causal=True)
+    assert (np.abs(got - d2["out"].get()) <= 2.01 * bound).all()
+
+
+def test_shared_refuses(pkg):
+    c = scase("bf16", S=900, B=5, Lq=1, Lk=70, H=8, KV=2, D=128, causal=True)
+    p, ws, d, m, _ = shared_setup(pkg, c, shared_inputs(c))
+    a = {n: x.array for n, x in d.items()}
+    A = pkg.ops.Array
+    host = np.zeros(64, np.float32)
+    T.refused(pkg, "workspace", lambda: p(**a))
+    T.refused(pkg, "workspace", lambda: p(**a, workspace=A(ws.buf.ptr, (p.workspace_bytes - 1,), "u8")))
+    w = dict(workspace=ws.array)
+    T.refused(pkg, "out is an input", lambda: p(**{**a, "q": a["out"]}, **w))
+    T.refused(pkg, "out is an input", lambda: p(**{**a, "shared_v": A(a["out"].ptr, (900, 2, 128), "bf16")}, **w))
+    T.refused(pkg, "shared_k is null", lambda: p(**{**a, "shared_k": A(0, (900, 2, 128), "bf16")}, **w))
+    T.refused(pkg, "shared_v is not device memory", lambda: p(**{**a, "shared_v": A(host.ctypes.data, (900, 2, 128), "bf16")}, **w))
+    T.refused(pkg, "shared_lens is not device memory", lambda: p(**a, **w, shared_lens=A(host.ctypes.data, (5,), "i32")))
+    T.refused(pkg, "2.22", lambda: p(**{**a, "shared_k": A(a["shared_k"].ptr, (900, 2, 128), "bf16", (1 << 23, 128, 1))}, **w))
+    T.refused(pkg, "stride", lambda: p(**{**a, "shared_k": A(a["shared_k"].ptr, (900, 2, 128), "bf16", (-128, 128, 1))}, **w))
+    assert np.all(d["out"].get() == 7.5)

@@ -96,9 +96,75 @@ def test_window_workspace_goes_by_the_window(pkg):
     assert plan(pkg, window=2 ** 30, **sizes).workspace_bytes == plan(pkg, **sizes).workspace_bytes
 
 
+# ---- attention of a batch that shares its first keys ------------------------------------
+
+
+def shared(pkg, **more):
+    a = dict(dtype="bf16", batch=2, q_tokens=5, shared_tokens=9, k_tokens=7, q_heads=4, k_heads=2, width=64)
+    a.update(more)
+    return pkg.ops.SharedAttention(**a)
+
+
+def shared_tensors(pkg):
+    return dict(tensors(pkg), shared_k=arr(pkg, (9, 2, 64)), shared_v=arr(pkg, (9, 2, 64)))
+
+
+@pytest.mark.parametrize("more,word", [
+    (dict(dtype="f64"), "dtype"), (dict(batch=-1), "negative"), (dict(shared_tokens=-1), "negative shared"), (dict(k_tokens=-1), "negative"),
+    (dict(q_heads=3), "multiple"), (dict(width=129), "width"), (dict(shared_tokens=2 ** 30), "2.30 shared"),
+    (dict(shared_tokens=2 ** 31), "int"), (dict(batch=2 ** 12, q_tokens=2 ** 12 + 1, q_heads=4), "2.26"),
+])
+def test_shared_sizes_refused(pkg, more, word):
+    with pytest.raises(pkg.S2SError, match=word):
+        shared(pkg, **more)
+
+
+@pytest.mark.parametrize("name,bad", [
+    ("q", dict(shape=(2, 5, 4, 63))), ("k", dict(shape=(2, 9, 2, 64))), ("shared_k", dict(shape=(2, 9, 2, 64))),
+    ("shared_k", dict(shape=(8, 2, 64))), ("shared_v", dict(shape=(9, 4, 64))), ("shared_v", dict(shape=(9, 2, 64), dtype="f16")),
+    ("shared_k", dict(shape=(9, 2, 64), strides=(128, 1, 2))), ("out", dict(shape=(2, 5, 4, 64), dtype="f32")),
+])
+def test_shared_arrays_refused(pkg, name, bad):
+    t = shared_tensors(pkg)
+    t[name] = arr(pkg, **bad)
+    with pytest.raises(pkg.S2SError, match=name):
+        shared(pkg)(**t)
+
+
+@pytest.mark.parametrize("extra,word", [
+    (dict(shared_lens=((3,), "i32")), "shared_lens"), (dict(shared_lens=((2,), "f32")), "shared_lens"), (dict(k_lens=((3,), "i32")), "k_lens"),
+    (dict(q_lens=((2, 1), "i32")), "q_lens"), (dict(slopes=((2,), "f32")), "slopes"),
+])
+def test_shared_extras_refused(pkg, extra, word):
+    with pytest.raises(pkg.S2SError, match=word):
+        shared(pkg)(**shared_tensors(pkg), **{n: arr(pkg, *x) for n, x in extra.items()})
+
+
+@pytest.mark.parametrize("more,word", [(dict(scale=float("nan")), "scale"), (dict(scale=2e30), "scale"), (dict(cap=-1.0), "cap"), (dict(cap=1e-9), "cap")])
+def test_shared_numbers_refused(pkg, more, word):
+    with pytest.raises(pkg.S2SError, match=word):
+        shared(pkg, **more)(**shared_tensors(pkg))
+
+
+@pytest.mark.parametrize("name", ["prefix", "q_docs", "k_docs", "q_pos", "k_pos", "table"])
+def test_shared_other_masks_refused(pkg, name):
+    a = pkg.abi.SharedAttention_(pkg.abi.Attention_(2, 2, 5, 7, 4, 2, 64, 1, 1.0, 0.0), 9)
+    setattr(a.own, name, 4096)
+    lib = pkg.load_library()
+    assert lib.s2s_shared_attention(C.addressof(a), None, 0, None) != 0 and b"not taken" in lib.s2s_last_error()
+
+
+def test_shared_nothing_to_do(pkg):
+    for more in (dict(batch=0), dict(q_tokens=0)):
+        b, n = more.get("batch", 2), more.get("q_tokens", 5)
+        s = arr(pkg, (9, 2, 64))
+        shared(pkg, **more)(arr(pkg, (b, n, 4, 64)), s, s, arr(pkg, (b, 7, 2, 64)), arr(pkg, (b, 7, 2, 64)), arr(pkg, (b, n, 4, 64)))
+
+
 # ---- the C interface ------------------------------------------------------------------
 
-STRUCTS = [("S2sNormRotaryArgs", "s2s_norm_rotary_args", "NormRotary_", "_NORM_ROTARY")]
+STRUCTS = [("S2sSharedAttentionArgs", "s2s_shared_attention_args", "SharedAttention_", "_SHARED"),
+           ("S2sNormRotaryArgs", "s2s_norm_rotary_args", "NormRotary_", "_NORM_ROTARY")]
 RUST = {"s2s_rotary_args": "S2sRotaryArgs", "s2s_attention_args": "S2sAttentionArgs", "s2s_tokens": "S2sTokens", "int": "c_int",
         "float": "f32", "int64_t": "i64"}
 
@@ -145,6 +211,8 @@ def test_structs_are_the_headers(pkg, rust, c, py, pack):
 def test_null_arguments_refused(pkg):
     lib = pkg.load_library()
     assert lib.s2s_norm_rotary(None, None) != 0 and b"null" in lib.s2s_last_error()
+    assert lib.s2s_shared_attention_workspace(None, None) != 0 and b"null" in lib.s2s_last_error()
+    assert lib.s2s_shared_attention(None, None, 0, None) != 0 and b"null" in lib.s2s_last_error()
     assert lib.s2s_window_attention_workspace(None, 1, 0, None) != 0 and b"null" in lib.s2s_last_error()
     assert lib.s2s_window_attention(None, 1, 0, None, 0, None) != 0 and b"null" in lib.s2s_last_error()
 
