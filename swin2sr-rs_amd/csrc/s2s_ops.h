@@ -34,7 +34,7 @@ struct AttnOpArgs {
     int own_nk;
 };
 
-struct RotaryArgs {
+struct RotaryArrays {
     int batch, tokens, hq, hk, width, axes, pairs;
     int adjacent;
     const void *q, *k;
@@ -43,16 +43,25 @@ struct RotaryArgs {
     const int *pos;
     long long pos_b;
     const int *lens;
-    unsigned long long freq[128];  // 2^64 turns per position, negated for the inverse
-    unsigned char axis[128];
 };
 
+// The turns of P pairs at most.
+template <int P>
+struct RotaryTurns {
+    unsigned long long freq[P];  // 2^64 turns per position, negated for the inverse
+    unsigned char axis[P];
+};
+
+struct RotaryArgs : RotaryArrays, RotaryTurns<128> {};
+
 // Rotary positions behind a norm of every head.
-struct NormRotaryArgs {
-    RotaryArgs r;
+struct HeadNorm {
     const float *qw, *kw;
     long long qw_head, kw_head;  // the weights' head strides (0: one row for all heads)
     float offset, eps;
+};
+struct NormRotaryArgs : HeadNorm {
+    RotaryArgs r;
 };
 
 struct RmsNormArgs {

@@ -539,152 +539,231 @@ __global__ __launch_bounds__(256) void k_norm_rotary_heads(NormRotaryArgs a) {
     }
 }
 
+// One access of a VecOf at a 32-bit byte offset; past the resource zeros are read and nothing is written.
+template <typename P>
+__device__ __forceinline__ P buf_read(__amdgpu_buffer_rsrc_t r, int off) {
+    if constexpr (sizeof(P) == 16) return __builtin_bit_cast(P, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+    else if constexpr (sizeof(P) == 8) return __builtin_bit_cast(P, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+    else if constexpr (sizeof(P) == 4) return __builtin_bit_cast(P, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+    else return __builtin_bit_cast(P, __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
+}
+template <typename P>
+__device__ __forceinline__ void buf_write(__amdgpu_buffer_rsrc_t r, int off, P x) {
+    if constexpr (sizeof(P) == 16) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x), r, off, 0, 0);
+    else if constexpr (sizeof(P) == 8) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, x), r, off, 0, 0);
+    else if constexpr (sizeof(P) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), r, off, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, x), r, off, 0, 0);
+}
+
+// How k_norm_rotary walks: the tokens of a workgroup, the units of a head, and for q and k the arrays'
+// strides in units of V elements, with what the next batch entry's first token lies further on than
+// the token behind this one's last.
+struct NormRotaryWalk {
+    int tb, per_head;
+    struct Of {
+        int in_t, in_h, in_b, out_t, out_h, out_b;
+        unsigned by_heads;  // ceil(2^32 / heads)
+    } of[2];
+};
+
 // A head in the registers of G lanes (a power of two): lane g holds V pairs, or V channels that are
 // not turned, reads them once, and the squares' sum is made across the lanes. The sines of the
-// workgroup's `tb` tokens are made once, in LDS; a lane keeps its channels' weights while it goes
-// from head to head, neighbouring lanes' heads side by side in memory.
-template <typename T, bool ADJ, int V, int G>
-__global__ __launch_bounds__(256) void k_norm_rotary(NormRotaryArgs a, int tb, int per_head) {
+// workgroup's tokens are made once, in LDS. A wave takes 64 / G heads at a time, side by side in memory,
+// first of q, then of k, so that what differs between the two is in scalar registers; the next heads are
+// read while these are normed and turned. Offsets are 32-bit ones from the workgroup's first token.
+// (The turns as an argument of 64 or 128 pairs: a launch's time goes by its arguments' bytes.)
+template <typename T, bool ADJ, int V, int G, bool EACH, int P>
+__global__ __launch_bounds__(256) void k_norm_rotary(RotaryArrays r, HeadNorm a, NormRotaryWalk w, RotaryTurns<P> x) {
     typedef VecOf<T, V> Part;
-    const RotaryArgs &r = a.r;
+    typedef VecOf<T, 2 * V> Both;
+    constexpr int H = 64 / G, UNIT = V * (int)sizeof(T);  // heads a wave takes at a time
     extern __shared__ float2 turn[];  // [tb][pairs]
-    const int tid = threadIdx.x, heads = r.hq + r.hk, rot = r.pairs / V, g = tid % G;
-    const unsigned tok0 = blockIdx.x * (unsigned)tb, all = (unsigned)r.batch * (unsigned)r.tokens;  // (at most 2^30)
-    const int n_tok = (int)min((unsigned)tb, all - tok0);
+    const int tid = threadIdx.x, lane = tid & 63, g = tid % G, rot = r.pairs / V;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned tok0 = blockIdx.x * (unsigned)w.tb, all = (unsigned)r.batch * (unsigned)r.tokens;  // (at most 2^30)
+    const int n_tok = (int)min((unsigned)w.tb, all - tok0);
+    const int b0 = (int)(tok0 / (unsigned)r.tokens), at0 = (int)(tok0 - (unsigned)b0 * r.tokens);
+    const int cross = r.tokens - at0;  // tokens from here on are the next batch entry's (one at most: tb <= tokens)
     for (int i = tid; i < n_tok * r.pairs; i += 256) {
-        const unsigned t = (unsigned)i / (unsigned)r.pairs, p = i - t * r.pairs, b = (tok0 + t) / (unsigned)r.tokens;
-        const int pos = r.pos[b * r.pos_b + (long long)(tok0 + t - b * r.tokens) * r.axes + r.axis[p]];
-        float2 x;
-        sincos_turns((unsigned long long)(long long)pos * r.freq[p], x.y, x.x);
-        turn[i] = x;
+        const int t = (int)((unsigned)i / (unsigned)r.pairs), p = i - t * r.pairs;
+        const int *pos = r.pos + (t < cross ? b0 * r.pos_b + (long long)(at0 + t) * r.axes : (b0 + 1) * r.pos_b + (long long)(t - cross) * r.axes);
+        float2 c;
+        sincos_turns((unsigned long long)(long long)pos[x.axis[p]] * x.freq[p], c.y, c.x);
+        turn[i] = c;
     }
+    const int len0 = r.lens ? min(r.lens[b0] - at0, n_tok) : n_tok;
+    const int len1 = r.lens && cross < n_tok ? min(r.lens[b0 + 1] + cross, n_tok) : n_tok;
     // this lane's channels: two runs of V (ADJ: one of 2 V), or one of V that is not turned
-    const bool turns = g < rot, there = g < per_head;
-    const int c0 = !there ? 0 : turns ? (ADJ ? 2 * V : V) * g : 2 * r.pairs + (g - rot) * V;
-    const int c1 = turns ? (ADJ ? c0 + V : c0 + r.pairs) : c0;
-    float wt[2][2][V];  // [k][run]
-    auto weights = [&](const float *w, float (*to)[V]) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) to[0][i] = w[c0 + i] + a.offset, to[1][i] = w[c1 + i] + a.offset;
-    };
-    if (!a.qw_head) weights(a.qw, wt[0]);
-    if (!a.kw_head && r.hk) weights(a.kw, wt[1]);
+    const bool turns = g < rot, there = g < w.per_head;
+    const int u0 = !there ? 0 : turns ? (ADJ ? 2 : 1) * g : 2 * rot + (g - rot), u1 = turns ? (ADJ ? u0 + 1 : u0 + rot) : u0;
+    const int c0 = u0 * V, c1 = u1 * V;
+    const float mean = 1.f / (float)r.width;
     __syncthreads();
-    constexpr int STEP = 256 / G;
-    int h = tid / G, t = 0, b = (int)(tok0 / (unsigned)r.tokens), at = (int)(tok0 - (unsigned)b * r.tokens);
-    auto wrap = [&] {
-        while (h >= heads) {
-            h -= heads, ++t;
-            if (++at == r.tokens) at = 0, ++b;
-        }
-    };
-    wrap();
-    // (a wave's lanes all stay to its end: the sums are made across them)
-    for (int left = n_tok * heads - (tid / 64) * (64 / G); left > 0; left -= STEP) {
-        const bool isq = h < r.hq;
-        const int hh = isq ? h : h - r.hq;
-        const bool ok = t < n_tok && there && (!r.lens || at < r.lens[b]);
-        const Strides si = isq ? r.sq : r.sk, so = isq ? r.sqo : r.sko;
-        const T *src = (const T *)(isq ? r.q : r.k) + b * si.b + at * si.t + hh * si.h;
-        T *dst = (T *)(isq ? r.qo : r.ko) + b * so.b + at * so.t + hh * so.h;
-        Part x{}, y{};
-        if (ok) {
-            if (ADJ && turns) {
-                const VecOf<T, 2 * V> z = *(const VecOf<T, 2 * V> *)(src + c0);
-#pragma unroll
-                for (int i = 0; i < V; ++i) x.e[i] = z.e[i], y.e[i] = z.e[V + i];
-            } else {
-                x = *(const Part *)(src + c0);
-                if (turns) y = *(const Part *)(src + c1);
-            }
-        }
-        float u[2][V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) u[0][i] = (float)x.e[i], u[1][i] = (float)y.e[i];
-        auto squares = [&](float f) {
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float p = u[0][i] * f, q = u[1][i] * f;
-                ss = fmaf(p, p, fmaf(q, q, ss));
-            }
-            return lanes_sum<G>(ss);
+    auto walk = [&](const void *src, void *dst, const Strides &ss, const Strides &ds, const float *weight, long long weight_head, int heads,
+                    const NormRotaryWalk::Of &o, int first) {
+        const auto in = buf_rsrc((const T *)src + b0 * ss.b + at0 * ss.t, BUF_MAX_BYTES);
+        const auto out = buf_rsrc((const T *)dst + b0 * ds.b + at0 * ds.t, BUF_MAX_BYTES);
+        const int end = (n_tok * heads + H - 1) / H;
+        struct Item {
+            int t, out;
+            bool ok;
+            Part x, y;
+            Both z;
+            float w[EACH ? 2 : 1][EACH ? V : 1];
         };
-        const float ss = squares(1.f);
-        float inv = 1.0f / sqrtf(ss / (float)r.width + a.eps);
-        if constexpr (!std::is_same<T, half_t>::value) {
+        float wt[2][V];
+        auto weights = [&](const float *p, auto &to) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) to[0][i] = p[c0 + i], to[1][i] = p[c1 + i];
+        };
+        auto read = [&](int n) {
+            Item m;
+            const int item = n * H + lane / G;
+            m.t = heads == 1 ? item : (int)__umulhi((unsigned)item, o.by_heads);
+            const int h = item - __mul24(m.t, heads), next = m.t < cross ? 0 : 1;
+            m.ok = there && m.t < (next ? len1 : len0);
+            const int at = __mul24(m.t, o.in_t) + __mul24(h, o.in_h) + (next ? o.in_b : 0);
+            m.out = __mul24(m.t, o.out_t) + __mul24(h, o.out_h) + (next ? o.out_b : 0);
+            const int i0 = m.ok ? (at + u0) * UNIT : BUF_OOB, i1 = m.ok && turns ? (at + u1) * UNIT : BUF_OOB;
+            if constexpr (ADJ) {
+                // (a lane of channels that are not turned reads V of them)
+                m.z = buf_read<Both>(in, turns ? i0 : BUF_OOB);
+                if (rot < w.per_head) m.x = buf_read<Part>(in, turns ? BUF_OOB : i0);
+            } else {
+                m.x = buf_read<Part>(in, i0);
+                m.y = buf_read<Part>(in, i1);
+            }
+            if constexpr (EACH) weights(weight + (m.ok ? h : 0) * weight_head, m.w);
+            return m;
+        };
+        if (first >= end) return;
+        if constexpr (!EACH) {
+            weights(weight, wt);
+#pragma unroll
+            for (int i = 0; i < V; ++i) wt[0][i] += a.offset, wt[1][i] += a.offset;
+        }
+        Item m = read(first);
+        for (int n = first; n < end; n += 4) {
+            Item later;
+            if (n + 4 < end) later = read(n + 4);
+            float u[2][V];
+            if constexpr (ADJ) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) u[0][i] = (float)m.z.e[i], u[1][i] = (float)m.z.e[V + i];
+                if (rot < w.per_head) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) u[0][i] = turns ? u[0][i] : (float)m.x.e[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) u[0][i] = (float)m.x.e[i], u[1][i] = (float)m.y.e[i];
+            }
+            auto squares = [&](float f) {
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float p = u[0][i] * f, q = u[1][i] * f;
+                    ss = fmaf(p, p, fmaf(q, q, ss));
+                }
+                return lanes_sum<G>(ss);
+            };
+            const float ss = squares(1.f);
+            float inv = __builtin_amdgcn_rsqf(fmaf(ss, mean, a.eps));
             // heads whose squares pass an f32's range, either way (as of a row of the norm)
             const bool far = ss > 0x1p127f, near = ss < 0x1p-100f && a.eps < 0x1p-100f;
             if (__builtin_expect(__any(far || near), 0)) {
                 const float f = far ? 0x1p-80f : near ? 0x1p80f : 1.f;
-                inv = f / sqrtf(squares(f) / (float)r.width + a.eps * f * f);
-            }
-        }
-        if (ok) {
-            float w[2][V];
-            if (isq ? a.qw_head : a.kw_head) weights(isq ? a.qw + hh * a.qw_head : a.kw + hh * a.kw_head, w);
-            else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) w[0][i] = isq ? wt[0][0][i] : wt[1][0][i], w[1][i] = isq ? wt[0][1][i] : wt[1][1][i];
+                inv = f * __builtin_amdgcn_rsqf(fmaf(squares(f), mean, a.eps * f * f));
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i) u[0][i] = u[0][i] * inv * w[0][i], u[1][i] = u[1][i] * inv * w[1][i];
-            if (turns) {
-                const float2 *cs = turn + t * r.pairs + g * V;
-                if (ADJ) {
-                    VecOf<T, 2 * V> z;
+            for (int i = 0; i < V; ++i) {
+                const float w0 = EACH ? m.w[0][EACH ? i : 0] + a.offset : wt[0][i], w1 = EACH ? m.w[EACH ? 1 : 0][EACH ? i : 0] + a.offset : wt[1][i];
+                u[0][i] = u[0][i] * inv * w0, u[1][i] = u[1][i] * inv * w1;
+            }
+            const int o0 = m.ok ? (m.out + u0) * UNIT : BUF_OOB, o1 = m.ok && turns ? (m.out + u1) * UNIT : BUF_OOB;
+            const float2 *cs = turn + (m.ok && turns ? __mul24(m.t, r.pairs) + g * V : 0);
+            if constexpr (ADJ) {
+                Both z;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float p = u[2 * i / V][2 * i % V], q = u[(2 * i + 1) / V][(2 * i + 1) % V];
-                        z.e[2 * i] = (T)fmaf(p, cs[i].x, -q * cs[i].y);
-                        z.e[2 * i + 1] = (T)fmaf(p, cs[i].y, q * cs[i].x);
-                    }
-                    *(VecOf<T, 2 * V> *)(dst + c0) = z;
-                } else {
+                for (int i = 0; i < V; ++i) {
+                    const float p = u[2 * i / V][2 * i % V], q = u[(2 * i + 1) / V][(2 * i + 1) % V];
+                    z.e[2 * i] = (T)fmaf(p, cs[i].x, -q * cs[i].y);
+                    z.e[2 * i + 1] = (T)fmaf(p, cs[i].y, q * cs[i].x);
+                }
+                buf_write(out, turns ? o0 : BUF_OOB, z);
+                if (rot < w.per_head) {
+                    Part x;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        x.e[i] = (T)fmaf(u[0][i], cs[i].x, -u[1][i] * cs[i].y);
-                        y.e[i] = (T)fmaf(u[0][i], cs[i].y, u[1][i] * cs[i].x);
-                    }
-                    *(Part *)(dst + c0) = x;
-                    *(Part *)(dst + c1) = y;
+                    for (int i = 0; i < V; ++i) x.e[i] = (T)u[0][i];
+                    buf_write(out, turns ? BUF_OOB : o0, x);
                 }
             } else {
+                Part x, y;
 #pragma unroll
-                for (int i = 0; i < V; ++i) x.e[i] = (T)u[0][i];
-                *(Part *)(dst + c0) = x;
+                for (int i = 0; i < V; ++i) {
+                    const float c = cs[i].x, s = cs[i].y;
+                    x.e[i] = (T)(turns ? fmaf(u[0][i], c, -u[1][i] * s) : u[0][i]);
+                    y.e[i] = (T)fmaf(u[0][i], s, u[1][i] * c);
+                }
+                buf_write(out, o0, x);
+                buf_write(out, o1, y);
             }
+            m = later;
         }
-        h += STEP;
-        wrap();
-    }
+    };
+    walk(r.q, r.qo, r.sq, r.sqo, a.qw, a.qw_head, r.hq, w.of[0], wave);
+    // (k's turns follow q's from wave to wave)
+    if (r.hk) walk(r.k, r.ko, r.sk, r.sko, a.kw, a.kw_head, r.hk, w.of[1], (wave - (n_tok * r.hq + H - 1) / H) & 3);
 }
 
-template <typename T, bool ADJ, int V, int G>
-hipError_t norm_rotary_launch(const NormRotaryArgs &a, int per_head, hipStream_t st) {
-    const RotaryArgs &r = a.r;
-    const long long all = (long long)r.batch * r.tokens;
-    const int heads = r.hq + r.hk;
-    const long long fill = std::max(1LL, all / (4LL * cu_count()));
-    const int tb = (int)std::max({1LL, std::min({std::max((256LL + heads * G - 1) / (heads * G), (128LL + r.pairs - 1) / r.pairs), fill, 16LL}), all / 0xffffff + 1});
-    return enqueue(k_norm_rotary<T, ADJ, V, G>, dim3((unsigned)((all + tb - 1) / tb)), dim3(256), (size_t)tb * r.pairs * sizeof(float2), st, a,
-                   tb, per_head);
+template <typename T, bool ADJ, int V, int G, int P>
+hipError_t norm_rotary_launch(const NormRotaryArgs &a, const NormRotaryWalk &w, hipStream_t st) {
+    const long long all = (long long)a.r.batch * a.r.tokens;
+    const dim3 grid((unsigned)((all + w.tb - 1) / w.tb));
+    const size_t lds = (size_t)w.tb * a.r.pairs * sizeof(float2);
+    RotaryTurns<P> x;
+    std::copy_n(a.r.freq, P, x.freq);
+    std::copy_n(a.r.axis, P, x.axis);
+    // (where only one of q and k has a row of weights for each head, the other takes its one row for each)
+    if (a.qw_head || a.kw_head) return enqueue(k_norm_rotary<T, ADJ, V, G, true, P>, grid, dim3(256), lds, st, a.r, a, w, x);
+    return enqueue(k_norm_rotary<T, ADJ, V, G, false, P>, grid, dim3(256), lds, st, a.r, a, w, x);
 }
 
 template <typename T, bool ADJ, int V>
-hipError_t norm_rotary_of(const NormRotaryArgs &a, hipStream_t st) {
-    const int per_head = (a.r.width - a.r.pairs) / V;
-    if (per_head <= 4) return norm_rotary_launch<T, ADJ, V, 4>(a, per_head, st);
-    if (per_head <= 8) return norm_rotary_launch<T, ADJ, V, 8>(a, per_head, st);
-    if (per_head <= 16) return norm_rotary_launch<T, ADJ, V, 16>(a, per_head, st);
-    if (per_head <= 32) return norm_rotary_launch<T, ADJ, V, 32>(a, per_head, st);
-    return norm_rotary_launch<T, ADJ, V, 64>(a, per_head, st);
+hipError_t norm_rotary_of(const NormRotaryArgs &a, const NormRotaryWalk &w, hipStream_t st) {
+    if (a.r.pairs > 64) {  // (nine lanes at least)
+        if (w.per_head <= 16) return norm_rotary_launch<T, ADJ, V, 16, 128>(a, w, st);
+        if (w.per_head <= 32) return norm_rotary_launch<T, ADJ, V, 32, 128>(a, w, st);
+        return norm_rotary_launch<T, ADJ, V, 64, 128>(a, w, st);
+    }
+    if (w.per_head <= 4) return norm_rotary_launch<T, ADJ, V, 4, 64>(a, w, st);
+    if (w.per_head <= 8) return norm_rotary_launch<T, ADJ, V, 8, 64>(a, w, st);
+    if (w.per_head <= 16) return norm_rotary_launch<T, ADJ, V, 16, 64>(a, w, st);
+    if (w.per_head <= 32) return norm_rotary_launch<T, ADJ, V, 32, 64>(a, w, st);
+    return norm_rotary_launch<T, ADJ, V, 64, 64>(a, w, st);
+}
+
+// Whether offsets of an array within a workgroup's tokens, and across an entry's end, are 32-bit ones.
+bool norm_rotary_offsets(const Strides &s, int tb, int tokens, int heads, int width, int size, int unit, int &t, int &h, int &b) {
+    const __int128 next = ((__int128)s.b - (__int128)tokens * s.t) * size, most = BUF_MAX_BYTES / 4;
+    if ((__int128)tb * s.t * size > most || (__int128)heads * s.h * size > most || next > most || next < -most || width * size > (1 << 20)) return false;
+    // (factors of 24 bits)
+    if (s.t / unit >= (1 << 23) || s.h / unit >= (1 << 23)) return false;
+    t = (int)(s.t / unit), h = (int)(s.h / unit), b = (int)(next / (unit * size));
+    return true;
 }
 
 template <typename T>
 hipError_t norm_rotary_type(const NormRotaryArgs &a, hipStream_t st) {
     constexpr int size = sizeof(T);
-    const RotaryArgs &r = a.r;
+    NormRotaryArgs c = a;
+    RotaryArgs &r = c.r;
+    // entries of one token without lengths are the tokens of one entry
+    if (r.tokens == 1 && !r.lens && r.pos_b % r.axes == 0 && (r.pos_b == r.axes || r.batch == 1)) {
+        r.tokens = r.batch, r.batch = 1;
+        r.sq.t = r.sq.b, r.sk.t = r.sk.b, r.sqo.t = r.sqo.b, r.sko.t = r.sko.b;
+        r.sq.b = r.sk.b = r.sqo.b = r.sko.b = r.pos_b = 0;
+    }
     int v = std::min(aligned_elements(r.q, r.sq, size), aligned_elements(r.qo, r.sqo, size));
     if (r.hk) v = std::min(v, std::min(aligned_elements(r.k, r.sk, size), aligned_elements(r.ko, r.sko, size)));
     const int most = v;
@@ -692,24 +771,42 @@ hipError_t norm_rotary_type(const NormRotaryArgs &a, hipStream_t st) {
     if (r.adjacent) v /= 2;
     while (v > 1 && (r.pairs % v || (r.width - 2 * r.pairs) % v)) v /= 2;
     // (adjacent pairs of odd addresses, and heads of more than a wave's lanes, element by element)
-    if (most >= (r.adjacent ? 2 : 1) && (r.width - r.pairs) / v <= 64) {
+    NormRotaryWalk w{};
+    bool fits = most >= (r.adjacent ? 2 : 1) && (r.width - r.pairs) / v <= 64;
+    if (fits) {
+        w.per_head = (r.width - r.pairs) / v;
+        const long long all = (long long)r.batch * r.tokens, fill = std::max(1LL, all / (4LL * cu_count()));
+        // tokens of 12 KB in all, fewer where that leaves CUs without work (16384 tokens, 32 + 8 bf16 heads
+        // of 128, 10 KB each: 62.9 us, by two 65.3, by four 68; 2 x 23400, 6 + 6 f32 heads of 30, 1.4 KB each: 37.3
+        // by eight, 73 by one, 39.4 by four and by sixteen)
+        w.tb = (int)std::max(1LL, std::min({12288 / ((long long)(r.hq + r.hk) * r.width * size), fill, (long long)r.tokens}));
+        fits = all / w.tb < (1 << 24) - 1 && w.tb * std::max(r.hq, r.hk) <= (1 << 15);  // (by_heads is exact that far)
+        auto set = [&](int k, const Strides &in, const Strides &out, int heads) {
+            NormRotaryWalk::Of &o = w.of[k];
+            o.by_heads = (unsigned)(((1ULL << 32) + heads - 1) / heads);
+            return norm_rotary_offsets(in, w.tb, r.tokens, heads, r.width, size, v, o.in_t, o.in_h, o.in_b) &&
+                   norm_rotary_offsets(out, w.tb, r.tokens, heads, r.width, size, v, o.out_t, o.out_h, o.out_b);
+        };
+        fits = fits && set(0, r.sq, r.sqo, r.hq) && (!r.hk || set(1, r.sk, r.sko, r.hk));
+    }
+    if (fits) {
         if (r.adjacent) switch (v) {
                 case 4:
-                    if constexpr (size == 2) return norm_rotary_of<T, true, 4>(a, st);
+                    if constexpr (size == 2) return norm_rotary_of<T, true, 4>(c, w, st);
                     break;
-                case 2: return norm_rotary_of<T, true, 2>(a, st);
-                case 1: return norm_rotary_of<T, true, 1>(a, st);
+                case 2: return norm_rotary_of<T, true, 2>(c, w, st);
+                case 1: return norm_rotary_of<T, true, 1>(c, w, st);
             }
         else switch (v) {
                 case 8:
-                    if constexpr (size == 2) return norm_rotary_of<T, false, 8>(a, st);
+                    if constexpr (size == 2) return norm_rotary_of<T, false, 8>(c, w, st);
                     break;
-                case 4: return norm_rotary_of<T, false, 4>(a, st);
-                case 2: return norm_rotary_of<T, false, 2>(a, st);
-                case 1: return norm_rotary_of<T, false, 1>(a, st);
+                case 4: return norm_rotary_of<T, false, 4>(c, w, st);
+                case 2: return norm_rotary_of<T, false, 2>(c, w, st);
+                case 1: return norm_rotary_of<T, false, 1>(c, w, st);
             }
     }
-    const long long items = (long long)r.batch * r.tokens * (r.hq + r.hk);
+    const long long items = (long long)a.r.batch * a.r.tokens * (a.r.hq + a.r.hk);
     return enqueue(k_norm_rotary_heads<T>, dim3((unsigned)std::min((items + 3) / 4, 1LL << 20)), dim3(256), 0, st, a);
 }
 

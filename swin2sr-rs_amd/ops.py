@@ -322,11 +322,11 @@ class Rotary:
             k_arrays = _tokens(k, ks, dt, op, "k"), _tokens(k_out, ks, dt, op, "k_out")
         else:
             _need(k_out is None, f"{op}: k_out without k")
-        ps, pstr = tuple(pos.shape), pos.stride()
-        _need(_is_int32(pos.dtype) and ps in ((shape[1],) + ps[-1:], (shape[0], shape[1]) + ps[-1:]),
-              f"{op}: pos is {ps} of {pos.dtype}, wanted int32 [batch][tokens][axes] or [tokens][axes]")
-        _need((pstr[-1] == 1 or ps[-1] == 1) and (pstr[-2] == ps[-1] or ps[-2] <= 1),
-              f"{op}: the tokens and axes of pos are not adjacent")
+        ps, pstr = pos.shape, pos.stride()
+        if not _is_int32(pos.dtype) or len(ps) not in (2, 3) or ps[:-1] != (shape[:2] if len(ps) == 3 else shape[1:2]):
+            raise S2SError(f"{op}: pos is {tuple(ps)} of {pos.dtype}, wanted int32 [batch][tokens][axes] or [tokens][axes]")
+        if (pstr[-1] != 1 and ps[-1] != 1) or (pstr[-2] != ps[-1] and ps[-2] > 1):
+            raise S2SError(f"{op}: the tokens and axes of pos are not adjacent")
         return (dt, shape[0], shape[1], shape[2], k_heads, shape[3], min(ps[-1], 2 ** 31 - 1), *self.flags, *arrays[0],
                 *k_arrays[0], *arrays[1], *k_arrays[1], pos.data_ptr(), pstr[0] if len(ps) == 3 else 0,
                 _vector(lens, shape[0], op, "lens"), *self.host), q_out, k_out
@@ -370,10 +370,10 @@ class NormRotary(Rotary):
 
 def _head_weight(w, shape, op: str, name: str):
     """f32 [width], or [heads][width] with adjacent channels: address and head stride."""
-    ws = tuple(w.shape)
-    _need(_is_f32(w.dtype) and ws in (tuple(shape[3:]), tuple(shape[2:])) and (w.stride()[-1] == 1 or shape[3] == 1),
-          f"{op}: {name} is {ws} of {w.dtype}, wanted f32 [{shape[3]}] or [{shape[2]}][{shape[3]}] with adjacent channels")
-    return w.data_ptr(), (w.stride()[0] if len(ws) == 2 else 0)
+    ws, st = w.shape, w.stride()
+    if not _is_f32(w.dtype) or (ws != shape[3:] and ws != shape[2:]) or (st[-1] != 1 and shape[3] != 1):
+        raise S2SError(f"{op}: {name} is {tuple(ws)} of {w.dtype}, wanted f32 [{shape[3]}] or [{shape[2]}][{shape[3]}] with adjacent channels")
+    return w.data_ptr(), (st[0] if len(ws) == 2 else 0)
 
 
 def _rows(a, shape, dtype: int, op: str, name: str):
