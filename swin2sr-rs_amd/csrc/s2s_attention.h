@@ -123,7 +123,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = kAttnLog2e;
 
-enum { CAP = 1, SLOPES = 2, ANY = 8, DOCS = 16, GENERAL = 32, WINDOW = 64, SHARED = 128 };
+enum { CAP = 1, SLOPES = 2, ANY = 8, DOCS = 16, GENERAL = 32, WINDOW = 64, SHARED = 128, WHOLE = 256 };
 
 template <typename T>
 struct Type;
@@ -246,7 +246,7 @@ __device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane
 // otherwise take scalar registers through the loop.
 struct AttnParams {
     AttnOpArgs a;
-    AttnLaunch L;
+    AttnLaunch L[2];  // (the second only of a kernel that has two)
 };
 __device__ __forceinline__ const __attribute__((address_space(4))) AttnParams *late_params() {
     auto p = (const __attribute__((address_space(4))) AttnParams *)__builtin_amdgcn_kernarg_segment_ptr();
@@ -351,7 +351,8 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 //  MODE: CAP and SLOPES are known (0 to 3), or asked for in every tile (ANY); documents
 //  (DOCS); or all of that and what AttnScore::general stands for (GENERAL); each with a
 //  sliding window or without (WINDOW); or for the columns of all batch entries over keys that
-//  they share (SHARED: k and v are the shared ones, and the sums go to the ranges' join). Paths that a
+//  they share (SHARED: the sums go to the ranges' join); or over those first, then over the
+//  entry's own (WHOLE). Paths that a
 //  kernel might take and does not cost it registers, spilled around its loop, and copies
 //  where they meet.
 // K and V tiles of TK keys are copied straight into LDS, two buffers each (three and four
@@ -360,12 +361,13 @@ __device__ __forceinline__ bool any_wild(f4v x) { return wild(x[0]) || wild(x[1]
 // (16, or 4 for rows of 4-byte multiples), or 0: through registers, by elements.
 template <typename T, int DP, int NB, bool WK, int ALIGN, int MODE>
 struct Kernel {
-    static constexpr bool WIN = MODE & WINDOW, SHARE = MODE & SHARED;
-    static constexpr int KIND = MODE & ~(WINDOW | SHARED);
+    static constexpr bool WIN = MODE & WINDOW, SHARE = MODE & SHARED, ALL = MODE & WHOLE;
+    static constexpr int KIND = MODE & ~(WINDOW | SHARED | WHOLE);
     static constexpr bool GEN = KIND == GENERAL, DOC = GEN || (KIND & DOCS), KNOWN = KIND < ANY;
     typedef Type<T> Ty;
     typedef typename Ty::V Vec;
     static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr bool RETRY = WK && !F32;
     static constexpr int E = Ty::kElems;
     // keys per tile: 64, so that the barriers and the softmax's steps across lanes come half as often
     // (2048 f32 tokens, 64 wide, 147 us against 160 with 32; windows of 16 x 16, 57 and 73); 32 for f32 rows
@@ -398,27 +400,33 @@ struct Kernel {
     };
 
     // (inlined into the kernel always: late_params has no meaning in a called function)
-    static __device__ __forceinline__ void run(const AttnOpArgs &a, const AttnLaunch &L, char *lds) {
+    // LAUNCH: which of the kernel's launches L is
+    template <int LAUNCH = 0>
+    static __device__ __forceinline__ void run(const AttnOpArgs &a, const AttnLaunch &L, int block, char *lds) {
         const int tid = threadIdx.x, lane = tid & 63, wave = wave_of();
         const int n16 = lane & 15, q = lane >> 4;
         // tile-major, so that with a multiple of 8 (batch, key head) pairs one XCD
         // keeps a pair's keys in its L2, and the tiles with the most keys (the last
         // ones, under the causal mask) start first
-        const int rest = L.by_pairs.of(blockIdx.x), bh = blockIdx.x - rest * (SHARE ? a.hk : a.batch * a.hk);
+        const int rest = L.by_pairs.of(block), bh = block - rest * (SHARE ? a.hk : a.batch * a.hk);
         const int split = L.by_tiles.of(rest), rank = rest - split * L.tiles;
         const int b = SHARE ? 0 : L.by_hk.of(bh), kvh = SHARE ? bh : bh - b * a.hk;
         const int ct = L.order ? L.order[b * L.tiles + rank] : L.tiles - 1 - rank;
         const int ql = SHARE ? a.batch * a.nq : a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
         int kl = !SHARE && a.k_lens ? min(max(a.k_lens[b], 0), a.nk) : a.nk;
+        // the place of the first query among the keys
+        int first = kl - ql;
+        const int own = kl, mine = !ALL ? 0 : a.shared_lens ? min(max(a.shared_lens[b], 0), a.shared_nk) : a.shared_nk;
+        if (ALL) first += mine, kl = mine;
         const int c0 = ct * COLS;
         if (c0 >= ql * a.group) return;  // (the whole workgroup; ql * group <= 2^30)
         const int pre = a.prefix ? a.prefix[b] : 0;
         auto limit = [&](int i) {
-            if (WIN && !a.causal) return min(kl, max(kl - ql + i + a.window, 0));
-            return a.causal ? min(kl, max(max(kl - ql + i + 1, pre), 0)) : kl;
+            if (WIN && !a.causal) return min(kl, max(first + i + a.window, 0));
+            return a.causal ? min(kl, max(max(first + i + 1, pre), 0)) : kl;
         };
         // the first key of a query's window; before it lie only sinks that it reads
-        auto start = [&](int i) { return WIN ? max(kl - ql + i + 1 - a.window, 0) : 0; };
+        auto start = [&](int i) { return WIN ? max(first + i + 1 - a.window, 0) : 0; };
 
         // the columns of this lane
         const int wc0 = WK ? c0 : c0 + wave * 16 * NB;
@@ -434,22 +442,22 @@ struct Kernel {
             if constexpr (SHARE) {
                 // the entry's lengths and the query's place behind its part of the shared keys
                 const int e = ok ? L.by_nq.of(i) : 0, ie = i - e * a.nq;
-                const int n = a.q_lens ? min(max(a.q_lens[e], 0), a.nq) : a.nq, own = a.k_lens ? min(max(a.k_lens[e], 0), a.own_nk) : a.own_nk;
-                const int mine = a.shared_lens ? min(max(a.shared_lens[e], 0), a.nk) : a.nk;
+                const int n = a.q_lens ? min(max(a.q_lens[e], 0), a.nq) : a.nq, own = a.k_lens ? min(max(a.k_lens[e], 0), a.nk) : a.nk;
+                const int mine = a.shared_lens ? min(max(a.shared_lens[e], 0), a.shared_nk) : a.shared_nk;
                 ok = ok && ie < n;
                 at[nb] = mine + own - n + ie;
                 lim[nb] = !ok ? -1 : a.causal ? min(mine, max(at[nb] + 1, 0)) : mine;
                 low[nb] = doc[nb] = tab[nb] = 0;
                 row = (const T *)a.q + e * a.sq.b + (long long)ie * a.sq.t + h * a.sq.h;
             } else {
-            lim[nb] = ok ? limit(i) : 0;
-            low[nb] = ok ? start(i) : 0;
-            // (a column of no document computes what it may, and is zeroed at the end)
-            doc[nb] = 0;
-            if (DOC && a.q_docs && ok) doc[nb] = a.q_docs[b * a.q_docs_b + i];
-            at[nb] = a.q_pos && ok ? a.q_pos[b * a.q_pos_b + i] : kl - ql + i;
-            tab[nb] = ok ? (L.table_lds ? c - i * a.group : h) * a.table_size : 0;
-            row = (const T *)a.q + b * a.sq.b + (long long)(ok ? i : 0) * a.sq.t + h * a.sq.h;
+                lim[nb] = ok ? limit(i) : 0;
+                low[nb] = ok ? start(i) : 0;
+                // (a column of no document computes what it may, and is zeroed at the end)
+                doc[nb] = 0;
+                if (DOC && a.q_docs && ok) doc[nb] = a.q_docs[b * a.q_docs_b + i];
+                at[nb] = a.q_pos && ok ? a.q_pos[b * a.q_pos_b + i] : first + i;
+                tab[nb] = ok ? (L.table_lds ? c - i * a.group : h) * a.table_size : 0;
+                row = (const T *)a.q + b * a.sq.b + (long long)(ok ? i : 0) * a.sq.t + h * a.sq.h;
             }
             slope[nb] = a.slopes && ok ? slope_of(a.slopes[h]) : 0.f;
 #pragma unroll
@@ -463,166 +471,8 @@ struct Kernel {
                 qf[nb][ks] = __builtin_bit_cast(Vec, x);
             }
         }
-        // keys that any column of the workgroup (of the wave) may read, and that all may
-        const int i_last = min(ql - 1, L.by_group.of(c0 + COLS - 1));
-        int wg_max = 0, wg_min = 0;
-        const int w_first = min(ql - 1, L.by_group.of(wc0)), w_last = min(ql - 1, L.by_group.of(wc0 + 16 * NB - 1));
-        const bool w_any = wc0 < ql * a.group;
-        int w_max = 0, w_min = 0, w_at = 0;  // (w_at: the first place among the wave's queries)
-        if constexpr (SHARE) {
-            // the limits in no order: over the wave's columns (those of no query aside), then the workgroup's
-            w_min = w_at = 0x7fffffff;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-                if (lim[nb] >= 0) w_max = max(w_max, lim[nb]), w_min = min(w_min, lim[nb]), w_at = min(w_at, at[nb]);
-#pragma unroll
-            for (int m = 1; m < 16; m *= 2) {
-                w_max = max(w_max, __shfl_xor(w_max, m));
-                w_min = min(w_min, __shfl_xor(w_min, m));
-                w_at = min(w_at, __shfl_xor(w_at, m));
-            }
-            w_max = __builtin_amdgcn_readfirstlane(w_max);
-            w_min = __builtin_amdgcn_readfirstlane(w_min);
-            w_at = __builtin_amdgcn_readfirstlane(w_at);
-            w_at = w_at == 0x7fffffff ? 0 : w_at;
-            if (lane == 0) ((int2 *)lds)[wave] = make_int2(w_max, w_min);
-            __syncthreads();
-            wg_min = 0x7fffffff;
-            for (int w = 0; w < 4; ++w) wg_max = max(wg_max, ((int2 *)lds)[w].x), wg_min = min(wg_min, ((int2 *)lds)[w].y);
-            __syncthreads();
-            wg_max = __builtin_amdgcn_readfirstlane(wg_max);
-            wg_min = __builtin_amdgcn_readfirstlane(wg_min);
-            kl = wg_max;
-        } else {
-            wg_max = limit(i_last), wg_min = limit(L.by_group.of(c0));
-            w_max = w_any ? limit(w_last) : 0, w_min = limit(w_first);
-            w_at = kl - ql + w_first;
-        }
-        // what all columns' windows hold begins here, and what any holds
-        const int wg_from = start(i_last), w_from = start(w_last), w_low = start(w_first);
-        // documents of the workgroup's columns and of the wave's, where key tiles can be passed
-        // over
-        int q_lo = 0, q_hi = 0, w_lo = 0, w_hi = 0;
-        const bool summary = DOC && L.meta;
-        if (summary) {
-            const int4 x = L.col_docs[b * L.tiles + ct];
-            q_lo = x.x, q_hi = x.y;
-            w_lo = 0x7fffffff, w_hi = -1;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-                if (lim[nb] > 0 && doc[nb] >= 0) w_lo = min(w_lo, doc[nb]), w_hi = max(w_hi, doc[nb]);
-#pragma unroll
-            for (int m = 1; m < 16; m *= 2) {
-                w_lo = min(w_lo, __shfl_xor(w_lo, m));
-                w_hi = max(w_hi, __shfl_xor(w_hi, m));
-            }
-            w_lo = __builtin_amdgcn_readfirstlane(w_lo);
-            w_hi = __builtin_amdgcn_readfirstlane(w_hi);
-        }
-        const int nt = q_hi < 0 ? 0 : (wg_max + TK - 1) / TK;
-        // under a window the tiles between the sinks' and its first one are passed over
-        const int t_sinks = WIN ? min((a.sinks + TK - 1) / TK, nt) : 0;
-        const int t_win = WIN ? max(t_sinks, min(start(L.by_group.of(c0)) / TK, nt)) : 0;
-        const int live_tiles = nt - (t_win - t_sinks);
-        const int per = L.splits == 1 ? live_tiles : (live_tiles + L.splits - 1) / L.splits;
-        auto tile_of = [&](int n) { return WIN && n >= t_sinks ? n + (t_win - t_sinks) : n; };
-        const int t_end = min(nt, tile_of((split + 1) * per));
-
-        // the next tile from t on that holds a key some column's document has, and
-        // whether all its keys and the columns are of one document
-        unsigned long long live = 0, whole = 0;
-        int live_at = -64, t_lo = 0, t_hi = 0, t_all = 0;
-        auto next = [&](int t) {
-            if (WIN && t >= t_sinks && t < t_win) t = t_win;
-            if (!summary) return t;
-            while (t < t_end) {
-                if (t >= live_at + 64) {
-                    live_at = t;
-                    const int m = t + lane;
-                    bool l = false, w = false;
-                    if (m < t_end) {
-                        const int4 x = L.meta[(long long)b * L.meta_tiles + m];
-                        t_lo = x.x, t_hi = x.y, t_all = x.z;
-                        l = x.x <= q_hi && x.y >= q_lo;
-                        w = x.z == x.y && q_lo == q_hi && x.y == q_hi;
-                    }
-                    live = __ballot(l);
-                    whole = __ballot(w);
-                }
-                const unsigned long long m = live >> (t - live_at);
-                if (m) {
-                    t += (int)__builtin_ctzll(m);
-                    if (!WIN || t < t_sinks || t >= t_win) return t;
-                    t = t_win;
-                    continue;
-                }
-                t = live_at + 64;
-            }
-            return t_end;
-        };
-
-        // copying a tile: this thread's chunks. With the DMA a row past the keys lies
-        // past the resource, which ends with the last row that is left (token strides are
-        // no smaller than the width on this path), and reads as zeros, as does a
-        // chunk past the width
-        const T *kp = (const T *)a.k + b * a.sk.b + kvh * a.sk.h;
-        const T *vp = (const T *)a.v + b * a.sv.b + kvh * a.sv.h;
-        const int kst = (int)a.sk.t, vst = (int)a.sv.t, kstep = TK * kst, vstep = TK * vst;  // (strides up to 2^22)
-        // a wave's next units are STEP rows on; the permutations repeat every 16
-        constexpr int ROW = CH * SUB, STEP = 256 / ROW, PER = STEP < 16 ? 16 / STEP : 1;
-        int koff[PER], voff[PER];
-#pragma unroll
-        for (int p = 0; ALIGN && p < PER; ++p) {
-            const int i = wave * 64 + lane, r = i / ROW + p * STEP, sl = i % ROW / SUB, sub = i % SUB * (E / SUB);
-            const int kc = (k_slot<CH>(r, sl) & (CH - 1)) * E + sub, vc = (v_slot<CH, F32>(r, sl) & (CH - 1)) * E + sub;
-            koff[p] = kc < a.width ? (r * kst + kc) * (int)sizeof(T) : 0x60000000;
-            voff[p] = vc < a.width ? (r * vst + vc) * (int)sizeof(T) : 0x60000000;
-        }
-        const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(const lds_t *)lds);
         const int *doc_keys = DOC && a.k_docs ? a.k_docs + b * a.k_docs_b : nullptr;
         const int *pos_keys = GEN && a.k_pos ? a.k_pos + b * a.k_pos_b : nullptr;
-        auto stage = [&](int t, int buf) {
-            const int left = min(kl - t * TK, TK);
-            if (DOC && doc_keys && wave == 0)
-                tile_dma<4>(tile_rsrc(doc_keys + t * TK, left * 4), lds0 + kIds + buf * 256, lane * 4);
-            if (GEN && pos_keys && wave == 1)
-                tile_dma<4>(tile_rsrc(pos_keys + t * TK, left * 4), lds0 + kPos + buf * 256, lane * 4);
-            if constexpr (ALIGN > 0) {
-                const v4u kr = tile_rsrc(kp, ((left - 1) * kst + a.width) * (int)sizeof(T)),
-                          vr = tile_rsrc(vp, ((left - 1) * vst + a.width) * (int)sizeof(T));
-                const unsigned to = lds0 + buf * 2 * (unsigned)kTile + wave * 64 * UNIT;
-                int ko[PER], vo[PER];
-#pragma unroll
-                for (int p = 0; p < PER; ++p) {
-                    ko[p] = koff[p], vo[p] = voff[p];
-                    asm volatile("" : "+v"(ko[p]), "+v"(vo[p]));  // (sums formed here, not kept)
-                }
-#pragma unroll
-                for (int n = 0; n < LOADS * SUB; ++n) {
-                    tile_dma<UNIT>(kr, to + n * 256 * UNIT, ko[n % PER] + n / PER * (PER * STEP) * kst * (int)sizeof(T));
-                    tile_dma<UNIT>(vr, to + (unsigned)kTile + n * 256 * UNIT, vo[n % PER] + n / PER * (PER * STEP) * vst * (int)sizeof(T));
-                }
-            } else {
-                v4u x[2][LOADS];
-#pragma unroll
-                for (int n = 0; n < LOADS; ++n) {
-                    const int s = n * 256 + tid, r = s / CH, c = s & (CH - 1);
-                    x[0][n] = x[1][n] = v4u{0, 0, 0, 0};
-                    if (r < left && c * E < a.width) {
-                        x[0][n] = load_chunk<T>(kp + (long long)r * kst, c * E, a.width, L.vec);
-                        x[1][n] = load_chunk<T>(vp + (long long)r * vst, c * E, a.width, L.vec);
-                    }
-                }
-                char *kd = lds + buf * 2 * kTile, *vd = kd + kTile;
-#pragma unroll
-                for (int n = 0; n < LOADS; ++n) {
-                    const int s = n * 256 + tid, r = s / CH, c = s & (CH - 1);
-                    *(v4u *)(kd + k_slot<CH>(r, c) * 16) = x[0][n];
-                    *(v4u *)(vd + v_slot<CH, F32>(r, c) * 16) = x[1][n];
-                }
-            }
-        };
-
         // the sums of the weights: f32 per lane and key, over the lanes at the end; 16-bit types by
         // the matrix cores, of the rounded weights (a product with ones, half the additions' time)
         typedef typename std::conditional<F32, float, f4v>::type Sum;
@@ -650,7 +500,6 @@ struct Kernel {
         u.k_pos = pos_keys;
         u.table = GEN ? a.table : nullptr;
         u.half = a.table_size >> 1;
-        u.kl = kl;
         u.sinks = WIN ? a.sinks : 0;
         u.capped = a.cap > 0.f;
         u.slopes = a.slopes != nullptr;
@@ -663,65 +512,271 @@ struct Kernel {
             for (int i = tid; i < a.group * a.table_size; i += 256)
                 *(__attribute__((address_space(3))) float *)((lds_t *)lds + kTab + 4 * i) = a.table[kvh * a.group * a.table_size + i];
 
-        // A found tile's documents: whether it and the workgroup's columns are of one, whether
-        // the wave's columns have keys in it, and whether those are of one
-        enum { ONE = 1, MINE = 2, SAME = 4 };
-        auto documents = [&](int t) {
-            if (!DOC || !doc_keys) return ONE | MINE | SAME;
-            if (!summary || t >= t_end) return (int)MINE;
-            const int at = t - live_at, lo = __builtin_amdgcn_readlane(t_lo, at), hi = __builtin_amdgcn_readlane(t_hi, at),
-                      all = __builtin_amdgcn_readlane(t_all, at);
-            return ((whole >> at) & 1 ? ONE : 0) | (lo <= w_hi && hi >= w_lo ? MINE : 0) |
-                   (all == hi && w_lo == w_hi && hi == w_hi ? SAME : 0);
-        };
-
-        // the first two tiles set out together; then the next one's buffer is free when the one
-        // before has been computed
-        constexpr int W = 2 * LOADS * SUB;  // copies per thread and tile
-        int t = next(tile_of(split * per)), buf = 0, docs = documents(t);
-        kp += (long long)t * kstep, vp += (long long)t * vstep;
-        if (t < t_end) stage(t, 0);
-        int tn = t < t_end ? next(t + 1) : t_end, docs_n = documents(tn);
-        kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
-        bool ahead = DOC && tn < t_end;
-        if (ahead) stage(tn, 1);
-        while (t < t_end) {
-            if constexpr (ALIGN > 0) {
-                if (ahead) WAIT_VMCNT(W < 63 ? W : 63);
-                else WAIT_VMCNT(0);
-            } else if (DOC) WAIT_VMCNT(0);
-            lds_sync();
-            if (!ahead && tn < t_end) stage(tn, buf ^ 1);
-            ahead = false;
-            const int at_buf = buf * 2 * (int)kTile;
-            const bool inside = !WIN || t * TK >= wg_from || t * TK + TK <= a.sinks;
-            if (!(t * TK + TK <= wg_min && (docs & ONE) && inside) || (GEN && u.table)) {
-                // a masked key's weight is zero, and zero times an infinity is none: with
-                // such values in the V of a tile that not every column reads whole, they are
-                // added by themselves to the columns that do read them, and taken out
-                lds_t *vd = (lds_t *)lds + at_buf + kTile;
-                auto *flag = (__attribute__((address_space(3))) int *)((lds_t *)lds + kFlag);
-                const bool w = __any(any_wild_chunk(vd));
-                if (lane == 0) flag[wave] = w;
-                lds_sync();
-                if (__builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3])) {
-                    wild_products(u, vd, t * TK + (WK ? 16 * wave : 0), lim, low, doc, at, tab, o);
-                    lds_sync();
-                    remove_wild(vd);
-                    lds_sync();
+        // the keys' one part, or the shared ones' and the entry's own. (`careful`: all over again, below)
+        bool careful = false;
+        int shared_tiles = 0;
+#pragma unroll 1
+        for (int part = 0; part < (ALL ? 2 : 1); ++part) {
+            if (ALL) {
+                kl = part ? own : mine, first = (part ? own : mine + own) - ql;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const int i = L.by_group.of(wc0 + nb * 16 + n16);
+                    lim[nb] = i < ql ? limit(i) : 0;
+                    at[nb] = first + i;
                 }
             }
-            const int j0 = t * TK + (WK ? 16 * wave : 0);  // the wave's first key
-            if (j0 < w_max && (docs & MINE) && (!WIN || j0 + 16 * KB > w_low || j0 < a.sinks)) {
-                const bool all = !WIN || j0 >= w_from || j0 + 16 * KB <= a.sinks;
-                const bool full = j0 + 16 * KB <= w_min && all && (docs & SAME) && !(GEN && u.table);
-                tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, j0 + 16 * KB <= w_at + 1, base + kIds + buf * 256 + (WK ? 64 * wave : 0), lim, low, doc, at, slope, tab, qf, o, m, l);
+            if ((ALL && part) || (RETRY && careful)) lds_sync();  // the buffers have been read
+            // keys that any column of the workgroup (of the wave) may read, and that all may
+            const int i_last = min(ql - 1, L.by_group.of(c0 + COLS - 1));
+            int wg_max = 0, wg_min = 0;
+            const int w_first = min(ql - 1, L.by_group.of(wc0)), w_last = min(ql - 1, L.by_group.of(wc0 + 16 * NB - 1));
+            const bool w_any = wc0 < ql * a.group;
+            int w_max = 0, w_min = 0, w_at = 0;  // (w_at: the first place among the wave's queries)
+            if constexpr (SHARE) {
+                // the limits in no order: over the wave's columns (those of no query aside), then the workgroup's
+                w_min = w_at = 0x7fffffff;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                    if (lim[nb] >= 0) w_max = max(w_max, lim[nb]), w_min = min(w_min, lim[nb]), w_at = min(w_at, at[nb]);
+#pragma unroll
+                for (int m = 1; m < 16; m *= 2) {
+                    w_max = max(w_max, __shfl_xor(w_max, m));
+                    w_min = min(w_min, __shfl_xor(w_min, m));
+                    w_at = min(w_at, __shfl_xor(w_at, m));
+                }
+                w_max = __builtin_amdgcn_readfirstlane(w_max);
+                w_min = __builtin_amdgcn_readfirstlane(w_min);
+                w_at = __builtin_amdgcn_readfirstlane(w_at);
+                w_at = w_at == 0x7fffffff ? 0 : w_at;
+                if (lane == 0) ((int2 *)lds)[wave] = make_int2(w_max, w_min);
+                __syncthreads();
+                wg_min = 0x7fffffff;
+                for (int w = 0; w < 4; ++w) wg_max = max(wg_max, ((int2 *)lds)[w].x), wg_min = min(wg_min, ((int2 *)lds)[w].y);
+                __syncthreads();
+                wg_max = __builtin_amdgcn_readfirstlane(wg_max);
+                wg_min = __builtin_amdgcn_readfirstlane(wg_min);
+                kl = wg_max;
+            } else {
+                wg_max = limit(i_last), wg_min = limit(L.by_group.of(c0));
+                w_max = w_any ? limit(w_last) : 0, w_min = limit(w_first);
+                w_at = first + w_first;
             }
-            t = tn, docs = docs_n;
-            buf ^= 1;
-            if (t < t_end) {
-                tn = next(t + 1), docs_n = documents(tn);
-                kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
+            u.kl = kl;
+            // what all columns' windows hold begins here, and what any holds
+            const int wg_from = start(i_last), w_from = start(w_last), w_low = start(w_first);
+            // documents of the workgroup's columns and of the wave's, where key tiles can be passed
+            // over
+            int q_lo = 0, q_hi = 0, w_lo = 0, w_hi = 0;
+            const bool summary = DOC && L.meta;
+            if (summary) {
+                const int4 x = L.col_docs[b * L.tiles + ct];
+                q_lo = x.x, q_hi = x.y;
+                w_lo = 0x7fffffff, w_hi = -1;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                    if (lim[nb] > 0 && doc[nb] >= 0) w_lo = min(w_lo, doc[nb]), w_hi = max(w_hi, doc[nb]);
+#pragma unroll
+                for (int m = 1; m < 16; m *= 2) {
+                    w_lo = min(w_lo, __shfl_xor(w_lo, m));
+                    w_hi = max(w_hi, __shfl_xor(w_hi, m));
+                }
+                w_lo = __builtin_amdgcn_readfirstlane(w_lo);
+                w_hi = __builtin_amdgcn_readfirstlane(w_hi);
+            }
+            const int nt = q_hi < 0 ? 0 : (wg_max + TK - 1) / TK;
+            // under a window the tiles between the sinks' and its first one are passed over
+            const int t_sinks = WIN ? min((a.sinks + TK - 1) / TK, nt) : 0;
+            const int t_win = WIN ? max(t_sinks, min(start(L.by_group.of(c0)) / TK, nt)) : 0;
+            const int live_tiles = nt - (t_win - t_sinks);
+            // (of both parts: the own keys' tiles are counted behind the shared ones')
+            const int ahead_tiles = ALL && part ? shared_tiles : 0;
+            if (ALL && part == 0) shared_tiles = nt;
+            const int all_tiles = ALL ? shared_tiles + (own + TK - 1) / TK : live_tiles;
+            const int per = L.splits == 1 ? all_tiles : (all_tiles + L.splits - 1) / L.splits;
+            auto tile_of = [&](int n) { return WIN && n >= t_sinks ? n + (t_win - t_sinks) : n; };
+            const int t_end = min(nt, tile_of((split + 1) * per) - ahead_tiles), t_begin = max(tile_of(split * per) - ahead_tiles, 0);
+
+            // the next tile from t on that holds a key some column's document has, and
+            // whether all its keys and the columns are of one document
+            unsigned long long live = 0, whole = 0;
+            int live_at = -64, t_lo = 0, t_hi = 0, t_all = 0;
+            auto next = [&](int t) {
+                if (WIN && t >= t_sinks && t < t_win) t = t_win;
+                if (!summary) return t;
+                while (t < t_end) {
+                    if (t >= live_at + 64) {
+                        live_at = t;
+                        const int m = t + lane;
+                        bool l = false, w = false;
+                        if (m < t_end) {
+                            const int4 x = L.meta[(long long)b * L.meta_tiles + m];
+                            t_lo = x.x, t_hi = x.y, t_all = x.z;
+                            l = x.x <= q_hi && x.y >= q_lo;
+                            w = x.z == x.y && q_lo == q_hi && x.y == q_hi;
+                        }
+                        live = __ballot(l);
+                        whole = __ballot(w);
+                    }
+                    const unsigned long long m = live >> (t - live_at);
+                    if (m) {
+                        t += (int)__builtin_ctzll(m);
+                        if (!WIN || t < t_sinks || t >= t_win) return t;
+                        t = t_win;
+                        continue;
+                    }
+                    t = live_at + 64;
+                }
+                return t_end;
+            };
+
+            // copying a tile: this thread's chunks. With the DMA a row past the keys lies
+            // past the resource, which ends with the last row that is left (token strides are
+            // no smaller than the width on this path), and reads as zeros, as does a
+            // chunk past the width
+            const bool shared_part = SHARE || (ALL && part == 0);
+            const T *kp = shared_part ? (const T *)a.shared_k + kvh * a.shared_sk.h : (const T *)a.k + b * a.sk.b + kvh * a.sk.h;
+            const T *vp = shared_part ? (const T *)a.shared_v + kvh * a.shared_sv.h : (const T *)a.v + b * a.sv.b + kvh * a.sv.h;
+            const int kst = (int)(shared_part ? a.shared_sk.t : a.sk.t), vst = (int)(shared_part ? a.shared_sv.t : a.sv.t), kstep = TK * kst, vstep = TK * vst;  // (strides up to 2^22)
+            // a wave's next units are STEP rows on; the permutations repeat every 16
+            constexpr int ROW = CH * SUB, STEP = 256 / ROW, PER = STEP < 16 ? 16 / STEP : 1;
+            int koff[PER], voff[PER];
+#pragma unroll
+            for (int p = 0; ALIGN && p < PER; ++p) {
+                const int i = wave * 64 + lane, r = i / ROW + p * STEP, sl = i % ROW / SUB, sub = i % SUB * (E / SUB);
+                const int kc = (k_slot<CH>(r, sl) & (CH - 1)) * E + sub, vc = (v_slot<CH, F32>(r, sl) & (CH - 1)) * E + sub;
+                koff[p] = kc < a.width ? (r * kst + kc) * (int)sizeof(T) : 0x60000000;
+                voff[p] = vc < a.width ? (r * vst + vc) * (int)sizeof(T) : 0x60000000;
+            }
+            const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(const lds_t *)lds);
+            auto stage = [&](int t, int buf) {
+                const int left = min(kl - t * TK, TK);
+                if (DOC && doc_keys && wave == 0)
+                    tile_dma<4>(tile_rsrc(doc_keys + t * TK, left * 4), lds0 + kIds + buf * 256, lane * 4);
+                if (GEN && pos_keys && wave == 1)
+                    tile_dma<4>(tile_rsrc(pos_keys + t * TK, left * 4), lds0 + kPos + buf * 256, lane * 4);
+                if constexpr (ALIGN > 0) {
+                    v4u kr = tile_rsrc(kp, ((left - 1) * kst + a.width) * (int)sizeof(T)),
+                              vr = tile_rsrc(vp, ((left - 1) * vst + a.width) * (int)sizeof(T));
+                    unsigned to = lds0 + buf * 2 * (unsigned)kTile + wave * 64 * UNIT;
+                    if constexpr (ALL) {  // (uniform over the two parts too, which the compiler does not see)
+#pragma unroll
+                        for (int i = 0; i < 3; ++i) kr[i] = __builtin_amdgcn_readfirstlane(kr[i]), vr[i] = __builtin_amdgcn_readfirstlane(vr[i]);
+                        to = __builtin_amdgcn_readfirstlane(to);
+                    }
+                    int ko[PER], vo[PER];
+#pragma unroll
+                    for (int p = 0; p < PER; ++p) {
+                        ko[p] = koff[p], vo[p] = voff[p];
+                        asm volatile("" : "+v"(ko[p]), "+v"(vo[p]));  // (sums formed here, not kept)
+                    }
+#pragma unroll
+                    for (int n = 0; n < LOADS * SUB; ++n) {
+                        tile_dma<UNIT>(kr, to + n * 256 * UNIT, ko[n % PER] + n / PER * (PER * STEP) * kst * (int)sizeof(T));
+                        tile_dma<UNIT>(vr, to + (unsigned)kTile + n * 256 * UNIT, vo[n % PER] + n / PER * (PER * STEP) * vst * (int)sizeof(T));
+                    }
+                } else {
+                    v4u x[2][LOADS];
+#pragma unroll
+                    for (int n = 0; n < LOADS; ++n) {
+                        const int s = n * 256 + tid, r = s / CH, c = s & (CH - 1);
+                        x[0][n] = x[1][n] = v4u{0, 0, 0, 0};
+                        if (r < left && c * E < a.width) {
+                            x[0][n] = load_chunk<T>(kp + (long long)r * kst, c * E, a.width, L.vec);
+                            x[1][n] = load_chunk<T>(vp + (long long)r * vst, c * E, a.width, L.vec);
+                        }
+                    }
+                    char *kd = lds + buf * 2 * kTile, *vd = kd + kTile;
+#pragma unroll
+                    for (int n = 0; n < LOADS; ++n) {
+                        const int s = n * 256 + tid, r = s / CH, c = s & (CH - 1);
+                        *(v4u *)(kd + k_slot<CH>(r, c) * 16) = x[0][n];
+                        *(v4u *)(vd + v_slot<CH, F32>(r, c) * 16) = x[1][n];
+                    }
+                }
+            };
+
+            // A found tile's documents: whether it and the workgroup's columns are of one, whether
+            // the wave's columns have keys in it, and whether those are of one
+            enum { ONE = 1, MINE = 2, SAME = 4 };
+            auto documents = [&](int t) {
+                if (!DOC || !doc_keys) return ONE | MINE | SAME;
+                if (!summary || t >= t_end) return (int)MINE;
+                const int at = t - live_at, lo = __builtin_amdgcn_readlane(t_lo, at), hi = __builtin_amdgcn_readlane(t_hi, at),
+                          all = __builtin_amdgcn_readlane(t_all, at);
+                return ((whole >> at) & 1 ? ONE : 0) | (lo <= w_hi && hi >= w_lo ? MINE : 0) |
+                       (all == hi && w_lo == w_hi && hi == w_hi ? SAME : 0);
+            };
+
+            // the first two tiles set out together; then the next one's buffer is free when the one
+            // before has been computed
+            constexpr int W = 2 * LOADS * SUB;  // copies per thread and tile
+            int t = next(t_begin), buf = 0, docs = documents(t);
+            kp += (long long)t * kstep, vp += (long long)t * vstep;
+            if (t < t_end) stage(t, 0);
+            int tn = t < t_end ? next(t + 1) : t_end, docs_n = documents(tn);
+            kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
+            bool ahead = DOC && tn < t_end;
+            if (ahead) stage(tn, 1);
+            while (t < t_end) {
+                if constexpr (ALIGN > 0) {
+                    if (ahead) WAIT_VMCNT(W < 63 ? W : 63);
+                    else WAIT_VMCNT(0);
+                } else if (DOC) WAIT_VMCNT(0);
+                lds_sync();
+                if (!ahead && tn < t_end) stage(tn, buf ^ 1);
+                ahead = false;
+                const int at_buf = buf * 2 * (int)kTile;
+                const bool inside = !WIN || t * TK >= wg_from || t * TK + TK <= a.sinks;
+                if ((RETRY && careful) || !(t * TK + TK <= wg_min && (docs & ONE) && inside) || (GEN && u.table)) {
+                    // a masked key's weight is zero, and zero times an infinity is none: with
+                    // such values in the V of a tile that not every column reads whole, they are
+                    // added by themselves to the columns that do read them, and taken out
+                    lds_t *vd = (lds_t *)lds + at_buf + kTile;
+                    auto *flag = (__attribute__((address_space(3))) int *)((lds_t *)lds + kFlag);
+                    const bool w = __any(any_wild_chunk(vd));
+                    if (lane == 0) flag[wave] = w;
+                    lds_sync();
+                    if (__builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3])) {
+                        wild_products(u, vd, t * TK + (WK ? 16 * wave : 0), lim, low, doc, at, tab, o);
+                        lds_sync();
+                        remove_wild(vd);
+                        lds_sync();
+                    }
+                }
+                const int j0 = t * TK + (WK ? 16 * wave : 0);  // the wave's first key
+                if (j0 < w_max && (docs & MINE) && (!WIN || j0 + 16 * KB > w_low || j0 < a.sinks)) {
+                    const bool all = !WIN || j0 >= w_from || j0 + 16 * KB <= a.sinks;
+                    const bool full = j0 + 16 * KB <= w_min && all && (docs & SAME) && !(GEN && u.table);
+                    tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, j0 + 16 * KB <= w_at + 1, base + kIds + buf * 256 + (WK ? 64 * wave : 0), lim, low, doc, at, slope, tab, qf, o, m, l);
+                }
+                t = tn, docs = docs_n;
+                buf ^= 1;
+                if (t < t_end) {
+                    tn = next(t + 1), docs_n = documents(tn);
+                    kp += (long long)(tn - t) * kstep, vp += (long long)(tn - t) * vstep;
+                }
+            }
+            // What the rounding of a weight left may be zero, and zero times an infinity is none: a sum that is
+            // no number of weights that are is made again, with the infinities of v by themselves.
+            if (RETRY && !careful && part == (ALL ? 1 : 0)) {
+                bool none = false;
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) none |= o[db][0][i] != o[db][0][i];
+                auto *flag = (__attribute__((address_space(3))) int *)((lds_t *)lds + kFlag);
+                lds_sync();
+                if (lane == 0) flag[wave] = 0;
+                if (__any(none && total_of(l[0]) == total_of(l[0])) && lane == 0) flag[wave] = 1;
+                lds_sync();
+                if (__builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3])) {
+                    careful = true;
+                    part = -1;
+                    m[0] = -INFINITY, l[0] = Sum{};
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) o[db][0] = f4v{0.f, 0.f, 0.f, 0.f};
+                }
             }
         }
 
@@ -774,14 +829,15 @@ struct Kernel {
         }
         // out, or the sums of this key range
         const auto *late = late_params();
-        const int group = late->a.group, splits = late->L.splits, width = late->a.width, vec = late->L.out_vec;
+        const auto *launch = &late->L[LAUNCH];
+        const int group = late->a.group, splits = launch->splits, width = late->a.width, vec = launch->out_vec;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const int c = wc0 + nb * 16 + n16, i = (int)((__umulhi((unsigned)c, late->L.by_group.m) + (unsigned)c) >> late->L.by_group.s);
+            const int c = wc0 + nb * 16 + n16, i = (int)((__umulhi((unsigned)c, launch->by_group.m) + (unsigned)c) >> launch->by_group.s);
             if (SHARE ? lim[nb] < 0 : i >= ql) continue;
-            if (SHARE || late->L.part_o) {
-                const long long row = ((long long)bh * splits + split) * late->L.cols + c;
-                float *po = late->L.part_o + row * DP, *ml = late->L.part_ml + 2 * row;
+            if (SHARE || launch->part_o) {
+                const long long row = ((long long)bh * splits + split) * launch->cols + c;
+                float *po = launch->part_o + row * DP, *ml = launch->part_ml + 2 * row;
                 if (q == 0 && (!WK || wave == 0)) ml[0] = m[nb], ml[1] = total[nb];
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
@@ -798,6 +854,9 @@ struct Kernel {
             }
         }
     }
+
+    static __device__ __forceinline__ float total_of(float l) { return l; }
+    static __device__ __forceinline__ float total_of(const f4v &l) { return l[0]; }
 
     // V^T's operand for channel block db (vl: the lane's address for it): the keys of
     // blocks 2 j and 2 j + 1 (f32: of block j, one key per lane group and register). With
@@ -1133,7 +1192,16 @@ template <typename T, int DP, int NB, bool WK, int ALIGN, int MODE>
 __global__ __launch_bounds__(256, 2) void k_attn(AttnOpArgs a, AttnLaunch L) {
     static_assert(sizeof(AttnOpArgs) % 8 == 0 && alignof(AttnLaunch) == 8, "late_params reads the two as one struct");
     extern __shared__ __align__(16) char lds[];
-    Kernel<T, DP, NB, WK, ALIGN, MODE>::run(a, L, lds);
+    Kernel<T, DP, NB, WK, ALIGN, MODE>::run(a, L, blockIdx.x, lds);
+}
+
+// The columns of all entries over the shared keys, `shared` workgroups, and each entry's few columns over its own keys
+// in one launch: the first are bound by instructions, the second by HBM, and a CU takes both.
+template <typename T, int DP, int NB, bool WK, int ALIGN>
+__global__ __launch_bounds__(256, 2) void k_attn_both(AttnOpArgs a, AttnLaunch own, AttnLaunch shared, int blocks) {
+    extern __shared__ __align__(16) char lds[];
+    if ((int)blockIdx.x < blocks) Kernel<T, DP, NB, WK, ALIGN, ANY | SHARED>::template run<1>(a, shared, blockIdx.x, lds);
+    else Kernel<T, DP, 1, true, ALIGN, ANY>::run(a, own, blockIdx.x - blocks, lds);
 }
 
 // The key ranges' sums of one column: a workgroup each, its threads over the ranges
@@ -1265,6 +1333,53 @@ __global__ __launch_bounds__(256) void k_attn_join_few(AttnOpArgs a, AttnLaunch 
     store((T *)a.out + b * a.so.b + (long long)i * a.so.t + h * a.so.h, d, a.width, L.out_vec, o * r);
 }
 
+// The same for up to kSomeRanges ranges, eight at a time, their weights first.
+constexpr int kSomeRanges = 32;
+template <typename T, int DP, bool SHARE>
+__global__ __launch_bounds__(256) void k_attn_join_some(AttnOpArgs a, AttnLaunch L, int rows) {
+    constexpr int R = DP / 4, N = 256 / R, W = 8;
+    const int tid = threadIdx.x, slot = tid / R, lane = tid % R, id = blockIdx.x * N + slot;
+    __shared__ float weight[N][kSomeRanges], total[N][kSomeRanges];
+    const bool there = tid < N * R && id < rows;
+    const int bh = there ? id / L.cols : 0, c = id - bh * L.cols, b = L.by_hk.of(bh), kvh = bh - b * a.hk;
+    const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.nq) : a.nq;
+    const int i = there ? L.by_group.of(c) : 0;
+    const bool ok = there && i < ql;
+    const Ranges<SHARE> at(a, L, b, kvh, there ? c : 0);
+    const int count = at.count();
+    f4v x[W];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) x[k] = ok && s0 + k < count ? *(const f4v *)(at.template o<DP>(s0 + k) + lane * 4) : f4v{0.f, 0.f, 0.f, 0.f};
+    };
+    if (ok)
+        for (int s = lane; s < count; s += R) {
+            const float *ml = at.ml(s);
+            weight[slot][s] = ml[0], total[slot][s] = ml[1];
+        }
+    load(0);
+    __syncthreads();
+    if (!ok) return;
+    float top = -INFINITY, ls = 0.f;
+    for (int s = 0; s < count; ++s) top = fmaxf(top, weight[slot][s]);
+    f4v o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < count; s0 += W) {
+        if (s0) load(s0);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            if (s0 + k >= count) break;
+            // a range without keys has weight zero; one whose sum is NaN passes it on
+            const float m = weight[slot][s0 + k], l = total[slot][s0 + k];
+            const float f = l == 0.f ? 0.f : (m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top));
+            ls += l == 0.f ? 0.f : f * l;
+            if (f != 0.f) o += x[k] * f;
+        }
+    }
+    const int h = kvh * a.group + (c - i * a.group);
+    const float r = ls == 0.f ? 0.f : 1.f / ls;
+    store((T *)a.out + b * a.so.b + (long long)i * a.so.t + h * a.so.h, lane * 4, a.width, L.out_vec, o * r);
+}
+
 // How a call is cut.
 struct Cut {
     int dp, nb, tk;
@@ -1279,7 +1394,7 @@ hipError_t launch(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
     AttnLaunch M = L;
     M.table_lds = a.table && (long long)a.group * a.table_size <= K::kTabEntries;
     const size_t lds = K::kTab + (M.table_lds ? (size_t)a.group * a.table_size * 4 : 0);
-    const long long blocks = (long long)((MODE & SHARED) ? 1 : a.batch) * a.hk * L.tiles * L.splits;  // (below 2^24 by the entry's checks)
+    const long long blocks = (long long)a.batch * a.hk * L.tiles * L.splits;  // (below 2^24 by the entry's checks)
     return enqueue(k_attn<T, DP, NB, WK, ALIGN, MODE>, dim3((unsigned)blocks), dim3(256), lds, st, a, M);
 }
 
@@ -1288,9 +1403,11 @@ hipError_t launch(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
 template <typename T, int DP, bool WK, int W>
 hipError_t launch_narrow(const AttnOpArgs &a, const AttnLaunch &L, int align, hipStream_t st) {
     if (align == 0) return launch<T, DP, 1, WK, 0, GENERAL | W>(a, L, st);
+    if constexpr (W != 0)
+        if (align < 16 && !L.score.general && !a.k_docs) return launch<T, DP, 1, WK, 4, ANY | W>(a, L, st);
     if (align < 16) return launch<T, DP, 1, WK, 4, GENERAL | W>(a, L, st);
     if (L.score.general) return launch<T, DP, 1, WK, 16, GENERAL | W>(a, L, st);
-    if constexpr (W != SHARED)
+    if constexpr (W == 0 || W == WINDOW)
         if (a.k_docs) return launch<T, DP, 1, WK, 16, ANY | DOCS | W>(a, L, st);
     return launch<T, DP, 1, WK, 16, ANY | W>(a, L, st);
 }
@@ -1304,43 +1421,29 @@ hipError_t join(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
     constexpr int N = 256 / (DP / 4);
     if (L.splits + (SHARE ? L.shared_splits : 0) <= kFewRanges && rows >= 4 * cu_count())
         return enqueue(k_attn_join_few<T, DP, SHARE>, dim3((unsigned)((rows + N - 1) / N)), dim3(256), 0, st, a, L, (int)rows);
+    // up to 32 ranges: 2048 columns of 17 ranges (64 steps over 16384 shared keys) 5.9 us, 8.0 by a workgroup a column
+    if constexpr (SHARE)
+        if (L.splits + L.shared_splits <= kSomeRanges && rows >= 4 * cu_count())
+            return enqueue(k_attn_join_some<T, DP, SHARE>, dim3((unsigned)((rows + N - 1) / N)), dim3(256), 0, st, a, L, (int)rows);
     return enqueue(k_attn_join<T, DP, SHARE>, dim3((unsigned)rows), dim3(256), 0, st, a, L);
 }
 
 template <typename T, int DP, int W>
 hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, int align, hipStream_t st) {
-    hipError_t e;
+    hipError_t e = hipErrorInvalidValue;
     if (c.wk)
         e = launch_narrow<T, DP, true, W>(a, L, align, st);
     else if (c.nb == 1)
         e = launch_narrow<T, DP, false, W>(a, L, align, st);
-    else if (a.k_docs)
-        e = launch<T, DP, 2, false, 16, ANY | DOCS | W>(a, L, st);
+    else if (W != 0 && align < 16)
+        e = launch<T, DP, 2, false, W != 0 ? 4 : 16, ANY | W>(a, L, st);
+    else if (W != WHOLE && a.k_docs)
+        e = launch<T, DP, 2, false, 16, W != WHOLE ? ANY | DOCS | W : W>(a, L, st);
     else if (a.cap > 0.f)
         e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES | W>(a, L, st) : launch<T, DP, 2, false, 16, CAP | W>(a, L, st);
     else
         e = a.slopes ? launch<T, DP, 2, false, 16, SLOPES | W>(a, L, st) : launch<T, DP, 2, false, 16, W>(a, L, st);
     return e != hipSuccess || !L.join ? e : join<T, DP>(a, L, st);
-}
-
-// The columns of all entries over the shared keys (`s`, cut by `c`); then each entry's own keys' sums
-// are there already, and all are joined by `own`.
-template <typename T, int DP>
-hipError_t launch_shared_width(const AttnOpArgs &s, const AttnLaunch &L, const Cut &c, int align, const AttnOpArgs &own, const AttnLaunch &J, hipStream_t st) {
-    hipError_t e;
-    if (c.nb == 2) e = launch<T, DP, 2, false, 16, ANY | SHARED>(s, L, st);
-    else e = c.wk ? launch_narrow<T, DP, true, SHARED>(s, L, align, st) : launch_narrow<T, DP, false, SHARED>(s, L, align, st);
-    return e != hipSuccess ? e : join<T, DP, true>(own, J, st);
-}
-
-template <typename T>
-hipError_t launch_shared_type(const AttnOpArgs &s, const AttnLaunch &L, const Cut &c, int align, const AttnOpArgs &own, const AttnLaunch &J, hipStream_t st) {
-    switch (c.dp) {
-        case 32: return launch_shared_width<T, 32>(s, L, c, align, own, J, st);
-        case 64: return launch_shared_width<T, 64>(s, L, c, align, own, J, st);
-        case 96: return launch_shared_width<T, 96>(s, L, c, align, own, J, st);
-        default: return launch_shared_width<T, 128>(s, L, c, align, own, J, st);
-    }
 }
 
 template <typename T, int W>
@@ -1353,6 +1456,36 @@ hipError_t launch_type(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, i
     }
 }
 
+// Both in one launch, and the join (c: how the shared keys are cut).
+template <typename T, int DP, int NB, bool WK, int ALIGN>
+hipError_t launch_both(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, hipStream_t st) {
+    typedef Kernel<T, DP, NB, WK, ALIGN, ANY | SHARED> S;
+    typedef Kernel<T, DP, 1, true, ALIGN, ANY> O;
+    static_assert(std::max(S::kTab, O::kTab) <= 163840, "LDS");
+    const int blocks = a.hk * shared.tiles * shared.splits;
+    const long long all = blocks + (long long)a.batch * a.hk * own.tiles * own.splits;
+    const hipError_t e = enqueue(k_attn_both<T, DP, NB, WK, ALIGN>, dim3((unsigned)all), dim3(256), std::max(S::kTab, O::kTab), st, a, own, shared, blocks);
+    return e != hipSuccess ? e : join<T, DP, true>(a, own, st);
+}
+template <typename T, int DP>
+hipError_t launch_both_width(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const Cut &c, int align, hipStream_t st) {
+    if (align < 16) {
+        if (c.wk) return launch_both<T, DP, 1, true, 4>(a, own, shared, st);
+        return c.nb == 1 ? launch_both<T, DP, 1, false, 4>(a, own, shared, st) : launch_both<T, DP, 2, false, 4>(a, own, shared, st);
+    }
+    if (c.wk) return launch_both<T, DP, 1, true, 16>(a, own, shared, st);
+    return c.nb == 1 ? launch_both<T, DP, 1, false, 16>(a, own, shared, st) : launch_both<T, DP, 2, false, 16>(a, own, shared, st);
+}
+template <typename T>
+hipError_t launch_both_type(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const Cut &c, int align, hipStream_t st) {
+    switch (c.dp) {
+        case 32: return launch_both_width<T, 32>(a, own, shared, c, align, st);
+        case 64: return launch_both_width<T, 64>(a, own, shared, c, align, st);
+        case 96: return launch_both_width<T, 96>(a, own, shared, c, align, st);
+        default: return launch_both_width<T, 128>(a, own, shared, c, align, st);
+    }
+}
+
 }  // namespace attn
 
 hipError_t launch_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
@@ -1361,9 +1494,9 @@ hipError_t launch_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const
 hipError_t launch_window_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
 hipError_t launch_window_attention_f16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
 hipError_t launch_window_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
-hipError_t launch_shared_attention_f32(const AttnOpArgs &s, const AttnLaunch &L, const attn::Cut &c, int align, const AttnOpArgs &own,
-                                        const AttnLaunch &J, hipStream_t st);
-hipError_t launch_shared_attention_f16(const AttnOpArgs &s, const AttnLaunch &L, const attn::Cut &c, int align, const AttnOpArgs &own,
-                                        const AttnLaunch &J, hipStream_t st);
-hipError_t launch_shared_attention_bf16(const AttnOpArgs &s, const AttnLaunch &L, const attn::Cut &c, int align, const AttnOpArgs &own,
-                                        const AttnLaunch &J, hipStream_t st);
+hipError_t launch_whole_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_whole_attention_f16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_whole_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_both_attention_f32(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_both_attention_f16(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_both_attention_bf16(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const attn::Cut &c, int align, hipStream_t st);

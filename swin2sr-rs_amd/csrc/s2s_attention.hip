@@ -34,8 +34,12 @@ attn::Cut cut_of(int dtype, const AttnOpArgs &a, bool narrow) {
     const long long blocks = std::max(1LL, pairs * c.tiles);
     long long nt = ((long long)a.nk + c.tk - 1) / c.tk;
     // of a window the tiles that a column tile's queries and the sinks lie in
-    if (a.window)
+    if (a.window) {
         nt = std::min(nt, ((long long)(a.causal ? 1 : 2) * a.window + per / a.group + c.tk) / c.tk + 1 + ((long long)a.sinks + c.tk - 1) / c.tk);
+        // few tiles are not cut: a launch less (5 queries over windows of 128 of 700 keys, 8 f16 heads of 64, 8.7 us with
+        // the host's call, 12.2 in ranges)
+        if (c.wk && nt <= 6) nt = 1;
+    }
     const long long ranges = c.wk && nt > 4 ? std::max({nt / 4, std::min(nt / 2, 32LL), std::min(nt, 16LL)}) : nt / 4;
     c.splits = (int)std::max(1LL, std::min({2LL * cus / blocks, ranges, 256LL}));
     return c;
@@ -276,7 +280,7 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
     // across two documents and mask both's tiles (nine images, 11003 tokens, 12 heads: 64
     // wide 153 us with waves of 32 and 127 with 16, 32 wide 132 and 105; 128 wide, 32 / 8
     // heads, where a wave of 16 reads LDS twice as often for its products, 369 and 483).
-    const attn::Cut c = cut_of(dtype, a, align < 16 || L.score.general || (a.k_docs && a.width <= 64));
+    const attn::Cut c = cut_of(dtype, a, (a.window && !a.k_docs ? align < 4 : align < 16) || L.score.general || (a.k_docs && a.width <= 64));
     L.cols = a.group * a.nq;
     L.tiles = c.tiles;
     L.splits = c.splits;
@@ -323,69 +327,103 @@ hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStre
 
 namespace {
 
-// How the columns of all entries go over the shared keys.
-attn::Cut shared_cut(int dtype, const AttnOpArgs &s, bool narrow) {
-    AttnOpArgs one = s;
-    one.nq = s.batch * s.nq;
+// How the columns of all entries go over the shared keys, in one launch with the entries' own: ranges for one
+// workgroup a CU, beside which it takes one of the own keys' (64 steps over 16384 shared keys, 640 own, 32 / 8 bf16
+// heads of 128: 54 us, 67 with two and 87 with a half); waves of 32 columns from 257 columns a head on
+// (200 steps over 8192 keys: 73 us against 86; 64 steps, 256 columns, over 4096 keys 46 against 41).
+attn::Cut shared_cut(int dtype, const AttnOpArgs &a) {
+    AttnOpArgs one = a;
+    one.nq = a.batch * a.nq;
     one.batch = 1;
-    attn::Cut c = cut_of(dtype, one, narrow);
-    c.splits = std::min(c.splits, 128);  // (the join takes 256 ranges)
+    one.nk = a.shared_nk;
+    attn::Cut c = cut_of(dtype, one, true);
+    const long long cols = (long long)one.nq * one.group, nt = ((long long)one.nk + c.tk - 1) / c.tk;
+    if (cols > 256) c.nb = 2;
+    const int per = c.wk ? 16 : 64 * c.nb;
+    c.tiles = (int)((cols + per - 1) / per);
+    c.splits = (int)std::max(1LL, std::min({cu_count() / ((long long)c.tiles * a.hk), nt / 2, 128LL}));  // (the join takes 256 ranges)
     return c;
 }
-attn::Cut own_cut(int dtype, const AttnOpArgs &a, bool narrow) {
-    attn::Cut c = cut_of(dtype, a, narrow);
+// How an entry's columns go over the shared keys and its own, as over keys of its own.
+attn::Cut whole_cut(int dtype, const AttnOpArgs &a, bool narrow) {
+    AttnOpArgs one = a;
+    one.nk = a.shared_nk + a.nk;
+    attn::Cut c = cut_of(dtype, one, narrow);
+    // up to eight tiles one launch is faster than two (16 steps over 256 + 128 keys, 32 / 8 bf16 heads of 128, 11.1 us
+    // uncut and 12.1 in ranges, and the host has one launch less)
+    if (c.wk && one.nk <= 8 * c.tk) c.splits = 1;
+    return c;
+}
+attn::Cut own_cut(int dtype, const AttnOpArgs &a) {
+    attn::Cut c = cut_of(dtype, a, true);
     c.splits = std::min(c.splits, 128);
     return c;
 }
 
-size_t sums_bytes(const attn::Cut &c, size_t columns) { return columns * c.splits * ((size_t)c.dp * 4 + 8); }
+size_t columns_of(const AttnOpArgs &a) { return (size_t)a.batch * a.nq * a.hq; }
+size_t sums_bytes(const attn::Cut &c, const AttnOpArgs &a) { return round16(columns_of(a) * c.splits * ((size_t)c.dp * 4 + 8)); }
+
+// Whether every column tile walks the shared keys by itself, and its entry's own behind them. For more than 16 columns
+// an entry always, since the shared keys' sums of every range, written and read again, cost more than the keys
+// (8 x 512 tokens behind 1024, 4096 and 16384 shared keys, 32 / 8 bf16 heads of 128: 98, 294 and 1077 us
+// against 177, 379 and 1188; 4 x 16 tokens 16, 27 and 40 against 20, 31 and 43); for few columns over few keys.
+bool goes_whole(const attn::Cut &c, const AttnOpArgs &a, int align, bool general) {
+    return !c.wk || align == 0 || general || (long long)a.shared_nk + a.nk <= 8 * c.tk;
+}
 
 }  // namespace
 
-size_t shared_attn_op_workspace(int dtype, const AttnOpArgs &s, const AttnOpArgs &a) {
-    size_t own = 0, shared = 0;
-    const size_t columns = (size_t)a.batch * a.nq * a.hq;
+// The most that any way of these sizes needs: which one runs goes by strides and numbers too.
+size_t shared_attn_op_workspace(int dtype, const AttnOpArgs &a) {
+    size_t most = sums_bytes(own_cut(dtype, a), a) + sums_bytes(shared_cut(dtype, a), a);
+    if (!cut_of(dtype, a, true).wk) most = 0;
     for (const bool narrow : {false, true}) {
-        own = std::max(own, sums_bytes(own_cut(dtype, a, narrow), columns));
-        shared = std::max(shared, sums_bytes(shared_cut(dtype, s, narrow), columns));
+        const attn::Cut c = whole_cut(dtype, a, narrow);
+        if (c.splits > 1) most = std::max(most, sums_bytes(c, a));
     }
-    return round16(own) + shared;
+    return most;
 }
 
-hipError_t launch_shared_attention_op(int dtype, const AttnOpArgs &s, const AttnOpArgs &a, void *ws, hipStream_t st) {
+hipError_t launch_shared_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStream_t st) {
     const int size = dtype == 0 ? 4 : 2;
-    const size_t columns = (size_t)a.batch * a.nq * a.hq;
-    auto fill = [&](const AttnOpArgs &x, const attn::Cut &c, int al, float *sums) {
+    AttnOpArgs s = a;  // the shared keys as the keys
+    s.k = a.shared_k, s.v = a.shared_v, s.sk = a.shared_sk, s.sv = a.shared_sv, s.nk = a.shared_nk;
+    const int own_al = aligned_inputs(a, size), own_align = copies_of(a, own_al);
+    const int shared_al = aligned_inputs(s, size), shared_align = copies_of(s, shared_al);
+    AttnScore score;
+    score.set(a);
+    auto fill = [&](const attn::Cut &c, int al, float *sums) {
         AttnLaunch L{};
-        L.score.set(x);
+        L.score = score;
         L.vec = std::min(al, 8);
         L.out_vec = std::min(4, aligned_bytes(a.out, a.so, a.width, size) / size);
+        L.cols = a.group * a.nq;
         L.tiles = c.tiles;
         L.splits = c.splits;
+        L.by_pairs.set(a.batch * a.hk);
         L.by_tiles.set(c.tiles);
         L.by_hk.set(a.hk);
         L.by_group.set(a.group);
         L.by_nq.set(a.nq);
         L.part_o = sums;
-        L.part_ml = sums + columns * c.splits * c.dp;
+        L.part_ml = sums + columns_of(a) * c.splits * c.dp;
         return L;
     };
-    // each entry's own keys
-    const int own_al = aligned_inputs(a, size), own_align = copies_of(a, own_al);
-    AttnScore score;
-    score.set(a);
-    const attn::Cut oc = own_cut(dtype, a, own_align < 16 || score.general);
-    AttnLaunch O = fill(a, oc, own_al, (float *)ws);
-    O.cols = a.group * a.nq;
-    O.by_pairs.set(a.batch * a.hk);
-    hipError_t e = launch_of(dtype, a, O, oc, own_align, st);
-    if (e != hipSuccess) return e;
-    // the shared ones, and the join
-    const int al = aligned_inputs(s, size), align = copies_of(s, al);
-    const attn::Cut sc = shared_cut(dtype, s, align < 16 || score.general);
-    size_t own_most = 0;
-    for (const bool narrow : {false, true}) own_most = std::max(own_most, sums_bytes(own_cut(dtype, a, narrow), columns));
-    AttnLaunch S = fill(s, sc, al, (float *)((char *)ws + round16(own_most)));
+    const int align = std::min(own_align, shared_align), al = std::min(own_al, shared_al);
+    const attn::Cut wc = whole_cut(dtype, a, align < 4 || score.general);
+    if (goes_whole(wc, a, align, score.general)) {
+        AttnLaunch L = fill(wc, al, (float *)ws);
+        if (wc.splits > 1) L.join = 1;
+        else L.part_o = L.part_ml = nullptr;
+        switch (dtype) {
+            case 0: return launch_whole_attention_f32(a, L, wc, align, st);
+            case 1: return launch_whole_attention_f16(a, L, wc, align, st);
+            case 2: return launch_whole_attention_bf16(a, L, wc, align, st);
+        }
+        return hipErrorInvalidValue;
+    }
+    const attn::Cut oc = own_cut(dtype, a), sc = shared_cut(dtype, a);
+    AttnLaunch O = fill(oc, al, (float *)ws), S = fill(sc, al, (float *)((char *)ws + sums_bytes(oc, a)));
     S.cols = a.group * a.nq * a.batch;
     S.by_pairs.set(a.hk);
     O.shared_o = S.part_o;
@@ -393,9 +431,9 @@ hipError_t launch_shared_attention_op(int dtype, const AttnOpArgs &s, const Attn
     O.shared_splits = sc.splits;
     O.shared_cols = S.cols;
     switch (dtype) {
-        case 0: return launch_shared_attention_f32(s, S, sc, align, a, O, st);
-        case 1: return launch_shared_attention_f16(s, S, sc, align, a, O, st);
-        case 2: return launch_shared_attention_bf16(s, S, sc, align, a, O, st);
+        case 0: return launch_both_attention_f32(a, O, S, sc, align, st);
+        case 1: return launch_both_attention_f16(a, O, S, sc, align, st);
+        case 2: return launch_both_attention_bf16(a, O, S, sc, align, st);
     }
     return hipErrorInvalidValue;
 }

@@ -1,7 +1,6 @@
-// s2s_attention_shared_bf16.hip - the attention kernels of s2s_attention.h over keys that a batch shares, for bf16 arrays.
+// s2s_attention_shared_bf16.hip - the attention kernels of s2s_attention.h for steps over keys that a batch shares, for bf16 arrays.
 #include "s2s_attention.h"
 
-hipError_t launch_shared_attention_bf16(const AttnOpArgs &s, const AttnLaunch &L, const attn::Cut &c, int align, const AttnOpArgs &own,
-                                        const AttnLaunch &J, hipStream_t st) {
-    return attn::launch_shared_type<bfloat_t>(s, L, c, align, own, J, st);
+hipError_t launch_both_attention_bf16(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const attn::Cut &c, int align, hipStream_t st) {
+    return attn::launch_both_type<bfloat_t>(a, own, shared, c, align, st);
 }

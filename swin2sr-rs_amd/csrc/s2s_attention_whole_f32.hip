@@ -1,0 +1,6 @@
+// s2s_attention_whole_f32.hip - the attention kernels of s2s_attention.h over shared keys and an entry's own, for f32 arrays.
+#include "s2s_attention.h"
+
+hipError_t launch_whole_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st) {
+    return attn::launch_type<float, attn::WHOLE>(a, L, c, align, st);
+}

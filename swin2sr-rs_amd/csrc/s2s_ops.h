@@ -28,10 +28,11 @@ struct AttnOpArgs {
     const float *slopes, *table;
     int table_size;
     int window, sinks;  // window 0: none
-    // keys that the batch shares (k, v and nk are theirs then): each entry's part of them, and how many keys
-    // of its own there are at most
+    // keys that the batch shares, ahead of each entry's own, and each entry's part of them
+    const void *shared_k, *shared_v;
+    Strides shared_sk, shared_sv;  // (b counts for nothing)
     const int *shared_lens;
-    int own_nk;
+    int shared_nk;
 };
 
 struct RotaryArrays {
@@ -95,8 +96,8 @@ hipError_t enqueue(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipS
 
 size_t attn_op_workspace(int dtype, const AttnOpArgs &a);
 hipError_t launch_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStream_t st);
-size_t shared_attn_op_workspace(int dtype, const AttnOpArgs &shared, const AttnOpArgs &own);
-hipError_t launch_shared_attention_op(int dtype, const AttnOpArgs &shared, const AttnOpArgs &own, void *ws, hipStream_t st);
+size_t shared_attn_op_workspace(int dtype, const AttnOpArgs &a);
+hipError_t launch_shared_attention_op(int dtype, const AttnOpArgs &a, void *ws, hipStream_t st);
 hipError_t launch_rotary_op(int dtype, const RotaryArgs &a, hipStream_t st);
 hipError_t launch_norm_rotary_op(int dtype, const NormRotaryArgs &a, hipStream_t st);
 hipError_t launch_rms_norm_op(int dtype, bool e4m3, const RmsNormArgs &a, hipStream_t st);

@@ -185,16 +185,14 @@ int shared_sizes(const char *op, const s2s_shared_attention_args *s) {
     return 0;
 }
 
-// The shared keys' part of a call whose own part is `own`.
-AttnOpArgs shared_args(const s2s_shared_attention_args *s, const AttnOpArgs &own) {
-    AttnOpArgs k = own;
-    k.k = s->shared_k.data;
-    k.v = s->shared_v.data;
-    k.sk = strides(s->shared_k, 1, s->shared_tokens, s->own.k_heads);
-    k.sv = strides(s->shared_v, 1, s->shared_tokens, s->own.k_heads);
-    if (s->shared_tokens <= 1) k.sk.t = k.sv.t = own.width;
-    k.nk = s->shared_tokens;
-    k.own_nk = own.nk;
+AttnOpArgs shared_args(const s2s_shared_attention_args *s) {
+    AttnOpArgs k = attention_args(&s->own);
+    k.shared_k = s->shared_k.data;
+    k.shared_v = s->shared_v.data;
+    k.shared_sk = strides(s->shared_k, 1, s->shared_tokens, s->own.k_heads);
+    k.shared_sv = strides(s->shared_v, 1, s->shared_tokens, s->own.k_heads);
+    if (s->shared_tokens <= 1) k.shared_sk.t = k.shared_sv.t = s->own.width;
+    k.shared_nk = s->shared_tokens;
     k.shared_lens = s->shared_lens;
     return k;
 }
@@ -266,16 +264,15 @@ int attention_call(const char *op, const s2s_attention_args *a, int window, int 
     for (const auto &x : arrays)
         if (x.p)
             if (int rc = check_array(op, x.name, x.p, 4, on.dev)) return rc;
-    const AttnOpArgs k = attention_args(a, window, sinks);
-    const AttnOpArgs ks = s ? shared_args(s, k) : k;
-    const size_t need = s ? shared_attn_op_workspace(a->dtype, ks, k) : attn_op_workspace(a->dtype, k);
+    const AttnOpArgs k = s ? shared_args(s) : attention_args(a, window, sinks);
+    const size_t need = s ? shared_attn_op_workspace(a->dtype, k) : attn_op_workspace(a->dtype, k);
     if (need) {
         if (!workspace || workspace_bytes < need)
             return refuse("%s: a workspace of %zu bytes is needed, %llu are given", op, need,
                           workspace ? (unsigned long long)workspace_bytes : 0ULL);
         if (int rc = check_array(op, "workspace", workspace, 16, on.dev)) return rc;
     }
-    e = s ? launch_shared_attention_op(a->dtype, ks, k, workspace, st) : launch_attention_op(a->dtype, k, workspace, st);
+    e = s ? launch_shared_attention_op(a->dtype, k, workspace, st) : launch_attention_op(a->dtype, k, workspace, st);
     return e == hipSuccess ? 0 : refuse_hip(op, "the launch", e);
 }
 
@@ -425,8 +422,7 @@ int s2s_shared_attention_workspace(const s2s_shared_attention_args *s, uint64_t 
     if (!s || !bytes) return refuse("%s: null argument", op);
     if (int rc = attention_sizes(op, &s->own)) return rc;
     if (int rc = shared_sizes(op, s)) return rc;
-    const AttnOpArgs k = attention_args(&s->own);
-    *bytes = shared_attn_op_workspace(s->own.dtype, shared_args(s, k), k);
+    *bytes = shared_attn_op_workspace(s->own.dtype, shared_args(s));
     return 0;
 }
 

@@ -23,7 +23,8 @@ fn build_hip() {
     let srcs = ["s2s_kernels.hip", "s2s_split.hip", "s2s_attention.hip", "s2s_attention_f32.hip",
                 "s2s_attention_f16.hip", "s2s_attention_bf16.hip", "s2s_attention_window_f32.hip",
                 "s2s_attention_window_f16.hip", "s2s_attention_window_bf16.hip", "s2s_attention_shared_f32.hip",
-                "s2s_attention_shared_f16.hip", "s2s_attention_shared_bf16.hip", "s2s_ops.hip", "s2s_ops_api.cpp",
+                "s2s_attention_shared_f16.hip", "s2s_attention_shared_bf16.hip", "s2s_attention_whole_f32.hip",
+                "s2s_attention_whole_f16.hip", "s2s_attention_whole_bf16.hip", "s2s_ops.hip", "s2s_ops_api.cpp",
                 "s2s_api.cpp", "s2s_test_api.cpp", "s2s_selftest.cpp"];
     let status = Command::new(&hipcc)
         .arg(format!("--offload-arch={arch}"))

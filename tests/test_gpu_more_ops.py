@@ -457,3 +457,26 @@ def test_shared_refuses(pkg):
     T.refused(pkg, "2.22", lambda: p(**{**a, "shared_k": A(a["shared_k"].ptr, (900, 2, 128), "bf16", (1 << 23, 128, 1))}, **w))
     T.refused(pkg, "stride", lambda: p(**{**a, "shared_k": A(a["shared_k"].ptr, (900, 2, 128), "bf16", (-128, 128, 1))}, **w))
     assert np.all(d["out"].get() == 7.5)
+
+
+# ---- infinities that a step sees -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("op", ["attention", "window", "shared"])
+@pytest.mark.parametrize("keys", [120, 2000])
+def test_steps_see_infinities(pkg, dtype, op, keys):
+    """An infinity of v in the middle of what a step reads is infinite in its channel and nowhere else; one of either
+    sign is NaN."""
+    H, KV, D = 4, 2, 64
+    sizes = dict(B=2, Lq=1, Lk=keys, H=H, KV=KV, D=D, causal=True, order="cache")
+
+    def put(v):
+        v[..., keys // 2, 0, 3], v[..., keys // 2 + 1, 1, 9], v[..., 70, 1, 5], v[..., keys - 60, 1, 5] = np.inf, -np.inf, np.inf, -np.inf
+    if op == "shared":
+        check_shared(pkg, scase(dtype, S=keys, **dict(sizes, Lk=50)), lambda q, k, v, sk, sv, more: put(sv))
+        check_shared(pkg, scase(dtype, S=50, **sizes), lambda q, k, v, sk, sv, more: put(v))
+    elif op == "window":
+        check_window(pkg, wcase(dtype, window=keys - 3, sinks=1, **sizes), lambda q, k, v, more: put(v))
+    else:
+        T.check_attention(pkg, T.case(dtype, **sizes), lambda q, k, v, more: put(v))
