@@ -341,7 +341,7 @@ attn::Cut shared_cut(int dtype, const AttnOpArgs &a) {
     if (cols > 256) c.nb = 2;
     const int per = c.wk ? 16 : 64 * c.nb;
     c.tiles = (int)((cols + per - 1) / per);
-    c.splits = (int)std::max(1LL, std::min({cu_count() / ((long long)c.tiles * a.hk), nt / 2, 128LL}));  // (the join takes 256 ranges)
+    c.splits = (int)std::max(1LL, std::min({cu_count() / std::max(1LL, (long long)c.tiles * a.hk), nt / 2, 128LL}));  // (the join takes 256 ranges)
     return c;
 }
 // How an entry's columns go over the shared keys and its own, as over keys of its own.
