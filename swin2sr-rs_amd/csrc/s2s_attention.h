@@ -1197,11 +1197,11 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnOpArgs a, AttnLaunch L) {
 
 // The columns of all entries over the shared keys, `shared` workgroups, and each entry's few columns over its own keys
 // in one launch: the first are bound by instructions, the second by HBM, and a CU takes both.
-template <typename T, int DP, int NB, bool WK, int ALIGN>
+template <typename T, int DP, int NB, bool WK, int ALIGN, bool OWN_WK>
 __global__ __launch_bounds__(256, 2) void k_attn_both(AttnOpArgs a, AttnLaunch own, AttnLaunch shared, int blocks) {
     extern __shared__ __align__(16) char lds[];
     if ((int)blockIdx.x < blocks) Kernel<T, DP, NB, WK, ALIGN, ANY | SHARED>::template run<1>(a, shared, blockIdx.x, lds);
-    else Kernel<T, DP, 1, true, ALIGN, ANY>::run(a, own, blockIdx.x - blocks, lds);
+    else Kernel<T, DP, 1, OWN_WK, ALIGN, ANY>::run(a, own, blockIdx.x - blocks, lds);
 }
 
 // The key ranges' sums of one column: a workgroup each, its threads over the ranges
@@ -1457,32 +1457,33 @@ hipError_t launch_type(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, i
 }
 
 // Both in one launch, and the join (c: how the shared keys are cut).
-template <typename T, int DP, int NB, bool WK, int ALIGN>
+template <typename T, int DP, int NB, bool WK, int ALIGN, bool OWN_WK = true>
 hipError_t launch_both(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, hipStream_t st) {
     typedef Kernel<T, DP, NB, WK, ALIGN, ANY | SHARED> S;
-    typedef Kernel<T, DP, 1, true, ALIGN, ANY> O;
+    typedef Kernel<T, DP, 1, OWN_WK, ALIGN, ANY> O;
     static_assert(std::max(S::kTab, O::kTab) <= 163840, "LDS");
     const int blocks = a.hk * shared.tiles * shared.splits;
     const long long all = blocks + (long long)a.batch * a.hk * own.tiles * own.splits;
-    const hipError_t e = enqueue(k_attn_both<T, DP, NB, WK, ALIGN>, dim3((unsigned)all), dim3(256), std::max(S::kTab, O::kTab), st, a, own, shared, blocks);
+    const hipError_t e = enqueue(k_attn_both<T, DP, NB, WK, ALIGN, OWN_WK>, dim3((unsigned)all), dim3(256), std::max(S::kTab, O::kTab), st, a, own, shared, blocks);
     return e != hipSuccess ? e : join<T, DP, true>(a, own, st);
 }
+template <typename T, int DP, int ALIGN>
+hipError_t launch_both_align(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const Cut &c, bool own_wk, hipStream_t st) {
+    if (!own_wk) return launch_both<T, DP, 2, false, ALIGN, false>(a, own, shared, st);
+    if (c.wk) return launch_both<T, DP, 1, true, ALIGN>(a, own, shared, st);
+    return c.nb == 1 ? launch_both<T, DP, 1, false, ALIGN>(a, own, shared, st) : launch_both<T, DP, 2, false, ALIGN>(a, own, shared, st);
+}
 template <typename T, int DP>
-hipError_t launch_both_width(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const Cut &c, int align, hipStream_t st) {
-    if (align < 16) {
-        if (c.wk) return launch_both<T, DP, 1, true, 4>(a, own, shared, st);
-        return c.nb == 1 ? launch_both<T, DP, 1, false, 4>(a, own, shared, st) : launch_both<T, DP, 2, false, 4>(a, own, shared, st);
-    }
-    if (c.wk) return launch_both<T, DP, 1, true, 16>(a, own, shared, st);
-    return c.nb == 1 ? launch_both<T, DP, 1, false, 16>(a, own, shared, st) : launch_both<T, DP, 2, false, 16>(a, own, shared, st);
+hipError_t launch_both_width(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const Cut &c, bool own_wk, int align, hipStream_t st) {
+    return align < 16 ? launch_both_align<T, DP, 4>(a, own, shared, c, own_wk, st) : launch_both_align<T, DP, 16>(a, own, shared, c, own_wk, st);
 }
 template <typename T>
-hipError_t launch_both_type(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const Cut &c, int align, hipStream_t st) {
+hipError_t launch_both_type(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const Cut &c, bool own_wk, int align, hipStream_t st) {
     switch (c.dp) {
-        case 32: return launch_both_width<T, 32>(a, own, shared, c, align, st);
-        case 64: return launch_both_width<T, 64>(a, own, shared, c, align, st);
-        case 96: return launch_both_width<T, 96>(a, own, shared, c, align, st);
-        default: return launch_both_width<T, 128>(a, own, shared, c, align, st);
+        case 32: return launch_both_width<T, 32>(a, own, shared, c, own_wk, align, st);
+        case 64: return launch_both_width<T, 64>(a, own, shared, c, own_wk, align, st);
+        case 96: return launch_both_width<T, 96>(a, own, shared, c, own_wk, align, st);
+        default: return launch_both_width<T, 128>(a, own, shared, c, own_wk, align, st);
     }
 }
 
@@ -1497,6 +1498,9 @@ hipError_t launch_window_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L
 hipError_t launch_whole_attention_f32(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
 hipError_t launch_whole_attention_f16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
 hipError_t launch_whole_attention_bf16(const AttnOpArgs &a, const AttnLaunch &L, const attn::Cut &c, int align, hipStream_t st);
-hipError_t launch_both_attention_f32(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const attn::Cut &c, int align, hipStream_t st);
-hipError_t launch_both_attention_f16(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const attn::Cut &c, int align, hipStream_t st);
-hipError_t launch_both_attention_bf16(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const attn::Cut &c, int align, hipStream_t st);
+hipError_t launch_both_attention_f32(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const attn::Cut &c, bool own_wk,
+                                      int align, hipStream_t st);
+hipError_t launch_both_attention_f16(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const attn::Cut &c, bool own_wk,
+                                      int align, hipStream_t st);
+hipError_t launch_both_attention_bf16(const AttnOpArgs &a, const AttnLaunch &own, const AttnLaunch &shared, const attn::Cut &c, bool own_wk,
+                                      int align, hipStream_t st);

@@ -338,7 +338,7 @@ attn::Cut shared_cut(int dtype, const AttnOpArgs &a) {
     one.nk = a.shared_nk;
     attn::Cut c = cut_of(dtype, one, true);
     const long long cols = (long long)one.nq * one.group, nt = ((long long)one.nk + c.tk - 1) / c.tk;
-    if (cols > 256) c.nb = 2;
+    if (cols > 256 || (long long)a.nq * a.group > 16) c.nb = 2, c.wk = false;
     const int per = c.wk ? 16 : 64 * c.nb;
     c.tiles = (int)((cols + per - 1) / per);
     c.splits = (int)std::max(1LL, std::min({cu_count() / std::max(1LL, (long long)c.tiles * a.hk), nt / 2, 128LL}));  // (the join takes 256 ranges)
@@ -363,12 +363,18 @@ attn::Cut own_cut(int dtype, const AttnOpArgs &a) {
 size_t columns_of(const AttnOpArgs &a) { return (size_t)a.batch * a.nq * a.hq; }
 size_t sums_bytes(const attn::Cut &c, const AttnOpArgs &a) { return round16(columns_of(a) * c.splits * ((size_t)c.dp * 4 + 8)); }
 
-// Whether every column tile walks the shared keys by itself, and its entry's own behind them. For more than 16 columns
+// Whether every column tile walks the shared keys by itself, and its entry's own behind them. For more than 32 columns
 // an entry always, since the shared keys' sums of every range, written and read again, cost more than the keys
 // (8 x 512 tokens behind 1024, 4096 and 16384 shared keys, 32 / 8 bf16 heads of 128: 98, 294 and 1077 us
-// against 177, 379 and 1188; 4 x 16 tokens 16, 27 and 40 against 20, 31 and 43); for few columns over few keys.
-bool goes_whole(const attn::Cut &c, const AttnOpArgs &a, int align, bool general) {
-    return !c.wk || align == 0 || general || (long long)a.shared_nk + a.nk <= 8 * c.tk;
+// against 177, 379 and 1188; 16 x 16 tokens, 64 columns, 26, 31 and 60 behind 1024, 2048 and 8192, 29, 34 and 68). 17 to 32,
+// which leave the half of a tile of their own empty: of 16-bit types but for many keys times entries (16 x 8 tokens behind 1024
+// and 8192 keys 20 and 52 us, 26 and 39 by the ranges), of f32, whose products take longer, never (16 x 24 tokens of 6
+// heads of 30 behind 1024 and 8192 keys 23 and 83, 17 and 44). Steps over up to eight tiles.
+bool goes_whole(int dtype, const AttnOpArgs &a, int tk, int align, bool general) {
+    const long long cols = (long long)a.nq * a.group, tiles = ((long long)a.shared_nk + tk - 1) / tk;
+    if (align == 0 || general || cols > 32) return true;
+    if (cols > 16) return dtype != 0 && a.batch * a.hk * tiles < 48LL * cu_count();
+    return (long long)a.shared_nk + a.nk <= 8 * tk;
 }
 
 }  // namespace
@@ -376,7 +382,6 @@ bool goes_whole(const attn::Cut &c, const AttnOpArgs &a, int align, bool general
 // The most that any way of these sizes needs: which one runs goes by strides and numbers too.
 size_t shared_attn_op_workspace(int dtype, const AttnOpArgs &a) {
     size_t most = sums_bytes(own_cut(dtype, a), a) + sums_bytes(shared_cut(dtype, a), a);
-    if (!cut_of(dtype, a, true).wk) most = 0;
     for (const bool narrow : {false, true}) {
         const attn::Cut c = whole_cut(dtype, a, narrow);
         if (c.splits > 1) most = std::max(most, sums_bytes(c, a));
@@ -411,7 +416,7 @@ hipError_t launch_shared_attention_op(int dtype, const AttnOpArgs &a, void *ws, 
     };
     const int align = std::min(own_align, shared_align), al = std::min(own_al, shared_al);
     const attn::Cut wc = whole_cut(dtype, a, align < 4 || score.general);
-    if (goes_whole(wc, a, align, score.general)) {
+    if (goes_whole(dtype, a, wc.tk, align, score.general)) {
         AttnLaunch L = fill(wc, al, (float *)ws);
         if (wc.splits > 1) L.join = 1;
         else L.part_o = L.part_ml = nullptr;
@@ -431,9 +436,9 @@ hipError_t launch_shared_attention_op(int dtype, const AttnOpArgs &a, void *ws, 
     O.shared_splits = sc.splits;
     O.shared_cols = S.cols;
     switch (dtype) {
-        case 0: return launch_both_attention_f32(a, O, S, sc, align, st);
-        case 1: return launch_both_attention_f16(a, O, S, sc, align, st);
-        case 2: return launch_both_attention_bf16(a, O, S, sc, align, st);
+        case 0: return launch_both_attention_f32(a, O, S, sc, oc.wk, align, st);
+        case 1: return launch_both_attention_f16(a, O, S, sc, oc.wk, align, st);
+        case 2: return launch_both_attention_bf16(a, O, S, sc, oc.wk, align, st);
     }
     return hipErrorInvalidValue;
 }

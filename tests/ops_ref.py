@@ -104,7 +104,8 @@ class Dev:
 
 
 def attention(dtype, q, k, v, scale, cap=0.0, causal=False, q_lens=None, k_lens=None, prefix=None, q_docs=None,
-              k_docs=None, q_pos=None, k_pos=None, slopes=None, table=None, window=0, sinks=0):
+              k_docs=None, q_pos=None, k_pos=None, slopes=None, table=None, window=0, sinks=0,
+              least=0.0):
     """(out, bound, written): the result in 64 bits for inputs that are values of
     `dtype`, the error a 32-bit evaluation may have, and which rows are written.
 
@@ -117,6 +118,7 @@ def attention(dtype, q, k, v, scale, cap=0.0, causal=False, q_lens=None, k_lens=
     rounded to the type before it multiplies v (HALF), the f16 one also by half
     its smallest step, 2^-25 at weights that have 2^0 or more for the row's
     largest. The result is rounded once (HALF of it, or half the smallest step).
+    `least`: keys of smaller weights, for the row's largest, are left out.
     """
     B, Lq, H, D = q.shape
     Lk, G = k.shape[1], H // k.shape[2]
@@ -183,7 +185,7 @@ def attention(dtype, q, k, v, scale, cap=0.0, causal=False, q_lens=None, k_lens=
                 w = p / np.where(total == 0, 1, total)
                 va = np.abs(vv)
                 for r in range(m):
-                    live = use[r]
+                    live = use[r] & ~(p[r] < least)
                     if not live.any():
                         continue
                     out[b, r, h] = w[r, live] @ vv[live]

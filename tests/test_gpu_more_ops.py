@@ -312,14 +312,14 @@ def shared_inputs(c):
     return q, k, v, sk, sv, more
 
 
-def shared_want(c, q, k, v, sk, sv, more, scale):
+def shared_want(c, q, k, v, sk, sv, more, scale, least=0.0):
     """Entry by entry, the entry's shared keys ahead of its own."""
     outs = []
     for b in range(c["B"]):
         n = int(np.clip(more["shared_lens"][b], 0, c["S"])) if "shared_lens" in more else c["S"]
         own = int(np.clip(more["k_lens"][b], 0, c["Lk"])) if "k_lens" in more else c["Lk"]
         kk, vv = (np.concatenate((x[:n], y[b, :own]))[None] for x, y in ((sk, k), (sv, v)))
-        extra = {"q_lens": more["q_lens"][b:b + 1]} if "q_lens" in more else {}
+        extra = {"q_lens": more["q_lens"][b:b + 1], "least": least} if "q_lens" in more else {"least": least}
         if "slopes" in more:
             extra["slopes"] = more["slopes"].astype(np.float64)
         outs.append(R.attention(c["dtype"], q[b:b + 1], kk, vv, scale, np.float64(np.float32(c["cap"])), c["causal"], **extra))
@@ -356,6 +356,12 @@ def check_shared(pkg, c, change=None):
     w = written[:, :, None, None] & np.ones(got.shape, bool)
     assert np.all(got[~w] == 7.5), "rows past the sequence were written"
     got, want, bound = got[w], want[w], bound[w]
+    if not np.isfinite(want).all():
+        # a key whose weight is below 2^-126 of its row's largest has none in 32 bits (e^(s - max) is no normal number), so
+        # that an infinity it holds may count or not: such rows are not compared
+        held = np.isfinite(shared_want(c, *arrays, scale, least=2.0 ** -126)[0][w]) == np.isfinite(want)
+        assert held.mean() > 0.5
+        got, want, bound = got[held], want[held], bound[held]
     assert np.array_equal(np.isnan(got), np.isnan(want))
     fine = np.isfinite(want)
     worst = (np.abs(got[fine] - want[fine]) / np.maximum(bound[fine], 1e-300)).max(initial=0.0)
@@ -480,3 +486,44 @@ def test_steps_see_infinities(pkg, dtype, op, keys):
         check_window(pkg, wcase(dtype, window=keys - 3, sinks=1, **sizes), lambda q, k, v, more: put(v))
     else:
         T.check_attention(pkg, T.case(dtype, **sizes), lambda q, k, v, more: put(v))
+
+
+# ---- every way over shared keys ---------------------------------------------------------------
+
+WAYS = {
+    # 17 to 32 columns an entry beside the shared keys' ranges: f32 always, 16-bit types from many keys times entries on
+    "f32_24": scase("f32", S=500, B=7, Lq=24, Lk=50, H=6, KV=6, D=30, causal=True, slopes=True),
+    "f32_20_128": scase("f32", S=300, B=5, Lq=5, Lk=70, H=8, KV=2, D=128, causal=True, q_lens=[5, 0, 3, 5, 1], k_lens=[70, 9, 64, 65, 0]),
+    "f32_32_part": scase("f32", S=400, B=6, Lq=16, Lk=40, H=4, KV=2, D=64, shared_lens=[0, 400, 64, 1, 333, 65], cap=20.0),
+    "bf16_32_many": scase("bf16", S=3100, B=64, Lq=8, Lk=20, H=16, KV=4, D=64, causal=True),
+    "f16_17_many": scase("f16", S=3100, B=64, Lq=17, Lk=20, H=4, KV=4, D=32, causal=True, shared_lens=[(97 * i) % 3200 for i in range(64)]),
+    # ranges of whole keys
+    "whole_ranges": scase("bf16", S=1500, B=3, Lq=20, Lk=200, H=8, KV=4, D=64, causal=True),
+    "whole_ranges_part": scase("f16", S=900, B=4, Lq=40, Lk=300, H=4, KV=2, D=96, causal=True, shared_lens=[0, 900, 100, 449], k_lens=[300, 20, 0, 100], q_lens=[40, 20, 0, 33]),
+    "whole_ranges_own": scase("f32", S=10, B=2, Lq=40, Lk=1900, H=4, KV=2, D=64, causal=True, order="cache"),
+    "whole_general": scase("bf16", S=1500, B=3, Lq=1, Lk=200, H=8, KV=4, D=64, causal=True, scale=-0.1, slopes=True),
+    "whole_odd": scase("bf16", S=1500, B=3, Lq=1, Lk=200, H=8, KV=4, D=63, causal=True, gap=3, lead=1, slopes=True),
+    # steps in ranges, rows of 4-byte multiples, waves of 16 and of 32 columns over the shared keys
+    "step_30_f32": scase("f32", S=1500, B=9, Lq=1, Lk=200, H=6, KV=6, D=30, causal=True),
+    "step_30_f32_many": scase("f32", S=1100, B=270, Lq=1, Lk=20, H=2, KV=2, D=30, causal=True),
+    "step_62_f16": scase("f16", S=1100, B=70, Lq=1, Lk=80, H=8, KV=2, D=62, causal=True, cap=30.0),
+    "step_300_columns": scase("bf16", S=1100, B=75, Lq=1, Lk=80, H=8, KV=2, D=128, causal=True, k_lens=[i % 81 for i in range(75)]),
+    "step_nine_tiles": scase("bf16", S=505, B=3, Lq=1, Lk=10, H=8, KV=2, D=64, causal=True),
+}
+
+
+@pytest.mark.parametrize("name", WAYS)
+def test_shared_ways(pkg, name):
+    check_shared(pkg, WAYS[name])
+
+
+@pytest.mark.parametrize("name", ["f32_24", "bf16_32_many", "whole_ranges", "step_30_f32_many", "step_300_columns"])
+def test_shared_ways_hide_what_keys_hold(pkg, name):
+    c = dict(WAYS[name])
+    S, B = c["S"], c["B"]
+    c["shared_lens"] = [(S - 90) * i // (B - 1) for i in range(B)]
+
+    def past(q, k, v, sk, sv, more):
+        sk[S - 80:], sv[S - 70:] = np.nan, -np.inf
+        sv[S // 2, 0, 3], sv[S // 2 + 1, -1, 5], sk[S // 2 + 70, -1, 0] = np.inf, np.nan, np.nan
+    check_shared(pkg, c, past)
