@@ -570,13 +570,17 @@ struct NormRotaryWalk {
 // not turned, reads them once, and the squares' sum is made across the lanes. The sines of the
 // workgroup's tokens are made once, in LDS. A wave takes 64 / G heads at a time, side by side in memory,
 // first of q, then of k, so that what differs between the two is in scalar registers; the next heads are
-// read while these are normed and turned. Offsets are 32-bit ones from the workgroup's first token.
+// read while these are normed and turned. HBM bounds it: the 16384 tokens below take 61.4 us (5.5 TB/s, a part from the last-level
+// cache), the f32 heads of 30 35.9 (3.8 TB/s: lanes of 8 bytes). Offsets are 32-bit ones from the workgroup's first token.
 // (The turns as an argument of 64 or 128 pairs: a launch's time goes by its arguments' bytes.)
 template <typename T, bool ADJ, int V, int G, bool EACH, int P>
 __global__ __launch_bounds__(256) void k_norm_rotary(RotaryArrays r, HeadNorm a, NormRotaryWalk w, RotaryTurns<P> x) {
     typedef VecOf<T, V> Part;
     typedef VecOf<T, 2 * V> Both;
     constexpr int H = 64 / G, UNIT = V * (int)sizeof(T);  // heads a wave takes at a time
+    // turns read ahead: two of short units (2 x 23400 tokens of 6 + 6 f32 heads of 30, 8 bytes a lane, 35.9 us; one 44.3,
+    // three 37.2), one of 32 bytes a lane (16384 tokens of 32 + 8 bf16 heads of 128 61.4 us; two 62.8, three 66)
+    constexpr int AHEAD = 2 * UNIT <= 16 ? 2 : 1;
     extern __shared__ float2 turn[];  // [tb][pairs]
     const int tid = threadIdx.x, lane = tid & 63, g = tid % G, rot = r.pairs / V;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -613,8 +617,17 @@ __global__ __launch_bounds__(256) void k_norm_rotary(RotaryArrays r, HeadNorm a,
         };
         float wt[2][V];
         auto weights = [&](const float *p, auto &to) {
+            if constexpr (ADJ) {
+                // one run of 2 V (of V channels that are not turned, its last ones where the head ends)
+                const int back = min(c0, r.width - 2 * V);
+                const auto z = *(const VecOf<float, 2 * V, 1> *)(p + back);
 #pragma unroll
-            for (int i = 0; i < V; ++i) to[0][i] = p[c0 + i], to[1][i] = p[c1 + i];
+                for (int i = 0; i < V; ++i) to[0][i] = back == c0 ? z.e[i] : z.e[V + i], to[1][i] = z.e[V + i];
+            } else {
+                const auto x = *(const VecOf<float, V, 1> *)(p + c0), y = *(const VecOf<float, V, 1> *)(p + c1);
+#pragma unroll
+                for (int i = 0; i < V; ++i) to[0][i] = x.e[i], to[1][i] = y.e[i];
+            }
         };
         auto read = [&](int n) {
             Item m;
@@ -642,10 +655,15 @@ __global__ __launch_bounds__(256) void k_norm_rotary(RotaryArrays r, HeadNorm a,
 #pragma unroll
             for (int i = 0; i < V; ++i) wt[0][i] += a.offset, wt[1][i] += a.offset;
         }
-        Item m = read(first);
+        Item ahead[AHEAD];
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d)
+            if (first + 4 * d < end) ahead[d] = read(first + 4 * d);
         for (int n = first; n < end; n += 4) {
-            Item later;
-            if (n + 4 < end) later = read(n + 4);
+            const Item m = ahead[0];
+#pragma unroll
+            for (int d = 1; d < AHEAD; ++d) ahead[d - 1] = ahead[d];
+            if (n + 4 * AHEAD < end) ahead[AHEAD - 1] = read(n + 4 * AHEAD);
             float u[2][V];
             if constexpr (ADJ) {
 #pragma unroll
@@ -708,7 +726,6 @@ __global__ __launch_bounds__(256) void k_norm_rotary(RotaryArrays r, HeadNorm a,
                 buf_write(out, o0, x);
                 buf_write(out, o1, y);
             }
-            m = later;
         }
     };
     walk(r.q, r.qo, r.sq, r.sqo, a.qw, a.qw_head, r.hq, w.of[0], wave);
