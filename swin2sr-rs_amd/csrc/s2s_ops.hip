@@ -595,8 +595,9 @@ __global__ __launch_bounds__(256) void k_norm_rotary(RotaryArrays r, HeadNorm a,
         sincos_turns((unsigned long long)(long long)pos[x.axis[p]] * x.freq[p], c.y, c.x);
         turn[i] = c;
     }
-    const int len0 = r.lens ? min(r.lens[b0] - at0, n_tok) : n_tok;
-    const int len1 = r.lens && cross < n_tok ? min(r.lens[b0 + 1] + cross, n_tok) : n_tok;
+    // (lengths of any size, past the tokens or negative)
+    const int len0 = r.lens ? min(min(max(r.lens[b0], 0), r.tokens) - at0, n_tok) : n_tok;
+    const int len1 = r.lens && cross < n_tok ? min(min(max(r.lens[b0 + 1], 0), r.tokens) + cross, n_tok) : n_tok;
     // this lane's channels: two runs of V (ADJ: one of 2 V), or one of V that is not turned
     const bool turns = g < rot, there = g < w.per_head;
     const int u0 = !there ? 0 : turns ? (ADJ ? 2 : 1) * g : 2 * rot + (g - rot), u1 = turns ? (ADJ ? u0 + 1 : u0 + rot) : u0;
@@ -605,8 +606,10 @@ __global__ __launch_bounds__(256) void k_norm_rotary(RotaryArrays r, HeadNorm a,
     __syncthreads();
     auto walk = [&](const void *src, void *dst, const Strides &ss, const Strides &ds, const float *weight, long long weight_head, int heads,
                     const NormRotaryWalk::Of &o, int first) {
-        const auto in = buf_rsrc((const T *)src + b0 * ss.b + at0 * ss.t, BUF_MAX_BYTES);
-        const auto out = buf_rsrc((const T *)dst + b0 * ds.b + at0 * ds.t, BUF_MAX_BYTES);
+        // (the resources begin where the first token of either entry lies: the next one's may lie ahead of this one's)
+        const int i_low = cross < n_tok ? min(cross * o.in_t + o.in_b, 0) : 0, o_low = cross < n_tok ? min(cross * o.out_t + o.out_b, 0) : 0;
+        const auto in = buf_rsrc((const T *)src + b0 * ss.b + at0 * ss.t + (long long)i_low * V, BUF_MAX_BYTES);
+        const auto out = buf_rsrc((const T *)dst + b0 * ds.b + at0 * ds.t + (long long)o_low * V, BUF_MAX_BYTES);
         const int end = (n_tok * heads + H - 1) / H;
         struct Item {
             int t, out;
@@ -635,8 +638,8 @@ __global__ __launch_bounds__(256) void k_norm_rotary(RotaryArrays r, HeadNorm a,
             m.t = heads == 1 ? item : (int)__umulhi((unsigned)item, o.by_heads);
             const int h = item - __mul24(m.t, heads), next = m.t < cross ? 0 : 1;
             m.ok = there && m.t < (next ? len1 : len0);
-            const int at = __mul24(m.t, o.in_t) + __mul24(h, o.in_h) + (next ? o.in_b : 0);
-            m.out = __mul24(m.t, o.out_t) + __mul24(h, o.out_h) + (next ? o.out_b : 0);
+            const int at = __mul24(m.t, o.in_t) + __mul24(h, o.in_h) + (next ? o.in_b : 0) - i_low;
+            m.out = __mul24(m.t, o.out_t) + __mul24(h, o.out_h) + (next ? o.out_b : 0) - o_low;
             const int i0 = m.ok ? (at + u0) * UNIT : BUF_OOB, i1 = m.ok && turns ? (at + u1) * UNIT : BUF_OOB;
             if constexpr (ADJ) {
                 // (a lane of channels that are not turned reads V of them)

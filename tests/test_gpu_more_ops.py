@@ -527,3 +527,310 @@ def test_shared_ways_hide_what_keys_hold(pkg, name):
         sk[S - 80:], sv[S - 70:] = np.nan, -np.inf
         sv[S // 2, 0, 3], sv[S // 2 + 1, -1, 5], sk[S // 2 + 70, -1, 0] = np.inf, np.nan, np.nan
     check_shared(pkg, c, past)
+
+
+# ---- calls at the edges ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("L", [1, 3, 50])
+def test_norm_rotary_lengths_of_any_size(pkg, L):
+    """Lengths past the tokens write them all, negative ones none, at an int's ends too."""
+    lens = [2 ** 31 - 1, -2 ** 31, 2, 0, 2 ** 31 - 1, -1, L]
+    turned(pkg, "bf16", 7, L, 3, 2, 64, (16, 16), lens=lens)
+    turned(pkg, "f32", 7, L, 3, 2, 31, (5,), lens=lens, adjacent=True)
+
+
+def test_norm_rotary_strides_past_32_bits(pkg):
+    """Tokens, heads and batch entries 3 GB apart."""
+    D, g = 16, np.random.default_rng(2)
+    x, w = R.round_to(g.standard_normal((2, 2, 2, D)), "f16"), np.ones(D, np.float32)
+    pos = R.Dev(pkg, g.integers(0, 100, (2, 2, 1)).astype(np.int32), "f32", whole=True)
+    dw, plain, rot, A = R.Dev(pkg, w, "f32"), R.Dev(pkg, x, "f16"), pkg.ops.NormRotary.of((8,)), pkg.ops.Array
+    rot(plain.array, pos.array, dw.array)
+    want, far, vp = plain.get(), (3 << 30) // 2, C.c_void_p
+    for strides in ((far, D, 2 * D, 1), (2 * D, far, D, 1), (4 * D, 2 * D, far, 1)):
+        buf = pkg.hip.DeviceBuffer((far + 8 * D) // 2)
+        places = [(b, t, h, (b * strides[0] + t * strides[1] + h * strides[2]) * 2) for b in (0, 1) for t in (0, 1) for h in (0, 1)]
+        for b, t, h, at in places:
+            row = np.ascontiguousarray(R.to_bits(x[b, t, h], "f16"))
+            assert pkg.hip.rt().hipMemcpy(vp(buf.ptr + at), row.ctypes.data_as(vp), row.nbytes, 1) == 0
+        rot(A(buf.ptr, (2, 2, 2, D), "f16", strides), pos.array, dw.array)
+        for b, t, h, at in places:
+            row = np.empty(D, np.uint16)
+            assert pkg.hip.rt().hipMemcpy(row.ctypes.data_as(vp), vp(buf.ptr + at), row.nbytes, 2) == 0
+            # (another kernel where strides pass 32 bits: two evaluations of at most the bound each, and a step of f16)
+            assert np.abs(R.from_bits(row, "f16") - want[b, t, h]).max() <= 2.0 ** -10 * np.abs(want[b, t, h]).max()
+        buf.free()
+
+
+def test_norm_rotary_more_tokens_than_workgroups(pkg):
+    """2^28 + 2^14 tokens of one pair, the batch's entries all the same: each is the first one."""
+    batch, tokens = 2 ** 14 + 1, 2 ** 14
+    g = np.random.default_rng(3)
+    q, w = R.Dev(pkg, R.round_to(g.standard_normal((1, tokens, 1, 2)), "f16"), "f16"), R.Dev(pkg, np.array([1.0, 0.5]), "f32")
+    pos = R.Dev(pkg, g.integers(0, 2 ** 31 - 1, (1, tokens, 1)).astype(np.int32), "f32", whole=True)
+    out, one = pkg.hip.DeviceBuffer(batch * tokens), R.Dev(pkg, np.zeros((1, tokens, 1, 2)), "f16")
+    rot, A = pkg.ops.NormRotary([0.7], [0]), pkg.ops.Array
+    rot(q.array, pos.array, w.array, one.array)
+    rot(A(q.array.ptr, (batch, tokens, 1, 2), "f16", (0, 2, 2, 1)), A(pos.array.ptr, (tokens, 1), "i32"), w.array,
+        A(out.ptr, (batch, tokens, 1, 2), "f16"))
+    pkg.hip.synchronize()
+    want, got = one.bits().view(np.uint32).reshape(-1)[:tokens], out.download().view(np.uint32).reshape(batch, tokens)
+    out.free()
+    assert (got == want).all()
+
+
+@pytest.mark.parametrize("order", [(1, 0, 2, 3), (2, 1, 0, 3), (1, 2, 0, 3), (2, 0, 1, 3)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_norm_rotary_entries_side_by_side(pkg, order, in_place):
+    """A token's entries, or a head's, next to each other: the next entry's first token lies ahead of this one's last."""
+    for dtype, adjacent, D in (("bf16", False, 64), ("f32", True, 30)):
+        T.ORDERS["other"] = order
+        try:
+            turned(pkg, dtype, 9, 7, 3, 2, D, (5, 4), adjacent=adjacent, order="other", in_place=in_place)
+            turned(pkg, dtype, 3, 500, 3, 2, D, (5, 4), adjacent=adjacent, order="other", in_place=in_place, lens=[500, 13, 499])
+        finally:
+            del T.ORDERS["other"]
+
+
+@pytest.mark.parametrize("op", ["window", "shared"])
+@pytest.mark.parametrize("Lq", [1, 40])
+def test_offsets_past_32_bits(pkg, op, Lq):
+    """Keys 4 MiB apart: 8.8 GB from the first to the last."""
+    Lk, D, stride, vp = 2100, 64, 1 << 21, C.c_void_p
+    g = np.random.default_rng(1)
+    q, k, v = (R.round_to(g.standard_normal(s), "bf16") for s in ((1, Lq, 2, D), (1, Lk, 1, D), (1, Lk, 1, D)))
+    buf = pkg.hip.DeviceBuffer((stride * (Lk - 1) + 2 * D + 1) // 2)
+    rows = np.concatenate([R.to_bits(k[0, :, 0], "bf16"), R.to_bits(v[0, :, 0], "bf16")], 1)
+    for j in range(Lk):
+        row = np.ascontiguousarray(rows[j])
+        assert pkg.hip.rt().hipMemcpy(vp(buf.ptr + j * stride * 2), row.ctypes.data_as(vp), row.nbytes, 1) == 0
+    qd, out, A = R.Dev(pkg, q, "bf16"), R.Dev(pkg, np.zeros(q.shape), "bf16"), pkg.ops.Array
+    scale = np.float64(np.float32(D ** -0.5))
+    if op == "window":
+        kd, vd = (A(buf.ptr + off, (1, Lk, 1, D), "bf16", (0, stride, 0, 1)) for off in (0, 2 * D))
+        p = pkg.ops.Attention("bf16", 1, Lq, Lk, 2, 1, D, causal=True, window=700, sinks=70)
+        ws = R.Dev(pkg, np.zeros(max(p.workspace_bytes // 4, 1)), "f32")
+        p(qd.array, kd, vd, out.array, workspace=ws.array)
+        want, bound, _ = R.attention("bf16", q, k, v, scale, causal=True, window=700, sinks=70)
+    else:
+        n = Lk - 60
+        sk, sv = (A(buf.ptr + off, (n, 1, D), "bf16", (stride, 0, 1)) for off in (0, 2 * D))
+        kd, vd = (A(buf.ptr + off + n * stride * 2, (1, 60, 1, D), "bf16", (0, stride, 0, 1)) for off in (0, 2 * D))
+        p = pkg.ops.SharedAttention("bf16", 1, Lq, n, 60, 2, 1, D, causal=True)
+        ws = R.Dev(pkg, np.zeros(max(p.workspace_bytes // 4, 1)), "f32")
+        p(qd.array, sk, sv, kd, vd, out.array, workspace=ws.array)
+        want, bound, _ = R.attention("bf16", q, k, v, scale, causal=True)
+    got = out.get()
+    buf.free()
+    assert (np.abs(got - want) <= bound + 8 * 2.0 ** -24 * np.abs(want)).all()
+
+
+def test_strides_of_one(pkg):
+    """The stride of a dimension of one counts for nothing, the shared keys' batch stride neither."""
+    c = scase("bf16", S=1, B=1, Lq=1, Lk=1, H=2, KV=1, D=64)
+    arrays = shared_inputs(c)
+    p, ws, d, m, scale = shared_setup(pkg, c, arrays)
+    want, bound, _ = shared_want(c, *arrays, scale)
+    A = pkg.ops.Array
+    for odd in (0, 1, (1 << 23) + 1):
+        d["out"].buf.upload(np.zeros(d["out"].buf.n, np.float32))
+        a = {n: A(d[n].array.ptr, d[n].array.shape, "bf16", (odd, odd, 64 if n in ("q", "out") else odd, 1)) for n in ("q", "k", "v", "out")}
+        s = {n: A(d[n].array.ptr, (1, 1, 64), "bf16", (odd, odd, 1)) for n in ("shared_k", "shared_v")}
+        p(a["q"], s["shared_k"], s["shared_v"], a["k"], a["v"], a["out"], workspace=ws.array)
+        assert (np.abs(d["out"].get() - want) <= bound + 8 * 2.0 ** -24 * np.abs(want)).all()
+
+
+def test_keys_of_all_tokens_one_row(pkg):
+    """Strides of zero: one shared row and one own row for all tokens."""
+    for dtype, Lq in (("bf16", 1), ("f32", 1), ("f16", 40)):
+        c = scase(dtype, S=700, B=3, Lq=Lq, Lk=70, H=2, KV=2, D=64)
+        q, k, v, sk, sv, more = shared_inputs(c)
+        k[:], v[:], sk[:], sv[:] = k[:1, :1], v[:1, :1], sk[:1], sv[:1]
+        p, ws, d, m, scale = shared_setup(pkg, c, (q, k, v, sk, sv, more))
+        want, bound, _ = shared_want(c, q, k, v, sk, sv, more, scale)
+        A = pkg.ops.Array
+        one = [A(d[n].array.ptr, (700, 2, 64), dtype, (0, 700 * 64, 1)) for n in ("shared_k", "shared_v")]
+        one += [A(d[n].array.ptr, (3, 70, 2, 64), dtype, (0, 0, 64, 1)) for n in "kv"]
+        p(d["q"].array, *one, d["out"].array, workspace=ws.array)
+        assert (np.abs(d["out"].get() - want) <= bound + 8 * 2.0 ** -24 * np.abs(want)).all()
+
+
+def test_operators_are_deterministic(pkg):
+    """The same call gives the same bits, whatever order its workgroups come in."""
+    for c in (wcase("bf16", B=2, Lq=700, Lk=700, H=4, KV=2, D=64, causal=True, window=99, sinks=3),
+              wcase("f16", Lq=1, Lk=20000, H=8, KV=1, D=64, order="cache", causal=True, window=9000, sinks=3)):
+        d, m = T.upload(pkg, c, *T.inputs(c))
+        p, ws, _ = window_plan(pkg, c)
+        seen = set()
+        for _ in range(6):
+            T.call(p, ws, d, m)
+            seen.add(d["out"].bits().tobytes())
+        assert len(seen) == 1
+    for c in (SHARED["step_many"], SHARED["tail"], WAYS["bf16_32_many"], WAYS["whole_ranges"]):
+        p, ws, d, m, _ = shared_setup(pkg, c, shared_inputs(c))
+        seen = set()
+        for _ in range(6):
+            shared_call(p, ws, d, m)
+            seen.add(d["out"].bits().tobytes())
+        assert len(seen) == 1
+
+
+# ---- the operators one after another, on streams and in graphs ------------------------------------
+
+
+class Tail:
+    """What several views of one image do with it, in one batch: the image's tokens are normed, turned and
+    attended to in a window once; then every view's tokens, normed and turned, attend to the image's keys (shared) and
+    their own, and one step of one token each follows, over the views' windows."""
+
+    def __init__(self, pkg, seed, tokens=600, views=5, own=40, heads=4, kv=2, D=64, dtype="bf16"):
+        self.pkg, self.D, self.heads, self.kv, self.dtype = pkg, D, heads, kv, dtype
+        self.tokens, self.views, self.own = tokens, views, own
+        g = np.random.default_rng(seed)
+        up = lambda v, t=dtype: R.Dev(pkg, v, t, whole=np.asarray(v).dtype == np.int32)  # noqa: E731
+        rows = heads + 2 * kv
+        self.x, self.y = (R.round_to(g.standard_normal((b, n, rows, D)), dtype) for b, n in ((1, tokens), (views, own)))
+        self.w = [(1 + 0.2 * g.standard_normal(s)).astype(np.float32) for s in ((heads, D), (D,))]
+        self.pos = [np.stack([np.arange(n) // 25, np.arange(n) % 25], 1)[None].repeat(b, 0).astype(np.int32) for b, n in ((1, tokens), (views, own))]
+        self.lens = np.array([own - 7 * i for i in range(views)], np.int32)
+        self.dx, self.dy, self.dw, self.dpos, self.dlens = up(self.x), up(self.y), [up(v, "f32") for v in self.w], [up(p) for p in self.pos], up(self.lens)
+        zeros = lambda *s: up(np.zeros(s))  # noqa: E731
+        self.tx, self.ty = zeros(1, tokens, heads + kv, D), zeros(views, own, heads + kv, D)
+        self.ox, self.oy, self.last = zeros(1, tokens, heads, D), zeros(views, own, heads, D), zeros(views, 1, heads, D)
+        self.turn = pkg.ops.NormRotary.of((16, 16), eps=1e-5)
+        self.windows = pkg.ops.Attention(dtype, 1, tokens, tokens, heads, kv, D, causal=True, window=100, sinks=4)
+        self.shared = pkg.ops.SharedAttention(dtype, views, own, tokens, own, heads, kv, D, causal=True)
+        self.step = pkg.ops.Attention(dtype, views, 1, own, heads, kv, D, causal=True, window=16, sinks=2)
+        self.steps = pkg.ops.SharedAttention(dtype, views, 1, tokens, own, heads, kv, D, causal=True)
+        self.last2 = zeros(views, 1, heads, D)
+        n = max(p.workspace_bytes for p in (self.windows, self.shared, self.step, self.steps))
+        self.ws = up(np.full(n // 4 + 1, np.nan), "f32")
+        self.outputs = (self.tx, self.ty, self.ox, self.oy, self.last, self.last2)
+
+    def part(self, dev, first, n):
+        """Heads first to first + n of an array, as an array."""
+        size = 4 if self.dtype == "f32" else 2
+        return self.pkg.ops.Array(dev.array.ptr + first * self.D * size, dev.shape[:2] + (n, self.D), self.dtype, dev.array.stride())
+
+    def run(self, stream=0):
+        H, KV, A = self.heads, self.kv, self.pkg.ops.Array
+        for x, t, pos, lens in ((self.dx, self.tx, self.dpos[0], None), (self.dy, self.ty, self.dpos[1], self.dlens)):
+            self.turn(self.part(x, 0, H), pos.array, self.dw[0].array, self.part(t, 0, H), k=self.part(x, H, KV), k_weight=self.dw[1].array,
+                      k_out=self.part(t, H, KV), lens=lens.array if lens else None, stream=stream)
+        k, v = self.part(self.tx, H, KV), self.part(self.dx, H + KV, KV)
+        self.windows(self.part(self.tx, 0, H), k, v, self.ox.array, workspace=self.ws.array, stream=stream)
+        sk, sv = (A(a.ptr, a.shape[1:], self.dtype, a.stride()[1:]) for a in (k, v))
+        yk, yv = self.part(self.ty, H, KV), self.part(self.dy, H + KV, KV)
+        self.shared(self.part(self.ty, 0, H), sk, sv, yk, yv, self.oy.array, workspace=self.ws.array, stream=stream, q_lens=self.dlens.array,
+                    k_lens=self.dlens.array)
+        one = self.part(self.ty, 0, H)
+        q = A(one.ptr, (self.views, 1, H, self.D), self.dtype, one.stride())
+        self.step(q, yk, yv, self.last.array, workspace=self.ws.array, stream=stream, k_lens=self.dlens.array)
+        self.steps(q, sk, sv, yk, yv, self.last2.array, workspace=self.ws.array, stream=stream, k_lens=self.dlens.array)
+
+    def bits(self):
+        return b"".join(d.bits().tobytes() for d in self.outputs)
+
+    def clear(self):
+        for d in self.outputs:
+            d.buf.upload(np.zeros(d.buf.n, np.float32))
+        self.pkg.hip.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_operators_together(pkg, dtype):
+    """Each stage against 64 bits from what the stage before left in memory."""
+    b = Tail(pkg, 0, dtype=dtype)
+    b.run()
+    pkg.hip.synchronize()
+    H, KV, D = b.heads, b.kv, b.D
+    axis, freq = np.array(b.turn.pair_axis[:]), np.array(b.turn.inv_freq[:])
+    for x, t, pos, lens in ((b.x, b.tx.get(), b.pos[0], [b.tokens]), (b.y, b.ty.get(), b.pos[1], b.lens)):
+        angle = pos[..., axis] * freq
+        for first, n, w in ((0, H, b.w[0]), (H, KV, b.w[1])):
+            want, bound = R.norm_rotary(dtype, x[:, :, first:first + n], w, 0.0, np.float64(np.float32(1e-5)), angle, 32, False, False)
+            for i, m in enumerate(lens):
+                assert (np.abs(t[i, :m, first:first + n] - want[i, :m]) <= bound[i, :m]).all()
+                assert not t[i, m:].any()
+    tx, ty, scale = b.tx.get(), b.ty.get(), np.float64(np.float32(D ** -0.5))
+    k, v = tx[:, :, H:], b.x[:, :, H + KV:]
+    want, bound, _ = R.attention(dtype, tx[:, :, :H], k, v, scale, causal=True, window=100, sinks=4)
+    assert (np.abs(b.ox.get() - want) <= bound).all()
+    oy, last, last2 = b.oy.get(), b.last.get(), b.last2.get()
+    for i, m in enumerate(b.lens):
+        q, yk, yv = ty[i:i + 1, :m, :H], ty[i:i + 1, :m, H:], b.y[i:i + 1, :m, H + KV:]
+        kk, vv = np.concatenate((k, yk), 1), np.concatenate((v, yv), 1)
+        want, bound, _ = R.attention(dtype, q, kk, vv, scale, causal=True)
+        assert (np.abs(oy[i, :m] - want[0]) <= bound[0] + 8 * 2.0 ** -24 * np.abs(want[0])).all() and not oy[i, m:].any()
+        want, bound, _ = R.attention(dtype, ty[i:i + 1, :1, :H], yk, yv, scale, causal=True, window=16, sinks=2)
+        assert (np.abs(last[i] - want[0]) <= bound[0]).all()
+        want, bound, _ = R.attention(dtype, ty[i:i + 1, :1, :H], kk, vv, scale, causal=True)
+        assert (np.abs(last2[i] - want[0]) <= bound[0] + 8 * 2.0 ** -24 * np.abs(want[0])).all()
+
+
+def test_operators_together_on_streams(pkg):
+    """Two runs on streams of their own, at once, are each the run on the default stream."""
+    runs, want = [Tail(pkg, s) for s in (1, 2)], []
+    for b in runs:
+        b.run()
+        pkg.hip.synchronize()
+        want.append(b.bits())
+        b.clear()
+    streams = [T.new_stream(pkg) for _ in runs]
+    for _ in range(3):
+        for b, st in zip(runs, streams):
+            b.run(stream=st.value)
+    for st in streams:
+        pkg.hip.stream_synchronize(st.value)
+    assert [b.bits() for b in runs] == want
+    for st in streams:
+        pkg.hip.rt().hipStreamDestroy(st)
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2])
+def test_operators_together_captured(pkg, mode):
+    """Captured in each mode: every replay, with eager work of another run between, is the eager run on the inputs of the
+    moment; two graphs with workspaces of their own run at once."""
+    h, vp = pkg.hip.rt(), C.c_void_p
+    for name, args in {"hipStreamBeginCapture": [vp, C.c_int], "hipStreamEndCapture": [vp, C.POINTER(vp)],
+                       "hipGraphInstantiate": [C.POINTER(vp), vp, vp, vp, C.c_size_t], "hipGraphLaunch": [vp, vp],
+                       "hipGraphExecDestroy": [vp], "hipGraphDestroy": [vp]}.items():
+        getattr(h, name).argtypes = args
+    runs, other, st, two = [Tail(pkg, s) for s in (3, 4)], Tail(pkg, 5), T.new_stream(pkg), T.new_stream(pkg)
+    graphs, execs = [], []
+    for b in runs:
+        b.run()
+        pkg.hip.synchronize()
+        assert h.hipStreamBeginCapture(st, mode) == 0
+        b.run(stream=st.value)
+        g, e = vp(), vp()
+        assert h.hipStreamEndCapture(st, C.byref(g)) == 0
+        assert h.hipGraphInstantiate(C.byref(e), g, None, None, 0) == 0
+        graphs.append(g)
+        execs.append(e)
+    for turn in range(4):
+        want = []
+        for b, e in zip(runs, execs):
+            b.x = R.round_to(np.random.default_rng(10 + turn).standard_normal(b.x.shape), b.dtype)
+            b.dx.buf.upload(np.frombuffer(R.to_bits(b.x, b.dtype).tobytes(), np.float32))
+            b.run()
+            pkg.hip.synchronize()
+            want.append(b.bits())
+            b.clear()
+            assert h.hipGraphLaunch(e, st) == 0
+            other.run()
+            pkg.hip.stream_synchronize(st.value)
+            pkg.hip.synchronize()
+            assert b.bits() == want[-1], turn
+            b.clear()
+        for e, s in zip(execs, (st, two)):
+            assert h.hipGraphLaunch(e, s) == 0
+        for s in (st, two):
+            pkg.hip.stream_synchronize(s.value)
+        assert [b.bits() for b in runs] == want
+    for e, g in zip(execs, graphs):
+        h.hipGraphExecDestroy(e)
+        h.hipGraphDestroy(g)
+    for s in (st, two):
+        h.hipStreamDestroy(s)
