@@ -155,9 +155,9 @@ class Attention:
         self.q_shape, self.k_shape = (batch, q_tokens, q_heads, width), (batch, k_tokens, k_heads, width)
         a = Attention_(*self.head)
         n = C.c_uint64()
-        self.window = (window, sinks)
+        self.window = (int(window), int(sinks))
         if window:
-            check(self.lib.s2s_window_attention_workspace(C.byref(a), window, sinks, C.byref(n)), "attention")
+            check(self.lib.s2s_window_attention_workspace(C.byref(a), *self.window, C.byref(n)), "attention")
         else:
             _need(sinks == 0, "attention: sinks without a window")
             check(self.lib.s2s_attention_workspace(C.byref(a), C.byref(n)), "attention")

@@ -508,6 +508,8 @@ WAYS = {
     "step_30_f32_many": scase("f32", S=1100, B=270, Lq=1, Lk=20, H=2, KV=2, D=30, causal=True),
     "step_62_f16": scase("f16", S=1100, B=70, Lq=1, Lk=80, H=8, KV=2, D=62, causal=True, cap=30.0),
     "step_300_columns": scase("bf16", S=1100, B=75, Lq=1, Lk=80, H=8, KV=2, D=128, causal=True, k_lens=[i % 81 for i in range(75)]),
+    "no_shared_long": scase("bf16", S=0, B=4, Lq=1, Lk=900, H=8, KV=2, D=64, causal=True),
+    "no_own_step": scase("f16", S=1500, B=4, Lq=1, Lk=0, H=8, KV=2, D=64, causal=True),
     "step_nine_tiles": scase("bf16", S=505, B=3, Lq=1, Lk=10, H=8, KV=2, D=64, causal=True),
 }
 
