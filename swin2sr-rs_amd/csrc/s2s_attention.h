@@ -564,7 +564,8 @@ struct Kernel {
             }
             u.kl = kl;
             // what all columns' windows hold begins here, and what any holds
-            const int wg_from = start(i_last), w_from = start(w_last), w_low = start(w_first);
+            // (in tiles: t_from, and the sinks' whole ones)
+            const int w_low = start(w_first), t_from = WIN ? (start(i_last) + TK - 1) / TK : 0, t_whole = WIN ? a.sinks / TK : 0;
             // documents of the workgroup's columns and of the wave's, where key tiles can be passed
             // over
             int q_lo = 0, q_hi = 0, w_lo = 0, w_hi = 0;
@@ -727,7 +728,7 @@ struct Kernel {
                 if (!ahead && tn < t_end) stage(tn, buf ^ 1);
                 ahead = false;
                 const int at_buf = buf * 2 * (int)kTile;
-                const bool inside = !WIN || t * TK >= wg_from || t * TK + TK <= a.sinks;
+                const bool inside = !WIN || t >= t_from || t < t_whole;
                 if ((RETRY && careful) || !(t * TK + TK <= wg_min && (docs & ONE) && inside) || (GEN && u.table)) {
                     // a masked key's weight is zero, and zero times an infinity is none: with
                     // such values in the V of a tile that not every column reads whole, they are
@@ -745,9 +746,8 @@ struct Kernel {
                     }
                 }
                 const int j0 = t * TK + (WK ? 16 * wave : 0);  // the wave's first key
-                if (j0 < w_max && (docs & MINE) && (!WIN || j0 + 16 * KB > w_low || j0 < a.sinks)) {
-                    const bool all = !WIN || j0 >= w_from || j0 + 16 * KB <= a.sinks;
-                    const bool full = j0 + 16 * KB <= w_min && all && (docs & SAME) && !(GEN && u.table);
+                if (j0 < w_max && (docs & MINE) && (!WIN || j0 + 16 * KB > w_low || t < t_sinks)) {
+                    const bool full = j0 + 16 * KB <= w_min && inside && (docs & SAME) && !(GEN && u.table);
                     tile(u, opaque(kl0 + at_buf), opaque(vl0 + at_buf), j0, full, j0 + 16 * KB <= w_at + 1, base + kIds + buf * 256 + (WK ? 64 * wave : 0), lim, low, doc, at, slope, tab, qf, o, m, l);
                 }
                 t = tn, docs = docs_n;
