@@ -256,7 +256,8 @@ int s2s_profile_only(s2s_ctx *ctx, const char *kernel);
 int s2s_rstb_device(s2s_ctx *ctx, int stage, int hp, int wp, const float *d_in, float *d_out);
 
 /* ---- transformer operators on device buffers ------------------------------- */
-/* Attention, rotary positions and the root-mean-square norm for tokens of any
+/* Attention (also with a sliding window, and of a batch that shares its first keys),
+ * rotary positions (also of normed heads) and the root-mean-square norm for tokens of any
  * count and layout, where the forward above has window attention on 8x8
  * windows, a 15x15 position-bias table and LayerNorm. No reference counterpart.
  *
@@ -348,7 +349,8 @@ int s2s_window_attention(const s2s_attention_args *args, int window, int sinks, 
  * memory once and are read once for all of them: entry b's keys are the shared ones
  * j < shared_lens[b], and behind them its own. The query's place is P(i) =
  * shared_lens[b] + k_lens[b] - q_lens[b] + i; masks (`causal`, lengths), cap and slopes are as
- * above. `own` holds the call's sizes (k_tokens of each entry's own keys, 0
+ * above. (For f16 and bf16 the weights of shared keys are rounded to the type unless
+ * at most 16 queries times heads of the whole batch read a key head.) `own` holds the call's sizes (k_tokens of each entry's own keys, 0
  * allowed), arrays and masks; its prefix, documents, positions and table have to be
  * NULL. Lengths are taken as clamped to the tokens. Up to 2^30 shared and own
  * tokens, 2^26 query tokens times heads of the batch. The workspace goes by dtype

@@ -4,8 +4,9 @@ Layout of this package:
   csrc/            the HIP kernels and the C ABI (include/swin2sr_hip.h)
   Makefile         builds libswin2sr_hip.so with hipcc --offload-arch=gfx950
   abi.py           ctypes binding of the ABI and the `Backend` mirror (HipBackend)
-  ops.py           the transformer operators on device buffers: attention, rotary
-                   positions, root-mean-square norm
+  ops.py           the transformer operators on device buffers: attention (whole, windowed,
+                   over a shared prefix), rotary positions (of normed heads too),
+                   root-mean-square norm
   model.py         architectures, synthetic checkpoints (crate tensor names) and inputs
   tiling.py        the crate's tile loop and memory policy over the Backend interface
   formats.py       the crate's on-disk formats: converted-checkpoint safetensors with the

@@ -28,6 +28,13 @@
 // sequences of up to 8192 keys, 8 x 128 bf16: 135 us, 5.07 TB/s). Small windows (1089
 // of 64 f32 tokens, 6 heads of 30, table and bands): the 733 VALU and 584 scalar instructions of a
 // wave for 16 columns, 79 us.
+//
+// With a sliding window (WINDOW) a column has a first key beside its last, and the key tiles between the sinks'
+// and the workgroup's first window are passed over: 16391 causal bf16 tokens, 16 / 4 heads of 128, window 4096,
+// 495 us (970 TFLOP/s), the next token of 32 sequences over 4096 keys 101 us (5.3 TB/s). Keys that a batch
+// shares are walked by every entry's columns ahead of its own (WHOLE: 8 x 500 bf16 tokens behind 8191 shared keys, 32 / 8 heads
+// of 128, 517 us, 1,070 TFLOP/s), or once by the columns of all entries (SHARED), in one launch with the entries' own
+// keys (k_attn_both: 64 steps over 16384 and up to 1024 keys 66 us with the join, 80 in three launches).
 #pragma once
 
 #include <algorithm>
@@ -1426,7 +1433,7 @@ hipError_t join(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
     constexpr int N = 256 / (DP / 4);
     if (L.splits + (SHARE ? L.shared_splits : 0) <= kFewRanges && rows >= 4 * cu_count())
         return enqueue(k_attn_join_few<T, DP, SHARE>, dim3((unsigned)((rows + N - 1) / N)), dim3(256), 0, st, a, L, (int)rows);
-    // up to 32 ranges: 2048 columns of 17 ranges (64 steps over 16384 shared keys) 5.9 us, 8.0 by a workgroup a column
+    // up to 32 ranges: 2048 columns of 9 ranges (64 steps over 16384 shared keys) 5.9 us, 8.0 by a workgroup a column
     if constexpr (SHARE)
         if (L.splits + L.shared_splits <= kSomeRanges && rows >= 4 * cu_count())
             return enqueue(k_attn_join_some<T, DP, SHARE>, dim3((unsigned)((rows + N - 1) / N)), dim3(256), 0, st, a, L, (int)rows);

@@ -1,5 +1,5 @@
-// s2s_ops.hip - rotary positions with several axes, and the root-mean-square
-// norm with the residual's addition and an e4m3 output. Both are bound by HBM:
+// s2s_ops.hip - rotary positions with several axes, the same behind a norm of each head, and the
+// root-mean-square norm with the residual's addition and an e4m3 output. All are bound by HBM:
 // every element is read once and written once. Measured on an MI355X, whose plain
 // copy of 1 GiB makes 5.05 TB/s: rotary of 16384 tokens, 32 + 8 bf16 heads of 128, 64 us
 // (5.2 TB/s); the norm of 16391 x 5120 bf16 with residual, sum and e4m3 groups of 128, 115 us

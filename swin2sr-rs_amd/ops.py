@@ -1,7 +1,9 @@
 """The transformer operators of include/swin2sr_hip.h on arrays in HBM: attention
 (capped scores, distance biases, document, causal and prefix masks, padded
-batches, grouped heads), rotary positions with several axes, and the
-root-mean-square norm with the residual's addition and an 8-bit output.
+batches, grouped heads, sliding windows with sinks) and attention of a batch that
+shares its first keys, rotary positions with several axes, of heads that are normed
+first too, and the root-mean-square norm with the residual's addition and an 8-bit
+output.
 
 Arrays are anything with `data_ptr()`, `shape`, `stride()` and `dtype` as torch
 tensors have them (torch itself is not imported here; a process that uses it
