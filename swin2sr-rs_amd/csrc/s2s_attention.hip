@@ -381,7 +381,8 @@ bool goes_whole(int dtype, const AttnOpArgs &a, int tk, int align, bool general)
 
 // The most that any way of these sizes needs: which one runs goes by strides and numbers too.
 size_t shared_attn_op_workspace(int dtype, const AttnOpArgs &a) {
-    size_t most = sums_bytes(own_cut(dtype, a), a) + sums_bytes(shared_cut(dtype, a), a);
+    const bool ranges = !goes_whole(dtype, a, cut_of(dtype, a, true).tk, 16, false);
+    size_t most = ranges ? sums_bytes(own_cut(dtype, a), a) + sums_bytes(shared_cut(dtype, a), a) : 0;
     for (const bool narrow : {false, true}) {
         const attn::Cut c = whole_cut(dtype, a, narrow);
         if (c.splits > 1) most = std::max(most, sums_bytes(c, a));

@@ -161,6 +161,14 @@ def test_shared_nothing_to_do(pkg):
         shared(pkg, **more)(arr(pkg, (b, n, 4, 64)), s, s, arr(pkg, (b, 7, 2, 64)), arr(pkg, (b, 7, 2, 64)), arr(pkg, (b, n, 4, 64)))
 
 
+def test_shared_workspace_goes_by_the_way(pkg):
+    """Whole keys over enough column tiles need no sums, a step over long keys does."""
+    assert shared(pkg, batch=64, q_tokens=500, shared_tokens=8000, k_tokens=500, q_heads=32, k_heads=8, width=128).workspace_bytes == 0
+    step = dict(q_tokens=1, k_tokens=64, q_heads=32, k_heads=8, width=128)
+    assert shared(pkg, batch=4, shared_tokens=300, **step).workspace_bytes == 0
+    assert 0 < shared(pkg, batch=4, shared_tokens=3000, **step).workspace_bytes < shared(pkg, batch=40, shared_tokens=3000, **step).workspace_bytes
+
+
 # ---- the C interface ------------------------------------------------------------------
 
 STRUCTS = [("S2sSharedAttentionArgs", "s2s_shared_attention_args", "SharedAttention_", "_SHARED"),
