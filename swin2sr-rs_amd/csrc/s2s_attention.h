@@ -765,7 +765,8 @@ struct Kernel {
                 }
             }
             // What the rounding of a weight left may be zero, and zero times an infinity is none: a sum that is
-            // no number of weights that are is made again, with the infinities of v by themselves.
+            // no number of weights that are is made again, with the infinities of v by themselves. (One query over 131071
+            // keys 20.9 -> 21.3 us for the look; no other call by more than two runs differ.)
             if (RETRY && !careful && part == (ALL ? 1 : 0)) {
                 bool none = false;
 #pragma unroll
@@ -1208,7 +1209,8 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnOpArgs a, AttnLaunch L) {
 }
 
 // The columns of all entries over the shared keys, `shared` workgroups, and each entry's few columns over its own keys
-// in one launch: the first are bound by instructions, the second by HBM, and a CU takes both.
+// in one launch: the first are bound by instructions, the second by HBM, and a CU takes both (64 steps over 16384 shared
+// and 640 own keys, 32 / 8 bf16 heads of 128: 56 us with the join, 78 in a launch each).
 template <typename T, int DP, int NB, bool WK, int ALIGN, bool OWN_WK>
 __global__ __launch_bounds__(256, 2) void k_attn_both(AttnOpArgs a, AttnLaunch own, AttnLaunch shared, int blocks) {
     extern __shared__ __align__(16) char lds[];

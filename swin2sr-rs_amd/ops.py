@@ -94,7 +94,7 @@ def _contiguous(a) -> bool:
 
 def _tokens(a, shape, dtype: int, op: str, name: str):
     """An array [batch][tokens][heads][width] as its C struct's fields."""
-    if a.shape != shape or _type(a.dtype) != dtype:
+    if a.shape != shape or (_codes.get(a.dtype) != dtype and _type(a.dtype) != dtype):
         raise S2SError(f"{op}: {name} is {tuple(a.shape)} of {a.dtype}, wanted {shape} of the call's type")
     b, t, h, d = a.stride()
     if d != 1 and shape[3] > 1:
@@ -115,7 +115,8 @@ def _vector(a, n: int, op: str, name: str):
     """A contiguous int32 vector of n: its address, 0 for none."""
     if a is None:
         return 0
-    _need(tuple(a.shape) == (n,) and _is_int32(a.dtype) and _contiguous(a), f"{op}: {name} is no int32 vector of {n}")
+    if tuple(a.shape) != (n,) or not _is_int32(a.dtype) or not _contiguous(a):
+        raise S2SError(f"{op}: {name} is no int32 vector of {n}")
     return a.data_ptr()
 
 
@@ -124,8 +125,8 @@ def _per_token(a, batch: int, tokens: int, op: str, name: str):
     if a is None:
         return 0, 0
     shape, s = tuple(a.shape), tuple(a.stride())
-    _need(_is_int32(a.dtype) and shape in ((tokens,), (batch, tokens)) and (s[-1] == 1 or tokens <= 1),
-          f"{op}: {name} is not int32 [{batch}][{tokens}] or [{tokens}] with adjacent tokens")
+    if not _is_int32(a.dtype) or shape not in ((tokens,), (batch, tokens)) or (s[-1] != 1 and tokens > 1):
+        raise S2SError(f"{op}: {name} is not int32 [{batch}][{tokens}] or [{tokens}] with adjacent tokens")
     return a.data_ptr(), (s[0] if len(shape) == 2 else 0)
 
 
@@ -184,8 +185,8 @@ class Attention:
             pos = (a, b, sa, sb)
         slope_ptr = table_ptr = entries = 0
         if slopes is not None:
-            _need(slopes.shape == (self.q_heads,) and _is_f32(slopes.dtype) and _contiguous(slopes),
-                  f"{op}: slopes is no f32 vector of {self.q_heads}")
+            if slopes.shape != (self.q_heads,) or not _is_f32(slopes.dtype) or not _contiguous(slopes):
+                raise S2SError(f"{op}: slopes is no f32 vector of {self.q_heads}")
             slope_ptr = slopes.data_ptr()
         if table is not None:
             _need(len(table.shape) == 2 and table.shape[0] == self.q_heads and _is_f32(table.dtype) and _contiguous(table),
@@ -234,8 +235,8 @@ class SharedAttention:
                   *_tokens(v, self.k_shape, dt, op, "v"), *_tokens(out, self.q_shape, dt, op, "out"))
         slope_ptr = 0
         if slopes is not None:
-            _need(slopes.shape == (self.q_heads,) and _is_f32(slopes.dtype) and _contiguous(slopes),
-                  f"{op}: slopes is no f32 vector of {self.q_heads}")
+            if slopes.shape != (self.q_heads,) or not _is_f32(slopes.dtype) or not _contiguous(slopes):
+                raise S2SError(f"{op}: slopes is no f32 vector of {self.q_heads}")
             slope_ptr = slopes.data_ptr()
         args = _SHARED.pack(*self.head, *arrays, _vector(q_lens, batch, op, "q_lens"), _vector(k_lens, batch, op, "k_lens"),
                             0, 0, 0, 0, 0, 0, 0, 0, 0, slope_ptr, 0, 0, self.shared_tokens,
@@ -260,15 +261,18 @@ _SIZES = {}
 
 
 def _bytes(a) -> int:
-    n = 1
-    for d in a.shape:
-        n *= d
+    shape, n = a.shape, 1
+    if len(shape) == 1:
+        n = shape[0]
+    else:
+        for d in shape:
+            n *= d
     size = _SIZES.get(a.dtype)
     if size is None:
         size = {"u8": 1, "uint8": 1, "i32": 4, "int32": 4, "f32": 4, "float32": 4}.get(str(a.dtype).replace("torch.", ""))
         _need(size is not None, f"workspace: of {a.dtype}, wanted u8, i32 or f32")
         _SIZES[a.dtype] = size
-    _need(len(a.shape) == 1 and a.stride()[0] == 1 or _contiguous(a), "workspace: not contiguous")
+    _need(len(shape) == 1 and a.stride()[0] == 1 or _contiguous(a), "workspace: not contiguous")
     return n * size
 
 
@@ -308,7 +312,8 @@ class Rotary:
     def _arrays(self, op, q, pos, q_out, k, k_out, lens):
         """The struct's fields, and the outputs."""
         shape = q.shape
-        _need(len(shape) == 4 and max(shape) < 2 ** 31, f"{op}: q is {tuple(shape)}, wanted [batch][tokens][heads][width]")
+        if len(shape) != 4 or max(shape) >= 2 ** 31:
+            raise S2SError(f"{op}: q is {tuple(shape)}, wanted [batch][tokens][heads][width]")
         dt = _type(q.dtype)
         if q_out is None:
             q_out = q
@@ -316,16 +321,17 @@ class Rotary:
         k_arrays, k_heads = ((0, 0, 0, 0), (0, 0, 0, 0)), 0
         if k is not None:
             ks = k.shape
-            _need(len(ks) == 4 and 1 <= ks[2] < 2 ** 31, f"{op}: k is {tuple(ks)}, wanted [batch][tokens][heads][width]")
+            if len(ks) != 4 or not 1 <= ks[2] < 2 ** 31:
+                raise S2SError(f"{op}: k is {tuple(ks)}, wanted [batch][tokens][heads][width]")
             k_heads = ks[2]
             ks = (shape[0], shape[1], k_heads, shape[3])
             if k_out is None:
                 k_out = k
             k_arrays = _tokens(k, ks, dt, op, "k"), _tokens(k_out, ks, dt, op, "k_out")
-        else:
-            _need(k_out is None, f"{op}: k_out without k")
-        ps, pstr = pos.shape, pos.stride()
-        if not _is_int32(pos.dtype) or len(ps) not in (2, 3) or ps[:-1] != (shape[:2] if len(ps) == 3 else shape[1:2]):
+        elif k_out is not None:
+            raise S2SError(f"{op}: k_out without k")
+        ps, pstr = tuple(pos.shape), pos.stride()
+        if not _is_int32(pos.dtype) or len(ps) not in (2, 3) or ps[:-1] != tuple(shape[:2] if len(ps) == 3 else shape[1:2]):
             raise S2SError(f"{op}: pos is {tuple(ps)} of {pos.dtype}, wanted int32 [batch][tokens][axes] or [tokens][axes]")
         if (pstr[-1] != 1 and ps[-1] != 1) or (pstr[-2] != ps[-1] and ps[-2] > 1):
             raise S2SError(f"{op}: the tokens and axes of pos are not adjacent")
@@ -361,10 +367,11 @@ class NormRotary(Rotary):
         qw, qs = _head_weight(q_weight, q.shape, op, "q_weight")
         kw = ks = 0
         if k is not None:
-            _need(k_weight is not None, f"{op}: k without k_weight")
+            if k_weight is None:
+                raise S2SError(f"{op}: k without k_weight")
             kw, ks = _head_weight(k_weight, k.shape, op, "k_weight")
-        else:
-            _need(k_weight is None, f"{op}: k_weight without k")
+        elif k_weight is not None:
+            raise S2SError(f"{op}: k_weight without k")
         if self.lib.s2s_norm_rotary(_NORM_ROTARY.pack(*args, qw, kw, qs, ks, *self.numbers), stream):
             raise S2SError(f"{op}: {last_error()}")
         return q_out if k is None else (q_out, k_out)
@@ -395,22 +402,24 @@ def rms_norm(x, weight, out, eps: float = 1e-6, res=None, sum=None, scales=None,
     or e4m3 (then with `scales` f32 [rows][ceil(cols / group)], group 0 being the
     row); weight f32 [cols]."""
     op, shape = "rms_norm", x.shape
-    _need(len(shape) == 2, f"{op}: x is {tuple(shape)}, wanted [rows][cols]")
+    if len(shape) != 2:
+        raise S2SError(f"{op}: x is {tuple(shape)}, wanted [rows][cols]")
     rows, cols = shape
-    _need(cols < 2 ** 31 and 0 <= group < 2 ** 31, f"{op}: columns or a group that are negative or no 32-bit int")
+    if cols >= 2 ** 31 or not 0 <= group < 2 ** 31:
+        raise S2SError(f"{op}: columns or a group that are negative or no 32-bit int")
     dt = _type(x.dtype)
     odt = E4M3 if _type(out.dtype) == E4M3 else dt
     xp, xs = _rows(x, shape, dt, op, "x")
     rp, rs = _rows(res, shape, dt, op, "res")
     sp, ss = _rows(sum, shape, dt, op, "sum")
     op_, os_ = _rows(out, shape, odt, op, "out")
-    _need(weight.shape == (cols,) and _is_f32(weight.dtype) and (weight.stride()[0] == 1 or cols <= 1),
-          f"{op}: weight is no f32 vector of {cols}")
+    if weight.shape != (cols,) or not _is_f32(weight.dtype) or (weight.stride()[0] != 1 and cols > 1):
+        raise S2SError(f"{op}: weight is no f32 vector of {cols}")
     scale_ptr = 0
     if scales is not None:
         n = -(-cols // group) if group else 1
-        _need(scales.shape == (rows, n) and _is_f32(scales.dtype) and _contiguous(scales),
-              f"{op}: scales is no contiguous f32 [{rows}][{n}]")
+        if scales.shape != (rows, n) or not _is_f32(scales.dtype) or not _contiguous(scales):
+            raise S2SError(f"{op}: scales is no contiguous f32 [{rows}][{n}]")
         scale_ptr = scales.data_ptr()
     args = _RMS.pack(dt, odt, rows, cols, xp, rp, sp, op_, xs, rs, ss, os_, weight.data_ptr(), _f32(weight_offset), _f32(eps), scale_ptr,
                      group)
