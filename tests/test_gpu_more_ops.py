@@ -836,3 +836,47 @@ def test_operators_together_captured(pkg, mode):
         h.hipGraphDestroy(g)
     for s in (st, two):
         h.hipStreamDestroy(s)
+
+
+# ---- hidden keys in the kernels of large calls -------------------------------------------------
+
+LARGE = {
+    "f16": dict(dtype="f16", D=128),
+    "cap_bf16": dict(dtype="bf16", D=128, cap=50.0, spread=4.0),
+    "cap_f32": dict(dtype="f32", D=32, cap=50.0, spread=4.0),
+    "slopes_bf16": dict(dtype="bf16", D=64, slopes=True),
+    "slopes_f32": dict(dtype="f32", D=128, slopes=True),
+    "cap_slopes_f16": dict(dtype="f16", D=96, slopes=True, cap=30.0),
+    "rows_of_4_bytes_f32": dict(dtype="f32", D=30, slopes=True),
+    "rows_of_4_bytes_f16": dict(dtype="f16", D=62, cap=30.0),
+    "odd_bf16": dict(dtype="bf16", D=63, gap=1),
+}
+
+
+@pytest.mark.parametrize("name", LARGE)
+@pytest.mark.parametrize("causal", [True, False])
+def test_window_large_calls_hide_what_keys_hold(pkg, name, causal):
+    def change(q, k, v, more):
+        # left behind by all but the first queries, ahead of all but the last ones, and a sink
+        v[:, 25, 0, 5], v[:, 30, 1, 2], k[:, 27, 2, 0] = np.nan, np.inf, np.nan
+        v[:, 180, 3, 7], v[:, 1, 5, 3] = -np.inf, np.inf
+    check_window(pkg, wcase(**LARGE[name], window=20, sinks=3, causal=causal, **WIDE), change)
+
+
+@pytest.mark.parametrize("name", LARGE)
+def test_shared_large_calls_hide_what_keys_hold(pkg, name):
+    """Whole keys by waves of 32 columns: keys past an entry's part, past its own, and in the future."""
+    c = dict(LARGE[name])
+    cap = c.pop("slopes", False)  # (slopes leave far keys without a weight in 32 bits: gentle ones)
+    c = scase(**c, B=23, S=130, Lq=70, Lk=80, H=12, KV=12, causal=True, slopes=cap, shared_lens=[5 * i for i in range(23)],
+              k_lens=[80 - i for i in range(23)], q_lens=[70 - i for i in range(23)])
+
+    def change(q, k, v, sk, sv, more):
+        if "slopes" in more:
+            more["slopes"] /= 64
+        sk[111:], sv[115:] = np.nan, -np.inf
+        sv[60, 0, 3], sv[61, 1, 5], sk[62, 2, 0] = np.inf, np.nan, np.nan
+        for b in range(23):
+            k[b, 80 - b:], v[b, 80 - b:] = np.nan, (np.inf, np.nan)[b % 2]
+            v[b, 79 - b, 4, 1] = np.inf
+    check_shared(pkg, c, change)
