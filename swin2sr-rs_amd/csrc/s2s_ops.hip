@@ -752,10 +752,14 @@ hipError_t norm_rotary_launch(const NormRotaryArgs &a, const NormRotaryWalk &w, 
 
 template <typename T, bool ADJ, int V>
 hipError_t norm_rotary_of(const NormRotaryArgs &a, const NormRotaryWalk &w, hipStream_t st) {
-    if (a.r.pairs > 64) {  // (nine lanes at least)
-        if (w.per_head <= 16) return norm_rotary_launch<T, ADJ, V, 16, 128>(a, w, st);
-        if (w.per_head <= 32) return norm_rotary_launch<T, ADJ, V, 32, 128>(a, w, st);
-        return norm_rotary_launch<T, ADJ, V, 64, 128>(a, w, st);
+    if constexpr (V > 1) {
+        if (a.r.pairs > 64) {  // over 64 / V lanes
+            if constexpr (V == 8)
+                if (w.per_head <= 16) return norm_rotary_launch<T, ADJ, V, 16, 128>(a, w, st);
+            if constexpr (V >= 4)
+                if (w.per_head <= 32) return norm_rotary_launch<T, ADJ, V, 32, 128>(a, w, st);
+            return norm_rotary_launch<T, ADJ, V, 64, 128>(a, w, st);
+        }
     }
     if (w.per_head <= 4) return norm_rotary_launch<T, ADJ, V, 4, 64>(a, w, st);
     if (w.per_head <= 8) return norm_rotary_launch<T, ADJ, V, 8, 64>(a, w, st);

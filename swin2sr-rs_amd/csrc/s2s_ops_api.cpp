@@ -128,7 +128,7 @@ int attention_sizes(const char *op, const s2s_attention_args *a) {
     return 0;
 }
 
-int window_sizes(const char *op, const s2s_attention_args *a, int window, int sinks) {
+int window_sizes(const char *op, int window, int sinks) {
     if (window < 1 || window > (1 << 30)) return refuse("%s: a window of %d keys is not in 1 to 2^30", op, window);
     if (sinks < 0 || sinks > (1 << 30)) return refuse("%s: %d sinks are not in 0 to 2^30", op, sinks);
     return 0;
@@ -401,7 +401,7 @@ int s2s_window_attention_workspace(const s2s_attention_args *a, int window, int 
     const char *op = "s2s_window_attention_workspace";
     if (!a || !bytes) return refuse("%s: null argument", op);
     if (int rc = attention_sizes(op, a)) return rc;
-    if (int rc = window_sizes(op, a, window, sinks)) return rc;
+    if (int rc = window_sizes(op, window, sinks)) return rc;
     *bytes = attn_op_workspace(a->dtype, attention_args(a, window, sinks));
     return 0;
 }
@@ -411,7 +411,7 @@ int s2s_window_attention(const s2s_attention_args *a, int window, int sinks, voi
     const char *op = "s2s_window_attention";
     if (!a) return refuse("%s: null argument", op);
     if (int rc = attention_sizes(op, a)) return rc;
-    if (int rc = window_sizes(op, a, window, sinks)) return rc;
+    if (int rc = window_sizes(op, window, sinks)) return rc;
     // (a document's own first keys are not known)
     if (sinks > 0 && (a->q_docs || a->k_docs)) return refuse("%s: sinks with documents", op);
     return attention_call(op, a, window, sinks, nullptr, workspace, workspace_bytes, stream);

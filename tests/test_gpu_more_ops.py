@@ -880,3 +880,11 @@ def test_shared_large_calls_hide_what_keys_hold(pkg, name):
             k[b, 80 - b:], v[b, 80 - b:] = np.nan, (np.inf, np.nan)[b % 2]
             v[b, 79 - b, 4, 1] = np.inf
     check_shared(pkg, c, change)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,pairs", [(136, 66), (144, 72), (160, 80), (200, 65), (192, 96), (256, 128), (258, 65), (300, 128)])
+def test_norm_rotary_many_pairs(pkg, dtype, D, pairs):
+    """More than 64 pairs, in lanes of one to eight."""
+    for adjacent in (False, True):
+        turned(pkg, dtype, 2, 21, 3, 1, D, (pairs - 30, 30), adjacent=adjacent, each=D % 16 == 0)
