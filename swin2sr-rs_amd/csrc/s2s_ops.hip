@@ -203,19 +203,30 @@ __device__ __forceinline__ float nan_max(float m, float v) {
     return v > m || v != v ? v : m;
 }
 
-// 1 / sqrt(mean of n squares + eps) from the squares' sum. Where that lies past an f32's range, or
-// (with so small an eps) where its precision ends, it is made again of the row times 2^-80 or
-// 2^80: `again(factor)`, which all threads of the row call or none. (Squares of f16 lie within 2^-48
+// What norms a row whose squares' sum passes an f32's range (FAR), or (with so small an eps) lies where
+// its precision ends (NEAR): the sum is made again of the row times 2^-80 or 2^100, and that factor is
+// multiplied in by itself, ahead of the reciprocal root for a NEAR row and behind it for a FAR one, since a
+// product of the two is no normal number for rows of 2^-128 or 2^127 (and a small channel of a FAR row times 2^-80
+// none either). 2^100 takes the smallest f32, 2^-149, to squares of 2^-98, and what is below the border, 2^-50, to 2^50.
+constexpr float kFar = 0x1p127f, kNear = 0x1p-100f, kFarUnit = 0x1p-80f, kNearUnit = 0x1p100f;
+struct Root {
+    float inv, before = 1.f, after = 1.f;
+    __device__ bool plain() const { return before * after == 1.f; }
+    __device__ float of(float v) const { return v * before * inv * after; }
+};
+
+// 1 / sqrt(mean of n squares + eps) from the squares' sum. `again(factor)` makes the sum of the row
+// times a factor; all threads of the row call it or none. (Squares of f16 lie within 2^-48
 // and 2^34, and 2^24 of them within both ends.)
 template <typename T, typename F>
-__device__ __forceinline__ float inverse_root(float ss, int n, float eps, const F &again) {
+__device__ __forceinline__ Root inverse_root(float ss, int n, float eps, const F &again) {
     constexpr bool F16 = std::is_same<T, half_t>::value;
-    const bool far = !F16 && ss > 0x1p127f, near = !F16 && ss < 0x1p-100f && eps < 0x1p-100f;
+    const bool far = !F16 && ss > kFar, near = !F16 && ss < kNear && eps < kNear;
     if (__builtin_expect(far || near, 0)) {
-        const float f = far ? 0x1p-80f : 0x1p80f;
-        return f / sqrtf(again(f) / (float)n + eps * f * f);
+        const float f = far ? kFarUnit : kNearUnit;
+        return {1.0f / sqrtf(again(f) / (float)n + eps * f * f), far ? 1.f : f, far ? f : 1.f};
     }
-    return 1.0f / sqrtf(ss / (float)n + eps);
+    return {1.0f / sqrtf(ss / (float)n + eps)};
 }
 
 __device__ __forceinline__ float e4m3_scale(float top) {
@@ -246,20 +257,20 @@ __global__ __launch_bounds__(256) void k_rms_norm_rows(RmsNormArgs a) {
             __syncthreads();
             return (part[0] + part[1]) + (part[2] + part[3]);
         };
-        const float inv = inverse_root<T>(squares(1.f), a.cols, a.eps, [&](float f) {
+        const Root root = inverse_root<T>(squares(1.f), a.cols, a.eps, [&](float f) {
             __syncthreads();  // `part` has been read
             return squares(f);
         });
         auto value = [&](int c) {
             const float h = (float)x[c] + (res ? (float)res[c] : 0.f);
-            return h * inv * (a.weight[c] + a.offset);
+            return root.of(h) * (a.weight[c] + a.offset);
         };
         if constexpr (!E4M3) {
             T *out = (T *)a.out + row * a.os;
             for (int c = tid; c < a.cols; c += 256) {
                 const float h = (float)x[c] + (res ? (float)res[c] : 0.f);
                 if (sum) sum[c] = (T)h;
-                out[c] = (T)(h * inv * (a.weight[c] + a.offset));
+                out[c] = (T)(root.of(h) * (a.weight[c] + a.offset));
             }
         } else {
             unsigned char *out = (unsigned char *)a.out + row * a.os;
@@ -373,10 +384,18 @@ __global__ __launch_bounds__(256) void k_rms_norm(RmsNormArgs a) {
                 if (i < chunks) *(Vec *)(sum + i * V) = u;
             }
         }
-        const float inv = inverse_root<T>(of_row(own), a.cols, a.eps, [&](float f) {
+        const Root root = inverse_root<T>(of_row(own), a.cols, a.eps, [&](float f) {
             if constexpr (TPR == 256) __syncthreads();  // `part` has been read
             return of_row(squares(f));
         });
+        float inv = root.inv;
+        if (__builtin_expect(!root.plain(), 0)) {  // (all of the row)
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int e = 0; e < V; ++e) h[n][e] = root.of(h[n][e]);
+            inv = 1.f;
+        }
 #pragma unroll
         for (int n = 0; n < NC; ++n)
 #pragma unroll
@@ -526,8 +545,8 @@ __global__ __launch_bounds__(256) void k_norm_rotary_heads(NormRotaryArgs a) {
             }
             return wave_sum(ss);
         };
-        const float inv = inverse_root<T>(squares(1.f), r.width, a.eps, squares);
-        auto value = [&](int c) { return (float)x[c] * inv * (w[c] + a.offset); };
+        const Root root = inverse_root<T>(squares(1.f), r.width, a.eps, squares);
+        auto value = [&](int c) { return root.of((float)x[c]) * (w[c] + a.offset); };
         for (int p = lane; p < r.pairs; p += 64) {
             const int c0 = r.adjacent ? 2 * p : p, c1 = r.adjacent ? c0 + 1 : c0 + r.pairs;
             const float u = value(c0), v = value(c1);
@@ -692,10 +711,13 @@ __global__ __launch_bounds__(256) void k_norm_rotary(RotaryArrays r, HeadNorm a,
             const float ss = squares(1.f);
             float inv = __builtin_amdgcn_rsqf(fmaf(ss, mean, a.eps));
             // heads whose squares pass an f32's range, either way (as of a row of the norm)
-            const bool far = ss > 0x1p127f, near = ss < 0x1p-100f && a.eps < 0x1p-100f;
+            const bool far = ss > kFar, near = ss < kNear && a.eps < kNear;
             if (__builtin_expect(__any(far || near), 0)) {
-                const float f = far ? 0x1p-80f : near ? 0x1p80f : 1.f;
-                inv = f * __builtin_amdgcn_rsqf(fmaf(squares(f), mean, a.eps * f * f));
+                const float f = far ? kFarUnit : near ? kNearUnit : 1.f;
+                const Root root = {__builtin_amdgcn_rsqf(fmaf(squares(f), mean, a.eps * f * f)), far ? 1.f : f, far ? f : 1.f};
+#pragma unroll
+                for (int i = 0; i < V; ++i) u[0][i] = root.of(u[0][i]), u[1][i] = root.of(u[1][i]);
+                inv = 1.f;
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
