@@ -790,9 +790,11 @@ hipError_t norm_rotary_of(const NormRotaryArgs &a, const NormRotaryWalk &w, hipS
     return norm_rotary_launch<T, ADJ, V, 64, 64>(a, w, st);
 }
 
-// Whether offsets of an array within a workgroup's tokens, and across an entry's end, are 32-bit ones.
-bool norm_rotary_offsets(const Strides &s, int tb, int tokens, int heads, int width, int size, int unit, int &t, int &h, int &b) {
-    const __int128 next = ((__int128)s.b - (__int128)tokens * s.t) * size, most = BUF_MAX_BYTES / 4;
+// Whether offsets of an array within a workgroup's tokens, and across an entry's end where another follows, are
+// 32-bit ones. (65536 tokens of 32 + 8 + 8 bf16 heads of 128 in one array of 805 MB, one entry: 247 us; by a wave a
+// head, as if an entry followed 805 MB back, 1539.)
+bool norm_rotary_offsets(const Strides &s, int tb, int batch, int tokens, int heads, int width, int size, int unit, int &t, int &h, int &b) {
+    const __int128 next = batch > 1 ? ((__int128)s.b - (__int128)tokens * s.t) * size : 0, most = BUF_MAX_BYTES / 4;
     if ((__int128)tb * s.t * size > most || (__int128)heads * s.h * size > most || next > most || next < -most || width * size > (1 << 20)) return false;
     // (factors of 24 bits)
     if (s.t / unit >= (1 << 23) || s.h / unit >= (1 << 23)) return false;
@@ -831,8 +833,8 @@ hipError_t norm_rotary_type(const NormRotaryArgs &a, hipStream_t st) {
         auto set = [&](int k, const Strides &in, const Strides &out, int heads) {
             NormRotaryWalk::Of &o = w.of[k];
             o.by_heads = (unsigned)(((1ULL << 32) + heads - 1) / heads);
-            return norm_rotary_offsets(in, w.tb, r.tokens, heads, r.width, size, v, o.in_t, o.in_h, o.in_b) &&
-                   norm_rotary_offsets(out, w.tb, r.tokens, heads, r.width, size, v, o.out_t, o.out_h, o.out_b);
+            return norm_rotary_offsets(in, w.tb, r.batch, r.tokens, heads, r.width, size, v, o.in_t, o.in_h, o.in_b) &&
+                   norm_rotary_offsets(out, w.tb, r.batch, r.tokens, heads, r.width, size, v, o.out_t, o.out_h, o.out_b);
         };
         fits = fits && set(0, r.sq, r.sqo, r.hq) && (!r.hk || set(1, r.sk, r.sko, r.hk));
     }
