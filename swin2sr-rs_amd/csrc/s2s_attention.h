@@ -1444,19 +1444,20 @@ hipError_t join(const AttnOpArgs &a, const AttnLaunch &L, hipStream_t st) {
 
 template <typename T, int DP, int W>
 hipError_t launch_width(const AttnOpArgs &a, const AttnLaunch &L, const Cut &c, int align, hipStream_t st) {
-    hipError_t e = hipErrorInvalidValue;
-    if (c.wk)
-        e = launch_narrow<T, DP, true, W>(a, L, align, st);
-    else if (c.nb == 1)
-        e = launch_narrow<T, DP, false, W>(a, L, align, st);
-    else if (W != 0 && align < 16)
-        e = launch<T, DP, 2, false, W != 0 ? 4 : 16, ANY | W>(a, L, st);
-    else if (W != WHOLE && a.k_docs)
-        e = launch<T, DP, 2, false, 16, W != WHOLE ? ANY | DOCS | W : W>(a, L, st);
-    else if (a.cap > 0.f)
-        e = a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES | W>(a, L, st) : launch<T, DP, 2, false, 16, CAP | W>(a, L, st);
-    else
-        e = a.slopes ? launch<T, DP, 2, false, 16, SLOPES | W>(a, L, st) : launch<T, DP, 2, false, 16, W>(a, L, st);
+    auto kernel = [&]() -> hipError_t {
+        if (c.wk) return launch_narrow<T, DP, true, W>(a, L, align, st);
+        if (c.nb == 1) return launch_narrow<T, DP, false, W>(a, L, align, st);
+        if constexpr (W != 0)
+            if (align < 16) return launch<T, DP, 2, false, 4, ANY | W>(a, L, st);
+        if (a.k_docs) {  // (of narrow heads never: waves of 16 take them)
+            if constexpr (W != WHOLE && DP > 64) return launch<T, DP, 2, false, 16, ANY | DOCS | W>(a, L, st);
+            return hipErrorInvalidValue;
+        }
+        if (a.cap > 0.f)
+            return a.slopes ? launch<T, DP, 2, false, 16, CAP | SLOPES | W>(a, L, st) : launch<T, DP, 2, false, 16, CAP | W>(a, L, st);
+        return a.slopes ? launch<T, DP, 2, false, 16, SLOPES | W>(a, L, st) : launch<T, DP, 2, false, 16, W>(a, L, st);
+    };
+    const hipError_t e = kernel();
     return e != hipSuccess || !L.join ? e : join<T, DP>(a, L, st);
 }
 
