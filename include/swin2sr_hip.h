@@ -346,12 +346,17 @@ int s2s_window_attention(const s2s_attention_args *args, int window, int sinks, 
                          void *stream);
 
 /* The attention of a batch whose entries all begin with the same keys, which lie in
- * memory once and are read once for all of them: entry b's keys are the shared ones
+ * memory once: entry b's keys are the shared ones
  * j < shared_lens[b], and behind them its own. The query's place is P(i) =
  * shared_lens[b] + k_lens[b] - q_lens[b] + i; masks (`causal`, lengths), cap and slopes are as
- * above. (For f16 and bf16 the weights of shared keys are rounded to the type unless
- * at most 16 queries times heads of the whole batch read a key head.) `own` holds the call's sizes (k_tokens of each entry's own keys, 0
- * allowed), arrays and masks; its prefix, documents, positions and table have to be
+ * above. Steps over many keys read the shared ones once for the whole batch, in ranges
+ * whose sums are joined; where more queries or few keys make that the slower way, and for
+ * arrays that are not of 4-byte multiples and scales of 0 and below, every entry's
+ * queries walk them. For f16 and bf16 the weights are rounded to the type before they
+ * multiply v where more than 16 (query, head) pairs of a key head go over the keys together:
+ * pairs of an entry or, for shared keys that are read once, of the whole batch. Of
+ * up to 16 what the rounding leaves is kept. `own` holds the call's sizes (k_tokens of
+ * each entry's own keys, 0 allowed), arrays and masks; its prefix, documents, positions and table have to be
  * NULL. Lengths are taken as clamped to the tokens. Up to 2^30 shared and own
  * tokens, 2^26 query tokens times heads of the batch. The workspace goes by dtype
  * and the seven sizes. */

@@ -106,7 +106,8 @@ struct AttnLaunch {
     int splits;     // key ranges per column tile
     int vec;        // bytes of one element-wise access (unaligned arrays): 8, 4 or 2
     int out_vec;    // elements that one store of the output takes: 4, 2 or 1
-    float *part_o;  // splits > 1: [batch * hk][splits][cols][DP] unnormalised sums
+    // what a join reads, of one range too where it joins shared keys as well (else null without a second range):
+    float *part_o;   // [batch * hk][splits][cols][DP] unnormalised sums
     float *part_ml;  // [batch * hk][splits][cols][2]: reference and sum of the weights
     const int4 *meta;  // documents: [batch][key tiles] {smallest, largest id >= 0, smallest id, 0}
     int meta_tiles;
@@ -765,8 +766,8 @@ struct Kernel {
                 }
             }
             // What the rounding of a weight left may be zero, and zero times an infinity is none: a sum that is
-            // no number of weights that are is made again, with the infinities of v by themselves. (One query over 131071
-            // keys 20.9 -> 21.3 us for the look; no other call by more than two runs differ.)
+            // no number of weights that are is made again, with the infinities of v by themselves. (For the look: one query over
+            // 131071 keys 20.9 -> 21.3 us, 32 of up to 8192 134.0 -> 134.5, in the join's own barriers 21.5 and 134.5.)
             if (RETRY && !careful && part == (ALL ? 1 : 0)) {
                 bool none = false;
 #pragma unroll
@@ -1117,7 +1118,11 @@ struct Kernel {
         const int i = tab + min(max(dist, -u.half), u.half) + u.half;
         return u.table_lds ? lds_read<float>(u.tab0 + 4 * i, 0) : u.table[i];
     }
-    // O^T += V^T P^T
+    // O^T += V^T P^T, with P of 16-bit types rounded to the type: v's products would run at the rate of f32 otherwise. The
+    // roundings of a row's weights, half a step each and independent, leave 1.2 to 1.4 times the error that the result's own
+    // rounding makes (bf16 2.0e-3 to 2.3e-3 against 64 bits, 1.65e-3 with f32 weights). Where the waves split the keys what they
+    // leave takes slots that are free. A product of its own for it over the keys that steps share (64 steps, 16384 bf16 keys: 1.65e-3 for
+    // 2.30e-3) would cost 66 -> 69 us, and 3 to 13% at other sizes (64 steps over 16384 and 320 to 640 keys of their own 57 -> 64).
     static __device__ __forceinline__ void products(const lds_t *vl0, const f4v (*s)[NB], f4v (*o)[NB],
                                                     typename std::conditional<F32, float, f4v>::type *l) {
         constexpr int J = F32 || WK ? KB : KB / 2;
@@ -1210,7 +1215,9 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnOpArgs a, AttnLaunch L) {
 
 // The columns of all entries over the shared keys, `shared` workgroups, and each entry's few columns over its own keys
 // in one launch: the first are bound by instructions, the second by HBM, and a CU takes both (64 steps over 16384 shared
-// and 640 own keys, 32 / 8 bf16 heads of 128: 56 us with the join, 78 in a launch each).
+// and 640 own keys, 32 / 8 bf16 heads of 128: 56 us with the join, 78 in a launch each). Of f32 heads over 64 wide a CU
+// takes one workgroup of either, since the own keys' two buffers fill 128 KB and a launch has one size of LDS: 64 steps over 4096
+// and 320 to 640 such keys 117 us, of 64 wide 52.
 template <typename T, int DP, int NB, bool WK, int ALIGN, bool OWN_WK>
 __global__ __launch_bounds__(256, 2) void k_attn_both(AttnOpArgs a, AttnLaunch own, AttnLaunch shared, int blocks) {
     extern __shared__ __align__(16) char lds[];

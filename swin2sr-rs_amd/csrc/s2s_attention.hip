@@ -33,7 +33,9 @@ attn::Cut cut_of(int dtype, const AttnOpArgs &a, bool narrow) {
     c.tiles = (int)((cols + per - 1) / per);
     const long long blocks = std::max(1LL, pairs * c.tiles);
     long long nt = ((long long)a.nk + c.tk - 1) / c.tk;
-    // of a window the tiles that a column tile's queries and the sinks lie in
+    // of a window the tiles that a column tile's queries and the sinks lie in. (Whether a call has a prefix is not known when its
+    // workspace is made. One past the window adds to a column tile's keys those of the queries behind it, which it then walks in
+    // as many ranges as the window alone would have.)
     if (a.window) {
         nt = std::min(nt, ((long long)(a.causal ? 1 : 2) * a.window + per / a.group + c.tk) / c.tk + 1 + ((long long)a.sinks + c.tk - 1) / c.tk);
         // few tiles are not cut: a launch less (5 queries over windows of 128 of 700 keys, 8 f16 heads of 64, 8.7 us with
@@ -366,7 +368,10 @@ size_t sums_bytes(const attn::Cut &c, const AttnOpArgs &a) { return round16(colu
 // Whether every column tile walks the shared keys by itself, and its entry's own behind them. For more than 32 columns
 // an entry always, since the shared keys' sums of every range, written and read again, cost more than the keys
 // (8 x 512 tokens behind 1024, 4096 and 16384 shared keys, 32 / 8 bf16 heads of 128: 98, 294 and 1077 us
-// against 177, 379 and 1188; 16 x 16 tokens, 64 columns, 26, 31 and 60 behind 1024, 2048 and 8192, 29, 34 and 68). 17 to 32,
+// against 177, 379 and 1188; 16 x 16 tokens, 64 columns, 26, 31 and 60 behind 1024, 2048 and 8192, 29, 34 and 68; 64 x 9, 12 and 16
+// tokens behind 8192 162, 162 and 175, 213, 216 and 221; 36 x 64 tokens of 6 f32 heads of 30 behind 1089 38.5 and 39.2. It is the slower way for
+// f32 of fewer columns: 33 and 48 such tokens 36 and 37.5, 27 and 31; 16 x 40 of 8 heads of 128 behind 4096 154 and 117; but
+// 64 x 40 of 64 behind 1024 83 and 91). 17 to 32,
 // which leave the half of a tile of their own empty: of 16-bit types but for many keys times entries (16 x 8 tokens behind 1024
 // and 8192 keys 20 and 52 us, 26 and 39 by the ranges), of f32, whose products take longer, never (16 x 24 tokens of 6
 // heads of 30 behind 1024 and 8192 keys 23 and 83, 17 and 44). Steps over up to eight tiles.

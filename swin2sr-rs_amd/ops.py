@@ -136,7 +136,8 @@ class Attention:
     `dtype` ("f32", "f16", "bf16") is the type of q, k, v and out; `scale` is
     1 / sqrt(width) by default, `cap` 0 for none, `window` 0 for none: with one, a
     query sees the `window` last keys up to its own place (not `causal`: those less than
-    `window` away either way) and the first `sinks` ones. `workspace_bytes` of device
+    `window` away either way) and the first `sinks` ones (not `causal`: up to the same
+    last key). `workspace_bytes` of device
     memory go with every call: one buffer serves all calls of a stream, calls
     that may overlap on the device (other streams, replays of captured graphs)
     need one each.
